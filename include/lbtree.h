@@ -33,6 +33,9 @@ extern "C" {
  * (src/cpp_utils/cpp_utils.h:177-182 type_dispatch_float). */
 #define LBT_F32 0
 #define LBT_F64 1
+/* further types of lbt_linear_log_loss and lbt_embed_rows */
+#define LBT_BF16 2
+#define LBT_F16 3
 
 /* Upper limit on split_samples, as in legateboost/models/tree.py:75-76. */
 #define LBT_MAX_SPLIT_SAMPLES 2048
@@ -528,6 +531,69 @@ int lbt_next_gradient(void* stream, int32_t objective, const double* leaf_value,
 int lbt_gather_rows(void* stream, const void* X, int32_t x_dtype, int64_t row_offset, int64_t n_rows,
                     int32_t n_features, const int64_t* sample_rows, int64_t n_samples,
                     int32_t samples_on_host, int64_t* staging, void* out);
+
+/* ---- vocabularies: linear scores over many classes, rows of a table (no counterpart in the reference) ----- */
+
+/*
+ * Log loss of linear scores over many classes (a vocabulary), where lbt_weighted_gradient takes the scores themselves:
+ *   s[r][c] = <X[r], weight[c]> + bias[c];   loss[r] = log sum_c exp(s[r][c]) - s[r][y[r]]
+ * The scores are formed in tiles of rows and classes and never written. Sums, tops and totals are held in 32 bits; LBT_F32
+ * inputs are multiplied as three planes of bfloat16 each, which gives products as exact as those of float.
+ *   X       device [n_rows][n_features], dtype LBT_F32, LBT_BF16 or LBT_F16, 16-byte aligned
+ *   weight  device [n_outputs][n_features], the same dtype, 16-byte aligned
+ *   bias    device float [n_outputs], or NULL. A class whose bias is -inf takes no part (p = 0; a row with that label has an
+ *           infinite loss); where that leaves no class, the losses are infinite and p is 0
+ *   y       device int64 [n_rows]. A row whose label is not in [0, n_outputs) does not count: its loss is 0, nothing that
+ *           it holds (NaN and infinities too) reaches any output
+ *   loss    device float [n_rows]
+ *   workspace  at least lbt_linear_log_loss_workspace_bytes(..., gradient = 0), 256-byte aligned
+ * Enqueues on the stream and does not wait. All results are the same from call to call.
+ */
+size_t lbt_linear_log_loss_workspace_bytes(int64_t n_rows, int32_t n_features, int32_t n_outputs, int32_t dtype, int32_t gradient);
+int lbt_linear_log_loss(void* stream, const void* X, const void* weight, int32_t dtype, int64_t n_rows, int32_t n_features,
+                        int32_t n_outputs, const float* bias, const int64_t* y, float* loss, void* workspace,
+                        size_t workspace_bytes);
+
+/*
+ * The same loss together with the gradients of sum_r sample_weight[r] loss[r]:
+ *   G[r][c] = sample_weight[r] (p[r][c] - [c = y[r]]),  p = softmax(s)
+ *   grad_X = G weight,  grad_weight = G^T X,  grad_bias[c] = sum_r G[r][c]
+ * G is formed for a piece of the classes at a time (at most 512 MiB of it), in the inputs' type (LBT_F16: times a power of two;
+ * LBT_F32: three planes of bfloat16), and multiplied both ways with sums in 32 bits.
+ *   sample_weight  device float [n_rows], or NULL for ones
+ *   grad_X, grad_weight  device, shape and dtype of X and weight, 16-byte aligned; overwritten (zeros for rows that do not count)
+ *   grad_bias      device float [n_outputs], or NULL; only with a bias
+ *   workspace      at least lbt_linear_log_loss_workspace_bytes(..., gradient = 1), 256-byte aligned
+ */
+int lbt_linear_log_loss_gradient(void* stream, const void* X, const void* weight, int32_t dtype, int64_t n_rows,
+                                 int32_t n_features, int32_t n_outputs, const float* bias, const int64_t* y,
+                                 const float* sample_weight, float* loss, void* grad_X, void* grad_weight, float* grad_bias,
+                                 void* workspace, size_t workspace_bytes);
+
+/*
+ * out[t] = scale * table[tokens[t]], multiplied in float and rounded once. lbt_gather_rows for the types that models use, for
+ * tokens and for categories; a tree's row_leaf is such an array too.
+ *   table   device [n_rows][n_features], dtype LBT_F32, LBT_BF16 or LBT_F16, 16-byte aligned
+ *   tokens  device int32 (token_bytes 4) or int64 (8) [n_tokens]. A token not in [0, n_rows) gives a row of zeros
+ *   out     device [n_tokens][n_features], dtype of the table, 16-byte aligned; may not overlap the table
+ * Enqueues on the stream and does not wait.
+ */
+int lbt_embed_rows(void* stream, const void* table, int32_t dtype, int32_t n_rows, int32_t n_features, const void* tokens,
+                   int32_t token_bytes, int64_t n_tokens, float scale, void* out);
+
+/*
+ * The gradient of lbt_embed_rows with respect to the table:
+ *   grad_table[v] = scale * sum over t with tokens[t] = v of grad[t]
+ * The tokens are sorted and each sum is formed in float in a fixed order: the same bits from call to call.
+ *   grad        device [n_tokens][n_features], 16-byte aligned; tokens not in [0, n_rows) add nothing
+ *   grad_table  device [n_rows][n_features], 16-byte aligned: every row is written; with add != 0 the sums are added to it and
+ *               rows without a token are left as they are (a table that is also lbt_linear_log_loss_gradient's weight)
+ *   workspace   at least lbt_embed_rows_gradient_workspace_bytes(...), 16-byte aligned
+ */
+size_t lbt_embed_rows_gradient_workspace_bytes(int64_t n_tokens, int32_t n_features, int32_t n_rows, int32_t dtype);
+int lbt_embed_rows_gradient(void* stream, const void* grad, int32_t dtype, const void* tokens, int32_t token_bytes,
+                            int64_t n_tokens, int32_t n_features, int32_t n_rows, float scale, int32_t add, void* grad_table,
+                            void* workspace, size_t workspace_bytes);
 
 /* ---- profiling (no counterpart in the reference) -------------------------- */
 

@@ -1,0 +1,583 @@
+// Rows of a table by their numbers, times a scale, and the gradient with respect to the table.
+//
+//   out[t] = scale * table[token[t]]                   (zeros where token[t] is no row of the table)
+//   grad_table[v] = scale * sum_{t: token[t] = v} grad[t]
+//
+// The gradient sorts the places by their token, equal tokens by place, so that the sums have one order whatever the hardware
+// does first: no atomics touch a sum. The sorted places are then cut into chunks of equal length, whatever their tokens are: a
+// wave adds up the rows of a chunk for its share of the columns, in 32 bits. A run of equal tokens inside a chunk is finished
+// there; of one that crosses a chunk's end each chunk leaves its part, and join_runs_kernel adds the parts in order. A token
+// that takes a twentieth of all places is thus the work of many waves.
+// Bound by memory: grad is read once and the table's gradient written once.
+#include <algorithm>
+#include <type_traits>
+
+#include "lbt_internal.h"
+
+namespace lbt {
+
+namespace {
+
+template <int kDtype>
+__device__ __forceinline__ float widen(uint32_t bits)
+{
+  if constexpr (kDtype == LBT_F32) return __builtin_bit_cast(float, bits);
+  if constexpr (kDtype == LBT_F16) return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(bits)));
+  return __builtin_bit_cast(float, bits << 16);
+}
+
+template <int kDtype>
+__device__ __forceinline__ uint32_t narrow(float v)
+{
+  if constexpr (kDtype == LBT_F32) return __builtin_bit_cast(uint32_t, v);
+  if constexpr (kDtype == LBT_F16) return __builtin_bit_cast(uint16_t, static_cast<_Float16>(v));
+  return __builtin_bit_cast(uint16_t, static_cast<__bf16>(v));
+}
+
+// v * scale as a float, whatever follows: the compiler joins a product and its rounding to half precision into one instruction
+// where it can, which rounds once and not twice; the same value would then depend on how many of them a lane takes.
+__device__ __forceinline__ float scaled(float v, float scale)
+{
+  float p = v * scale;
+  asm("" : "+v"(p));
+  return p;
+}
+
+// kBytes consecutive bytes of a row: its values as floats and back.
+template <int kDtype, int kBytes>
+struct Pack {
+  static constexpr int kSize = kDtype == LBT_F32 ? 4 : 2, kValues = kBytes / kSize;
+  using Word = std::conditional_t<kBytes == 16, uint4, std::conditional_t<kBytes == 4, uint32_t, uint16_t>>;
+
+  static __device__ __forceinline__ void unpack(Word w, float (&v)[kValues])
+  {
+    if constexpr (kBytes == 16) {
+      const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int i = 0; i < kValues; i++)
+        v[i] = kSize == 4 ? widen<kDtype>(x[i % 4]) : widen<kDtype>((x[i / 2] >> (16 * (i & 1))) & 0xffffu);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kValues; i++) v[i] = kSize == 4 ? widen<kDtype>(w) : widen<kDtype>((uint32_t(w) >> (16 * i)) & 0xffffu);
+    }
+  }
+  static __device__ __forceinline__ Word pack(const float (&v)[kValues])
+  {
+    if constexpr (kBytes == 16) {
+      uint32_t x[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < kValues; i++) {
+        if constexpr (kSize == 4) x[i % 4] = narrow<kDtype>(v[i]);
+        else x[i / 2] |= narrow<kDtype>(v[i]) << (16 * (i & 1));
+      }
+      return make_uint4(x[0], x[1], x[2], x[3]);
+    } else {
+      uint32_t x = 0;
+#pragma unroll
+      for (int i = 0; i < kValues; i++) x |= narrow<kDtype>(v[i]) << (kSize == 4 ? 0 : 16 * i);
+      return static_cast<Word>(x);
+    }
+  }
+};
+
+// tokens as they come: 4 or 8 bytes each. What is no row of the table becomes n_rows.
+__device__ __forceinline__ int token_at(const void* tokens, int bytes, int64_t t, int n_rows)
+{
+  const int64_t v = bytes == 8 ? static_cast<const int64_t*>(tokens)[t] : static_cast<const int32_t*>(tokens)[t];
+  return v >= 0 && v < n_rows ? static_cast<int>(v) : n_rows;
+}
+
+constexpr int kRowThreads = 256;
+
+template <int kDtype, int kBytes>
+__global__ void __launch_bounds__(kRowThreads)
+  embed_rows_kernel(const void* __restrict__ table, int n_rows, int words, const void* __restrict__ tokens, int token_bytes,
+                    int64_t n_tokens, float scale, void* __restrict__ out)
+{
+  using P          = Pack<kDtype, kBytes>;
+  using Word       = typename P::Word;
+  const int64_t i  = blockIdx.x * int64_t(kRowThreads) + threadIdx.x;
+  if (i >= n_tokens * words) return;
+  const int64_t t = i / words;
+  const int at    = static_cast<int>(i % words);
+  const int v     = token_at(tokens, token_bytes, t, n_rows);
+  float x[P::kValues];
+  if (v < n_rows) {
+    P::unpack(static_cast<const Word*>(table)[static_cast<int64_t>(v) * words + at], x);
+#pragma unroll
+    for (int e = 0; e < P::kValues; e++) x[e] = scaled(x[e], scale);
+  } else {
+#pragma unroll
+    for (int e = 0; e < P::kValues; e++) x[e] = 0.f;
+  }
+  static_cast<Word*>(out)[i] = P::pack(x);
+}
+
+// ---- places sorted by token ----------------------------------------------------------------------
+
+struct Sorted {
+  int32_t* key;    // tokens, ascending; places that name no row come last, as n_rows
+  int32_t* place;  // where in `grad` each is; equal tokens in ascending order
+};
+
+constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64;
+
+// Few tokens: the place of each among the sorted ones is the number of those before it, counted. A workgroup counts for 64
+// tokens; its waves share out the others, 64 at a time.
+__global__ void __launch_bounds__(kSortThreads)
+  count_sort_kernel(const void* __restrict__ tokens, int token_bytes, int n_tokens, int n_rows, Sorted out)
+{
+  __shared__ int before[kSortWaves][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int own  = blockIdx.x * 64 + lane;
+  const int key  = own < n_tokens ? token_at(tokens, token_bytes, own, n_rows) : 0;
+  int count      = 0;
+  for (int b = wave; b * 64 < n_tokens; b += kSortWaves) {
+    const int j     = b * 64 + lane;
+    const int other = j < n_tokens ? token_at(tokens, token_bytes, j, n_rows) : 0x7fffffff;
+    const int bound = b < static_cast<int>(blockIdx.x) ? key + 1 : key;  // equal ones count where they come first
+    for (int l = 0; l < 64; l++) count += __builtin_amdgcn_readlane(other, l) < bound ? 1 : 0;
+    if (b == static_cast<int>(blockIdx.x))
+      for (int l = 0; l < 64; l++) count += __builtin_amdgcn_readlane(other, l) == key && l < lane ? 1 : 0;
+  }
+  before[wave][lane] = count;
+  __syncthreads();
+  if (wave != 0 || own >= n_tokens) return;
+  int rank = 0;
+  for (int w = 0; w < kSortWaves; w++) rank += before[w][lane];
+  out.key[rank]   = key;
+  out.place[rank] = own;
+}
+
+// Many tokens: by digits of up to 10 bits, least significant first; each pass counts, adds up and moves.
+constexpr int kDigits = 1024, kSortEach = 4, kSortBlock = kSortThreads * kSortEach;
+
+__device__ __forceinline__ int sort_key(const void* tokens, int token_bytes, const int32_t* keys, int64_t i, int n_rows)
+{
+  return keys != nullptr ? keys[i] : token_at(tokens, token_bytes, i, n_rows);
+}
+
+__global__ void __launch_bounds__(kSortThreads)
+  digit_count_kernel(const void* __restrict__ tokens, int token_bytes, const int32_t* __restrict__ keys, int64_t n, int n_rows,
+                     int shift, int digits, int blocks, int32_t* __restrict__ counts)
+{
+  __shared__ int count[kDigits];
+  count[threadIdx.x] = 0;
+  __syncthreads();
+  for (int e = 0; e < kSortEach; e++) {
+    const int64_t i = blockIdx.x * int64_t(kSortBlock) + e * kSortThreads + threadIdx.x;
+    if (i < n) atomicAdd(&count[(sort_key(tokens, token_bytes, keys, i, n_rows) >> shift) & (digits - 1)], 1);
+  }
+  __syncthreads();
+  if (static_cast<int>(threadIdx.x) < digits) counts[static_cast<int64_t>(threadIdx.x) * blocks + blockIdx.x] = count[threadIdx.x];
+}
+
+// counts [digits][blocks] become the number of entries before each: one workgroup, a thread per digit.
+__global__ void __launch_bounds__(kSortThreads) digit_offsets_kernel(int digits, int blocks, int32_t* __restrict__ counts)
+{
+  __shared__ int wave_sum[kSortWaves];
+  const int d = threadIdx.x, lane = d & 63, wave = d >> 6;
+  int sum = 0;
+  if (d < digits)
+    for (int b = 0; b < blocks; b++) sum += counts[static_cast<int64_t>(d) * blocks + b];
+  int upto = sum;
+  for (int s = 1; s < 64; s <<= 1) {
+    const int other = __shfl_up(upto, s);
+    if (lane >= s) upto += other;
+  }
+  if (lane == 63) wave_sum[wave] = upto;
+  __syncthreads();
+  int at = upto - sum;
+  for (int w = 0; w < wave; w++) at += wave_sum[w];
+  if (d < digits)
+    for (int b = 0; b < blocks; b++) {
+      const int64_t i = static_cast<int64_t>(d) * blocks + b;
+      const int c     = counts[i];
+      counts[i]       = at;
+      at += c;
+    }
+}
+
+// A wave takes 256 consecutive entries, 64 at a time: the lanes of equal digits find one another by ballots, the first of
+// them moves the wave's count on. Ranks are then the block's offset, the waves before, and the place in the wave: stable.
+__global__ void __launch_bounds__(kSortThreads)
+  digit_move_kernel(const void* __restrict__ tokens, int token_bytes, const int32_t* __restrict__ keys,
+                    const int32_t* __restrict__ places, int64_t n, int n_rows, int shift, int bits, int blocks,
+                    const int32_t* __restrict__ offsets, Sorted out)
+{
+  __shared__ uint16_t count[kSortWaves][kDigits];
+  __shared__ int first[kDigits];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int digits = 1 << bits;
+  for (int w = 0; w < kSortWaves; w++) count[w][threadIdx.x] = 0;
+  if (static_cast<int>(threadIdx.x) < digits) first[threadIdx.x] = offsets[static_cast<int64_t>(threadIdx.x) * blocks + blockIdx.x];
+  __syncthreads();
+  const int64_t begin = blockIdx.x * int64_t(kSortBlock) + wave * (64 * kSortEach);
+  int key[kSortEach], digit[kSortEach], rank[kSortEach];
+  for (int e = 0; e < kSortEach; e++) {
+    const int64_t i = begin + e * 64 + lane;
+    const bool in   = i < n;
+    key[e]          = in ? sort_key(tokens, token_bytes, keys, i, n_rows) : 0;
+    digit[e]        = (key[e] >> shift) & (digits - 1);
+    uint64_t same   = __ballot(in);
+    for (int b = 0; b < bits; b++) {
+      const uint64_t set = __ballot((digit[e] >> b) & 1);
+      same &= (digit[e] >> b) & 1 ? set : ~set;
+    }
+    const int ahead = __popcll(same & ((uint64_t(1) << lane) - 1));
+    const int so_far = in ? count[wave][digit[e]] : 0;
+    rank[e]         = so_far + ahead;
+    __builtin_amdgcn_wave_barrier();
+    if (in && ahead == 0) count[wave][digit[e]] = static_cast<uint16_t>(so_far + __popcll(same));
+    __builtin_amdgcn_wave_barrier();
+  }
+  __syncthreads();
+  if (static_cast<int>(threadIdx.x) < digits) {
+    int sum = 0;
+    for (int w = 0; w < kSortWaves; w++) {
+      const int c               = count[w][threadIdx.x];
+      count[w][threadIdx.x]     = static_cast<uint16_t>(sum);
+      sum += c;
+    }
+  }
+  __syncthreads();
+  for (int e = 0; e < kSortEach; e++) {
+    const int64_t i = begin + e * 64 + lane;
+    if (i >= n) continue;
+    const int64_t to = static_cast<int64_t>(first[digit[e]]) + count[wave][digit[e]] + rank[e];
+    out.key[to]      = key[e];
+    out.place[to]    = places != nullptr ? places[i] : static_cast<int32_t>(i);
+  }
+}
+
+// ---- sums of runs -----------------------------------------------------------------------------------
+
+struct RunArgs {
+  const void* grad;
+  Sorted sorted;
+  int n_tokens, n_rows;
+  int words;   // of a row
+  int chunk;   // sorted places of a wave, at most 64
+  int slices;  // of 64 words
+  float scale;
+  void* out;
+  int add;     // to what `out` holds
+  float* part; // [chunks][2][words * values]: of the run that began before the chunk, of the run that goes on after it
+};
+
+template <int kDtype, int kBytes>
+__device__ __forceinline__ void write_row(const RunArgs& a, int row, int at, const float (&sum)[Pack<kDtype, kBytes>::kValues])
+{
+  using P    = Pack<kDtype, kBytes>;
+  using Word = typename P::Word;
+  Word* to   = static_cast<Word*>(a.out) + static_cast<int64_t>(row) * a.words + at;
+  float x[P::kValues];
+  if (a.add) {
+    P::unpack(*to, x);
+#pragma unroll
+    for (int e = 0; e < P::kValues; e++) x[e] += scaled(sum[e], a.scale);
+  } else {
+#pragma unroll
+    for (int e = 0; e < P::kValues; e++) x[e] = scaled(sum[e], a.scale);
+  }
+  *to = P::pack(x);
+}
+
+template <int kDtype, int kBytes>
+__global__ void __launch_bounds__(kRowThreads) sum_runs_kernel(const RunArgs a)
+{
+  using P    = Pack<kDtype, kBytes>;
+  using Word = typename P::Word;
+  const int lane      = threadIdx.x & 63;
+  const int64_t task  = static_cast<int64_t>(blockIdx.x) * (kRowThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t chunk = task / a.slices;
+  const int at        = static_cast<int>(task % a.slices) * 64 + lane;
+  const int64_t p0    = chunk * a.chunk;
+  if (p0 >= a.n_tokens) return;
+  const int count = static_cast<int>(min(static_cast<int64_t>(a.chunk), a.n_tokens - p0));
+  // lane l has the token and place of entry l; a run ends where the next entry has another token
+  const int key    = lane < count ? a.sorted.key[p0 + lane] : a.n_rows;
+  const int place  = lane < count ? a.sorted.place[p0 + lane] : 0;
+  const int before = p0 > 0 ? a.sorted.key[p0 - 1] : -1;
+  const int after  = p0 + count < a.n_tokens ? a.sorted.key[p0 + count] : -1;
+  const int below  = __shfl_down(key, 1);  // (by all lanes: what a lane reads from has to take part)
+  const int next   = lane + 1 < count ? below : after;
+  const uint64_t ends = __ballot(lane < count && key != next);
+  const bool inside   = at < a.words;
+  float sum[P::kValues];
+#pragma unroll
+  for (int e = 0; e < P::kValues; e++) sum[e] = 0.f;
+  constexpr int kAhead = 8;  // rows asked for together
+  int begin = 0;             // of the run
+  for (int i = 0; i < count; i += kAhead) {
+    Word w[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; j++) {
+      const int from = __builtin_amdgcn_readlane(place, min(i + j, count - 1));
+      if (inside) w[j] = static_cast<const Word*>(a.grad)[static_cast<int64_t>(from) * a.words + at];
+    }
+#pragma unroll
+    for (int j = 0; j < kAhead; j++) {
+      if (i + j >= count) break;
+      float x[P::kValues];
+      P::unpack(w[j], x);
+#pragma unroll
+      for (int e = 0; e < P::kValues; e++) sum[e] += x[e];
+      const bool end = (ends >> (i + j)) & 1;
+      if (!end && i + j + 1 < count) continue;
+      const int row    = __builtin_amdgcn_readlane(key, i + j);
+      const bool early = begin == 0 && before == row;  // began in an earlier chunk
+      if (row < a.n_rows && inside) {
+        if (end && !early) {
+          write_row<kDtype, kBytes>(a, row, at, sum);
+        } else {
+          float* to = a.part + ((chunk * 2 + (early ? 0 : 1)) * a.words + at) * P::kValues;
+#pragma unroll
+          for (int e = 0; e < P::kValues; e++) to[e] = sum[e];
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < P::kValues; e++) sum[e] = 0.f;
+      begin = i + j + 1;
+    }
+  }
+}
+
+// Runs that cross the end of a chunk: the wave of the chunk in which one begins adds up its parts.
+template <int kDtype, int kBytes>
+__global__ void __launch_bounds__(kRowThreads) join_runs_kernel(const RunArgs a)
+{
+  using P = Pack<kDtype, kBytes>;
+  const int64_t task  = static_cast<int64_t>(blockIdx.x) * (kRowThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t chunk = task / a.slices;
+  const int at        = static_cast<int>(task % a.slices) * 64 + (threadIdx.x & 63);
+  const int64_t p0    = chunk * a.chunk, p1 = p0 + a.chunk;
+  if (p1 >= a.n_tokens) return;
+  const int row = a.sorted.key[p1 - 1];
+  if (row >= a.n_rows || a.sorted.key[p1] != row) return;
+  if (p0 > 0 && a.sorted.key[p0 - 1] == row) return;  // it began earlier
+  if (at >= a.words) return;
+  const int64_t stride = static_cast<int64_t>(a.words) * P::kValues;
+  const float* from    = a.part + (chunk * 2 + 1) * stride + static_cast<int64_t>(at) * P::kValues;
+  float sum[P::kValues];
+#pragma unroll
+  for (int e = 0; e < P::kValues; e++) sum[e] = from[e];
+  from += stride;  // the part at the head of the next chunk
+  for (int64_t p = p1; p < a.n_tokens && a.sorted.key[p] == row; p += a.chunk, from += 2 * stride) {
+#pragma unroll
+    for (int e = 0; e < P::kValues; e++) sum[e] += from[e];
+  }
+  write_row<kDtype, kBytes>(a, row, at, sum);
+}
+
+// Zeros for the rows that no token names: a workgroup looks up 64 rows in the sorted tokens and clears those that are absent.
+constexpr int kClearRows = 64;
+template <int kBytes>
+__global__ void __launch_bounds__(kRowThreads)
+  clear_rows_kernel(const int32_t* __restrict__ keys, int n_tokens, int n_rows, int words, void* __restrict__ out)
+{
+  using Word = typename Pack<LBT_BF16, kBytes>::Word;
+  const int64_t first = blockIdx.x * int64_t(kClearRows);
+  const int64_t row   = first + (threadIdx.x & 63);
+  int lo = 0, hi = n_tokens;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (keys[mid] < row) lo = mid + 1;
+    else hi = mid;
+  }
+  const uint64_t absent = __ballot(row < n_rows && !(lo < n_tokens && keys[lo] == row));
+  Word* to = static_cast<Word*>(out) + first * words;
+  const int64_t total = static_cast<int64_t>(kClearRows) * words;
+  for (int64_t i = threadIdx.x; i < total; i += kRowThreads)
+    if ((absent >> (i / words)) & 1) to[i] = Word{};
+}
+
+// ---- host -------------------------------------------------------------------------------------------
+
+constexpr int kCountSortTokens = 8192;  // at most this many are sorted by counting
+
+int value_bytes(int dtype) { return dtype == LBT_F32 ? 4 : 2; }
+
+// Bytes of a row that a lane takes: 16 or 4 where rows are whole numbers of them, else one value.
+int lane_bytes(int n_features, int dtype)
+{
+  const int64_t row = static_cast<int64_t>(n_features) * value_bytes(dtype);
+  return row % 16 == 0 ? 16 : row % 4 == 0 ? 4 : 2;
+}
+
+struct EmbedCall {
+  int64_t n_tokens;
+  int n_features, n_rows, dtype;
+  int bytes, words, slices, chunk, bits, passes;
+  int64_t chunks, blocks;
+  Sorted sorted[2];
+  int32_t* counts;
+  float* part;
+
+  EmbedCall(int64_t t, int f, int rows, int type) : n_tokens(t), n_features(f), n_rows(rows), dtype(type)
+  {
+    bytes  = lane_bytes(f, type);
+    words  = static_cast<int>(static_cast<int64_t>(f) * value_bytes(type) / bytes);
+    slices = (words + 63) / 64;
+    // chunks as long as they may be while there are some thousands of waves
+    chunk = 64;
+    while (chunk > 8 && (t / chunk) * slices < 4096) chunk /= 2;
+    chunks = (t + chunk - 1) / chunk;
+    blocks = (t + kSortBlock - 1) / kSortBlock;
+    bits   = 1;
+    while ((int64_t(1) << bits) <= rows) bits++;  // keys go up to n_rows
+    passes = (bits + 9) / 10;
+  }
+
+  void carve(Arena& arena)
+  {
+    for (int i = 0; i < 2; i++) {
+      sorted[i].key   = arena.take<int32_t>(n_tokens);
+      sorted[i].place = arena.take<int32_t>(n_tokens);
+    }
+    counts = arena.take<int32_t>(static_cast<size_t>(kDigits) * blocks);
+    part   = arena.take<float>(static_cast<size_t>(chunks) * 2 * n_features);
+  }
+};
+
+template <int kDtype, int kBytes>
+int embed_gradient(hipStream_t s, const EmbedCall& c, const void* grad, const void* tokens, int token_bytes, float scale, bool add,
+                   void* out)
+{
+  int at = 0;
+  if (c.n_tokens <= kCountSortTokens) {
+    if (c.n_tokens > 0)
+      count_sort_kernel<<<static_cast<unsigned>((c.n_tokens + 63) / 64), kSortThreads, 0, s>>>(
+        tokens, token_bytes, static_cast<int>(c.n_tokens), c.n_rows, c.sorted[0]);
+  } else {
+    const int each = (c.bits + c.passes - 1) / c.passes;
+    for (int p = 0; p < c.passes; p++) {
+      const int shift     = p * each, bits = std::min(each, c.bits - shift);
+      const int32_t* keys = p == 0 ? nullptr : c.sorted[at].key;
+      const int32_t* from = p == 0 ? nullptr : c.sorted[at].place;
+      const Sorted to     = c.sorted[1 - at];
+      const unsigned grid = static_cast<unsigned>(c.blocks);
+      digit_count_kernel<<<grid, kSortThreads, 0, s>>>(tokens, token_bytes, keys, c.n_tokens, c.n_rows, shift, 1 << bits,
+                                                       static_cast<int>(c.blocks), c.counts);
+      digit_offsets_kernel<<<1, kSortThreads, 0, s>>>(1 << bits, static_cast<int>(c.blocks), c.counts);
+      digit_move_kernel<<<grid, kSortThreads, 0, s>>>(tokens, token_bytes, keys, from, c.n_tokens, c.n_rows, shift, bits,
+                                                      static_cast<int>(c.blocks), c.counts, to);
+      at = 1 - at;
+    }
+  }
+  LBT_HIP(hipGetLastError());
+  if (!add) {
+    const int64_t groups = (static_cast<int64_t>(c.n_rows) + kClearRows - 1) / kClearRows;
+    clear_rows_kernel<kBytes><<<static_cast<unsigned>(groups), kRowThreads, 0, s>>>(c.sorted[at].key, static_cast<int>(c.n_tokens),
+                                                                                   c.n_rows, c.words, out);
+    LBT_HIP(hipGetLastError());
+  }
+  if (c.n_tokens == 0) return LBT_OK;
+  const RunArgs a{grad,     c.sorted[at], static_cast<int>(c.n_tokens), c.n_rows, c.words, c.chunk, c.slices, scale, out, add ? 1 : 0,
+                  c.part};
+  const int64_t grid = (c.chunks * c.slices + kRowThreads / 64 - 1) / (kRowThreads / 64);
+  LBT_REQUIRE(grid < (int64_t(1) << 31), "too many elements");
+  sum_runs_kernel<kDtype, kBytes><<<static_cast<unsigned>(grid), kRowThreads, 0, s>>>(a);
+  LBT_HIP(hipGetLastError());
+  if (c.chunks > 1) {
+    join_runs_kernel<kDtype, kBytes><<<static_cast<unsigned>(grid), kRowThreads, 0, s>>>(a);
+    LBT_HIP(hipGetLastError());
+  }
+  return LBT_OK;
+}
+
+bool embed_shape(int64_t n_tokens, int32_t n_features, int32_t n_rows, int32_t dtype)
+{
+  return (dtype == LBT_F32 || dtype == LBT_BF16 || dtype == LBT_F16) && n_tokens >= 0 && n_tokens <= (1 << 30) &&
+         n_features >= 1 && n_features <= (1 << 24) && n_rows >= 1 && n_rows <= (1 << 30) &&
+         n_tokens * n_features < (int64_t(1) << 38) && int64_t(n_rows) * n_features < (int64_t(1) << 38);
+}
+
+// Calls `f` with the type and the bytes of a lane as constants.
+template <class F>
+int for_type(int dtype, int bytes, const F& f)
+{
+  using std::integral_constant;
+  if (dtype == LBT_F32)
+    return bytes == 16 ? f(integral_constant<int, LBT_F32>{}, integral_constant<int, 16>{})
+                       : f(integral_constant<int, LBT_F32>{}, integral_constant<int, 4>{});
+  if (dtype == LBT_BF16)
+    return bytes == 16  ? f(integral_constant<int, LBT_BF16>{}, integral_constant<int, 16>{})
+           : bytes == 4 ? f(integral_constant<int, LBT_BF16>{}, integral_constant<int, 4>{})
+                        : f(integral_constant<int, LBT_BF16>{}, integral_constant<int, 2>{});
+  return bytes == 16  ? f(integral_constant<int, LBT_F16>{}, integral_constant<int, 16>{})
+         : bytes == 4 ? f(integral_constant<int, LBT_F16>{}, integral_constant<int, 4>{})
+                      : f(integral_constant<int, LBT_F16>{}, integral_constant<int, 2>{});
+}
+
+}  // namespace
+}  // namespace lbt
+
+extern "C" {
+
+int lbt_embed_rows(void* stream, const void* table, int32_t dtype, int32_t n_rows, int32_t n_features, const void* tokens,
+                   int32_t token_bytes, int64_t n_tokens, float scale, void* out)
+{
+  LBT_REQUIRE(dtype == LBT_F32 || dtype == LBT_BF16 || dtype == LBT_F16, "unsupported dtype %d", dtype);
+  LBT_REQUIRE(lbt::embed_shape(n_tokens, n_features, n_rows, dtype), "bad shape");
+  LBT_REQUIRE(token_bytes == 4 || token_bytes == 8, "tokens of 4 or 8 bytes, not %d", token_bytes);
+  if (n_tokens == 0) return LBT_OK;
+  LBT_REQUIRE(table && tokens && out, "null pointer");
+  LBT_REQUIRE(((reinterpret_cast<uintptr_t>(table) | reinterpret_cast<uintptr_t>(out)) & 15) == 0,
+              "table and out must be 16-byte aligned");
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const lbt::EmbedCall c(n_tokens, n_features, n_rows, dtype);
+  lbt::ProfScope ps(LBT_PROF_OTHER, s);
+  return lbt::for_type(dtype, c.bytes, [&](auto type, auto bytes) -> int {
+    const int64_t blocks = (n_tokens * c.words + lbt::kRowThreads - 1) / lbt::kRowThreads;
+    LBT_REQUIRE(blocks < (int64_t(1) << 31), "too many elements");
+    lbt::embed_rows_kernel<decltype(type)::value, decltype(bytes)::value>
+      <<<static_cast<unsigned>(blocks), lbt::kRowThreads, 0, s>>>(table, n_rows, c.words, tokens, token_bytes, n_tokens, scale, out);
+    LBT_HIP(hipGetLastError());
+    return LBT_OK;
+  });
+}
+
+size_t lbt_embed_rows_gradient_workspace_bytes(int64_t n_tokens, int32_t n_features, int32_t n_rows, int32_t dtype)
+{
+  if (!lbt::embed_shape(n_tokens, n_features, n_rows, dtype)) return 0;
+  lbt::EmbedCall c(n_tokens, n_features, n_rows, dtype);
+  lbt::Arena arena;
+  arena.measure = true;
+  c.carve(arena);
+  return std::max<size_t>(arena.used, 256);
+}
+
+int lbt_embed_rows_gradient(void* stream, const void* grad, int32_t dtype, const void* tokens, int32_t token_bytes,
+                            int64_t n_tokens, int32_t n_features, int32_t n_rows, float scale, int32_t add, void* grad_table,
+                            void* workspace, size_t workspace_bytes)
+{
+  LBT_REQUIRE(dtype == LBT_F32 || dtype == LBT_BF16 || dtype == LBT_F16, "unsupported dtype %d", dtype);
+  LBT_REQUIRE(lbt::embed_shape(n_tokens, n_features, n_rows, dtype), "bad shape");
+  LBT_REQUIRE(token_bytes == 4 || token_bytes == 8, "tokens of 4 or 8 bytes, not %d", token_bytes);
+  if (n_tokens == 0 && add) return LBT_OK;
+  LBT_REQUIRE(grad_table && (n_tokens == 0 || (grad && tokens)), "null pointer");
+  LBT_REQUIRE(((reinterpret_cast<uintptr_t>(grad) | reinterpret_cast<uintptr_t>(grad_table)) & 15) == 0,
+              "grad and grad_table must be 16-byte aligned");
+  if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0) {
+    lbt::set_error("a workspace aligned to 16 bytes is needed");
+    return LBT_ERR_WORKSPACE;
+  }
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  lbt::EmbedCall c(n_tokens, n_features, n_rows, dtype);
+  lbt::Arena arena;
+  arena.base = static_cast<char*>(workspace);
+  arena.cap  = workspace_bytes;
+  c.carve(arena);
+  if (arena.failed) {
+    lbt::set_error("workspace of %zu bytes, %zu needed", workspace_bytes, arena.used);
+    return LBT_ERR_WORKSPACE;
+  }
+  lbt::ProfScope ps(LBT_PROF_OTHER, s);
+  return lbt::for_type(dtype, c.bytes, [&](auto type, auto bytes) {
+    return lbt::embed_gradient<decltype(type)::value, decltype(bytes)::value>(s, c, grad, tokens, token_bytes, scale, add != 0,
+                                                                              grad_table);
+  });
+}
+
+}  // extern "C"

@@ -1,0 +1,850 @@
+// Log loss of linear scores over many classes, and its gradient, without the scores in memory.
+//
+//   s[r][c] = <X[r], weight[c]> + bias[c]      top[r] = max_c s, total[r] = sum_c exp(s - top)
+//   loss[r] = log total[r] + top[r] - s[r][y[r]]
+//   G[r][c] = w[r] (exp(s - top) / total - [c = y[r]])
+//   grad_X = G weight,  grad_weight = G^T X,  grad_bias[c] = sum_r G[r][c]
+//
+// Rows whose label is no class are taken out first (prepare_rows_kernel, pack_rows_kernel): what follows has only rows that
+// count, side by side and padded with zeros, so a row that does not count costs nothing and what it holds reaches nothing.
+// The scores are formed tile by tile (lbt_products.h) and stay in registers: a first walk over the classes leaves the top and
+// the total of each tile's share of a row, which join_kernel joins. For the gradient the scores of a piece of the classes
+// are formed a second time, and G of the piece is written in the type of the products and multiplied both ways.
+//
+// Half precision: G is held times 2^14 and with the weight's exponent taken out of its row (w = f 2^e, 1 <= |f| < 2), so that
+// probabilities down to 2^-28 keep all their bits; grad_X gets 2^(e - 14) at its end, grad_weight multiplies rows of X times
+// 2^(e - m), m such that the largest value comes to lie just below 2^15 and those of rows with small weights, 2^-29 of it, keep
+// theirs. bfloat16 and float hold G as it is: their exponents reach far enough.
+#include <algorithm>
+
+#include "lbt_products.h"
+
+namespace lbt {
+
+namespace {
+
+constexpr int kHalfShift = 14;
+constexpr int64_t kPieceBytes = int64_t(512) << 20;  // of G, or of packed weights, at a time
+
+template <int kDtype>
+struct LossType;
+template <>
+struct LossType<LBT_BF16> {
+  using Value = uint16_t;
+  static constexpr int kProduct = LBT_BF16, kPlanes = 1;
+};
+template <>
+struct LossType<LBT_F16> {
+  using Value = uint16_t;
+  static constexpr int kProduct = LBT_F16, kPlanes = 1;
+};
+template <>
+struct LossType<LBT_F32> {
+  using Value = float;
+  static constexpr int kProduct = LBT_BF16, kPlanes = 3;
+};
+
+__device__ __forceinline__ uint16_t to_bf16(float v) { return __builtin_bit_cast(uint16_t, static_cast<__bf16>(v)); }
+__device__ __forceinline__ float from_bf16(uint16_t v) { return __builtin_bit_cast(float, static_cast<uint32_t>(v) << 16); }
+
+// One rounding to the type of an operand's plane.
+template <int kProduct>
+__device__ __forceinline__ uint16_t narrow_value(float v)
+{
+  if constexpr (kProduct == LBT_F16) return __builtin_bit_cast(uint16_t, static_cast<_Float16>(v));
+  return to_bf16(v);
+}
+
+// A float as the sum of three bfloat16: what is left after each goes on exactly. A value that rounds up to infinity keeps
+// the largest number instead; infinities and NaN are their own first plane and the others are 0.
+__device__ __forceinline__ void split_planes(float v, uint16_t (&out)[3])
+{
+  uint16_t hi = to_bf16(v);
+  if ((hi & 0x7fff) == 0x7f80 && fabsf(v) < INFINITY) hi = static_cast<uint16_t>(__builtin_bit_cast(uint32_t, v) >> 16);
+  out[0]        = hi;
+  const bool in = fabsf(v) < INFINITY;
+  const float r = in ? v - from_bf16(hi) : 0.f;
+  out[1]        = to_bf16(r);
+  out[2]        = to_bf16(r - from_bf16(out[1]));
+}
+
+template <int kDtype>
+__device__ __forceinline__ float load_value(const void* p, int64_t i)
+{
+  if constexpr (kDtype == LBT_F32) return static_cast<const float*>(p)[i];
+  const uint16_t v = static_cast<const uint16_t*>(p)[i];
+  if constexpr (kDtype == LBT_F16) return static_cast<float>(__builtin_bit_cast(_Float16, v));
+  return from_bf16(v);
+}
+
+template <int kDtype>
+__device__ __forceinline__ void store_value(void* p, int64_t i, float v)
+{
+  if constexpr (kDtype == LBT_F32)
+    static_cast<float*>(p)[i] = v;
+  else
+    static_cast<uint16_t*>(p)[i] = narrow_value<kDtype>(v);
+}
+
+// Four consecutive values of an output row of which `n` are inside.
+template <int kDtype>
+__device__ __forceinline__ void store_four(void* p, int64_t i, const float (&v)[4], int n, bool aligned)
+{
+  if (n >= 4 && aligned) {
+    if constexpr (kDtype == LBT_F32) {
+      *reinterpret_cast<float4*>(static_cast<float*>(p) + i) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+      const uint32_t a = narrow_value<kDtype>(v[0]) | static_cast<uint32_t>(narrow_value<kDtype>(v[1])) << 16;
+      const uint32_t b = narrow_value<kDtype>(v[2]) | static_cast<uint32_t>(narrow_value<kDtype>(v[3])) << 16;
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p) + i) = make_uint2(a, b);
+    }
+    return;
+  }
+  for (int e = 0; e < 4; e++)
+    if (e < n) store_value<kDtype>(p, i + e, v[e]);
+}
+
+// What is kept of each row that counts, in the order of the rows.
+struct LossRows {
+  int32_t* order;   // its number in the call
+  int32_t* place;   // [n_rows of the call] where it went, or -1
+  int32_t* label;
+  float* factor;    // its weight, or (half precision) the weight's significand times 2^14
+  int32_t* exponent;  // half precision: the weight's exponent
+  float* picked;    // score of its label
+  float* top;
+  float* inverse;   // 1 / total
+};
+
+constexpr int kPrepareThreads = 1024;
+
+// One workgroup goes through the labels: the rows that count, in order. Their weights' largest exponent is found on the way.
+// 8192 rows take 3 us and the work grows with the rows only; it runs beside nothing, as all that follows needs it.
+__global__ void __launch_bounds__(kPrepareThreads)
+  prepare_rows_kernel(const int64_t* __restrict__ y, const float* __restrict__ weight, int64_t n_rows, int64_t padded,
+                      int n_classes, int half, LossRows out, float* __restrict__ loss, RowCounts* counts, uint16_t* zeros)
+{
+  __shared__ int wave_sum[kPrepareThreads / 64];
+  __shared__ int largest;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (threadIdx.x < 8) zeros[threadIdx.x] = 0;
+  if (threadIdx.x == 0) largest = -1000;
+  int at = 0;  // rows that count so far
+  for (int64_t first = 0; first < n_rows; first += kPrepareThreads) {
+    const int64_t r     = first + threadIdx.x;
+    const int64_t label = r < n_rows ? y[r] : -1;
+    const bool in       = label >= 0 && label < n_classes;
+    const uint64_t set  = __ballot(in);
+    __syncthreads();
+    if (lane == 0) wave_sum[wave] = __popcll(set);
+    __syncthreads();
+    int before = at, all = 0;
+    for (int w = 0; w < kPrepareThreads / 64; w++) {
+      const int s = wave_sum[w];
+      before += w < wave ? s : 0;
+      all += s;
+    }
+    at += all;
+    if (in) {
+      const int p  = before + __popcll(set & ((uint64_t(1) << lane) - 1));
+      float w      = weight != nullptr ? weight[r] : 1.f;
+      int exponent = 0;
+      if (half) {
+        if (w != 0.f && fabsf(w) < INFINITY) {
+          w = 2.f * frexpf(w, &exponent);  // 1 <= |w| < 2
+          exponent -= 1;
+          atomicMax(&largest, exponent);
+        } else {
+          exponent = -1000;  // adds nothing to grad_weight where the weight is 0
+          if (w != 0.f) { exponent = 0; atomicMax(&largest, 0); }
+        }
+        w *= 1 << kHalfShift;
+      }
+      out.order[p]    = static_cast<int32_t>(r);
+      out.place[r]    = p;
+      out.label[p]    = static_cast<int32_t>(label);
+      out.factor[p]   = w;
+      out.exponent[p] = exponent;
+      out.picked[p]   = -INFINITY;
+    } else if (r < n_rows) {
+      out.place[r] = -1;
+      loss[r]      = 0.f;
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    counts->rows     = at;
+    counts->exponent = largest > -1000 ? largest : 0;
+    counts->reach    = -1000;
+  }
+  for (int64_t p = at + threadIdx.x; p < padded; p += kPrepareThreads) {
+    out.order[p]    = -1;
+    out.label[p]    = -1;
+    out.factor[p]   = 0.f;
+    out.exponent[p] = -1000;
+    out.picked[p]   = 0.f;
+  }
+}
+
+// Rows of an array as rows of an operand: in `order` where that is given, -1 and what lies past the end as zeros, columns
+// padded with zeros to `padded_cols`, floats as three planes. A thread takes 8 columns. Bound by the copy: it reads and writes
+// each value once. Half precision with weights: kMeasure finds counts->reach, kScale multiplies row p by 2^(exponent[p] + 14 - reach).
+enum { kCopy = 0, kMeasure = 1, kScale = 2 };
+constexpr int kReach = 14;
+template <int kDtype>
+__global__ void __launch_bounds__(256)
+  pack_rows_kernel(const void* __restrict__ from, int64_t first_row, int64_t rows, int cols, const int32_t* __restrict__ order,
+                   int mode, const int32_t* __restrict__ exponent, RowCounts* counts, int64_t out_rows, int padded_cols,
+                   int64_t plane, uint16_t* __restrict__ out)
+{
+  using L          = LossType<kDtype>;
+  const int groups = padded_cols / 8;
+  const int64_t i  = blockIdx.x * int64_t(256) + threadIdx.x;
+  if (i >= out_rows * groups) return;
+  const int64_t p = i / groups;
+  const int col   = static_cast<int>(i % groups) * 8;
+  const int64_t r = order != nullptr ? order[p] : (first_row + p < rows ? first_row + p : -1);
+  uint16_t v[L::kPlanes][8];
+  const bool whole = r >= 0 && col + 8 <= cols && cols % 8 == 0 && (reinterpret_cast<uintptr_t>(from) & 15) == 0;
+  float f[8];
+  if (whole) {
+    if constexpr (kDtype == LBT_F32) {
+      const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(from) + r * cols + col);
+      const float4 a = q[0], b = q[1];
+      f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+    } else {
+      *reinterpret_cast<uint4*>(v[0]) = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(from) + r * cols + col);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      const bool in = r >= 0 && col + e < cols;
+      if constexpr (kDtype == LBT_F32)
+        f[e] = in ? static_cast<const float*>(from)[r * cols + col + e] : 0.f;
+      else
+        v[0][e] = in ? static_cast<const uint16_t*>(from)[r * cols + col + e] : uint16_t(0);
+    }
+  }
+  if constexpr (kDtype == LBT_F32) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      uint16_t s[3];
+      split_planes(f[e], s);
+      v[0][e] = s[0];
+      v[1][e] = s[1];
+      v[2][e] = s[2];
+    }
+  }
+  if constexpr (kDtype == LBT_F16) {
+    if (mode == kMeasure) {
+      int reach = -1000;
+      if (r >= 0 && exponent[p] > -1000)
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const float x = load_value<kDtype>(v[0], e);
+          int own       = 16;  // (infinities and NaN)
+          if (fabsf(x) < INFINITY) (void)frexpf(x, &own);
+          if (x != 0.f) reach = max(reach, own - 1 + exponent[p]);
+        }
+      // (rows of one wave: the lanes that are still here)
+      for (int s = 32; s > 0; s >>= 1) reach = max(reach, __shfl_xor(reach, s));
+      if ((threadIdx.x & 63) == 0 && reach > -1000) atomicMax(&counts->reach, reach);
+    } else if (mode == kScale) {
+      const int shift = exponent[p] + kReach - counts->reach;
+#pragma unroll
+      for (int e = 0; e < 8; e++)
+        v[0][e] = exponent[p] <= -1000 ? uint16_t(0) : narrow_value<L::kProduct>(ldexpf(load_value<kDtype>(v[0], e), shift));
+    }
+  }
+#pragma unroll
+  for (int q = 0; q < L::kPlanes; q++)
+    *reinterpret_cast<uint4*>(out + q * plane + p * padded_cols + col) = *reinterpret_cast<const uint4*>(v[q]);
+}
+
+// ---- what the products end in -------------------------------------------------------------------
+
+__device__ __forceinline__ float exp_of(float d, bool exact) { return exact ? expf(d) : __expf(d); }
+
+// scores: m = classes, n = rows. Adds the bias; classes past the end count as masked.
+template <class Tile>
+__device__ __forceinline__ void add_bias(Float16v (&acc)[Tile::kMT][Tile::kNT], const float* bias, int class_first, int n_classes,
+                                         int lane)
+{
+#pragma unroll
+  for (int i = 0; i < Tile::kMT; i++)
+#pragma unroll
+    for (int e = 0; e < 16; e++) {
+      const int c   = class_first + i * 32 + block_m(e, lane);
+      const float b = bias != nullptr && c < n_classes ? bias[c] : 0.f;
+#pragma unroll
+      for (int j = 0; j < Tile::kNT; j++) acc[i][j][e] = c < n_classes ? acc[i][j][e] + b : -INFINITY;
+    }
+}
+
+// Each tile's share of the rows' tops and totals.
+template <bool kExact>
+struct LossEpilogue {
+  const float* bias;
+  int class_first, n_classes;  // of this launch: number of its first class; classes of the call
+  int tile_first;
+  int64_t padded;              // rows
+  LossRows rows;
+  float2* partial;             // [tiles][padded]: top, total
+
+  template <class Tile>
+  __device__ __forceinline__ void store(Float16v (&acc)[Tile::kMT][Tile::kNT], int tile_m, int tile_n, int wm, int wn, int lane,
+                                        int, const RowCounts*, char* lds) const
+  {
+    const int c0 = class_first + tile_m * Tile::kBM + wm * Tile::kWM;
+    add_bias<Tile>(acc, bias, c0, n_classes, lane);
+    float2(*share)[Tile::kBN] = reinterpret_cast<float2(*)[Tile::kBN]>(lds);
+#pragma unroll
+    for (int j = 0; j < Tile::kNT; j++) {
+      const int n         = wn * Tile::kWN + j * 32 + (lane & 31);
+      const int64_t row   = static_cast<int64_t>(tile_n) * Tile::kBN + n;
+      const int label     = rows.label[row] - c0;
+      float top           = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < Tile::kMT; i++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+          top = fmaxf(top, acc[i][j][e]);
+          if (i * 32 + block_m(e, lane) == label) rows.picked[row] = acc[i][j][e];
+        }
+      top              = fmaxf(top, __shfl_xor(top, 32));
+      const float from = top == -INFINITY ? 0.f : top;
+      float total      = 0.f;
+#pragma unroll
+      for (int i = 0; i < Tile::kMT; i++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) total += exp_of(acc[i][j][e] - from, kExact);
+      total += __shfl_xor(total, 32);
+      if (lane < 32) share[wm][n] = make_float2(top, total);
+    }
+    __syncthreads();
+    for (int n = threadIdx.x; n < Tile::kBN; n += Tile::kThreads) {
+      float top = share[0][n].x;
+      for (int w = 1; w < Tile::kWavesM; w++) top = fmaxf(top, share[w][n].x);
+      const float from = top == -INFINITY ? 0.f : top;
+      float total      = 0.f;
+      for (int w = 0; w < Tile::kWavesM; w++) total += share[w][n].y * exp_of(share[w][n].x - from, kExact);
+      partial[static_cast<int64_t>(tile_first + tile_m) * padded + static_cast<int64_t>(tile_n) * Tile::kBN + n] =
+        make_float2(top, total);
+    }
+  }
+};
+
+// G of a piece of the classes, [plane][rows][piece] in the products' type, and its sums over the tile's rows.
+template <bool kExact, int kProduct, int kPlanes>
+struct GradientEpilogue {
+  const float* bias;
+  int class_first, n_classes, piece;  // classes of a row of G
+  LossRows rows;
+  uint16_t* g;
+  int64_t plane;
+  float* bias_sums;  // [tiles of rows][classes], or null
+
+  template <class Tile>
+  __device__ __forceinline__ void store(Float16v (&acc)[Tile::kMT][Tile::kNT], int tile_m, int tile_n, int wm, int wn, int lane,
+                                        int counted, const RowCounts* counts, char* lds) const
+  {
+    const int in_piece = tile_m * Tile::kBM + wm * Tile::kWM;
+    const int c0       = class_first + in_piece;
+    add_bias<Tile>(acc, bias, c0, n_classes, lane);
+    float scale[Tile::kNT];  // of the sums over rows: half precision has the weights' exponents apart
+#pragma unroll
+    for (int j = 0; j < Tile::kNT; j++) {
+      const int64_t row   = static_cast<int64_t>(tile_n) * Tile::kBN + wn * Tile::kWN + j * 32 + (lane & 31);
+      const bool in       = row < counted;
+      const int label     = in ? rows.label[row] - c0 : -1;
+      const float top     = in ? rows.top[row] : 0.f;
+      const float inverse = in ? rows.inverse[row] : 0.f;
+      const float factor  = in ? rows.factor[row] : 0.f;
+      scale[j]            = 1.f;
+      if (bias_sums != nullptr && kProduct == LBT_F16) scale[j] = ldexpf(1.f, in ? rows.exponent[row] - counts->exponent : 0);
+      uint16_t* out = g + row * piece + in_piece + 4 * (lane >> 5);
+#pragma unroll
+      for (int i = 0; i < Tile::kMT; i++)
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+          uint16_t v[kPlanes][4];
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const int m   = i * 32 + block_m(q * 4 + e, lane);
+            const float p = exp_of(acc[i][j][q * 4 + e] - top, kExact) * inverse;
+            float d       = (m == label ? p - 1.f : p) * factor;
+            d             = in && c0 + m < n_classes ? d : 0.f;
+            acc[i][j][q * 4 + e] = d;
+            if constexpr (kPlanes == 1) {
+              v[0][e] = narrow_value<kProduct>(d);
+            } else {
+              uint16_t s[3];
+              split_planes(d, s);
+              v[0][e] = s[0];
+              v[1][e] = s[1];
+              v[2][e] = s[2];
+            }
+          }
+#pragma unroll
+          for (int l = 0; l < kPlanes; l++)
+            *reinterpret_cast<uint2*>(out + l * plane + i * 32 + q * 8) = *reinterpret_cast<const uint2*>(v[l]);
+        }
+    }
+    if (bias_sums == nullptr) return;
+    float(*share)[Tile::kBM] = reinterpret_cast<float(*)[Tile::kBM]>(lds);  // [waves over n][m]
+#pragma unroll
+    for (int i = 0; i < Tile::kMT; i++)
+#pragma unroll
+      for (int e = 0; e < 16; e++) {
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < Tile::kNT; j++) sum += acc[i][j][e] * scale[j];
+        for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor(sum, s);
+        if ((lane & 31) == 0) share[wn][wm * Tile::kWM + i * 32 + block_m(e, lane)] = sum;
+      }
+    __syncthreads();
+    for (int m = threadIdx.x; m < Tile::kBM; m += Tile::kThreads) {
+      float sum = 0.f;
+      for (int w = 0; w < Tile::kWavesN; w++) sum += share[w][m];
+      const int c = class_first + tile_m * Tile::kBM + m;
+      if (c < n_classes) bias_sums[static_cast<int64_t>(tile_n) * n_classes + c] = sum;
+    }
+  }
+};
+
+// grad_X: m = features, n = rows. Adds to (or begins) the sums of this split of the classes, [split][rows][padded_cols].
+struct RowsEpilogue {
+  float* sums;
+  int64_t split;  // values of a split
+  int padded_cols;
+  bool begin;
+
+  template <class Tile>
+  __device__ __forceinline__ void store(Float16v (&acc)[Tile::kMT][Tile::kNT], int tile_m, int tile_n, int wm, int wn, int lane,
+                                        int counted, const RowCounts*, char*) const
+  {
+#pragma unroll
+    for (int j = 0; j < Tile::kNT; j++) {
+      const int64_t row = static_cast<int64_t>(tile_n) * Tile::kBN + wn * Tile::kWN + j * 32 + (lane & 31);
+      if (row >= counted) continue;
+#pragma unroll
+      for (int i = 0; i < Tile::kMT; i++)
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+          const int col = tile_m * Tile::kBM + wm * Tile::kWM + i * 32 + q * 8 + 4 * (lane >> 5);
+          if (col >= padded_cols) continue;
+          float4* at = reinterpret_cast<float4*>(sums + blockIdx.y * split + row * padded_cols + col);
+          float4 v   = make_float4(acc[i][j][q * 4], acc[i][j][q * 4 + 1], acc[i][j][q * 4 + 2], acc[i][j][q * 4 + 3]);
+          if (!begin) {
+            const float4 o = *at;
+            v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
+          }
+          *at = v;
+        }
+    }
+  }
+};
+
+// grad_weight: m = features, n = classes of the piece. Complete: written in the output's type.
+template <int kDtype>
+struct ClassesEpilogue {
+  void* out;
+  int class_first, n_classes, cols;
+  bool scaled;  // the rows were multiplied by powers of two (half precision)
+
+  template <class Tile>
+  __device__ __forceinline__ void store(Float16v (&acc)[Tile::kMT][Tile::kNT], int tile_m, int tile_n, int wm, int wn, int lane,
+                                        int, const RowCounts* counts, char*) const
+  {
+    const int shift    = (scaled ? counts->reach - kReach : 0) - kHalfShift;
+    const bool aligned = cols % 4 == 0;
+#pragma unroll
+    for (int j = 0; j < Tile::kNT; j++) {
+      const int c = class_first + tile_n * Tile::kBN + wn * Tile::kWN + j * 32 + (lane & 31);
+      if (c >= n_classes) continue;
+#pragma unroll
+      for (int i = 0; i < Tile::kMT; i++)
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+          const int col = tile_m * Tile::kBM + wm * Tile::kWM + i * 32 + q * 8 + 4 * (lane >> 5);
+          if (col >= cols) continue;
+          float v[4];
+#pragma unroll
+          for (int e = 0; e < 4; e++) v[e] = kDtype == LBT_F16 ? ldexpf(acc[i][j][q * 4 + e], shift) : acc[i][j][q * 4 + e];
+          store_four<kDtype>(out, static_cast<int64_t>(c) * cols + col, v, cols - col, aligned);
+        }
+    }
+  }
+};
+
+// ---- joins ----------------------------------------------------------------------------------------
+
+constexpr int kJoinRows = 64, kJoinSlices = 16;
+
+// Top and total of each row from its shares by tile; its loss. 16 threads take the shares of a row between them, neighbours
+// in a wave are neighbouring rows.
+__global__ void __launch_bounds__(kJoinRows * kJoinSlices)
+  join_kernel(const float2* __restrict__ partial, int tiles, int64_t padded, LossRows rows, const RowCounts* __restrict__ counts,
+              float* __restrict__ loss)
+{
+  __shared__ float2 share[kJoinSlices][kJoinRows];
+  const int n       = threadIdx.x % kJoinRows, slice = threadIdx.x / kJoinRows;
+  const int64_t row = blockIdx.x * int64_t(kJoinRows) + n;
+  const int counted = counts->rows;
+  if (blockIdx.x * int64_t(kJoinRows) >= counted) return;
+  float top = -INFINITY, total = 0.f;
+  for (int t = slice; t < tiles; t += kJoinSlices) {
+    const float2 s   = partial[t * padded + row];
+    const float next = fmaxf(top, s.x);
+    const float from = next == -INFINITY ? 0.f : next;
+    total            = total * expf(top - from) + s.y * expf(s.x - from);
+    top              = next;
+  }
+  share[slice][n] = make_float2(top, total);
+  __syncthreads();
+  if (slice != 0 || row >= counted) return;
+  for (int s = 1; s < kJoinSlices; s++) top = fmaxf(top, share[s][n].x);
+  const float from = top == -INFINITY ? 0.f : top;
+  total            = 0.f;
+  for (int s = 0; s < kJoinSlices; s++) total += share[s][n].y * expf(share[s][n].x - from);
+  // where every class is masked there is no probability: the loss is infinite and p is 0
+  const bool none = top == -INFINITY && total == 0.f;
+  rows.top[row]     = from;
+  rows.inverse[row] = none ? 0.f : 1.f / total;
+  loss[rows.order[row]] = none ? INFINITY : (from - rows.picked[row]) + logf(total);
+}
+
+// grad_X from its sums over the splits; zeros for rows that do not count.
+template <int kDtype>
+__global__ void __launch_bounds__(256)
+  finish_rows_kernel(const float* __restrict__ sums, int splits, int64_t split, int padded_cols, int64_t n_rows, int cols,
+                     LossRows rows, void* __restrict__ out)
+{
+  const int groups = (cols + 3) / 4;
+  const int64_t i  = blockIdx.x * int64_t(256) + threadIdx.x;
+  if (i >= n_rows * groups) return;
+  const int64_t r = i / groups;
+  const int col   = static_cast<int>(i % groups) * 4;
+  const int p     = rows.place[r];
+  float v[4]      = {0.f, 0.f, 0.f, 0.f};
+  if (p >= 0) {
+    for (int s = 0; s < splits; s++) {
+      const float4 a = *reinterpret_cast<const float4*>(sums + s * split + static_cast<int64_t>(p) * padded_cols + col);
+      v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+    }
+    if (kDtype == LBT_F16) {
+      const int e = rows.exponent[p];
+      for (int q = 0; q < 4; q++) v[q] = e <= -1000 ? v[q] * 0.f : ldexpf(v[q], e - kHalfShift);
+    }
+  }
+  store_four<kDtype>(out, r * cols + col, v, cols - col, cols % 4 == 0);
+}
+
+__global__ void __launch_bounds__(256)
+  finish_bias_kernel(const float* __restrict__ sums, int n_classes, int tile_rows, const RowCounts* __restrict__ counts, int half,
+                     float* __restrict__ out)
+{
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c >= n_classes) return;
+  const int tiles = (counts->rows + tile_rows - 1) / tile_rows;
+  float sum       = 0.f;
+  for (int t = 0; t < tiles; t++) sum += sums[static_cast<int64_t>(t) * n_classes + c];
+  out[c] = half ? ldexpf(sum, counts->exponent - kHalfShift) : sum;
+}
+
+__global__ void __launch_bounds__(256) clear_kernel(uint16_t* __restrict__ out, int64_t n)
+{
+  const int64_t i = blockIdx.x * int64_t(256) + threadIdx.x;
+  if (i < n) out[i] = 0;
+}
+
+// ---- host -----------------------------------------------------------------------------------------
+
+using LargeTile = ProductTile<256, 256, 2, 4>;
+using SmallTile = ProductTile<128, 128, 2, 2>;
+
+int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+int64_t tiles_of(int64_t v, int64_t by) { return (v + by - 1) / by; }
+
+// Tiles of 256 x 256 where they give every CU one, else of 128 x 128.
+bool large_tiles(int64_t m, int64_t n) { return tiles_of(m, 256) * tiles_of(n, 256) >= 256; }
+
+struct LossCall {
+  int64_t n_rows;
+  int features, classes, dtype;
+  bool gradient;
+  int planes;
+  int64_t padded;   // rows
+  int cols;         // features, padded
+  bool packed;      // the weights are laid out piece by piece before they are multiplied
+  int64_t piece;    // classes at a time
+  int splits;       // of the classes in the products for grad_X
+  LossRows rows;
+  RowCounts* counts;
+  uint16_t *zeros, *x, *x_scaled, *weight, *g;
+  float2* partial;
+  float *row_sums, *bias_sums;
+
+  LossCall(int64_t n, int f, int k, int type, bool grad) : n_rows(n), features(f), classes(k), dtype(type), gradient(grad)
+  {
+    planes = type == LBT_F32 ? 3 : 1;
+    padded = round_up(n, 256);
+    cols   = static_cast<int>(round_up(f, kProductK));
+    packed = type == LBT_F32 || f % 8 != 0;
+    // a piece's G, and its packed weights, within kPieceBytes each; pieces of one size
+    int64_t most = round_up(k, 256);
+    if (grad) most = std::min(most, kPieceBytes / (2 * planes * padded) / 256 * 256);
+    if (packed) most = std::min(most, kPieceBytes / (2 * planes * int64_t(cols)) / 256 * 256);
+    most  = std::max<int64_t>(most, 256);
+    piece = round_up(tiles_of(k, tiles_of(k, most)), 256);
+    // grad_X has features / 256 x rows / 256 tiles: too few for 256 CUs unless the classes are split
+    const bool large    = large_tiles(f, n);
+    const int64_t tiles = large ? tiles_of(f, 256) * tiles_of(n, 256) : tiles_of(f, 128) * tiles_of(n, 128);
+    splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({512 / tiles, piece / 512, 16})));
+  }
+
+  template <typename A>
+  void carve(A& arena)
+  {
+    counts        = arena.template take<RowCounts>(1);
+    zeros         = arena.template take<uint16_t>(64);
+    rows.order    = arena.template take<int32_t>(padded);
+    rows.place    = arena.template take<int32_t>(padded);
+    rows.label    = arena.template take<int32_t>(padded);
+    rows.factor   = arena.template take<float>(padded);
+    rows.exponent = arena.template take<int32_t>(padded);
+    rows.picked   = arena.template take<float>(padded);
+    rows.top      = arena.template take<float>(padded);
+    rows.inverse  = arena.template take<float>(padded);
+    x             = arena.template take<uint16_t>(planes * padded * cols);
+    partial       = arena.template take<float2>(tiles_of(classes, 128) * padded);
+    weight = x_scaled = g = nullptr;
+    row_sums = bias_sums = nullptr;
+    if (packed) weight = arena.template take<uint16_t>(planes * piece * cols);
+    if (!gradient) return;
+    if (dtype == LBT_F16) x_scaled = arena.template take<uint16_t>(padded * cols);
+    g         = arena.template take<uint16_t>(planes * padded * piece);
+    row_sums  = arena.template take<float>(splits * padded * cols);
+    bias_sums = arena.template take<float>(tiles_of(padded, 128) * classes);
+  }
+};
+
+template <class Tile, class L, bool kAMajor, bool kBMajor, int kRowsSide, class Epilogue>
+int launch_tiles(hipStream_t s, ProductArgs args, int64_t m, int64_t n, int splits, const Epilogue& e)
+{
+  args.tiles_m = static_cast<int>(tiles_of(m, Tile::kBM));
+  args.tiles_n = static_cast<int>(tiles_of(n, Tile::kBN));
+  const int64_t blocks = static_cast<int64_t>(args.tiles_m) * args.tiles_n;
+  LBT_REQUIRE(blocks < (int64_t(1) << 31), "too many tiles");
+  product_kernel<Tile, L::kProduct, L::kPlanes, kAMajor, kBMajor, kRowsSide, Epilogue>
+    <<<dim3(static_cast<unsigned>(blocks), splits), Tile::kThreads, 0, s>>>(args, e);
+  LBT_HIP(hipGetLastError());
+  return LBT_OK;
+}
+
+template <class L, bool kAMajor, bool kBMajor, int kRowsSide, class Epilogue>
+int launch_product(hipStream_t s, const ProductArgs& args, int64_t m, int64_t n, int splits, const Epilogue& e)
+{
+  if (large_tiles(m, n)) return launch_tiles<LargeTile, L, kAMajor, kBMajor, kRowsSide>(s, args, m, n, splits, e);
+  return launch_tiles<SmallTile, L, kAMajor, kBMajor, kRowsSide>(s, args, m, n, splits, e);
+}
+
+template <int kDtype>
+int launch_pack(hipStream_t s, const void* from, int64_t first_row, int64_t rows, int cols, const int32_t* order,
+                int mode, const int32_t* exponent, RowCounts* counts, int64_t out_rows, int padded_cols, int64_t plane, uint16_t* out)
+{
+  const int64_t blocks = tiles_of(out_rows * (padded_cols / 8), 256);
+  LBT_REQUIRE(blocks < (int64_t(1) << 31), "too many values to lay out");
+  pack_rows_kernel<kDtype><<<static_cast<unsigned>(blocks), 256, 0, s>>>(from, first_row, rows, cols, order, mode, exponent, counts,
+                                                                         out_rows, padded_cols, plane, out);
+  LBT_HIP(hipGetLastError());
+  return LBT_OK;
+}
+
+template <int kDtype>
+int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void* weight, const float* bias, const int64_t* y,
+                    const float* sample_weight, float* loss, void* grad_X, void* grad_weight, float* grad_bias)
+{
+  using L              = LossType<kDtype>;
+  constexpr bool kFine = kDtype == LBT_F32;
+  constexpr bool kHalf = kDtype == LBT_F16;
+  prepare_rows_kernel<<<1, kPrepareThreads, 0, s>>>(y, sample_weight, c.n_rows, c.padded, c.classes, kHalf, c.rows, loss,
+                                                    c.counts, c.zeros);
+  LBT_HIP(hipGetLastError());
+  if (c.n_rows == 0) {  // no row: the gradients are zeros
+    const int64_t halves = int64_t(c.classes) * c.features * sizeof(typename L::Value) / 2;
+    LBT_REQUIRE(tiles_of(halves, 256) < (int64_t(1) << 31), "too many values");
+    clear_kernel<<<static_cast<unsigned>(tiles_of(halves, 256)), 256, 0, s>>>(static_cast<uint16_t*>(grad_weight), halves);
+    if (grad_bias != nullptr)
+      clear_kernel<<<static_cast<unsigned>(tiles_of(2 * int64_t(c.classes), 256)), 256, 0, s>>>(
+        reinterpret_cast<uint16_t*>(grad_bias), 2 * int64_t(c.classes));
+    LBT_HIP(hipGetLastError());
+    return LBT_OK;
+  }
+  const bool scaled = kHalf && sample_weight != nullptr;  // (without weights every exponent is 0)
+  LBT_TRY(launch_pack<kDtype>(s, X, 0, c.n_rows, c.features, c.rows.order, scaled ? kMeasure : kCopy, c.rows.exponent, c.counts, c.padded, c.cols,
+                              c.padded * c.cols, c.x));
+
+  // (rows that do not count are not there: x holds them side by side)
+  const ProductOperand x{c.x, c.cols, c.padded * c.cols, static_cast<int32_t>(c.padded), c.cols};
+  auto weights = [&](int64_t first, int64_t classes) {  // a piece, laid out by lay_out, or the caller's rows
+    if (c.packed) return ProductOperand{c.weight, c.cols, c.piece * c.cols, static_cast<int32_t>(classes), c.cols};
+    return ProductOperand{static_cast<const uint16_t*>(weight) + first * c.features, c.features, 0, static_cast<int32_t>(classes),
+                          c.features};
+  };
+  auto lay_out = [&](int64_t first) {
+    if (!c.packed) return LBT_OK;
+    return launch_pack<kDtype>(s, weight, first, c.classes, c.features, nullptr, kCopy, nullptr, c.counts, c.piece, c.cols,
+                               c.piece * c.cols, c.weight);
+  };
+  ProductArgs args{};
+  args.zeros  = c.zeros;
+  args.counts = c.counts;
+
+  // top and total of each row; weights that are multiplied where they lie need no pieces here
+  const int64_t step = c.packed ? c.piece : c.classes;
+  const int64_t by   = large_tiles(std::min<int64_t>(step, c.classes), c.n_rows) ? 256 : 128;
+  int64_t tiles      = 0;
+  for (int64_t first = 0; first < c.classes; first += step) {
+    const int64_t classes = std::min<int64_t>(step, c.classes - first);
+    LBT_TRY(lay_out(first));
+    args.a = weights(first, classes);
+    args.b = x;
+    args.k_extent = args.k_split = c.cols;
+    const LossEpilogue<kFine> e{bias, static_cast<int>(first), c.classes, static_cast<int>(tiles), c.padded, c.rows, c.partial};
+    // (every piece in tiles of one size: they share the numbering of `partial`)
+    LBT_TRY((by == 256 ? launch_tiles<LargeTile, L, false, false, kRowsN>(s, args, classes, c.n_rows, 1, e)
+                       : launch_tiles<SmallTile, L, false, false, kRowsN>(s, args, classes, c.n_rows, 1, e)));
+    tiles += tiles_of(classes, by);
+  }
+  join_kernel<<<static_cast<unsigned>(tiles_of(c.n_rows, kJoinRows)), kJoinRows * kJoinSlices, 0, s>>>(
+    c.partial, static_cast<int>(tiles), c.padded, c.rows, c.counts, loss);
+  LBT_HIP(hipGetLastError());
+  if (!c.gradient) return LBT_OK;
+
+  if (scaled)
+    LBT_TRY(launch_pack<kDtype>(s, X, 0, c.n_rows, c.features, c.rows.order, kScale, c.rows.exponent, c.counts, c.padded, c.cols,
+                                c.padded * c.cols, c.x_scaled));
+  ProductOperand x_scaled = x;
+  if (scaled) x_scaled.base = c.x_scaled;
+  const ProductOperand g{c.g, c.piece, c.padded * c.piece, static_cast<int32_t>(c.padded), static_cast<int32_t>(c.piece)};
+  const int64_t bias_tile = large_tiles(std::min<int64_t>(c.piece, c.classes), c.n_rows) ? 256 : 128;
+  for (int64_t first = 0; first < c.classes; first += c.piece) {
+    const int64_t classes = std::min<int64_t>(c.piece, c.classes - first);
+    if (first > 0 || c.piece < c.classes) LBT_TRY(lay_out(first));
+    const ProductOperand w = weights(first, classes);
+    args.a        = w;
+    args.b        = x;
+    args.k_extent = args.k_split = c.cols;
+    const GradientEpilogue<kFine, L::kProduct, L::kPlanes> ge{bias, static_cast<int>(first), c.classes, static_cast<int>(c.piece),
+                                                              c.rows, c.g, c.padded * c.piece,
+                                                              grad_bias != nullptr ? c.bias_sums : nullptr};
+    // (over the whole piece: what lies past its classes is written as zeros)
+    LBT_TRY((bias_tile == 256 ? launch_tiles<LargeTile, L, false, false, kRowsN>(s, args, c.piece, c.n_rows, 1, ge)
+                              : launch_tiles<SmallTile, L, false, false, kRowsN>(s, args, c.piece, c.n_rows, 1, ge)));
+    args.a        = w;
+    args.b        = g;
+    args.k_extent = static_cast<int32_t>(c.piece);
+    args.k_split  = static_cast<int32_t>(round_up(tiles_of(c.piece, c.splits), kProductK));
+    const RowsEpilogue re{c.row_sums, c.padded * c.cols, c.cols, first == 0};
+    LBT_TRY((launch_product<L, true, false, kRowsN>(s, args, c.features, c.n_rows, c.splits, re)));
+    args.a        = x_scaled;
+    args.b        = g;
+    args.k_extent = args.k_split = static_cast<int32_t>(c.padded);
+    const ClassesEpilogue<kDtype> ce{grad_weight, static_cast<int>(first), c.classes, c.features, scaled};
+    LBT_TRY((launch_product<L, true, true, kRowsK>(s, args, c.features, classes, 1, ce)));
+  }
+  const int64_t blocks = tiles_of(c.n_rows * ((c.features + 3) / 4), 256);
+  LBT_REQUIRE(blocks < (int64_t(1) << 31), "too many values");
+  finish_rows_kernel<kDtype><<<static_cast<unsigned>(blocks), 256, 0, s>>>(c.row_sums, c.splits, c.padded * c.cols, c.cols,
+                                                                           c.n_rows, c.features, c.rows, grad_X);
+  LBT_HIP(hipGetLastError());
+  if (grad_bias != nullptr) {
+    finish_bias_kernel<<<static_cast<unsigned>(tiles_of(c.classes, 256)), 256, 0, s>>>(c.bias_sums, c.classes,
+                                                                                       static_cast<int>(bias_tile), c.counts, kHalf,
+                                                                                       grad_bias);
+    LBT_HIP(hipGetLastError());
+  }
+  return LBT_OK;
+}
+
+bool loss_shape(int64_t n_rows, int32_t n_features, int32_t n_outputs, int32_t dtype)
+{
+  return (dtype == LBT_F32 || dtype == LBT_BF16 || dtype == LBT_F16) && n_rows >= 0 && n_features >= 1 && n_outputs >= 1 &&
+         n_rows <= (int64_t(1) << 30) && n_features <= (1 << 20) && n_outputs <= (1 << 30) &&
+         n_rows * n_features < (int64_t(1) << 38) && int64_t(n_outputs) * n_features < (int64_t(1) << 38);
+}
+
+int run_loss(void* stream, const void* X, const void* weight, int32_t dtype, int64_t n_rows, int32_t n_features, int32_t n_outputs,
+             const float* bias, const int64_t* y, const float* sample_weight, float* loss, void* grad_X, void* grad_weight,
+             float* grad_bias, bool gradient, void* workspace, size_t workspace_bytes)
+{
+  LBT_REQUIRE(dtype == LBT_F32 || dtype == LBT_BF16 || dtype == LBT_F16, "unsupported dtype %d", dtype);
+  LBT_REQUIRE(loss_shape(n_rows, n_features, n_outputs, dtype), "bad shape");
+  LBT_REQUIRE(grad_bias == nullptr || bias != nullptr, "a gradient of the bias without a bias");
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (n_rows == 0 && !gradient) return LBT_OK;
+  LBT_REQUIRE(weight != nullptr, "null pointer");
+  LBT_REQUIRE(n_rows == 0 || (X != nullptr && y != nullptr && loss != nullptr), "null pointer");
+  LBT_REQUIRE(!gradient || (grad_weight != nullptr && (n_rows == 0 || grad_X != nullptr)), "null pointer");
+  const uintptr_t places = reinterpret_cast<uintptr_t>(X) | reinterpret_cast<uintptr_t>(weight) |
+                           reinterpret_cast<uintptr_t>(grad_X) | reinterpret_cast<uintptr_t>(grad_weight);
+  LBT_REQUIRE((places & 15) == 0, "X, weight and their gradients must be 16-byte aligned");
+  if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0) {
+    set_error("a workspace aligned to 256 bytes is needed");
+    return LBT_ERR_WORKSPACE;
+  }
+  LossCall c(std::max<int64_t>(n_rows, 1), n_features, n_outputs, dtype, gradient);
+  c.n_rows = n_rows;
+  Arena arena;
+  arena.base = static_cast<char*>(workspace);
+  arena.cap  = workspace_bytes;
+  c.carve(arena);
+  if (arena.failed) {
+    set_error("workspace of %zu bytes, %zu needed", workspace_bytes, arena.used);
+    return LBT_ERR_WORKSPACE;
+  }
+  ProfScope ps(LBT_PROF_OTHER, s);
+  switch (dtype) {
+    case LBT_BF16:
+      return linear_log_loss<LBT_BF16>(s, c, X, weight, bias, y, sample_weight, loss, grad_X, grad_weight, grad_bias);
+    case LBT_F16:
+      return linear_log_loss<LBT_F16>(s, c, X, weight, bias, y, sample_weight, loss, grad_X, grad_weight, grad_bias);
+    default:
+      return linear_log_loss<LBT_F32>(s, c, X, weight, bias, y, sample_weight, loss, grad_X, grad_weight, grad_bias);
+  }
+}
+
+}  // namespace
+}  // namespace lbt
+
+extern "C" {
+
+size_t lbt_linear_log_loss_workspace_bytes(int64_t n_rows, int32_t n_features, int32_t n_outputs, int32_t dtype, int32_t gradient)
+{
+  if (!lbt::loss_shape(n_rows, n_features, n_outputs, dtype)) return 0;
+  lbt::LossCall c(std::max<int64_t>(n_rows, 1), n_features, n_outputs, dtype, gradient != 0);
+  lbt::Arena arena;
+  arena.measure = true;
+  c.carve(arena);
+  return arena.used;
+}
+
+int lbt_linear_log_loss(void* stream, const void* X, const void* weight, int32_t dtype, int64_t n_rows, int32_t n_features,
+                        int32_t n_outputs, const float* bias, const int64_t* y, float* loss, void* workspace,
+                        size_t workspace_bytes)
+{
+  return lbt::run_loss(stream, X, weight, dtype, n_rows, n_features, n_outputs, bias, y, nullptr, loss, nullptr, nullptr, nullptr,
+                       false, workspace, workspace_bytes);
+}
+
+int lbt_linear_log_loss_gradient(void* stream, const void* X, const void* weight, int32_t dtype, int64_t n_rows,
+                                 int32_t n_features, int32_t n_outputs, const float* bias, const int64_t* y,
+                                 const float* sample_weight, float* loss, void* grad_X, void* grad_weight, float* grad_bias,
+                                 void* workspace, size_t workspace_bytes)
+{
+  return lbt::run_loss(stream, X, weight, dtype, n_rows, n_features, n_outputs, bias, y, sample_weight, loss, grad_X, grad_weight,
+                       grad_bias, true, workspace, workspace_bytes);
+}
+
+}  // extern "C"

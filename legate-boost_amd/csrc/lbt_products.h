@@ -1,0 +1,218 @@
+// Tiled matrix products on the matrix cores, for the linear log loss (lbt_linear_loss.hip).
+//
+// C[m][n] = sum_k A(m, k) B(n, k), added in 32 bits. An operand is an array of 16-bit numbers in rows, and either of its two
+// directions may be the one that is contiguous:
+//   k contiguous   rows are the product's m (or n), read by ds_read_b128
+//   k in rows      rows are the product's k; ds_read_b64_tr_b16 turns 4 x 16 blocks on their way out of the LDS, so that
+//                  no operand is ever transposed in memory
+// A workgroup forms a tile of kBM x kBN, 64 values of k at a time, which go from memory into the LDS without passing
+// through registers (global_load_lds, 16 bytes a lane). What lies outside an operand is read from a page of zeros, lane by
+// lane, so the loop has no edges. The LDS holds 16-byte chunks in an order (an exclusive or with the row's number) in which
+// the 32 rows that a fragment reads lie on all banks.
+//
+// float operands are sums of three bfloat16 planes (8 + 8 + 8 significant bits, exact); of the nine products of planes the
+// six that reach above 2^-24 of the result are added up, one walk over k each.
+#pragma once
+
+#include "lbt_internal.h"
+
+namespace lbt {
+
+typedef __attribute__((ext_vector_type(4))) short Short4;
+typedef __attribute__((ext_vector_type(8))) short Short8;
+typedef __attribute__((ext_vector_type(8))) __bf16 Bf16x8;
+typedef __attribute__((ext_vector_type(8))) _Float16 Half8;
+typedef __attribute__((ext_vector_type(16))) float Float16v;
+
+constexpr int kProductK = 64;  // values of k in a stage of the LDS
+
+// One operand: plane p of row r begins at base + p * plane + r * ld (elements). cols is a multiple of 8.
+struct ProductOperand {
+  const uint16_t* base;
+  int64_t ld;
+  int64_t plane;
+  int32_t rows;
+  int32_t cols;
+};
+
+// What the rows of a call come down to; written on the device by prepare_rows_kernel.
+struct RowCounts {
+  int32_t rows;      // rows that count
+  int32_t exponent;  // the largest exponent of a row's weight (half precision)
+  int32_t reach;     // the largest exponent of a weight times a value of its row (half precision)
+};
+
+struct ProductArgs {
+  ProductOperand a, b;
+  int32_t k_extent;  // k ends here, or (row products over k) at the rows that count
+  int32_t k_split;   // values of k of one split, a multiple of kProductK
+  int32_t tiles_m, tiles_n;
+  const uint16_t* zeros;  // 16 bytes of zeros
+  const RowCounts* counts;
+};
+
+template <int kM, int kN, int kWaveM, int kWaveN>
+struct ProductTile {
+  static constexpr int kBM = kM, kBN = kN;              // tile of a workgroup
+  static constexpr int kWM = kM / kWaveM, kWN = kN / kWaveN;  // tile of a wave
+  static constexpr int kWavesM = kWaveM, kWavesN = kWaveN;
+  static constexpr int kWaves = kWaveM * kWaveN, kThreads = kWaves * 64;
+  static constexpr int kMT = kWM / 32, kNT = kWN / 32;  // 32 x 32 blocks of a wave
+};
+
+template <int kType>  // LBT_BF16 or LBT_F16
+__device__ __forceinline__ Float16v mfma_32x32x16(Short8 a, Short8 b, Float16v c)
+{
+  if constexpr (kType == LBT_F16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(Half8, a), __builtin_bit_cast(Half8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(Bf16x8, a), __builtin_bit_cast(Bf16x8, b), c, 0, 0, 0);
+}
+
+// Asks for the stage of one operand: kTile of its m (or n) from `tile0` on, 64 of its k from `k0` on.
+template <bool kRowsAreK, int kTile, int kWaves>
+__device__ __forceinline__ void load_stage(const ProductOperand& op, const uint16_t* base, int tile0, int k0,
+                                           const uint16_t* zeros, char* lds, int wave, int lane)
+{
+  constexpr int kChunks = kTile * kProductK / 8;  // of 16 bytes
+  static_assert(kChunks % (kWaves * 64) == 0, "every lane loads the same number of chunks");
+#pragma unroll
+  for (int j = 0; j < kChunks / (kWaves * 64); j++) {
+    const int q = (j * kWaves + wave) * 64 + lane;
+    const uint16_t* from;
+    bool inside;
+    if constexpr (kRowsAreK) {
+      constexpr int kRow = kTile / 8;  // chunks of a row
+      const int row = q / kRow;
+      const int col = ((q % kRow) ^ ((row & 3) << 2)) * 8;
+      inside = k0 + row < op.rows && tile0 + col < op.cols;
+      from   = base + static_cast<int64_t>(k0 + row) * op.ld + (tile0 + col);
+    } else {
+      const int row = q >> 3;
+      const int col = ((q & 7) ^ (row & 7)) * 8;
+      inside = tile0 + row < op.rows && k0 + col < op.cols;
+      from   = base + static_cast<int64_t>(tile0 + row) * op.ld + (k0 + col);
+    }
+    from = inside ? from : zeros;
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+                                     (__attribute__((address_space(3))) void*)(lds + (j * kWaves + wave) * 1024), 16, 0, 0);
+  }
+}
+
+// Eight values of k for each of 32 values of m (or n) from `first` on: lane l has m = l % 32, k = 16 kk + 8 (l / 32) ...
+template <bool kRowsAreK, int kTile>
+__device__ __forceinline__ Short8 fragment(const char* lds, int first, int kk, int lane)
+{
+  if constexpr (kRowsAreK) {
+    const int row   = kk * 16 + (lane >> 5) * 8 + ((lane & 15) >> 2);
+    const int col   = first + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+    const int chunk = (col >> 3) ^ ((row & 3) << 2);
+    const char* at  = lds + row * (kTile * 2) + chunk * 16 + (col & 7) * 2;
+    typedef __attribute__((address_space(3))) Short4* LdsPtr;
+    const Short4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)at);
+    const Short4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(at + 4 * (kTile * 2)));
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  } else {
+    const int row   = first + (lane & 31);
+    const int chunk = (kk * 2 + (lane >> 5)) ^ (row & 7);
+    return *reinterpret_cast<const Short8*>(lds + row * (kProductK * 2) + chunk * 16);
+  }
+}
+
+// Tile of this workgroup: workgroups go round the 8 XCDs by their number, each XCD takes a run of tiles, and a run goes
+// through `kGroup` tiles of m for every tile of n, so that what an XCD has in its L2 is used by several tiles.
+__device__ __forceinline__ void tile_of_block(int block, int tiles_m, int tiles_n, int* m, int* n)
+{
+  constexpr int kXcds = 8, kGroup = 8;
+  const int tiles = tiles_m * tiles_n;
+  const int share = tiles / kXcds, more = tiles % kXcds;
+  const int xcd   = block % kXcds;
+  const int at    = xcd * share + min(xcd, more) + block / kXcds;
+  const int width = kGroup * tiles_n;
+  const int group = at / width;
+  const int size  = min(tiles_m - group * kGroup, kGroup);
+  *m = group * kGroup + (at % width) % size;
+  *n = (at % width) / size;
+}
+
+// Which planes are multiplied: the small products first.
+template <int kPlanes>
+struct PlanePairs;
+template <>
+struct PlanePairs<1> {
+  static constexpr int kCount = 1;
+  __device__ static int a(int) { return 0; }
+  __device__ static int b(int) { return 0; }
+};
+template <>
+struct PlanePairs<3> {
+  static constexpr int kCount = 6;  // (2,0) (1,1) (0,2) (1,0) (0,1) (0,0)
+  __device__ static int a(int i) { return (0x001012 >> (4 * i)) & 15; }
+  __device__ static int b(int i) { return (0x010210 >> (4 * i)) & 15; }
+};
+
+// kRowsSide: which direction of the product is the call's rows: 0 n, 1 k, 2 m
+enum { kRowsN = 0, kRowsK = 1 };
+
+template <class Tile, int kType, int kPlanes, bool kAMajor, bool kBMajor, int kRowsSide, class Epilogue>
+__global__ void __launch_bounds__(Tile::kThreads, 1) product_kernel(const ProductArgs args, const Epilogue epilogue)
+{
+  constexpr int kStageA = Tile::kBM * kProductK * 2, kStageB = Tile::kBN * kProductK * 2;
+  __shared__ __attribute__((aligned(1024))) char lds[2 * (kStageA + kStageB)];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  int tile_m, tile_n;
+  tile_of_block(blockIdx.x, args.tiles_m, args.tiles_n, &tile_m, &tile_n);
+  const int rows = args.counts->rows;
+  int k_end      = args.k_extent;
+  if (kRowsSide == kRowsN && tile_n * Tile::kBN >= rows) return;
+  if (kRowsSide == kRowsK) k_end = min(k_end, rows);
+  const int k_first = blockIdx.y * args.k_split;
+  k_end             = min(k_end, k_first + args.k_split);
+  const int steps   = k_end > k_first ? (k_end - k_first + kProductK - 1) / kProductK : 0;
+
+  const int wm = wave / Tile::kWavesN, wn = wave % Tile::kWavesN;
+  Float16v acc[Tile::kMT][Tile::kNT];
+#pragma unroll
+  for (int i = 0; i < Tile::kMT; i++)
+#pragma unroll
+    for (int j = 0; j < Tile::kNT; j++)
+#pragma unroll
+      for (int e = 0; e < 16; e++) acc[i][j][e] = 0.f;
+
+  const int total = steps * PlanePairs<kPlanes>::kCount;
+  auto load       = [&](int t, int stage) {
+    const int pair = kPlanes == 1 ? 0 : t / steps;
+    const int k0   = k_first + (kPlanes == 1 ? t : t % steps) * kProductK;
+    char* at       = lds + stage * (kStageA + kStageB);
+    load_stage<kAMajor, Tile::kBM, Tile::kWaves>(args.a, args.a.base + PlanePairs<kPlanes>::a(pair) * args.a.plane,
+                                                 tile_m * Tile::kBM, k0, args.zeros, at, wave, lane);
+    load_stage<kBMajor, Tile::kBN, Tile::kWaves>(args.b, args.b.base + PlanePairs<kPlanes>::b(pair) * args.b.plane,
+                                                 tile_n * Tile::kBN, k0, args.zeros, at + kStageA, wave, lane);
+  };
+  if (total > 0) load(0, 0);
+  for (int t = 0; t < total; t++) {
+    __syncthreads();  // this stage has arrived, and the one before it has been read by all
+    if (t + 1 < total) load(t + 1, (t + 1) & 1);
+    const char* at = lds + (t & 1) * (kStageA + kStageB);
+#pragma unroll
+    for (int kk = 0; kk < kProductK / 16; kk++) {
+      Short8 a[Tile::kMT], b[Tile::kNT];
+#pragma unroll
+      for (int i = 0; i < Tile::kMT; i++) a[i] = fragment<kAMajor, Tile::kBM>(at, wm * Tile::kWM + i * 32, kk, lane);
+#pragma unroll
+      for (int j = 0; j < Tile::kNT; j++)
+        b[j] = fragment<kBMajor, Tile::kBN>(at + kStageA, wn * Tile::kWN + j * 32, kk, lane);
+#pragma unroll
+      for (int i = 0; i < Tile::kMT; i++)
+#pragma unroll
+        for (int j = 0; j < Tile::kNT; j++) acc[i][j] = mfma_32x32x16<kType>(a[i], b[j], acc[i][j]);
+    }
+  }
+  __syncthreads();  // the LDS is free for what follows
+  epilogue.template store<Tile>(acc, tile_m, tile_n, wm, wn, lane, rows, args.counts, lds);
+}
+
+// Element e of a 32 x 32 block: its m within the block; its n is lane % 32.
+__device__ __forceinline__ int block_m(int e, int lane) { return 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3); }
+
+}  // namespace lbt

@@ -21,6 +21,8 @@ SO_PATH = os.environ.get("LBTREE_SO") or os.path.join(os.path.dirname(_HERE), "c
 LBT_OK = 0
 LBT_F32 = 0
 LBT_F64 = 1
+LBT_BF16 = 2
+LBT_F16 = 3
 LBT_MAX_SPLIT_SAMPLES = 2048
 LBT_OBJ_SQUARED_ERROR = 0
 LBT_OBJ_LOG_LOSS = 1
@@ -221,6 +223,23 @@ def _load():
     lib.lbt_update_positions.restype = C.c_int
     lib.lbt_update_positions.argtypes = [C.c_void_p, C.c_void_p, C.c_int32, C.c_int64, C.c_int32, C.c_void_p, C.c_void_p,
                                          C.c_void_p, C.c_int32, C.c_void_p, C.c_size_t]
+    lib.lbt_linear_log_loss_workspace_bytes.restype = C.c_size_t
+    lib.lbt_linear_log_loss_workspace_bytes.argtypes = [C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_int32]
+    lib.lbt_linear_log_loss.restype = C.c_int
+    lib.lbt_linear_log_loss.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_int64, C.c_int32, C.c_int32, C.c_void_p,
+                                        C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t]
+    lib.lbt_linear_log_loss_gradient.restype = C.c_int
+    lib.lbt_linear_log_loss_gradient.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_int64, C.c_int32, C.c_int32,
+                                                 C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
+                                                 C.c_void_p, C.c_size_t]
+    lib.lbt_embed_rows.restype = C.c_int
+    lib.lbt_embed_rows.argtypes = [C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_void_p, C.c_int32, C.c_int64,
+                                   C.c_float, C.c_void_p]
+    lib.lbt_embed_rows_gradient_workspace_bytes.restype = C.c_size_t
+    lib.lbt_embed_rows_gradient_workspace_bytes.argtypes = [C.c_int64, C.c_int32, C.c_int32, C.c_int32]
+    lib.lbt_embed_rows_gradient.restype = C.c_int
+    lib.lbt_embed_rows_gradient.argtypes = [C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_int32, C.c_int64, C.c_int32, C.c_int32,
+                                            C.c_float, C.c_int32, C.c_void_p, C.c_void_p, C.c_size_t]
     lib.lbt_profile_enable.restype = None
     lib.lbt_profile_enable.argtypes = [C.c_int]
     lib.lbt_profile_reset.restype = None
@@ -263,6 +282,8 @@ EXPORTS = [
     "lbt_quantise_gradients_workspace_bytes", "lbt_quantise_gradients", "lbt_quantise_gradients_static",
     "lbt_histogram_level_workspace_bytes", "lbt_histogram_level", "lbt_scan", "lbt_best_split_workspace_bytes",
     "lbt_best_split", "lbt_update_positions_workspace_bytes", "lbt_update_positions",
+    "lbt_linear_log_loss_workspace_bytes", "lbt_linear_log_loss", "lbt_linear_log_loss_gradient",
+    "lbt_embed_rows", "lbt_embed_rows_gradient_workspace_bytes", "lbt_embed_rows_gradient",
     "lbt_profile_enable", "lbt_profile_reset",
     "lbt_profile_get", "lbt_small_levels_polls",
 ]

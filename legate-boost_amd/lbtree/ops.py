@@ -564,6 +564,147 @@ def gather_rows(X, samples, row_offset=0):
     return out
 
 
+# ---- vocabularies: linear scores over many classes, rows of a table (include/lbtree.h) ------------
+
+_DT_NARROW = {torch.float32: _lib.LBT_F32, torch.bfloat16: _lib.LBT_BF16, torch.float16: _lib.LBT_F16}
+
+
+def _narrow(a, dims, what):
+    """A contiguous CUDA tensor of one of the types above whose data is aligned as the kernels need it."""
+    a = as_device(a)
+    if a.dtype not in _DT_NARROW:
+        raise _lib.LbtError("%s must be float32, bfloat16 or float16, got %s" % (what, a.dtype))
+    if dims is not None and a.dim() != dims:
+        raise _lib.LbtError("%s must be %d-dimensional" % (what, dims))
+    return a if a.data_ptr() % 16 == 0 else a.clone()
+
+
+def _beside(a, device, what):
+    if a.device != device:
+        raise _lib.LbtError("%s is on %s, the others on %s" % (what, a.device, device))
+    return a
+
+
+def _scratch(nbytes, device):
+    """The workspace of a call. One that is being captured into a graph gets its own from the graph's memory: graphs are replayed
+    on any stream, and the buffers kept between calls are replaced by larger ones."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(int(nbytes), dtype=torch.uint8, device=device)
+    return _get_workspace(nbytes, device)
+
+
+def _whole_numbers(a, n, what):
+    a = as_device(a)
+    if a.dtype.is_floating_point or a.dtype.is_complex or a.dtype == torch.bool:
+        raise _lib.LbtError("%s must be whole numbers, got %s" % (what, a.dtype))
+    if n is not None and a.numel() != n:
+        raise _lib.LbtError("%s has %d elements, expected %d" % (what, a.numel(), n))
+    return a
+
+
+def _loss_arguments(X, weight, y, bias):
+    X, weight = _narrow(X, 2, "X"), _narrow(weight, 2, "weight")
+    dev = X.device
+    if weight.dtype != X.dtype or weight.shape[1] != X.shape[1]:
+        raise _lib.LbtError("weight must be [n_outputs, %d] of %s, got %s of %s" % (X.shape[1], X.dtype, list(weight.shape),
+                                                                                   weight.dtype))
+    if X.shape[1] == 0 or weight.shape[0] == 0:
+        raise _lib.LbtError("X and weight need a feature and a class at least")
+    y = _whole_numbers(y, X.shape[0], "y").to(torch.int64)
+    _beside(weight, dev, "weight")
+    _beside(y, dev, "y")
+    if bias is not None:
+        bias = _beside(as_device(bias, torch.float32), dev, "bias")
+        if bias.numel() != weight.shape[0]:
+            raise _lib.LbtError("bias must have one entry per class")
+    return X, weight, y, bias
+
+
+def _ptr(a):
+    return None if a is None else a.data_ptr()
+
+
+def linear_log_loss(X, weight, y, bias=None):
+    """Log loss per row of the linear scores X @ weight.T + bias over many classes, without the scores in memory: float32
+    [n_rows]. X [n_rows, n_features] and weight [n_classes, n_features]: both float32, bfloat16 or float16; y: whole numbers, a
+    row whose label is not in [0, n_classes) does not count and has loss 0; bias: float32 [n_classes], -inf masks a class.
+    No autograd graph is recorded: linear_log_loss_gradient returns the gradients."""
+    X, weight, y, bias = _loss_arguments(X, weight, y, bias)
+    n, f = X.shape
+    k, dt = weight.shape[0], _DT_NARROW[X.dtype]
+    with torch.cuda.device(X.device):
+        loss = torch.empty(n, dtype=torch.float32, device=X.device)
+        ws = _scratch(_lib.lib.lbt_linear_log_loss_workspace_bytes(n, f, k, dt, 0), X.device)
+        _lib.check(_lib.lib.lbt_linear_log_loss(_stream(), X.data_ptr(), weight.data_ptr(), dt, n, f, k, _ptr(bias), y.data_ptr(),
+                                                loss.data_ptr(), ws.data_ptr(), ws.numel()))
+    return loss
+
+
+def linear_log_loss_gradient(X, weight, y, sample_weight=None, bias=None):
+    """linear_log_loss with the gradients of sum_r sample_weight[r] * loss[r]: (loss, grad_X, grad_weight), and grad_bias (float32)
+    behind them where a bias is given. grad_X and grad_weight have the types of X and weight. sample_weight: [n_rows], all ones
+    where it is not given (1 / n_rows makes it the mean); the loss that is returned is not weighted."""
+    X, weight, y, bias = _loss_arguments(X, weight, y, bias)
+    n, f = X.shape
+    k, dt = weight.shape[0], _DT_NARROW[X.dtype]
+    w = None
+    if sample_weight is not None:
+        w = _beside(as_device(sample_weight, torch.float32), X.device, "sample_weight")
+        if w.numel() != n:
+            raise _lib.LbtError("sample_weight must have one entry per row")
+    with torch.cuda.device(X.device):
+        loss = torch.empty(n, dtype=torch.float32, device=X.device)
+        grad_X, grad_weight = torch.empty_like(X), torch.empty_like(weight)
+        grad_bias = None if bias is None else torch.empty(k, dtype=torch.float32, device=X.device)
+        ws = _scratch(_lib.lib.lbt_linear_log_loss_workspace_bytes(n, f, k, dt, 1), X.device)
+        _lib.check(_lib.lib.lbt_linear_log_loss_gradient(
+            _stream(), X.data_ptr(), weight.data_ptr(), dt, n, f, k, _ptr(bias), y.data_ptr(), _ptr(w), loss.data_ptr(),
+            grad_X.data_ptr(), grad_weight.data_ptr(), _ptr(grad_bias), ws.data_ptr(), ws.numel()))
+    return (loss, grad_X, grad_weight) if bias is None else (loss, grad_X, grad_weight, grad_bias)
+
+
+def _tokens(tokens, device):
+    tokens = _beside(_whole_numbers(tokens, None, "tokens"), device, "tokens")
+    return tokens if tokens.dtype in (torch.int32, torch.int64) else tokens.to(torch.int64)
+
+
+def embed_rows(table, tokens, scale=1.0):
+    """scale * table[tokens] for whole numbers `tokens` of any shape: [*tokens.shape, n_features] of the table's type (float32,
+    bfloat16 or float16), multiplied in float32 and rounded once. A token that is no row of the table gives zeros. tokens may be
+    a tree's row_leaf (build_tree(row_leaf=True))."""
+    table = _narrow(table, 2, "table")
+    tokens = _tokens(tokens, table.device)
+    with torch.cuda.device(table.device):
+        out = torch.empty(tuple(tokens.shape) + (table.shape[1],), dtype=table.dtype, device=table.device)
+        _lib.check(_lib.lib.lbt_embed_rows(_stream(), table.data_ptr(), _DT_NARROW[table.dtype], table.shape[0], table.shape[1],
+                                           tokens.data_ptr(), tokens.element_size(), tokens.numel(), float(scale), out.data_ptr()))
+    return out
+
+
+def embed_rows_gradient(grad, tokens, n_rows, scale=1.0, add_to=None):
+    """The gradient of embed_rows with respect to its table of n_rows rows: row v is scale times the sum of grad[t] over the t with
+    tokens[t] = v, in float32 and in a fixed order. grad: [*tokens.shape, n_features]. add_to: a contiguous [n_rows, n_features]
+    tensor of grad's type that the sums are added to in place, and which is returned, instead of a new one (a table that is also
+    the weight of linear_log_loss_gradient)."""
+    grad = _narrow(grad, None, "grad")
+    tokens = _tokens(tokens, grad.device)
+    if grad.dim() == 0 or grad.shape[:-1] != tokens.shape:
+        raise _lib.LbtError("grad must be [*tokens.shape, n_features], got %s for tokens %s" % (list(grad.shape), list(tokens.shape)))
+    f, n_rows, dt = grad.shape[-1], int(n_rows), _DT_NARROW[grad.dtype]
+    out = add_to
+    if add_to is not None and not (isinstance(add_to, torch.Tensor) and add_to.shape == (n_rows, f) and add_to.dtype == grad.dtype
+                                   and add_to.device == grad.device and add_to.is_contiguous() and add_to.data_ptr() % 16 == 0):
+        raise _lib.LbtError("add_to must be a contiguous, 16-byte aligned [%d, %d] tensor of %s beside grad" % (n_rows, f, grad.dtype))
+    with torch.cuda.device(grad.device):
+        if out is None:
+            out = torch.empty((max(n_rows, 0), f), dtype=grad.dtype, device=grad.device)
+        ws = _scratch(_lib.lib.lbt_embed_rows_gradient_workspace_bytes(tokens.numel(), f, n_rows, dt), grad.device)
+        _lib.check(_lib.lib.lbt_embed_rows_gradient(_stream(), grad.data_ptr(), dt, tokens.data_ptr(), tokens.element_size(),
+                                                    tokens.numel(), f, n_rows, float(scale), int(add_to is not None),
+                                                    out.data_ptr(), ws.data_ptr(), ws.numel()))
+    return out
+
+
 def select_split_samples(X, split_samples, seed, dataset_rows=None, row_offset=0):
     """SelectSplitSamples on its own (build_tree.cu:867-964): returns (proposals, row_pointers),
     the proposals of feature f at proposals[row_pointers[f]:row_pointers[f + 1]], ascending,

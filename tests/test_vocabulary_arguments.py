@@ -1,0 +1,92 @@
+"""The operators for vocabularies refuse bad arguments before they touch a GPU, and say how much scratch they need."""
+import ctypes as C
+
+import pytest
+
+from lbtree import _lib
+
+L = _lib.lib
+AT = C.c_void_p(4096)  # never followed: the checks come first
+ODD = C.c_void_p(4096 + 8)
+BIG = 1 << 40
+
+
+def loss(stream=None, X=AT, weight=AT, dtype=_lib.LBT_BF16, n=10, f=8, k=100, bias=None, y=AT, out=AT, ws=None, size=0):
+    return L.lbt_linear_log_loss(stream, X, weight, dtype, n, f, k, bias, y, out, ws, size)
+
+
+def gradient(X=AT, weight=AT, dtype=_lib.LBT_BF16, n=10, f=8, k=100, bias=None, y=AT, w=None, out=AT, gx=AT, gw=AT, gb=None,
+             ws=None, size=0):
+    return L.lbt_linear_log_loss_gradient(None, X, weight, dtype, n, f, k, bias, y, w, out, gx, gw, gb, ws, size)
+
+
+@pytest.mark.parametrize("arguments,message", [
+    (dict(dtype=_lib.LBT_F64), b"dtype"), (dict(dtype=9), b"dtype"), (dict(dtype=-1), b"dtype"),
+    (dict(n=-1), b"shape"), (dict(f=0), b"shape"), (dict(k=0), b"shape"), (dict(k=-5), b"shape"),
+    (dict(n=1 << 31), b"shape"), (dict(f=1 << 20, k=1 << 20), b"shape"),
+    (dict(X=None), b"null"), (dict(weight=None), b"null"), (dict(y=None), b"null"), (dict(out=None), b"null"),
+    (dict(X=ODD), b"aligned"), (dict(weight=ODD), b"aligned"),
+])
+def test_loss_refuses(arguments, message):
+    for call in (loss, gradient):
+        assert call(**arguments) == -1
+        assert message in L.lbt_last_error()
+
+
+@pytest.mark.parametrize("arguments,message", [
+    (dict(gx=None), b"null"), (dict(gw=None), b"null"), (dict(gx=ODD), b"aligned"), (dict(gw=ODD), b"aligned"),
+    (dict(gb=AT), b"without a bias"),
+])
+def test_gradient_refuses(arguments, message):
+    assert gradient(**arguments) == -1
+    assert message in L.lbt_last_error()
+
+
+def test_workspaces_are_checked():
+    for call, grad in ((loss, 0), (gradient, 1)):
+        need = L.lbt_linear_log_loss_workspace_bytes(10, 8, 100, _lib.LBT_BF16, grad)
+        assert need > 0
+        assert call(ws=None) == -3 and b"workspace" in L.lbt_last_error()
+        assert call(ws=AT, size=need - 1) == -3 and str(need).encode() in L.lbt_last_error()
+        assert call(ws=ODD, size=BIG) == -3 and b"aligned" in L.lbt_last_error()
+
+
+def test_workspace_sizes():
+    q = L.lbt_linear_log_loss_workspace_bytes
+    assert q(10, 8, 100, _lib.LBT_F64, 0) == 0 and q(-1, 8, 100, _lib.LBT_BF16, 0) == 0 and q(10, 0, 100, _lib.LBT_BF16, 1) == 0
+    assert q(0, 8, 100, _lib.LBT_BF16, 1) > 0
+    for dtype in (_lib.LBT_BF16, _lib.LBT_F16, _lib.LBT_F32):
+        assert q(1000, 64, 5000, dtype, 0) <= q(1000, 64, 5000, dtype, 1)
+        # a piece of the gradient and one of packed weights take 512 MiB each at most, whatever the vocabulary
+        assert q(8192, 4096, 1 << 20, dtype, 1) < (4 << 30)
+    # the scores of 8192 rows and a million classes would take 32 GiB
+    assert q(8192, 1024, 1 << 20, _lib.LBT_BF16, 0) < (1 << 30)
+
+
+def test_no_rows_no_work():
+    assert loss(n=0, X=None, y=None, out=None) == 0
+    assert gradient(n=0, X=None, y=None, out=None, gx=None, weight=None) == -1
+
+
+def test_embed_refuses():
+    def rows(table=AT, dtype=_lib.LBT_F32, n=10, f=8, tokens=AT, width=8, t=5, out=AT):
+        return L.lbt_embed_rows(None, table, dtype, n, f, tokens, width, t, 1.0, out)
+
+    def grad(g=AT, dtype=_lib.LBT_F32, tokens=AT, width=8, t=5, f=8, n=10, add=0, out=AT, ws=AT, size=BIG):
+        return L.lbt_embed_rows_gradient(None, g, dtype, tokens, width, t, f, n, 1.0, add, out, ws, size)
+
+    for call in (rows, grad):
+        for arguments, message in ((dict(dtype=_lib.LBT_F64), b"dtype"), (dict(n=0), b"shape"), (dict(f=0), b"shape"),
+                                   (dict(t=-1), b"shape"), (dict(t=1 << 31), b"shape"), (dict(n=1 << 30, f=1 << 20), b"shape"),
+                                   (dict(width=2), b"tokens"), (dict(tokens=None), b"null"), (dict(out=None), b"null"),
+                                   (dict(out=ODD), b"aligned")):
+            assert call(**arguments) == -1, arguments
+            assert message in L.lbt_last_error(), arguments
+    assert rows(table=ODD) == -1 and rows(table=None) == -1
+    assert grad(g=ODD) == -1 and grad(g=None) == -1
+    assert rows(t=0, tokens=None, out=None) == 0
+    assert grad(t=0, add=1, g=None, tokens=None) == 0
+    need = L.lbt_embed_rows_gradient_workspace_bytes(5, 8, 10, _lib.LBT_F32)
+    assert need > 0 and grad(size=need - 1) == -3 and grad(ws=None) == -3 and grad(ws=ODD) == -3
+    assert L.lbt_embed_rows_gradient_workspace_bytes(5, 8, 10, _lib.LBT_F64) == 0
+    assert L.lbt_embed_rows_gradient_workspace_bytes(0, 8, 10, _lib.LBT_F32) > 0
