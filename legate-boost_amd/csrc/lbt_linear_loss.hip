@@ -560,8 +560,8 @@ __global__ void __launch_bounds__(256) clear_kernel(uint16_t* __restrict__ out, 
 
 // ---- host -----------------------------------------------------------------------------------------
 
-using LargeTile = ProductTile<256, 256, 2, 4>;
-using SmallTile = ProductTile<128, 128, 2, 2>;
+using LargeTile = ProductTile<256, 256, 2, 4, 2>;
+using SmallTile = ProductTile<128, 128, 2, 2, 2>;
 
 int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 int64_t tiles_of(int64_t v, int64_t by) { return (v + by - 1) / by; }

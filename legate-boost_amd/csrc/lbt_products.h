@@ -14,6 +14,8 @@
 // six that reach above 2^-24 of the result are added up, one walk over k each.
 #pragma once
 
+#include <type_traits>
+
 #include "lbt_internal.h"
 
 namespace lbt {
@@ -51,13 +53,16 @@ struct ProductArgs {
   const RowCounts* counts;
 };
 
-template <int kM, int kN, int kWaveM, int kWaveN>
+template <int kM, int kN, int kWaveM, int kWaveN, int kDepth>
 struct ProductTile {
   static constexpr int kBM = kM, kBN = kN;              // tile of a workgroup
   static constexpr int kWM = kM / kWaveM, kWN = kN / kWaveN;  // tile of a wave
   static constexpr int kWavesM = kWaveM, kWavesN = kWaveN;
   static constexpr int kWaves = kWaveM * kWaveN, kThreads = kWaves * 64;
   static constexpr int kMT = kWM / 32, kNT = kWN / 32;  // 32 x 32 blocks of a wave
+  static constexpr int kStages = kDepth;                // of the LDS
+  static constexpr int kStageA = kM * kProductK * 2, kStageB = kN * kProductK * 2;  // bytes
+  static constexpr int kLoads = (kM + kN) * kProductK / 8 / kThreads;               // of a lane for a stage
 };
 
 template <int kType>  // LBT_BF16 or LBT_F16
@@ -69,35 +74,76 @@ __device__ __forceinline__ Float16v mfma_32x32x16(Short8 a, Short8 b, Float16v c
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(Bf16x8, a), __builtin_bit_cast(Bf16x8, b), c, 0, 0, 0);
 }
 
-// Asks for the stage of one operand: kTile of its m (or n) from `tile0` on, 64 of its k from `k0` on.
-template <bool kRowsAreK, int kTile, int kWaves>
-__device__ __forceinline__ void load_stage(const ProductOperand& op, const uint16_t* base, int tile0, int k0,
-                                           const uint16_t* zeros, char* lds, int wave, int lane)
+// 16 bytes a lane from memory into the LDS, in the order of the lanes from `lds` on. The compiler's own form of this load is waited
+// for before the next read of the LDS, whichever part that reads; here the waits are those of wait_and_meet.
+__device__ __forceinline__ void load_to_lds(const void* base, uint32_t offset, uint32_t lds)
 {
-  constexpr int kChunks = kTile * kProductK / 8;  // of 16 bytes
-  static_assert(kChunks % (kWaves * 64) == 0, "every lane loads the same number of chunks");
-#pragma unroll
-  for (int j = 0; j < kChunks / (kWaves * 64); j++) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory");
+}
+__device__ __forceinline__ void load_to_lds(const void* from, uint32_t lds)
+{
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(from) : "memory");
+}
+
+// All but the last kLater loads of this wave have arrived, and all it has read from the LDS; then the same holds for every wave.
+template <int kLater>
+__device__ __forceinline__ void wait_and_meet()
+{
+  static_assert(kLater < 64, "the counter's range");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kLater) : "memory");
+}
+
+// Where a lane's chunks of a stage lie in an operand, relative to the stage's first element.
+template <bool kRowsAreK, int kTile, int kWaves>
+struct StageLoader {
+  static constexpr int kEach = kTile * kProductK / 8 / (kWaves * 64);  // chunks of 16 bytes
+  static_assert(kEach * kWaves * 64 * 8 == kTile * kProductK, "every lane loads the same number of chunks");
+  uint32_t offset[kEach];
+
+  static __device__ __forceinline__ void place(int j, int wave, int lane, int* row, int* col)
+  {
     const int q = (j * kWaves + wave) * 64 + lane;
-    const uint16_t* from;
-    bool inside;
     if constexpr (kRowsAreK) {
       constexpr int kRow = kTile / 8;  // chunks of a row
-      const int row = q / kRow;
-      const int col = ((q % kRow) ^ ((row & 3) << 2)) * 8;
-      inside = k0 + row < op.rows && tile0 + col < op.cols;
-      from   = base + static_cast<int64_t>(k0 + row) * op.ld + (tile0 + col);
+      *row = q / kRow;
+      *col = ((q % kRow) ^ ((*row & 3) << 2)) * 8;
     } else {
-      const int row = q >> 3;
-      const int col = ((q & 7) ^ (row & 7)) * 8;
-      inside = tile0 + row < op.rows && k0 + col < op.cols;
-      from   = base + static_cast<int64_t>(tile0 + row) * op.ld + (k0 + col);
+      *row = q >> 3;
+      *col = ((q & 7) ^ (*row & 7)) * 8;
     }
-    from = inside ? from : zeros;
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
-                                     (__attribute__((address_space(3))) void*)(lds + (j * kWaves + wave) * 1024), 16, 0, 0);
   }
-}
+  __device__ __forceinline__ void init(const ProductOperand& op, int wave, int lane)
+  {
+#pragma unroll
+    for (int j = 0; j < kEach; j++) {
+      int row, col;
+      place(j, wave, lane, &row, &col);
+      offset[j] = (static_cast<uint32_t>(row) * static_cast<uint32_t>(op.ld) + col) * 2;
+    }
+  }
+  // Asks for kTile of its m (or n) from `tile0` on, 64 of its k from `k0` on; stages that reach past the operand, or past the
+  // product's end (not `live`), take zeros there.
+  __device__ __forceinline__ void load(const ProductOperand& op, const uint16_t* plane, int tile0, int k0, bool live,
+                                       const uint16_t* zeros, uint32_t lds, int wave, int lane) const
+  {
+    const int row0 = kRowsAreK ? k0 : tile0, col0 = kRowsAreK ? tile0 : k0;
+    constexpr int kRows = kRowsAreK ? kProductK : kTile, kCols = kRowsAreK ? kTile : kProductK;
+    const uint16_t* base = plane + static_cast<int64_t>(row0) * op.ld + col0;
+    if (live && row0 + kRows <= op.rows && col0 + kCols <= op.cols) {
+#pragma unroll
+      for (int j = 0; j < kEach; j++) load_to_lds(base, offset[j], lds + (j * kWaves + wave) * 1024);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kEach; j++) {
+        int row, col;
+        place(j, wave, lane, &row, &col);
+        const bool inside   = live && row0 + row < op.rows && col0 + col < op.cols;
+        const uint16_t* from = base + static_cast<int64_t>(row) * op.ld + col;
+        load_to_lds(inside ? from : zeros, lds + (j * kWaves + wave) * 1024);
+      }
+    }
+  }
+};
 
 // Eight values of k for each of 32 values of m (or n) from `first` on: lane l has m = l % 32, k = 16 kk + 8 (l / 32) ...
 template <bool kRowsAreK, int kTile>
@@ -157,8 +203,8 @@ enum { kRowsN = 0, kRowsK = 1 };
 template <class Tile, int kType, int kPlanes, bool kAMajor, bool kBMajor, int kRowsSide, class Epilogue>
 __global__ void __launch_bounds__(Tile::kThreads, 1) product_kernel(const ProductArgs args, const Epilogue epilogue)
 {
-  constexpr int kStageA = Tile::kBM * kProductK * 2, kStageB = Tile::kBN * kProductK * 2;
-  __shared__ __attribute__((aligned(1024))) char lds[2 * (kStageA + kStageB)];
+  constexpr int kStage = Tile::kStageA + Tile::kStageB, kSteps = kProductK / 16;
+  __shared__ __attribute__((aligned(1024))) char lds[Tile::kStages * kStage];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   int tile_m, tile_n;
   tile_of_block(blockIdx.x, args.tiles_m, args.tiles_n, &tile_m, &tile_n);
@@ -180,35 +226,66 @@ __global__ void __launch_bounds__(Tile::kThreads, 1) product_kernel(const Produc
       for (int e = 0; e < 16; e++) acc[i][j][e] = 0.f;
 
   const int total = steps * PlanePairs<kPlanes>::kCount;
-  auto load       = [&](int t, int stage) {
-    const int pair = kPlanes == 1 ? 0 : t / steps;
-    const int k0   = k_first + (kPlanes == 1 ? t : t % steps) * kProductK;
-    char* at       = lds + stage * (kStageA + kStageB);
-    load_stage<kAMajor, Tile::kBM, Tile::kWaves>(args.a, args.a.base + PlanePairs<kPlanes>::a(pair) * args.a.plane,
-                                                 tile_m * Tile::kBM, k0, args.zeros, at, wave, lane);
-    load_stage<kBMajor, Tile::kBN, Tile::kWaves>(args.b, args.b.base + PlanePairs<kPlanes>::b(pair) * args.b.plane,
-                                                 tile_n * Tile::kBN, k0, args.zeros, at + kStageA, wave, lane);
+  StageLoader<kAMajor, Tile::kBM, Tile::kWaves> load_a;
+  StageLoader<kBMajor, Tile::kBN, Tile::kWaves> load_b;
+  load_a.init(args.a, wave, lane);
+  load_b.init(args.b, wave, lane);
+  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds));
+  // (one operand of stage t of the product, to where `stage` lies)
+  auto load = [&](int t, int stage, auto second) {
+    const int pair  = kPlanes == 1 ? 0 : t / max(steps, 1);
+    const int k0    = k_first + (kPlanes == 1 ? t : t % max(steps, 1)) * kProductK;
+    const bool live = t < total;
+    const uint32_t at = lds0 + stage * kStage;
+    if constexpr (decltype(second)::value)
+      load_b.load(args.b, args.b.base + PlanePairs<kPlanes>::b(pair) * args.b.plane, tile_n * Tile::kBN, k0, live, args.zeros,
+                  at + Tile::kStageA, wave, lane);
+    else
+      load_a.load(args.a, args.a.base + PlanePairs<kPlanes>::a(pair) * args.a.plane, tile_m * Tile::kBM, k0, live, args.zeros,
+                  at, wave, lane);
   };
-  if (total > 0) load(0, 0);
-  for (int t = 0; t < total; t++) {
-    __syncthreads();  // this stage has arrived, and the one before it has been read by all
-    if (t + 1 < total) load(t + 1, (t + 1) & 1);
-    const char* at = lds + (t & 1) * (kStageA + kStageB);
+  constexpr std::false_type kA{};
+  constexpr std::true_type kB{};
+  Short8 a[2][Tile::kMT], b[2][Tile::kNT];
+  // The i-th part of the fragments of a step: one of each operand.
+  auto read = [&](const char* at, int kk, int to, int i) {
+    if (i < Tile::kMT) a[to][i] = fragment<kAMajor, Tile::kBM>(at, wm * Tile::kWM + i * 32, kk, lane);
+    if (i < Tile::kNT) b[to][i] = fragment<kBMajor, Tile::kBN>(at + Tile::kStageA, wn * Tile::kWN + i * 32, kk, lane);
+  };
+  // Stages are asked for kStages ahead. The fragments of a step are read while the step before is multiplied; those of a stage's
+  // first step while the last one of the stage before is, after all waves have met: then that stage has been read by all,
+  // and is filled again, and the next has arrived. Reads and loads are dealt out between the multiplications.
 #pragma unroll
-    for (int kk = 0; kk < kProductK / 16; kk++) {
-      Short8 a[Tile::kMT], b[Tile::kNT];
-#pragma unroll
-      for (int i = 0; i < Tile::kMT; i++) a[i] = fragment<kAMajor, Tile::kBM>(at, wm * Tile::kWM + i * 32, kk, lane);
-#pragma unroll
-      for (int j = 0; j < Tile::kNT; j++)
-        b[j] = fragment<kBMajor, Tile::kBN>(at + kStageA, wn * Tile::kWN + j * 32, kk, lane);
-#pragma unroll
-      for (int i = 0; i < Tile::kMT; i++)
-#pragma unroll
-        for (int j = 0; j < Tile::kNT; j++) acc[i][j] = mfma_32x32x16<kType>(a[i], b[j], acc[i][j]);
-    }
+  for (int s = 0; s < Tile::kStages; s++) {
+    load(s, s, kA);
+    load(s, s, kB);
   }
-  __syncthreads();  // the LDS is free for what follows
+  wait_and_meet<(Tile::kStages - 1) * Tile::kLoads>();
+  static_assert(Tile::kMT >= Tile::kNT, "the parts of a step are those of the first operand");
+#pragma unroll
+  for (int i = 0; i < Tile::kMT; i++) read(lds, 0, 0, i);
+  int stage = 0;
+  for (int t = 0; t < total; t++) {
+    const int next = stage + 1 == Tile::kStages ? 0 : stage + 1;
+#pragma unroll
+    for (int kk = 0; kk < kSteps; kk++) {
+      const bool last = kk + 1 == kSteps;
+      if (last) wait_and_meet<(Tile::kStages - 2) * Tile::kLoads>();
+#pragma unroll
+      for (int i = 0; i < Tile::kMT; i++) {
+        if (last) read(lds + next * kStage, 0, 0, i);
+        else read(lds + stage * kStage, kk + 1, (kk + 1) & 1, i);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < Tile::kNT; j++) acc[i][j] = mfma_32x32x16<kType>(a[kk & 1][i], b[kk & 1][j], acc[i][j]);
+        __builtin_amdgcn_sched_barrier(0);
+        if (last && i == 0) load(t + Tile::kStages, stage, kA);
+        if (last && i == Tile::kMT / 2) load(t + Tile::kStages, stage, kB);
+      }
+    }
+    stage = next;
+  }
+  wait_and_meet<0>();  // the LDS is free for what follows
   epilogue.template store<Tile>(acc, tile_m, tile_n, wm, wn, lane, rows, args.counts, lds);
 }
 
