@@ -514,6 +514,202 @@ __global__ void __launch_bounds__(kJoinRows * kJoinSlices)
   loss[rows.order[row]] = none ? INFINITY : (from - rows.picked[row]) + logf(total);
 }
 
+// ---- few rows -----------------------------------------------------------------------------------------
+//
+// A score of few rows is bound by reading the weights once. Each wave takes 16 classes, 16 bytes of a class a lane, straight from
+// memory into the operand of a 16 x 16 product, with up to four blocks of 16 rows beside it (they are read over and over, from the
+// L1): there is no stage in the LDS to wait for and nothing is laid out first. The order of k within 16 lanes' chunks is the same
+// for both operands, which is all a product asks of it. float goes to the float products of the matrix cores as it is. Rows are not
+// taken out: what a row that does not count holds stays in its own column.
+// kShared: the four waves of a workgroup share out k instead of taking 16 classes each, where the classes would give the CUs too
+// few waves to keep memory busy.
+
+typedef __attribute__((ext_vector_type(4))) float Float4v;
+
+constexpr int kFewThreads = 256, kFewRows = 64;
+
+template <int kDtype>
+struct FewStep {  // 16 bytes of a row: kValues of k
+  static constexpr int kValues = kDtype == LBT_F32 ? 4 : 8;
+  using Value                  = typename LossType<kDtype>::Value;
+  uint4 bits;
+
+  __device__ __forceinline__ void load(const Value* row, int k) { __builtin_memcpy(&bits, row + k, 16); }
+  __device__ __forceinline__ void load_end(const Value* row, int k, int cols)
+  {
+    Value v[kValues];
+#pragma unroll
+    for (int e = 0; e < kValues; e++) v[e] = k + e < cols ? row[k + e] : Value(0);
+    __builtin_memcpy(&bits, v, 16);
+  }
+  static __device__ __forceinline__ Float4v multiply(const FewStep& a, const FewStep& b, Float4v c)
+  {
+    if constexpr (kDtype == LBT_F32) {
+      const Float4v x = __builtin_bit_cast(Float4v, a.bits), y = __builtin_bit_cast(Float4v, b.bits);
+#pragma unroll
+      for (int e = 0; e < 4; e++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], y[e], c, 0, 0, 0);
+      return c;
+    } else if constexpr (kDtype == LBT_F16) {
+      return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(Half8, a.bits), __builtin_bit_cast(Half8, b.bits), c, 0, 0, 0);
+    } else {
+      return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(Bf16x8, a.bits), __builtin_bit_cast(Bf16x8, b.bits), c, 0, 0, 0);
+    }
+  }
+};
+
+template <int kDtype, int kBlocks, bool kShared>
+__global__ void __launch_bounds__(kFewThreads)
+  few_rows_kernel(const void* __restrict__ X, const void* __restrict__ weight, const float* __restrict__ bias,
+                  const int64_t* __restrict__ y, int n_rows, int cols, int n_classes, int tiles, float2* __restrict__ partial,
+                  float* __restrict__ picked)
+{
+  using S = FewStep<kDtype>;
+  using V = typename S::Value;
+  constexpr bool kExact = kDtype == LBT_F32;
+  constexpr int kWaves = kFewThreads / 64, kUnroll = kBlocks >= 4 ? 2 : 4, kStep = 4 * S::kValues;  // k of a product
+  __shared__ float4 sums[kShared ? kWaves * kBlocks * 64 : 1];
+  __shared__ float2 share[kWaves][16 * kBlocks];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c0 = blockIdx.x * (kShared ? 16 : 64) + (kShared ? 0 : wave * 16);  // of this wave
+  const V* w   = static_cast<const V*>(weight) + static_cast<int64_t>(min(c0 + (lane & 15), n_classes - 1)) * cols;
+  const V* x[kBlocks];
+#pragma unroll
+  for (int b = 0; b < kBlocks; b++)
+    x[b] = static_cast<const V*>(X) + static_cast<int64_t>(min(b * 16 + (lane & 15), n_rows - 1)) * cols;
+  const int at  = (lane >> 4) * S::kValues;
+  const int hop = kShared ? kWaves * kUnroll * kStep : kUnroll * kStep;  // k of a turn, from wave to wave
+  Float4v acc[kBlocks];
+#pragma unroll
+  for (int b = 0; b < kBlocks; b++) acc[b] = Float4v{0.f, 0.f, 0.f, 0.f};
+  int k = kShared ? wave * kUnroll * kStep : 0;
+  S a[kUnroll], m[kBlocks][kUnroll];
+  auto load = [&](int from) {
+#pragma unroll
+    for (int u = 0; u < kUnroll; u++) {
+      a[u].load(w, from + u * kStep + at);
+#pragma unroll
+      for (int b = 0; b < kBlocks; b++) m[b][u].load(x[b], from + u * kStep + at);
+    }
+  };
+  bool whole = k + kUnroll * kStep <= cols;
+  if (whole) load(k);
+  while (whole) {  // the next turn is asked for before this one is multiplied
+    S a1[kUnroll], m1[kBlocks][kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; u++) {
+      a1[u] = a[u];
+#pragma unroll
+      for (int b = 0; b < kBlocks; b++) m1[b][u] = m[b][u];
+    }
+    k += hop;
+    whole = k + kUnroll * kStep <= cols;
+    if (whole) load(k);
+#pragma unroll
+    for (int u = 0; u < kUnroll; u++)
+#pragma unroll
+      for (int b = 0; b < kBlocks; b++) acc[b] = S::multiply(a1[u], m1[b][u], acc[b]);
+  }
+  for (int u = 0; u < kUnroll && k + u * kStep < cols; u++) {  // the end of the rows
+    S e, f;
+    e.load_end(w, k + u * kStep + at, cols);
+#pragma unroll
+    for (int b = 0; b < kBlocks; b++) {
+      f.load_end(x[b], k + u * kStep + at, cols);
+      acc[b] = S::multiply(e, f, acc[b]);
+    }
+  }
+  if constexpr (kShared) {
+#pragma unroll
+    for (int b = 0; b < kBlocks; b++) sums[(wave * kBlocks + b) * 64 + lane] = make_float4(acc[b][0], acc[b][1], acc[b][2], acc[b][3]);
+    __syncthreads();
+  }
+#pragma unroll
+  for (int b = 0; b < kBlocks; b++) {  // lane: row lane % 16, classes 4 (lane / 16) ...
+    if constexpr (kShared) {
+      if (b % kWaves != wave) continue;
+      float4 t = sums[b * 64 + lane];
+      for (int v = 1; v < kWaves; v++) {
+        const float4 o = sums[(v * kBlocks + b) * 64 + lane];
+        t.x += o.x; t.y += o.y; t.z += o.z; t.w += o.w;
+      }
+      acc[b] = Float4v{t.x, t.y, t.z, t.w};
+    }
+    const int r     = b * 16 + (lane & 15);
+    const int first = c0 + 4 * (lane >> 4);
+    const int64_t label = r < n_rows ? y[r] : -1;
+    float top = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const int c = first + e;
+      acc[b][e]   = c < n_classes ? acc[b][e] + (bias != nullptr ? bias[c] : 0.f) : -INFINITY;
+      if (c == label && c < n_classes) picked[r] = acc[b][e];
+      top = fmaxf(top, acc[b][e]);
+    }
+    top = fmaxf(top, __shfl_xor(top, 16));
+    top = fmaxf(top, __shfl_xor(top, 32));
+    const float from = top == -INFINITY ? 0.f : top;
+    float total      = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; e++) total += exp_of(acc[b][e] - from, kExact);
+    total += __shfl_xor(total, 16);
+    total += __shfl_xor(total, 32);
+    if constexpr (kShared) {
+      if (lane < 16 && r < n_rows) partial[static_cast<int64_t>(r) * tiles + blockIdx.x] = make_float2(top, total);
+    } else {
+      if (lane < 16) share[wave][b * 16 + lane] = make_float2(top, total);
+    }
+  }
+  if constexpr (!kShared) {
+    __syncthreads();
+    const int r = threadIdx.x;
+    if (r >= n_rows || r >= 16 * kBlocks) return;
+    float top = share[0][r].x;
+    for (int v = 1; v < kWaves; v++) top = fmaxf(top, share[v][r].x);
+    const float from = top == -INFINITY ? 0.f : top;
+    float total      = 0.f;
+    for (int v = 0; v < kWaves; v++) total += share[v][r].y * exp_of(share[v][r].x - from, kExact);
+    partial[static_cast<int64_t>(r) * tiles + blockIdx.x] = make_float2(top, total);
+  }
+}
+
+// Top and total of a row from its shares, by a workgroup: [rows][tiles].
+__device__ __forceinline__ float2 join_row(const float2* __restrict__ shares, int tiles)
+{
+  constexpr int kWaves = kFewThreads / 64;
+  __shared__ float2 by_wave[kWaves];
+  float top = -INFINITY;
+  for (int t = threadIdx.x; t < tiles; t += kFewThreads) top = fmaxf(top, shares[t].x);
+  for (int s = 32; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor(top, s));
+  if ((threadIdx.x & 63) == 0) by_wave[threadIdx.x >> 6].x = top;
+  __syncthreads();
+  for (int v = 0; v < kWaves; v++) top = fmaxf(top, by_wave[v].x);
+  const float from = top == -INFINITY ? 0.f : top;
+  float total      = 0.f;
+  for (int t = threadIdx.x; t < tiles; t += kFewThreads) total += shares[t].y * expf(shares[t].x - from);
+  for (int s = 32; s > 0; s >>= 1) total += __shfl_xor(total, s);
+  if ((threadIdx.x & 63) == 0) by_wave[threadIdx.x >> 6].y = total;
+  __syncthreads();
+  total = 0.f;
+  for (int v = 0; v < kWaves; v++) total += by_wave[v].y;
+  return make_float2(top, total);
+}
+
+__device__ __forceinline__ float loss_of(float2 s, float picked)
+{
+  if (s.x == -INFINITY && s.y == 0.f) return INFINITY;  // every class is masked
+  return ((s.x == -INFINITY ? 0.f : s.x) - picked) + logf(s.y);
+}
+
+__global__ void __launch_bounds__(kFewThreads)
+  join_few_kernel(const float2* __restrict__ partial, int tiles, const float* __restrict__ picked, const int64_t* __restrict__ y,
+                  int n_classes, float* __restrict__ loss)
+{
+  const int r     = blockIdx.x;
+  const float2 s  = join_row(partial + static_cast<int64_t>(r) * tiles, tiles);
+  const int64_t l = y[r];
+  if (threadIdx.x == 0) loss[r] = l >= 0 && l < n_classes ? loss_of(s, picked[r]) : 0.f;
+}
+
 // grad_X from its sums over the splits; zeros for rows that do not count.
 template <int kDtype>
 __global__ void __launch_bounds__(256)
@@ -560,14 +756,38 @@ __global__ void __launch_bounds__(256) clear_kernel(uint16_t* __restrict__ out, 
 
 // ---- host -----------------------------------------------------------------------------------------
 
-using LargeTile = ProductTile<256, 256, 2, 4, 2>;
-using SmallTile = ProductTile<128, 128, 2, 2, 2>;
+using LargeTile  = ProductTile<256, 256, 2, 4, 2>;
+using MediumTile = ProductTile<128, 128, 2, 2, 2>;
+using SmallTile  = ProductTile<64, 64, 2, 2, 4>;
 
 int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 int64_t tiles_of(int64_t v, int64_t by) { return (v + by - 1) / by; }
 
-// Tiles of 256 x 256 where they give every CU one, else of 128 x 128.
-bool large_tiles(int64_t m, int64_t n) { return tiles_of(m, 256) * tiles_of(n, 256) >= 256; }
+// How a product of m x n over `stages` stages of k is cut: tiles of 256, 128 or 64, and k into splits. A CU's time is that of its
+// share of the tiles; a stage takes it 1.72 us, 0.5 and 0.2 (two workgroups at a time; 0.7 and 0.35 where it has only one, which
+// then waits for memory), and a tile 8, 3 and 2 us to begin and end. Each split adds a pass over the sums.
+struct Cut {
+  int tile, splits;
+};
+Cut cut_product(int64_t m, int64_t n, int64_t stages, int64_t most_splits)
+{
+  constexpr int kCus = 256;
+  constexpr struct { int tile; double stage, lone, ends; } kTiles[3] = {{256, 1.72, 1.72, 8.0}, {128, 0.5, 0.7, 3.0}, {64, 0.2, 0.35, 2.0}};
+  Cut best{256, 1};
+  double least = 1e30;
+  for (const auto& t : kTiles)
+    for (int splits = 1; splits <= 16; splits *= 2) {
+      if (splits > 1 && (splits > most_splits || stages / splits < 4)) break;
+      const int64_t each = tiles_of(tiles_of(m, t.tile) * tiles_of(n, t.tile) * splits, kCus);
+      const double time  = each * (tiles_of(stages, splits) * (each == 1 ? t.lone : t.stage) + t.ends) +
+                          (splits - 1) * (1.0 + m * n * 8e-6 / 4.0);
+      if (time < least) {
+        least = time;
+        best  = {t.tile, splits};
+      }
+    }
+  return best;
+}
 
 struct LossCall {
   int64_t n_rows;
@@ -578,7 +798,7 @@ struct LossCall {
   int cols;         // features, padded
   bool packed;      // the weights are laid out piece by piece before they are multiplied
   int64_t piece;    // classes at a time
-  int splits;       // of the classes in the products for grad_X
+  Cut all_scores, scores, row_product, class_product;
   LossRows rows;
   RowCounts* counts;
   uint16_t *zeros, *x, *x_scaled, *weight, *g;
@@ -597,10 +817,11 @@ struct LossCall {
     if (packed) most = std::min(most, kPieceBytes / (2 * planes * int64_t(cols)) / 256 * 256);
     most  = std::max<int64_t>(most, 256);
     piece = round_up(tiles_of(k, tiles_of(k, most)), 256);
-    // grad_X has features / 256 x rows / 256 tiles: too few for 256 CUs unless the classes are split
-    const bool large    = large_tiles(f, n);
-    const int64_t tiles = large ? tiles_of(f, 256) * tiles_of(n, 256) : tiles_of(f, 128) * tiles_of(n, 128);
-    splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({512 / tiles, piece / 512, 16})));
+    const int64_t pairs = type == LBT_F32 ? 6 : 1;
+    scores      = cut_product(std::min<int64_t>(piece, k), n, pairs * cols / kProductK, 1);
+    all_scores  = packed ? scores : cut_product(k, n, pairs * cols / kProductK, 1);
+    row_product = cut_product(f, n, pairs * piece / kProductK, 16);
+    class_product = cut_product(f, std::min<int64_t>(piece, k), pairs * padded / kProductK, 1);
   }
 
   template <typename A>
@@ -617,15 +838,15 @@ struct LossCall {
     rows.top      = arena.template take<float>(padded);
     rows.inverse  = arena.template take<float>(padded);
     x             = arena.template take<uint16_t>(planes * padded * cols);
-    partial       = arena.template take<float2>(tiles_of(classes, 128) * padded);
+    partial       = arena.template take<float2>((tiles_of(classes, all_scores.tile) + tiles_of(classes, piece)) * padded);
     weight = x_scaled = g = nullptr;
     row_sums = bias_sums = nullptr;
     if (packed) weight = arena.template take<uint16_t>(planes * piece * cols);
     if (!gradient) return;
     if (dtype == LBT_F16) x_scaled = arena.template take<uint16_t>(padded * cols);
     g         = arena.template take<uint16_t>(planes * padded * piece);
-    row_sums  = arena.template take<float>(splits * padded * cols);
-    bias_sums = arena.template take<float>(tiles_of(padded, 128) * classes);
+    row_sums  = arena.template take<float>(row_product.splits * padded * cols);
+    bias_sums = arena.template take<float>(tiles_of(padded, scores.tile) * classes);
   }
 };
 
@@ -643,10 +864,11 @@ int launch_tiles(hipStream_t s, ProductArgs args, int64_t m, int64_t n, int spli
 }
 
 template <class L, bool kAMajor, bool kBMajor, int kRowsSide, class Epilogue>
-int launch_product(hipStream_t s, const ProductArgs& args, int64_t m, int64_t n, int splits, const Epilogue& e)
+int launch_product(hipStream_t s, const ProductArgs& args, int64_t m, int64_t n, Cut cut, const Epilogue& e)
 {
-  if (large_tiles(m, n)) return launch_tiles<LargeTile, L, kAMajor, kBMajor, kRowsSide>(s, args, m, n, splits, e);
-  return launch_tiles<SmallTile, L, kAMajor, kBMajor, kRowsSide>(s, args, m, n, splits, e);
+  if (cut.tile == 256) return launch_tiles<LargeTile, L, kAMajor, kBMajor, kRowsSide>(s, args, m, n, cut.splits, e);
+  if (cut.tile == 128) return launch_tiles<MediumTile, L, kAMajor, kBMajor, kRowsSide>(s, args, m, n, cut.splits, e);
+  return launch_tiles<SmallTile, L, kAMajor, kBMajor, kRowsSide>(s, args, m, n, cut.splits, e);
 }
 
 template <int kDtype>
@@ -703,7 +925,6 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
 
   // top and total of each row; weights that are multiplied where they lie need no pieces here
   const int64_t step = c.packed ? c.piece : c.classes;
-  const int64_t by   = large_tiles(std::min<int64_t>(step, c.classes), c.n_rows) ? 256 : 128;
   int64_t tiles      = 0;
   for (int64_t first = 0; first < c.classes; first += step) {
     const int64_t classes = std::min<int64_t>(step, c.classes - first);
@@ -713,9 +934,8 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
     args.k_extent = args.k_split = c.cols;
     const LossEpilogue<kFine> e{bias, static_cast<int>(first), c.classes, static_cast<int>(tiles), c.padded, c.rows, c.partial};
     // (every piece in tiles of one size: they share the numbering of `partial`)
-    LBT_TRY((by == 256 ? launch_tiles<LargeTile, L, false, false, kRowsN>(s, args, classes, c.n_rows, 1, e)
-                       : launch_tiles<SmallTile, L, false, false, kRowsN>(s, args, classes, c.n_rows, 1, e)));
-    tiles += tiles_of(classes, by);
+    LBT_TRY((launch_product<L, false, false, kRowsN>(s, args, classes, c.n_rows, c.all_scores, e)));
+    tiles += tiles_of(classes, c.all_scores.tile);
   }
   join_kernel<<<static_cast<unsigned>(tiles_of(c.n_rows, kJoinRows)), kJoinRows * kJoinSlices, 0, s>>>(
     c.partial, static_cast<int>(tiles), c.padded, c.rows, c.counts, loss);
@@ -728,7 +948,6 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
   ProductOperand x_scaled = x;
   if (scaled) x_scaled.base = c.x_scaled;
   const ProductOperand g{c.g, c.piece, c.padded * c.piece, static_cast<int32_t>(c.padded), static_cast<int32_t>(c.piece)};
-  const int64_t bias_tile = large_tiles(std::min<int64_t>(c.piece, c.classes), c.n_rows) ? 256 : 128;
   for (int64_t first = 0; first < c.classes; first += c.piece) {
     const int64_t classes = std::min<int64_t>(c.piece, c.classes - first);
     if (first > 0 || c.piece < c.classes) LBT_TRY(lay_out(first));
@@ -740,32 +959,70 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
                                                               c.rows, c.g, c.padded * c.piece,
                                                               grad_bias != nullptr ? c.bias_sums : nullptr};
     // (over the whole piece: what lies past its classes is written as zeros)
-    LBT_TRY((bias_tile == 256 ? launch_tiles<LargeTile, L, false, false, kRowsN>(s, args, c.piece, c.n_rows, 1, ge)
-                              : launch_tiles<SmallTile, L, false, false, kRowsN>(s, args, c.piece, c.n_rows, 1, ge)));
+    LBT_TRY((launch_product<L, false, false, kRowsN>(s, args, c.piece, c.n_rows, c.scores, ge)));
     args.a        = w;
     args.b        = g;
     args.k_extent = static_cast<int32_t>(c.piece);
-    args.k_split  = static_cast<int32_t>(round_up(tiles_of(c.piece, c.splits), kProductK));
+    args.k_split  = static_cast<int32_t>(round_up(tiles_of(c.piece, c.row_product.splits), kProductK));
     const RowsEpilogue re{c.row_sums, c.padded * c.cols, c.cols, first == 0};
-    LBT_TRY((launch_product<L, true, false, kRowsN>(s, args, c.features, c.n_rows, c.splits, re)));
+    LBT_TRY((launch_product<L, true, false, kRowsN>(s, args, c.features, c.n_rows, c.row_product, re)));
     args.a        = x_scaled;
     args.b        = g;
     args.k_extent = args.k_split = static_cast<int32_t>(c.padded);
     const ClassesEpilogue<kDtype> ce{grad_weight, static_cast<int>(first), c.classes, c.features, scaled};
-    LBT_TRY((launch_product<L, true, true, kRowsK>(s, args, c.features, classes, 1, ce)));
+    LBT_TRY((launch_product<L, true, true, kRowsK>(s, args, c.features, classes, c.class_product, ce)));
   }
   const int64_t blocks = tiles_of(c.n_rows * ((c.features + 3) / 4), 256);
   LBT_REQUIRE(blocks < (int64_t(1) << 31), "too many values");
-  finish_rows_kernel<kDtype><<<static_cast<unsigned>(blocks), 256, 0, s>>>(c.row_sums, c.splits, c.padded * c.cols, c.cols,
+  finish_rows_kernel<kDtype><<<static_cast<unsigned>(blocks), 256, 0, s>>>(c.row_sums, c.row_product.splits, c.padded * c.cols, c.cols,
                                                                            c.n_rows, c.features, c.rows, grad_X);
   LBT_HIP(hipGetLastError());
   if (grad_bias != nullptr) {
     finish_bias_kernel<<<static_cast<unsigned>(tiles_of(c.classes, 256)), 256, 0, s>>>(c.bias_sums, c.classes,
-                                                                                       static_cast<int>(bias_tile), c.counts, kHalf,
+                                                                                       c.scores.tile, c.counts, kHalf,
                                                                                        grad_bias);
     LBT_HIP(hipGetLastError());
   }
   return LBT_OK;
+}
+
+// Workgroups of the scores of few rows; four waves share the classes of one where they would be fewer than four a CU.
+bool few_shared(int classes) { return classes < 65536; }
+int64_t few_tiles(int classes) { return tiles_of(classes, few_shared(classes) ? 16 : 64); }
+
+struct FewCall {
+  float2* partial;
+  float* picked;
+  void carve(Arena& arena, int64_t n_rows, int classes)
+  {
+    partial = arena.take<float2>(n_rows * few_tiles(classes));
+    picked  = arena.take<float>(n_rows);
+  }
+};
+
+template <int kDtype, int kBlocks>
+int few_log_loss(hipStream_t s, const FewCall& c, const void* X, const void* weight, const float* bias, const int64_t* y, int n_rows,
+                 int features, int classes, float* loss)
+{
+  const int tiles = static_cast<int>(few_tiles(classes));
+  if (few_shared(classes))
+    few_rows_kernel<kDtype, kBlocks, true>
+      <<<tiles, kFewThreads, 0, s>>>(X, weight, bias, y, n_rows, features, classes, tiles, c.partial, c.picked);
+  else
+    few_rows_kernel<kDtype, kBlocks, false>
+      <<<tiles, kFewThreads, 0, s>>>(X, weight, bias, y, n_rows, features, classes, tiles, c.partial, c.picked);
+  join_few_kernel<<<n_rows, kFewThreads, 0, s>>>(c.partial, tiles, c.picked, y, classes, loss);
+  LBT_HIP(hipGetLastError());
+  return LBT_OK;
+}
+
+template <int kDtype>
+int few_log_loss(hipStream_t s, const FewCall& c, const void* X, const void* weight, const float* bias, const int64_t* y, int n_rows,
+                 int features, int classes, float* loss)
+{
+  if (n_rows <= 16) return few_log_loss<kDtype, 1>(s, c, X, weight, bias, y, n_rows, features, classes, loss);
+  if (n_rows <= 32) return few_log_loss<kDtype, 2>(s, c, X, weight, bias, y, n_rows, features, classes, loss);
+  return few_log_loss<kDtype, 4>(s, c, X, weight, bias, y, n_rows, features, classes, loss);
 }
 
 bool loss_shape(int64_t n_rows, int32_t n_features, int32_t n_outputs, int32_t dtype)
@@ -795,16 +1052,25 @@ int run_loss(void* stream, const void* X, const void* weight, int32_t dtype, int
     return LBT_ERR_WORKSPACE;
   }
   LossCall c(std::max<int64_t>(n_rows, 1), n_features, n_outputs, dtype, gradient);
-  c.n_rows = n_rows;
+  c.n_rows       = n_rows;
+  const bool few = !gradient && n_rows <= kFewRows;
+  FewCall f;
   Arena arena;
   arena.base = static_cast<char*>(workspace);
   arena.cap  = workspace_bytes;
-  c.carve(arena);
+  if (few) f.carve(arena, n_rows, n_outputs);
+  else c.carve(arena);
   if (arena.failed) {
     set_error("workspace of %zu bytes, %zu needed", workspace_bytes, arena.used);
     return LBT_ERR_WORKSPACE;
   }
   ProfScope ps(LBT_PROF_OTHER, s);
+  if (few) {
+    const int n = static_cast<int>(n_rows);
+    if (dtype == LBT_BF16) return few_log_loss<LBT_BF16>(s, f, X, weight, bias, y, n, n_features, n_outputs, loss);
+    if (dtype == LBT_F16) return few_log_loss<LBT_F16>(s, f, X, weight, bias, y, n, n_features, n_outputs, loss);
+    return few_log_loss<LBT_F32>(s, f, X, weight, bias, y, n, n_features, n_outputs, loss);
+  }
   switch (dtype) {
     case LBT_BF16:
       return linear_log_loss<LBT_BF16>(s, c, X, weight, bias, y, sample_weight, loss, grad_X, grad_weight, grad_bias);
@@ -826,6 +1092,11 @@ size_t lbt_linear_log_loss_workspace_bytes(int64_t n_rows, int32_t n_features, i
   lbt::LossCall c(std::max<int64_t>(n_rows, 1), n_features, n_outputs, dtype, gradient != 0);
   lbt::Arena arena;
   arena.measure = true;
+  if (gradient == 0 && n_rows <= lbt::kFewRows) {
+    lbt::FewCall f;
+    f.carve(arena, n_rows, n_outputs);
+    return std::max<size_t>(arena.used, 256);
+  }
   c.carve(arena);
   return arena.used;
 }

@@ -93,6 +93,14 @@ __device__ __forceinline__ void wait_and_meet()
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kLater) : "memory");
 }
 
+// What the number of a chunk in a row of k is turned by, within the row's kTile / 8 chunks: rows that are read together lie on
+// different banks, 64 bytes apart.
+template <int kTile>
+__device__ __forceinline__ int turned(int row)
+{
+  return (row & (kTile >= 128 ? 3 : 1)) << 2;
+}
+
 // Where a lane's chunks of a stage lie in an operand, relative to the stage's first element.
 template <bool kRowsAreK, int kTile, int kWaves>
 struct StageLoader {
@@ -106,7 +114,7 @@ struct StageLoader {
     if constexpr (kRowsAreK) {
       constexpr int kRow = kTile / 8;  // chunks of a row
       *row = q / kRow;
-      *col = ((q % kRow) ^ ((*row & 3) << 2)) * 8;
+      *col = ((q % kRow) ^ turned<kTile>(*row)) * 8;
     } else {
       *row = q >> 3;
       *col = ((q & 7) ^ (*row & 7)) * 8;
@@ -152,7 +160,7 @@ __device__ __forceinline__ Short8 fragment(const char* lds, int first, int kk, i
   if constexpr (kRowsAreK) {
     const int row   = kk * 16 + (lane >> 5) * 8 + ((lane & 15) >> 2);
     const int col   = first + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
-    const int chunk = (col >> 3) ^ ((row & 3) << 2);
+    const int chunk = (col >> 3) ^ turned<kTile>(row);
     const char* at  = lds + row * (kTile * 2) + chunk * 16 + (col & 7) * 2;
     typedef __attribute__((address_space(3))) Short4* LdsPtr;
     const Short4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)at);

@@ -119,8 +119,22 @@ def test_several_pieces_of_the_classes(dtype, n, f, k):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
-def test_rows_that_do_not_count(dtype):
-    n, f, k = 300, 72, 700
+@pytest.mark.parametrize("n,f,k", [(1, 1024, 5000), (16, 40, 33), (17, 1000, 700), (32, 2053, 70001), (33, 7, 90000), (64, 130, 66000),
+                                   (65, 130, 66000), (3, 4096, 10)])
+def test_loss_of_few_rows(n, f, k, dtype):
+    x, w, y = inputs(n, f, k, dtype, seed=n * f)
+    rs = np.random.RandomState(k)
+    for bias in (None, torch.from_numpy(np.where(rs.rand(k) < 0.1, -np.inf, rs.normal(0, 2, k))).float().cuda()):
+        if bias is not None:
+            bias[y] = 0.25
+        want, bounds = reference(x, w, y, bias)
+        assert_within(ops.linear_log_loss(x, w, y, bias=bias), want[0], bounds(dtype)[0], "loss")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("n", [300, 40])
+def test_rows_that_do_not_count(n, dtype):
+    f, k = 72, 700
     x, w, y = inputs(n, f, k, dtype, seed=11)
     y[::3] = -1
     y[1], y[4], y[7], y[10] = k, 2 ** 31, -2 ** 40, 2 ** 62
