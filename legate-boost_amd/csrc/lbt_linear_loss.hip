@@ -24,7 +24,8 @@ namespace lbt {
 namespace {
 
 constexpr int kHalfShift = 14;
-constexpr int64_t kPieceBytes = int64_t(512) << 20;  // of G, or of packed weights, at a time
+constexpr int64_t kPieceBytes  = int64_t(512) << 20;  // of packed weights at a time
+constexpr int64_t kScoresBytes = int64_t(2) << 30;    // of G (float: and of what it is made from) at a time
 
 template <int kDtype>
 struct LossType;
@@ -246,9 +247,10 @@ __global__ void __launch_bounds__(256)
           if (fabsf(x) < INFINITY) (void)frexpf(x, &own);
           if (x != 0.f) reach = max(reach, own - 1 + exponent[p]);
         }
-      // (rows of one wave: the lanes that are still here)
       for (int s = 32; s > 0; s >>= 1) reach = max(reach, __shfl_xor(reach, s));
-      if ((threadIdx.x & 63) == 0 && reach > -1000) atomicMax(&counts->reach, reach);
+      // (most waves find a larger one there already: they need not wait their turn for the atomic)
+      if ((threadIdx.x & 63) == 0 && reach > __hip_atomic_load(&counts->reach, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT))
+        atomicMax(&counts->reach, reach);
     } else if (mode == kScale) {
       const int shift = exponent[p] + kReach - counts->reach;
 #pragma unroll
@@ -281,55 +283,70 @@ __device__ __forceinline__ void add_bias(Float16v (&acc)[Tile::kMT][Tile::kNT], 
     }
 }
 
-// Each tile's share of the rows' tops and totals.
-template <bool kExact>
+// The shares of the rows' tops and totals: one of each row for the kWM classes of a wave. With kKeep also u = exp(s - the share's
+// top), [rows][piece], for scale_kernel: float, or half times 2^15 (2^-12 of a step below the type it is for, and no smaller
+// than 2^-29 with all its bits).
+constexpr float kKeptScale = 32768.f;
+template <bool kExact, bool kKeep>
 struct LossEpilogue {
   const float* bias;
   int class_first, n_classes;  // of this launch: number of its first class; classes of the call
-  int tile_first;
+  int share_first;
   int64_t padded;              // rows
   LossRows rows;
-  float2* partial;             // [tiles][padded]: top, total
+  float2* partial;             // [shares][padded]: top, total
+  void* kept;
+  int piece;
 
   template <class Tile>
   __device__ __forceinline__ void store(Float16v (&acc)[Tile::kMT][Tile::kNT], int tile_m, int tile_n, int wm, int wn, int lane,
-                                        int, const RowCounts*, char* lds) const
+                                        int, const RowCounts*, char*) const
   {
-    const int c0 = class_first + tile_m * Tile::kBM + wm * Tile::kWM;
+    const int in_piece = tile_m * Tile::kBM + wm * Tile::kWM;
+    const int c0       = class_first + in_piece;
     add_bias<Tile>(acc, bias, c0, n_classes, lane);
-    float2(*share)[Tile::kBN] = reinterpret_cast<float2(*)[Tile::kBN]>(lds);
 #pragma unroll
     for (int j = 0; j < Tile::kNT; j++) {
-      const int n         = wn * Tile::kWN + j * 32 + (lane & 31);
-      const int64_t row   = static_cast<int64_t>(tile_n) * Tile::kBN + n;
-      const int label     = rows.label[row] - c0;
-      float top           = -INFINITY;
+      const int64_t row = static_cast<int64_t>(tile_n) * Tile::kBN + wn * Tile::kWN + j * 32 + (lane & 31);
+      const int label   = rows.label[row] - c0;
+      if (__any(label >= 0 && label < Tile::kWM)) {
+#pragma unroll
+        for (int i = 0; i < Tile::kMT; i++)
+#pragma unroll
+          for (int e = 0; e < 16; e++)
+            if (i * 32 + block_m(e, lane) == label) rows.picked[row] = acc[i][j][e];
+      }
+      float top = -INFINITY;
 #pragma unroll
       for (int i = 0; i < Tile::kMT; i++)
 #pragma unroll
-        for (int e = 0; e < 16; e++) {
-          top = fmaxf(top, acc[i][j][e]);
-          if (i * 32 + block_m(e, lane) == label) rows.picked[row] = acc[i][j][e];
-        }
+        for (int e = 0; e < 16; e++) top = fmaxf(top, acc[i][j][e]);
       top              = fmaxf(top, __shfl_xor(top, 32));
       const float from = top == -INFINITY ? 0.f : top;
       float total      = 0.f;
 #pragma unroll
       for (int i = 0; i < Tile::kMT; i++)
 #pragma unroll
-        for (int e = 0; e < 16; e++) total += exp_of(acc[i][j][e] - from, kExact);
+        for (int q = 0; q < 4; q++) {
+          float u[4];
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            u[e] = exp_of(acc[i][j][q * 4 + e] - from, kExact);
+            total += u[e];
+          }
+          if constexpr (kKeep) {
+            const int64_t at = row * piece + in_piece + i * 32 + q * 8 + 4 * (lane >> 5);
+            if constexpr (kExact) {
+              *reinterpret_cast<float4*>(static_cast<float*>(kept) + at) = make_float4(u[0], u[1], u[2], u[3]);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 4; e++) u[e] *= kKeptScale;
+              store_four<LBT_F16>(kept, at, u, 4, true);
+            }
+          }
+        }
       total += __shfl_xor(total, 32);
-      if (lane < 32) share[wm][n] = make_float2(top, total);
-    }
-    __syncthreads();
-    for (int n = threadIdx.x; n < Tile::kBN; n += Tile::kThreads) {
-      float top = share[0][n].x;
-      for (int w = 1; w < Tile::kWavesM; w++) top = fmaxf(top, share[w][n].x);
-      const float from = top == -INFINITY ? 0.f : top;
-      float total      = 0.f;
-      for (int w = 0; w < Tile::kWavesM; w++) total += share[w][n].y * exp_of(share[w][n].x - from, kExact);
-      partial[static_cast<int64_t>(tile_first + tile_m) * padded + static_cast<int64_t>(tile_n) * Tile::kBN + n] =
-        make_float2(top, total);
+      if (lane < 32) partial[static_cast<int64_t>(share_first + tile_m * Tile::kWavesM + wm) * padded + row] = make_float2(top, total);
     }
   }
 };
@@ -476,6 +493,9 @@ struct ClassesEpilogue {
     }
   }
 };
+
+// The rows that tiles of rows reach: those that count, filled up.
+__device__ __forceinline__ int64_t round_up_rows(int counted) { return (static_cast<int64_t>(counted) + 255) / 256 * 256; }
 
 // ---- joins ----------------------------------------------------------------------------------------
 
@@ -710,6 +730,69 @@ __global__ void __launch_bounds__(kFewThreads)
   if (threadIdx.x == 0) loss[r] = l >= 0 && l < n_classes ? loss_of(s, picked[r]) : 0.f;
 }
 
+// G from what LossEpilogue kept, once the rows' tops and totals are known: p = u exp(top of the share - top) / total. A workgroup
+// takes 16 rows and 2048 classes; bound by memory, each value is read and written once (bfloat16: in the same place).
+constexpr int kScaleRows = 16, kScaleClasses = 2048;
+template <bool kFloat>
+__global__ void __launch_bounds__(256)
+  scale_kernel(const void* kept, const float2* __restrict__ partial, int share_classes, int64_t padded, LossRows rows,
+               const RowCounts* __restrict__ counts, int piece, int64_t plane, uint16_t* g)
+{
+  __shared__ float factor[kScaleRows][kScaleClasses / 32 + 1];
+  const int wides    = (piece + kScaleClasses - 1) / kScaleClasses;
+  const int64_t row0 = blockIdx.x / wides * int64_t(kScaleRows);
+  const int counted  = counts->rows;
+  if (row0 >= round_up_rows(counted)) return;
+  const int class0 = static_cast<int>(blockIdx.x % wides) * kScaleClasses, shares = kScaleClasses / share_classes, first = class0 / share_classes;
+  for (int i = threadIdx.x; i < kScaleRows * shares; i += 256) {
+    const int64_t row = row0 + i % kScaleRows;
+    const int s       = i / kScaleRows;
+    float f           = 0.f;
+    if (row < counted && class0 + s * share_classes < piece) {
+      const float top = partial[(first + s) * padded + row].x;
+      f = top == -INFINITY ? 0.f : exp_of(top - rows.top[row], kFloat) * rows.inverse[row] * (kFloat ? 1.f : 1.f / kKeptScale);
+    }
+    factor[i % kScaleRows][s] = f;
+  }
+  __syncthreads();
+  const int wide = min(kScaleClasses, piece - class0) / 8;  // groups of 8 classes
+  for (int i = threadIdx.x; i < kScaleRows * wide; i += 256) {
+    const int r = i / wide, c = (i % wide) * 8;
+    const int64_t row = row0 + r, at = row * piece + class0 + c;
+    const float f = factor[r][c / share_classes];
+    const float w = rows.factor[row];
+    const int label = rows.label[row] - (class0 + c);
+    float u[8];
+    if constexpr (kFloat) {
+      const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(kept) + at);
+      const float4 a = q[0], b = q[1];
+      u[0] = a.x; u[1] = a.y; u[2] = a.z; u[3] = a.w; u[4] = b.x; u[5] = b.y; u[6] = b.z; u[7] = b.w;
+    } else {
+      const Half8 h = *reinterpret_cast<const Half8*>(static_cast<const uint16_t*>(kept) + at);
+#pragma unroll
+      for (int e = 0; e < 8; e++) u[e] = static_cast<float>(h[e]);
+    }
+    uint16_t v[kFloat ? 3 : 1][8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      const float p = u[e] * f;
+      float d       = (e == label ? p - 1.f : p) * w;
+      d             = row < counted ? d : 0.f;
+      if constexpr (kFloat) {
+        uint16_t s[3];
+        split_planes(d, s);
+        v[0][e] = s[0];
+        v[1][e] = s[1];
+        v[2][e] = s[2];
+      } else {
+        v[0][e] = to_bf16(d);
+      }
+    }
+#pragma unroll
+    for (int l = 0; l < (kFloat ? 3 : 1); l++) *reinterpret_cast<uint4*>(g + l * plane + at) = *reinterpret_cast<const uint4*>(v[l]);
+  }
+}
+
 // grad_X from its sums over the splits; zeros for rows that do not count.
 template <int kDtype>
 __global__ void __launch_bounds__(256)
@@ -798,12 +881,13 @@ struct LossCall {
   int cols;         // features, padded
   bool packed;      // the weights are laid out piece by piece before they are multiplied
   int64_t piece;    // classes at a time
+  bool keeps;       // all classes are one piece: G is made from the scores' exponentials instead of the scores once more
   Cut all_scores, scores, row_product, class_product;
   LossRows rows;
   RowCounts* counts;
   uint16_t *zeros, *x, *x_scaled, *weight, *g;
   float2* partial;
-  float *row_sums, *bias_sums;
+  float *row_sums, *bias_sums, *kept;
 
   LossCall(int64_t n, int f, int k, int type, bool grad) : n_rows(n), features(f), classes(k), dtype(type), gradient(grad)
   {
@@ -811,12 +895,14 @@ struct LossCall {
     padded = round_up(n, 256);
     cols   = static_cast<int>(round_up(f, kProductK));
     packed = type == LBT_F32 || f % 8 != 0;
-    // a piece's G, and its packed weights, within kPieceBytes each; pieces of one size
+    // a piece's G and its packed weights within their bounds; pieces of one size
     int64_t most = round_up(k, 256);
-    if (grad) most = std::min(most, kPieceBytes / (2 * planes * padded) / 256 * 256);
+    const int64_t bytes = type == LBT_F32 ? 10 : 2;  // of an entry of G
+    if (grad) most = std::min(most, kScoresBytes / (bytes * padded) / 256 * 256);
     if (packed) most = std::min(most, kPieceBytes / (2 * planes * int64_t(cols)) / 256 * 256);
     most  = std::max<int64_t>(most, 256);
     piece = round_up(tiles_of(k, tiles_of(k, most)), 256);
+    keeps = grad && piece >= k && type != LBT_F16;
     const int64_t pairs = type == LBT_F32 ? 6 : 1;
     scores      = cut_product(std::min<int64_t>(piece, k), n, pairs * cols / kProductK, 1);
     all_scores  = packed ? scores : cut_product(k, n, pairs * cols / kProductK, 1);
@@ -838,13 +924,14 @@ struct LossCall {
     rows.top      = arena.template take<float>(padded);
     rows.inverse  = arena.template take<float>(padded);
     x             = arena.template take<uint16_t>(planes * padded * cols);
-    partial       = arena.template take<float2>((tiles_of(classes, all_scores.tile) + tiles_of(classes, piece)) * padded);
+    partial       = arena.template take<float2>(2 * (tiles_of(round_up(classes, 256), all_scores.tile) + tiles_of(classes, piece)) * padded);
     weight = x_scaled = g = nullptr;
-    row_sums = bias_sums = nullptr;
+    row_sums = bias_sums = kept = nullptr;
     if (packed) weight = arena.template take<uint16_t>(planes * piece * cols);
     if (!gradient) return;
     if (dtype == LBT_F16) x_scaled = arena.template take<uint16_t>(padded * cols);
     g         = arena.template take<uint16_t>(planes * padded * piece);
+    if (keeps && dtype == LBT_F32) kept = arena.template take<float>(padded * piece);
     row_sums  = arena.template take<float>(row_product.splits * padded * cols);
     bias_sums = arena.template take<float>(tiles_of(padded, scores.tile) * classes);
   }
@@ -923,6 +1010,8 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
   args.zeros  = c.zeros;
   args.counts = c.counts;
 
+  // the sums of G for grad_bias are those of floats, which what is kept for bfloat16 is not
+  const bool keep = c.keeps && grad_bias == nullptr;
   // top and total of each row; weights that are multiplied where they lie need no pieces here
   const int64_t step = c.packed ? c.piece : c.classes;
   int64_t tiles      = 0;
@@ -932,13 +1021,22 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
     args.a = weights(first, classes);
     args.b = x;
     args.k_extent = args.k_split = c.cols;
-    const LossEpilogue<kFine> e{bias, static_cast<int>(first), c.classes, static_cast<int>(tiles), c.padded, c.rows, c.partial};
+    const int share = 2 * static_cast<int>(tiles);  // (all tiles are two waves high)
     // (every piece in tiles of one size: they share the numbering of `partial`)
-    LBT_TRY((launch_product<L, false, false, kRowsN>(s, args, classes, c.n_rows, c.all_scores, e)));
-    tiles += tiles_of(classes, c.all_scores.tile);
+    if (keep) {
+      void* kept = kDtype == LBT_F32 ? static_cast<void*>(c.kept) : c.g;
+      const LossEpilogue<kFine, true> e{bias, static_cast<int>(first), c.classes, share, c.padded, c.rows, c.partial, kept,
+                                        static_cast<int>(c.piece)};
+      LBT_TRY((launch_product<L, false, false, kRowsN>(s, args, c.piece, c.n_rows, c.all_scores, e)));
+      tiles += tiles_of(c.piece, c.all_scores.tile);
+    } else {
+      const LossEpilogue<kFine, false> e{bias, static_cast<int>(first), c.classes, share, c.padded, c.rows, c.partial, nullptr, 0};
+      LBT_TRY((launch_product<L, false, false, kRowsN>(s, args, classes, c.n_rows, c.all_scores, e)));
+      tiles += tiles_of(classes, c.all_scores.tile);
+    }
   }
   join_kernel<<<static_cast<unsigned>(tiles_of(c.n_rows, kJoinRows)), kJoinRows * kJoinSlices, 0, s>>>(
-    c.partial, static_cast<int>(tiles), c.padded, c.rows, c.counts, loss);
+    c.partial, 2 * static_cast<int>(tiles), c.padded, c.rows, c.counts, loss);
   LBT_HIP(hipGetLastError());
   if (!c.gradient) return LBT_OK;
 
@@ -952,6 +1050,13 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
     const int64_t classes = std::min<int64_t>(c.piece, c.classes - first);
     if (first > 0 || c.piece < c.classes) LBT_TRY(lay_out(first));
     const ProductOperand w = weights(first, classes);
+    if (keep) {
+      constexpr bool kKeeps = kDtype == LBT_F32;
+      scale_kernel<kKeeps><<<static_cast<unsigned>(tiles_of(c.piece, kScaleClasses) * tiles_of(c.padded, kScaleRows)), 256, 0, s>>>(
+                             kKeeps ? static_cast<const void*>(c.kept) : c.g, c.partial, c.all_scores.tile / 2, c.padded,
+                                          c.rows, c.counts, static_cast<int>(c.piece), c.padded * c.piece, c.g);
+      LBT_HIP(hipGetLastError());
+    } else {
     args.a        = w;
     args.b        = x;
     args.k_extent = args.k_split = c.cols;
@@ -960,6 +1065,7 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
                                                               grad_bias != nullptr ? c.bias_sums : nullptr};
     // (over the whole piece: what lies past its classes is written as zeros)
     LBT_TRY((launch_product<L, false, false, kRowsN>(s, args, c.piece, c.n_rows, c.scores, ge)));
+    }
     args.a        = w;
     args.b        = g;
     args.k_extent = static_cast<int32_t>(c.piece);
