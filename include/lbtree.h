@@ -546,7 +546,8 @@ int lbt_gather_rows(void* stream, const void* X, int32_t x_dtype, int64_t row_of
  *   y       device int64 [n_rows]. A row whose label is not in [0, n_outputs) does not count: its loss is 0, nothing that
  *           it holds (NaN and infinities too) reaches any output
  *   loss    device float [n_rows]
- *   workspace  at least lbt_linear_log_loss_workspace_bytes(..., gradient = 0), 256-byte aligned
+ *   workspace  at least lbt_linear_log_loss_workspace_bytes(..., gradient = 0), 256-byte aligned. `gradient`: 0 for this
+ *              call, 1 for lbt_linear_log_loss_gradient, 2 for that with grad_bias; 0 bytes for invalid arguments
  * Enqueues on the stream and does not wait. All results are the same from call to call.
  */
 size_t lbt_linear_log_loss_workspace_bytes(int64_t n_rows, int32_t n_features, int32_t n_outputs, int32_t dtype, int32_t gradient);
@@ -558,12 +559,13 @@ int lbt_linear_log_loss(void* stream, const void* X, const void* weight, int32_t
  * The same loss together with the gradients of sum_r sample_weight[r] loss[r]:
  *   G[r][c] = sample_weight[r] (p[r][c] - [c = y[r]]),  p = softmax(s)
  *   grad_X = G weight,  grad_weight = G^T X,  grad_bias[c] = sum_r G[r][c]
- * G is formed for a piece of the classes at a time (at most 512 MiB of it), in the inputs' type (LBT_F16: times a power of two;
- * LBT_F32: three planes of bfloat16), and multiplied both ways with sums in 32 bits.
+ * G is formed for a piece of the classes at a time, in the inputs' type (LBT_F16: times a power of two; LBT_F32: three planes of
+ * bfloat16), and multiplied both ways with sums in 32 bits. A piece's share of the workspace is at most 2 GiB, whatever the
+ * vocabulary; classes that are one piece have their scores formed once, those of more pieces twice.
  *   sample_weight  device float [n_rows], or NULL for ones
  *   grad_X, grad_weight  device, shape and dtype of X and weight, 16-byte aligned; overwritten (zeros for rows that do not count)
  *   grad_bias      device float [n_outputs], or NULL; only with a bias
- *   workspace      at least lbt_linear_log_loss_workspace_bytes(..., gradient = 1), 256-byte aligned
+ *   workspace      at least lbt_linear_log_loss_workspace_bytes(..., gradient = 1, or 2 with grad_bias), 256-byte aligned
  */
 int lbt_linear_log_loss_gradient(void* stream, const void* X, const void* weight, int32_t dtype, int64_t n_rows,
                                  int32_t n_features, int32_t n_outputs, const float* bias, const int64_t* y,

@@ -283,11 +283,12 @@ __device__ __forceinline__ void add_bias(Float16v (&acc)[Tile::kMT][Tile::kNT], 
     }
 }
 
-// The shares of the rows' tops and totals: one of each row for the kWM classes of a wave. With kKeep also u = exp(s - the share's
-// top), [rows][piece], for scale_kernel: float, or half times 2^15 (2^-12 of a step below the type it is for, and no smaller
-// than 2^-29 with all its bits).
+// The shares of the rows' tops and totals: one of each row for the kWM classes of a wave. For scale_kernel also
+// u = exp(s - the share's top), [rows][piece]: as float, or, for G in bfloat16, as half times 2^15. Half is off by 2^-12 where
+// bfloat16 is by 2^-9 afterwards, and has all its bits down to 2^-29 of the top.
+enum { kNotKept = 0, kKeptHalf = 1, kKeptFloat = 2 };
 constexpr float kKeptScale = 32768.f;
-template <bool kExact, bool kKeep>
+template <bool kExact, int kKeep>
 struct LossEpilogue {
   const float* bias;
   int class_first, n_classes;  // of this launch: number of its first class; classes of the call
@@ -334,9 +335,9 @@ struct LossEpilogue {
             u[e] = exp_of(acc[i][j][q * 4 + e] - from, kExact);
             total += u[e];
           }
-          if constexpr (kKeep) {
+          if constexpr (kKeep != kNotKept) {
             const int64_t at = row * piece + in_piece + i * 32 + q * 8 + 4 * (lane >> 5);
-            if constexpr (kExact) {
+            if constexpr (kKeep == kKeptFloat) {
               *reinterpret_cast<float4*>(static_cast<float*>(kept) + at) = make_float4(u[0], u[1], u[2], u[3]);
             } else {
 #pragma unroll
@@ -350,6 +351,21 @@ struct LossEpilogue {
     }
   }
 };
+
+template <int kCtrl, int kRows>
+__device__ __forceinline__ float add_lanes(float v)
+{
+  return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), kCtrl, kRows, 0xf, true));
+}
+// Sums over lanes 0 to 31 and over 32 to 63, in the lanes' own data paths: in lanes 16 to 31 and 48 to 63.
+__device__ __forceinline__ float sum_32_lanes(float v)
+{
+  v = add_lanes<0x128, 0xf>(v);  // row_ror:8 within 16 lanes
+  v = add_lanes<0x124, 0xf>(v);
+  v = add_lanes<0x122, 0xf>(v);
+  v = add_lanes<0x121, 0xf>(v);
+  return add_lanes<0x142, 0xa>(v);  // row_bcast:15 from the row of 16 lanes before
+}
 
 // G of a piece of the classes, [plane][rows][piece] in the products' type, and its sums over the tile's rows.
 template <bool kExact, int kProduct, int kPlanes>
@@ -416,8 +432,8 @@ struct GradientEpilogue {
         float sum = 0.f;
 #pragma unroll
         for (int j = 0; j < Tile::kNT; j++) sum += acc[i][j][e] * scale[j];
-        for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor(sum, s);
-        if ((lane & 31) == 0) share[wn][wm * Tile::kWM + i * 32 + block_m(e, lane)] = sum;
+        sum = sum_32_lanes(sum);
+        if ((lane & 31) == 16) share[wn][wm * Tile::kWM + i * 32 + block_m(e, lane)] = sum;
       }
     __syncthreads();
     for (int m = threadIdx.x; m < Tile::kBM; m += Tile::kThreads) {
@@ -732,65 +748,78 @@ __global__ void __launch_bounds__(kFewThreads)
 
 // G from what LossEpilogue kept, once the rows' tops and totals are known: p = u exp(top of the share - top) / total. A workgroup
 // takes 16 rows and 2048 classes; bound by memory, each value is read and written once (bfloat16: in the same place).
-constexpr int kScaleRows = 16, kScaleClasses = 2048;
-template <bool kFloat>
+// The sums of G over the workgroup's rows are those of floats. Where 16 rows each would be too few workgroups they take 4.
+constexpr int kScaleClasses = 2048;
+template <int kDtype, bool kKeptAsHalf, int kRows>
 __global__ void __launch_bounds__(256)
   scale_kernel(const void* kept, const float2* __restrict__ partial, int share_classes, int64_t padded, LossRows rows,
-               const RowCounts* __restrict__ counts, int piece, int64_t plane, uint16_t* g)
+               const RowCounts* __restrict__ counts, int n_classes, int piece, int64_t plane, uint16_t* g, float* bias_sums)
 {
-  __shared__ float factor[kScaleRows][kScaleClasses / 32 + 1];
-  const int wides    = (piece + kScaleClasses - 1) / kScaleClasses;
-  const int64_t row0 = blockIdx.x / wides * int64_t(kScaleRows);
-  const int counted  = counts->rows;
+  using L = LossType<kDtype>;
+  __shared__ float factor[kRows][kScaleClasses / 32 + 1];
+  const int wides       = (piece + kScaleClasses - 1) / kScaleClasses;
+  const int64_t block   = blockIdx.x / wides;
+  const int64_t row0    = block * kRows;
+  const int counted     = counts->rows;
   if (row0 >= round_up_rows(counted)) return;
   const int class0 = static_cast<int>(blockIdx.x % wides) * kScaleClasses, shares = kScaleClasses / share_classes, first = class0 / share_classes;
-  for (int i = threadIdx.x; i < kScaleRows * shares; i += 256) {
-    const int64_t row = row0 + i % kScaleRows;
-    const int s       = i / kScaleRows;
+  for (int i = threadIdx.x; i < kRows * shares; i += 256) {
+    const int64_t row = row0 + i % kRows;
+    const int s       = i / kRows;
     float f           = 0.f;
     if (row < counted && class0 + s * share_classes < piece) {
       const float top = partial[(first + s) * padded + row].x;
-      f = top == -INFINITY ? 0.f : exp_of(top - rows.top[row], kFloat) * rows.inverse[row] * (kFloat ? 1.f : 1.f / kKeptScale);
+      f = top == -INFINITY ? 0.f : exp_of(top - rows.top[row], kDtype == LBT_F32) * rows.inverse[row] * (kKeptAsHalf ? 1.f / kKeptScale : 1.f);
     }
-    factor[i % kScaleRows][s] = f;
+    factor[i % kRows][s] = f;
   }
   __syncthreads();
-  const int wide = min(kScaleClasses, piece - class0) / 8;  // groups of 8 classes
-  for (int i = threadIdx.x; i < kScaleRows * wide; i += 256) {
-    const int r = i / wide, c = (i % wide) * 8;
-    const int64_t row = row0 + r, at = row * piece + class0 + c;
-    const float f = factor[r][c / share_classes];
-    const float w = rows.factor[row];
-    const int label = rows.label[row] - (class0 + c);
+  const int c = class0 + static_cast<int>(threadIdx.x) * 8;
+  if (c >= piece) return;
+  float sum[8];
+#pragma unroll
+  for (int e = 0; e < 8; e++) sum[e] = 0.f;
+#pragma unroll 4
+  for (int r = 0; r < kRows; r++) {
+    const int64_t row = row0 + r, at = row * piece + c;
+    const float f   = factor[r][(c - class0) / share_classes];
+    const float w   = rows.factor[row];
+    const int label = rows.label[row] - c;
     float u[8];
-    if constexpr (kFloat) {
-      const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(kept) + at);
-      const float4 a = q[0], b = q[1];
-      u[0] = a.x; u[1] = a.y; u[2] = a.z; u[3] = a.w; u[4] = b.x; u[5] = b.y; u[6] = b.z; u[7] = b.w;
-    } else {
+    if constexpr (kKeptAsHalf) {
       const Half8 h = *reinterpret_cast<const Half8*>(static_cast<const uint16_t*>(kept) + at);
 #pragma unroll
       for (int e = 0; e < 8; e++) u[e] = static_cast<float>(h[e]);
+    } else {
+      const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(kept) + at);
+      const float4 a = q[0], b = q[1];
+      u[0] = a.x; u[1] = a.y; u[2] = a.z; u[3] = a.w; u[4] = b.x; u[5] = b.y; u[6] = b.z; u[7] = b.w;
     }
-    uint16_t v[kFloat ? 3 : 1][8];
+    const float scale = kDtype == LBT_F16 && bias_sums != nullptr && row < counted ? ldexpf(1.f, rows.exponent[row] - counts->exponent) : 1.f;
+    uint16_t v[L::kPlanes][8];
 #pragma unroll
     for (int e = 0; e < 8; e++) {
       const float p = u[e] * f;
       float d       = (e == label ? p - 1.f : p) * w;
       d             = row < counted ? d : 0.f;
-      if constexpr (kFloat) {
+      sum[e] += kDtype == LBT_F16 ? d * scale : d;
+      if constexpr (L::kPlanes == 3) {
         uint16_t s[3];
         split_planes(d, s);
         v[0][e] = s[0];
         v[1][e] = s[1];
         v[2][e] = s[2];
       } else {
-        v[0][e] = to_bf16(d);
+        v[0][e] = narrow_value<L::kProduct>(d);
       }
     }
 #pragma unroll
-    for (int l = 0; l < (kFloat ? 3 : 1); l++) *reinterpret_cast<uint4*>(g + l * plane + at) = *reinterpret_cast<const uint4*>(v[l]);
+    for (int l = 0; l < L::kPlanes; l++) *reinterpret_cast<uint4*>(g + l * plane + at) = *reinterpret_cast<const uint4*>(v[l]);
   }
+  if (bias_sums == nullptr) return;
+#pragma unroll
+  for (int e = 0; e < 8; e++)
+    if (c + e < n_classes) bias_sums[block * n_classes + c + e] = sum[e];
 }
 
 // grad_X from its sums over the splits; zeros for rows that do not count.
@@ -859,7 +888,7 @@ Cut cut_product(int64_t m, int64_t n, int64_t stages, int64_t most_splits)
   Cut best{256, 1};
   double least = 1e30;
   for (const auto& t : kTiles)
-    for (int splits = 1; splits <= 16; splits *= 2) {
+    for (int splits = 1; splits <= 16; splits++) {
       if (splits > 1 && (splits > most_splits || stages / splits < 4)) break;
       const int64_t each = tiles_of(tiles_of(m, t.tile) * tiles_of(n, t.tile) * splits, kCus);
       const double time  = each * (tiles_of(stages, splits) * (each == 1 ? t.lone : t.stage) + t.ends) +
@@ -875,21 +904,23 @@ Cut cut_product(int64_t m, int64_t n, int64_t stages, int64_t most_splits)
 struct LossCall {
   int64_t n_rows;
   int features, classes, dtype;
-  bool gradient;
+  bool gradient, with_bias;
   int planes;
   int64_t padded;   // rows
   int cols;         // features, padded
   bool packed;      // the weights are laid out piece by piece before they are multiplied
   int64_t piece;    // classes at a time
-  bool keeps;       // all classes are one piece: G is made from the scores' exponentials instead of the scores once more
+  int kept;         // all classes are one piece: G is made from the scores' exponentials instead of the scores once more
+  int scale_rows;   // of a workgroup of scale_kernel
   Cut all_scores, scores, row_product, class_product;
   LossRows rows;
   RowCounts* counts;
   uint16_t *zeros, *x, *x_scaled, *weight, *g;
   float2* partial;
-  float *row_sums, *bias_sums, *kept;
+  float *row_sums, *bias_sums, *exps;
 
-  LossCall(int64_t n, int f, int k, int type, bool grad) : n_rows(n), features(f), classes(k), dtype(type), gradient(grad)
+  LossCall(int64_t n, int f, int k, int type, int grad)
+    : n_rows(n), features(f), classes(k), dtype(type), gradient(grad != 0), with_bias(grad > 1)
   {
     planes = type == LBT_F32 ? 3 : 1;
     padded = round_up(n, 256);
@@ -897,15 +928,17 @@ struct LossCall {
     packed = type == LBT_F32 || f % 8 != 0;
     // a piece's G and its packed weights within their bounds; pieces of one size
     int64_t most = round_up(k, 256);
-    const int64_t bytes = type == LBT_F32 ? 10 : 2;  // of an entry of G
-    if (grad) most = std::min(most, kScoresBytes / (bytes * padded) / 256 * 256);
+    kept                = type == LBT_BF16 && !with_bias ? kKeptHalf : kKeptFloat;  // (the sums for the bias are those of floats)
+    const int64_t bytes = 2 * planes + (kept == kKeptFloat ? 4 : 0);                // of an entry of G
+    if (gradient) most = std::min(most, kScoresBytes / (bytes * padded) / 256 * 256);
     if (packed) most = std::min(most, kPieceBytes / (2 * planes * int64_t(cols)) / 256 * 256);
     most  = std::max<int64_t>(most, 256);
     piece = round_up(tiles_of(k, tiles_of(k, most)), 256);
-    keeps = grad && piece >= k && type != LBT_F16;
+    if (!gradient || piece < k) kept = kNotKept;
     const int64_t pairs = type == LBT_F32 ? 6 : 1;
     scores      = cut_product(std::min<int64_t>(piece, k), n, pairs * cols / kProductK, 1);
     all_scores  = packed ? scores : cut_product(k, n, pairs * cols / kProductK, 1);
+    scale_rows  = tiles_of(padded, 16) * tiles_of(piece, kScaleClasses) >= 1024 ? 16 : 4;
     row_product = cut_product(f, n, pairs * piece / kProductK, 16);
     class_product = cut_product(f, std::min<int64_t>(piece, k), pairs * padded / kProductK, 1);
   }
@@ -926,14 +959,14 @@ struct LossCall {
     x             = arena.template take<uint16_t>(planes * padded * cols);
     partial       = arena.template take<float2>(2 * (tiles_of(round_up(classes, 256), all_scores.tile) + tiles_of(classes, piece)) * padded);
     weight = x_scaled = g = nullptr;
-    row_sums = bias_sums = kept = nullptr;
+    row_sums = bias_sums = exps = nullptr;
     if (packed) weight = arena.template take<uint16_t>(planes * piece * cols);
     if (!gradient) return;
     if (dtype == LBT_F16) x_scaled = arena.template take<uint16_t>(padded * cols);
     g         = arena.template take<uint16_t>(planes * padded * piece);
-    if (keeps && dtype == LBT_F32) kept = arena.template take<float>(padded * piece);
+    if (kept == kKeptFloat) exps = arena.template take<float>(padded * piece);
     row_sums  = arena.template take<float>(row_product.splits * padded * cols);
-    bias_sums = arena.template take<float>(tiles_of(padded, scores.tile) * classes);
+    if (with_bias) bias_sums = arena.template take<float>(tiles_of(padded, kept ? scale_rows : scores.tile) * classes);
   }
 };
 
@@ -1010,8 +1043,6 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
   args.zeros  = c.zeros;
   args.counts = c.counts;
 
-  // the sums of G for grad_bias are those of floats, which what is kept for bfloat16 is not
-  const bool keep = c.keeps && grad_bias == nullptr;
   // top and total of each row; weights that are multiplied where they lie need no pieces here
   const int64_t step = c.packed ? c.piece : c.classes;
   int64_t tiles      = 0;
@@ -1023,17 +1054,20 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
     args.k_extent = args.k_split = c.cols;
     const int share = 2 * static_cast<int>(tiles);  // (all tiles are two waves high)
     // (every piece in tiles of one size: they share the numbering of `partial`)
-    if (keep) {
-      void* kept = kDtype == LBT_F32 ? static_cast<void*>(c.kept) : c.g;
-      const LossEpilogue<kFine, true> e{bias, static_cast<int>(first), c.classes, share, c.padded, c.rows, c.partial, kept,
-                                        static_cast<int>(c.piece)};
-      LBT_TRY((launch_product<L, false, false, kRowsN>(s, args, c.piece, c.n_rows, c.all_scores, e)));
-      tiles += tiles_of(c.piece, c.all_scores.tile);
-    } else {
-      const LossEpilogue<kFine, false> e{bias, static_cast<int>(first), c.classes, share, c.padded, c.rows, c.partial, nullptr, 0};
-      LBT_TRY((launch_product<L, false, false, kRowsN>(s, args, classes, c.n_rows, c.all_scores, e)));
-      tiles += tiles_of(classes, c.all_scores.tile);
-    }
+    auto scores = [&](auto kind) {
+      constexpr int kKind = decltype(kind)::value;
+      const int64_t m     = kKind == kNotKept ? classes : c.piece;  // (what is kept is kept for the whole piece)
+      const LossEpilogue<kFine, kKind> e{bias, static_cast<int>(first), c.classes, share, c.padded, c.rows, c.partial,
+                                         kKind == kKeptFloat ? static_cast<void*>(c.exps) : c.g, static_cast<int>(c.piece)};
+      tiles += tiles_of(m, c.all_scores.tile);
+      return launch_product<L, false, false, kRowsN>(s, args, m, c.n_rows, c.all_scores, e);
+    };
+    if constexpr (kDtype == LBT_BF16)
+      if (c.kept == kKeptHalf) {
+        LBT_TRY(scores(std::integral_constant<int, kKeptHalf>{}));
+        continue;
+      }
+    LBT_TRY(c.kept == kNotKept ? scores(std::integral_constant<int, kNotKept>{}) : scores(std::integral_constant<int, kKeptFloat>{}));
   }
   join_kernel<<<static_cast<unsigned>(tiles_of(c.n_rows, kJoinRows)), kJoinRows * kJoinSlices, 0, s>>>(
     c.partial, 2 * static_cast<int>(tiles), c.padded, c.rows, c.counts, loss);
@@ -1050,21 +1084,34 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
     const int64_t classes = std::min<int64_t>(c.piece, c.classes - first);
     if (first > 0 || c.piece < c.classes) LBT_TRY(lay_out(first));
     const ProductOperand w = weights(first, classes);
-    if (keep) {
-      constexpr bool kKeeps = kDtype == LBT_F32;
-      scale_kernel<kKeeps><<<static_cast<unsigned>(tiles_of(c.piece, kScaleClasses) * tiles_of(c.padded, kScaleRows)), 256, 0, s>>>(
-                             kKeeps ? static_cast<const void*>(c.kept) : c.g, c.partial, c.all_scores.tile / 2, c.padded,
-                                          c.rows, c.counts, static_cast<int>(c.piece), c.padded * c.piece, c.g);
+    if (c.kept != kNotKept) {
+      auto scale = [&](auto half, auto each) {
+        constexpr int kRows = decltype(each)::value;
+        scale_kernel<kDtype, decltype(half)::value, kRows>
+          <<<static_cast<unsigned>(tiles_of(c.piece, kScaleClasses) * tiles_of(c.padded, kRows)), 256, 0, s>>>(
+            decltype(half)::value ? static_cast<const void*>(c.g) : c.exps, c.partial, c.all_scores.tile / 2, c.padded, c.rows, c.counts,
+            c.classes, static_cast<int>(c.piece), c.padded * c.piece, c.g, grad_bias != nullptr ? c.bias_sums : nullptr);
+      };
+      auto scale_by = [&](auto half) {
+        if (c.scale_rows == 16) scale(half, std::integral_constant<int, 16>{});
+        else scale(half, std::integral_constant<int, 4>{});
+      };
+      if constexpr (kDtype == LBT_BF16) {
+        if (c.kept == kKeptHalf) scale_by(std::true_type{});
+        else scale_by(std::false_type{});
+      } else {
+        scale_by(std::false_type{});
+      }
       LBT_HIP(hipGetLastError());
     } else {
-    args.a        = w;
-    args.b        = x;
-    args.k_extent = args.k_split = c.cols;
-    const GradientEpilogue<kFine, L::kProduct, L::kPlanes> ge{bias, static_cast<int>(first), c.classes, static_cast<int>(c.piece),
-                                                              c.rows, c.g, c.padded * c.piece,
-                                                              grad_bias != nullptr ? c.bias_sums : nullptr};
-    // (over the whole piece: what lies past its classes is written as zeros)
-    LBT_TRY((launch_product<L, false, false, kRowsN>(s, args, c.piece, c.n_rows, c.scores, ge)));
+      args.a        = w;
+      args.b        = x;
+      args.k_extent = args.k_split = c.cols;
+      const GradientEpilogue<kFine, L::kProduct, L::kPlanes> ge{bias, static_cast<int>(first), c.classes, static_cast<int>(c.piece),
+                                                                c.rows, c.g, c.padded * c.piece,
+                                                                grad_bias != nullptr ? c.bias_sums : nullptr};
+      // (over the whole piece: what lies past its classes is written as zeros)
+      LBT_TRY((launch_product<L, false, false, kRowsN>(s, args, c.piece, c.n_rows, c.scores, ge)));
     }
     args.a        = w;
     args.b        = g;
@@ -1085,7 +1132,7 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
   LBT_HIP(hipGetLastError());
   if (grad_bias != nullptr) {
     finish_bias_kernel<<<static_cast<unsigned>(tiles_of(c.classes, 256)), 256, 0, s>>>(c.bias_sums, c.classes,
-                                                                                       c.scores.tile, c.counts, kHalf,
+                                                                                       c.kept ? c.scale_rows : c.scores.tile, c.counts, kHalf,
                                                                                        grad_bias);
     LBT_HIP(hipGetLastError());
   }
@@ -1157,7 +1204,7 @@ int run_loss(void* stream, const void* X, const void* weight, int32_t dtype, int
     set_error("a workspace aligned to 256 bytes is needed");
     return LBT_ERR_WORKSPACE;
   }
-  LossCall c(std::max<int64_t>(n_rows, 1), n_features, n_outputs, dtype, gradient);
+  LossCall c(std::max<int64_t>(n_rows, 1), n_features, n_outputs, dtype, !gradient ? 0 : grad_bias == nullptr ? 1 : 2);
   c.n_rows       = n_rows;
   const bool few = !gradient && n_rows <= kFewRows;
   FewCall f;
@@ -1194,8 +1241,8 @@ extern "C" {
 
 size_t lbt_linear_log_loss_workspace_bytes(int64_t n_rows, int32_t n_features, int32_t n_outputs, int32_t dtype, int32_t gradient)
 {
-  if (!lbt::loss_shape(n_rows, n_features, n_outputs, dtype)) return 0;
-  lbt::LossCall c(std::max<int64_t>(n_rows, 1), n_features, n_outputs, dtype, gradient != 0);
+  if (!lbt::loss_shape(n_rows, n_features, n_outputs, dtype) || gradient < 0 || gradient > 2) return 0;
+  lbt::LossCall c(std::max<int64_t>(n_rows, 1), n_features, n_outputs, dtype, gradient);
   lbt::Arena arena;
   arena.measure = true;
   if (gradient == 0 && n_rows <= lbt::kFewRows) {

@@ -656,7 +656,7 @@ def linear_log_loss_gradient(X, weight, y, sample_weight=None, bias=None):
         loss = torch.empty(n, dtype=torch.float32, device=X.device)
         grad_X, grad_weight = torch.empty_like(X), torch.empty_like(weight)
         grad_bias = None if bias is None else torch.empty(k, dtype=torch.float32, device=X.device)
-        ws = _scratch(_lib.lib.lbt_linear_log_loss_workspace_bytes(n, f, k, dt, 1), X.device)
+        ws = _scratch(_lib.lib.lbt_linear_log_loss_workspace_bytes(n, f, k, dt, 1 if bias is None else 2), X.device)
         _lib.check(_lib.lib.lbt_linear_log_loss_gradient(
             _stream(), X.data_ptr(), weight.data_ptr(), dt, n, f, k, _ptr(bias), y.data_ptr(), _ptr(w), loss.data_ptr(),
             grad_X.data_ptr(), grad_weight.data_ptr(), _ptr(grad_bias), ws.data_ptr(), ws.numel()))

@@ -111,11 +111,14 @@ def test_tiles_of_256(dtype):
     check(*inputs(3900, {"bf16": 4104, "f16": 4099, "f32": 4100}[dtype], 5100, dtype, seed=3), dtype)
 
 
-@pytest.mark.parametrize("dtype,n,f,k", [("bf16", 4100, 64, 62000), ("f16", 4100, 40, 62000), ("f32", 4100, 24, 21000),
-                                         ("bf16", 40, 2050, 131001)])
-def test_several_pieces_of_the_classes(dtype, n, f, k):
-    assert 2 * (3 if dtype == "f32" else 1) * ((n + 255) // 256 * 256) * k > 512 << 20 or 2 * 2112 * k > 512 << 20
-    check(*inputs(n, f, k, dtype, seed=5), dtype)
+@pytest.mark.parametrize("dtype,n,f,k,biased", [("bf16", 4100, 64, 250000, False), ("f16", 4100, 40, 85000, True),
+                                                ("f32", 4100, 24, 50000, False), ("bf16", 40, 2050, 131001, True)])
+def test_several_pieces_of_the_classes(dtype, n, f, k, biased):
+    """G of a piece takes 2 GiB, with float exponentials beside it but for bfloat16; weights that are laid out first 512 MiB."""
+    entry = {"bf16": 2, "f16": 6, "f32": 10}[dtype]
+    assert entry * ((n + 255) // 256 * 256) * k > 2 << 30 or 2 * 2112 * k > 512 << 20
+    bias = torch.randn(k, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda") if biased else None
+    check(*inputs(n, f, k, dtype, seed=5), dtype, bias=bias)
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
