@@ -87,30 +87,39 @@ __device__ __forceinline__ int token_at(const void* tokens, int bytes, int64_t t
   return v >= 0 && v < n_rows ? static_cast<int>(v) : n_rows;
 }
 
-constexpr int kRowThreads = 256;
+constexpr int kRowThreads = 256, kRowWaves = kRowThreads / 64;
 
-template <int kDtype, int kBytes>
+// A group of kLanes lanes copies a row, kEach words of a lane at a time.
+template <int kDtype, int kBytes, int kLanes>
 __global__ void __launch_bounds__(kRowThreads)
   embed_rows_kernel(const void* __restrict__ table, int n_rows, int words, const void* __restrict__ tokens, int token_bytes,
                     int64_t n_tokens, float scale, void* __restrict__ out)
 {
-  using P          = Pack<kDtype, kBytes>;
-  using Word       = typename P::Word;
-  const int64_t i  = blockIdx.x * int64_t(kRowThreads) + threadIdx.x;
-  if (i >= n_tokens * words) return;
-  const int64_t t = i / words;
-  const int at    = static_cast<int>(i % words);
-  const int v     = token_at(tokens, token_bytes, t, n_rows);
-  float x[P::kValues];
-  if (v < n_rows) {
-    P::unpack(static_cast<const Word*>(table)[static_cast<int64_t>(v) * words + at], x);
+  using P             = Pack<kDtype, kBytes>;
+  using Word          = typename P::Word;
+  constexpr int kEach = 4;
+  const int64_t t     = blockIdx.x * int64_t(kRowThreads / kLanes) + threadIdx.x / kLanes;
+  if (t >= n_tokens) return;
+  const int v      = token_at(tokens, token_bytes, t, n_rows);
+  const Word* from = static_cast<const Word*>(table) + static_cast<int64_t>(v) * words;
+  Word* to         = static_cast<Word*>(out) + t * words;
+  for (int at = threadIdx.x % kLanes; at < words; at += kLanes * kEach) {
+    Word w[kEach];
+    if (v < n_rows) {
 #pragma unroll
-    for (int e = 0; e < P::kValues; e++) x[e] = scaled(x[e], scale);
-  } else {
+      for (int e = 0; e < kEach; e++)
+        if (at + e * kLanes < words) w[e] = from[at + e * kLanes];
+    }
 #pragma unroll
-    for (int e = 0; e < P::kValues; e++) x[e] = 0.f;
+    for (int e = 0; e < kEach; e++) {
+      if (at + e * kLanes >= words) break;
+      float x[P::kValues];
+      if (v < n_rows) P::unpack(w[e], x);
+#pragma unroll
+      for (int i = 0; i < P::kValues; i++) x[i] = v < n_rows ? scaled(x[i], scale) : 0.f;
+      to[at + e * kLanes] = P::pack(x);
+    }
   }
-  static_cast<Word*>(out)[i] = P::pack(x);
 }
 
 // ---- places sorted by token ----------------------------------------------------------------------
@@ -159,7 +168,7 @@ __device__ __forceinline__ int sort_key(const void* tokens, int token_bytes, con
 
 __global__ void __launch_bounds__(kSortThreads)
   digit_count_kernel(const void* __restrict__ tokens, int token_bytes, const int32_t* __restrict__ keys, int64_t n, int n_rows,
-                     int shift, int digits, int blocks, int32_t* __restrict__ counts)
+                     int shift, int digits, int32_t* __restrict__ counts)
 {
   __shared__ int count[kDigits];
   count[threadIdx.x] = 0;
@@ -169,17 +178,25 @@ __global__ void __launch_bounds__(kSortThreads)
     if (i < n) atomicAdd(&count[(sort_key(tokens, token_bytes, keys, i, n_rows) >> shift) & (digits - 1)], 1);
   }
   __syncthreads();
-  if (static_cast<int>(threadIdx.x) < digits) counts[static_cast<int64_t>(threadIdx.x) * blocks + blockIdx.x] = count[threadIdx.x];
+  if (static_cast<int>(threadIdx.x) < digits) counts[static_cast<int64_t>(blockIdx.x) * digits + threadIdx.x] = count[threadIdx.x];
 }
 
-// counts [digits][blocks] become the number of entries before each: one workgroup, a thread per digit.
+// counts [blocks][digits] become the number of entries before each: one workgroup, a thread per digit.
 __global__ void __launch_bounds__(kSortThreads) digit_offsets_kernel(int digits, int blocks, int32_t* __restrict__ counts)
 {
   __shared__ int wave_sum[kSortWaves];
+  constexpr int kAhead = 16;  // counts asked for together
   const int d = threadIdx.x, lane = d & 63, wave = d >> 6;
-  int sum = 0;
-  if (d < digits)
-    for (int b = 0; b < blocks; b++) sum += counts[static_cast<int64_t>(d) * blocks + b];
+  int c[kAhead], sum = 0;
+  auto load = [&](int b0) {
+#pragma unroll
+    for (int e = 0; e < kAhead; e++) c[e] = d < digits && b0 + e < blocks ? counts[static_cast<int64_t>(b0 + e) * digits + d] : 0;
+  };
+  for (int b0 = 0; b0 < blocks; b0 += kAhead) {
+    load(b0);
+#pragma unroll
+    for (int e = 0; e < kAhead; e++) sum += c[e];
+  }
   int upto = sum;
   for (int s = 1; s < 64; s <<= 1) {
     const int other = __shfl_up(upto, s);
@@ -189,20 +206,21 @@ __global__ void __launch_bounds__(kSortThreads) digit_offsets_kernel(int digits,
   __syncthreads();
   int at = upto - sum;
   for (int w = 0; w < wave; w++) at += wave_sum[w];
-  if (d < digits)
-    for (int b = 0; b < blocks; b++) {
-      const int64_t i = static_cast<int64_t>(d) * blocks + b;
-      const int c     = counts[i];
-      counts[i]       = at;
-      at += c;
+  for (int b0 = 0; b0 < blocks; b0 += kAhead) {
+    if (blocks > kAhead) load(b0);
+#pragma unroll
+    for (int e = 0; e < kAhead; e++) {
+      if (d < digits && b0 + e < blocks) counts[static_cast<int64_t>(b0 + e) * digits + d] = at;
+      at += c[e];
     }
+  }
 }
 
 // A wave takes 256 consecutive entries, 64 at a time: the lanes of equal digits find one another by ballots, the first of
 // them moves the wave's count on. Ranks are then the block's offset, the waves before, and the place in the wave: stable.
 __global__ void __launch_bounds__(kSortThreads)
   digit_move_kernel(const void* __restrict__ tokens, int token_bytes, const int32_t* __restrict__ keys,
-                    const int32_t* __restrict__ places, int64_t n, int n_rows, int shift, int bits, int blocks,
+                    const int32_t* __restrict__ places, int64_t n, int n_rows, int shift, int bits,
                     const int32_t* __restrict__ offsets, Sorted out)
 {
   __shared__ uint16_t count[kSortWaves][kDigits];
@@ -210,7 +228,7 @@ __global__ void __launch_bounds__(kSortThreads)
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int digits = 1 << bits;
   for (int w = 0; w < kSortWaves; w++) count[w][threadIdx.x] = 0;
-  if (static_cast<int>(threadIdx.x) < digits) first[threadIdx.x] = offsets[static_cast<int64_t>(threadIdx.x) * blocks + blockIdx.x];
+  if (static_cast<int>(threadIdx.x) < digits) first[threadIdx.x] = offsets[static_cast<int64_t>(blockIdx.x) * digits + threadIdx.x];
   __syncthreads();
   const int64_t begin = blockIdx.x * int64_t(kSortBlock) + wave * (64 * kSortEach);
   int key[kSortEach], digit[kSortEach], rank[kSortEach];
@@ -262,6 +280,7 @@ struct RunArgs {
   float scale;
   void* out;
   int add;     // to what `out` holds
+  unsigned clears;  // workgroups that clear rows without a token
   float* part; // [chunks][2][words * values]: of the run that began before the chunk, of the run that goes on after it
 };
 
@@ -283,13 +302,39 @@ __device__ __forceinline__ void write_row(const RunArgs& a, int row, int at, con
   *to = P::pack(x);
 }
 
+// Zeros for the rows that no token names: a workgroup looks up 64 rows in the sorted tokens and clears those that are absent.
+constexpr int kClearRows = 64;
+template <class Word>
+__device__ __forceinline__ void clear_rows(const RunArgs& a, int64_t group)
+{
+  const int64_t first = group * kClearRows;
+  const int64_t row   = first + (threadIdx.x & 63);
+  int lo = 0, hi = a.n_tokens;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (a.sorted.key[mid] < row) lo = mid + 1;
+    else hi = mid;
+  }
+  const uint64_t absent = __ballot(row < a.n_rows && !(lo < a.n_tokens && a.sorted.key[lo] == row));
+  for (int r = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); r < kClearRows; r += kRowWaves)
+    if ((absent >> r) & 1) {
+      Word* to = static_cast<Word*>(a.out) + (first + r) * a.words;
+      for (int i = threadIdx.x & 63; i < a.words; i += 64) to[i] = Word{};
+    }
+}
+
 template <int kDtype, int kBytes>
 __global__ void __launch_bounds__(kRowThreads) sum_runs_kernel(const RunArgs a)
 {
   using P    = Pack<kDtype, kBytes>;
   using Word = typename P::Word;
+  // (the first workgroups clear: they are writes alone, and those that add are mostly reads)
+  if (blockIdx.x < a.clears) {
+    clear_rows<Word>(a, blockIdx.x);
+    return;
+  }
   const int lane      = threadIdx.x & 63;
-  const int64_t task  = static_cast<int64_t>(blockIdx.x) * (kRowThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t task  = static_cast<int64_t>(blockIdx.x - a.clears) * kRowWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t chunk = task / a.slices;
   const int at        = static_cast<int>(task % a.slices) * 64 + lane;
   const int64_t p0    = chunk * a.chunk;
@@ -348,7 +393,7 @@ template <int kDtype, int kBytes>
 __global__ void __launch_bounds__(kRowThreads) join_runs_kernel(const RunArgs a)
 {
   using P = Pack<kDtype, kBytes>;
-  const int64_t task  = static_cast<int64_t>(blockIdx.x) * (kRowThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t task  = static_cast<int64_t>(blockIdx.x) * kRowWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t chunk = task / a.slices;
   const int at        = static_cast<int>(task % a.slices) * 64 + (threadIdx.x & 63);
   const int64_t p0    = chunk * a.chunk, p1 = p0 + a.chunk;
@@ -356,45 +401,123 @@ __global__ void __launch_bounds__(kRowThreads) join_runs_kernel(const RunArgs a)
   const int row = a.sorted.key[p1 - 1];
   if (row >= a.n_rows || a.sorted.key[p1] != row) return;
   if (p0 > 0 && a.sorted.key[p0 - 1] == row) return;  // it began earlier
-  if (at >= a.words) return;
   const int64_t stride = static_cast<int64_t>(a.words) * P::kValues;
   const float* from    = a.part + (chunk * 2 + 1) * stride + static_cast<int64_t>(at) * P::kValues;
   float sum[P::kValues];
 #pragma unroll
-  for (int e = 0; e < P::kValues; e++) sum[e] = from[e];
+  for (int e = 0; e < P::kValues; e++) sum[e] = at < a.words ? from[e] : 0.f;
   from += stride;  // the part at the head of the next chunk
-  for (int64_t p = p1; p < a.n_tokens && a.sorted.key[p] == row; p += a.chunk, from += 2 * stride) {
+  // 64 chunks at a time: how many of them begin with this token
+  for (int64_t p = p1;; p += 64 * static_cast<int64_t>(a.chunk)) {
+    const int64_t own   = p + static_cast<int64_t>(threadIdx.x & 63) * a.chunk;
+    const uint64_t same = __ballot(own < a.n_tokens && a.sorted.key[min(own, static_cast<int64_t>(a.n_tokens) - 1)] == row);
+    const int parts     = same == ~uint64_t(0) ? 64 : __builtin_ctzll(~same);
+    constexpr int kAhead = 8;
+    for (int i = 0; i < parts; i += kAhead) {
+      float x[kAhead][P::kValues];
 #pragma unroll
-    for (int e = 0; e < P::kValues; e++) sum[e] += from[e];
+      for (int j = 0; j < kAhead; j++)
+        if (at < a.words && i + j < parts)
+#pragma unroll
+          for (int e = 0; e < P::kValues; e++) x[j][e] = from[(i + j) * 2 * stride + e];
+#pragma unroll
+      for (int j = 0; j < kAhead; j++)
+        if (i + j < parts)
+#pragma unroll
+          for (int e = 0; e < P::kValues; e++) sum[e] += x[j][e];
+    }
+    if (parts < 64) break;
+    from += 64 * 2 * stride;
   }
+  if (at >= a.words) return;
   write_row<kDtype, kBytes>(a, row, at, sum);
 }
 
-// Zeros for the rows that no token names: a workgroup looks up 64 rows in the sorted tokens and clears those that are absent.
-constexpr int kClearRows = 64;
-template <int kBytes>
+// ---- few places -----------------------------------------------------------------------------------------
+
+// Few tokens need no sorting: a workgroup takes some rows of the table, lists the places that name one of them in ascending order,
+// and its waves add up a row each. One launch.
+constexpr int kDirectTokens = 2048;
+
+template <int kDtype, int kBytes>
 __global__ void __launch_bounds__(kRowThreads)
-  clear_rows_kernel(const int32_t* __restrict__ keys, int n_tokens, int n_rows, int words, void* __restrict__ out)
+  direct_rows_kernel(const RunArgs a, const void* __restrict__ tokens, int token_bytes, int rows_each)
 {
-  using Word = typename Pack<LBT_BF16, kBytes>::Word;
-  const int64_t first = blockIdx.x * int64_t(kClearRows);
-  const int64_t row   = first + (threadIdx.x & 63);
-  int lo = 0, hi = n_tokens;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (keys[mid] < row) lo = mid + 1;
-    else hi = mid;
+  using P    = Pack<kDtype, kBytes>;
+  using Word = typename P::Word;
+  __shared__ int list[kDirectTokens];  // row of the workgroup << 16 | place
+  __shared__ int count[kRowWaves];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int first = blockIdx.x * rows_each;
+  int listed = 0;
+  for (int base = 0; base < a.n_tokens; base += kRowThreads) {
+    const int t    = base + threadIdx.x;
+    const int row  = t < a.n_tokens ? token_at(tokens, token_bytes, t, a.n_rows) : a.n_rows;
+    const bool in  = row < a.n_rows && row >= first && row < first + rows_each;
+    const uint64_t set = __ballot(in);
+    if (lane == 0) count[wave] = __popcll(set);
+    __syncthreads();
+    int at = listed;
+#pragma unroll
+    for (int w = 0; w < kRowWaves; w++) {
+      at += w < wave ? count[w] : 0;
+      listed += count[w];
+    }
+    if (in) list[at + __popcll(set & ((uint64_t(1) << lane) - 1))] = (row - first) << 16 | t;
+    __syncthreads();
   }
-  const uint64_t absent = __ballot(row < n_rows && !(lo < n_tokens && keys[lo] == row));
-  Word* to = static_cast<Word*>(out) + first * words;
-  const int64_t total = static_cast<int64_t>(kClearRows) * words;
-  for (int64_t i = threadIdx.x; i < total; i += kRowThreads)
-    if ((absent >> (i / words)) & 1) to[i] = Word{};
+  listed = __builtin_amdgcn_readfirstlane(listed);
+  for (int r = wave; r < rows_each && first + r < a.n_rows; r += kRowWaves) {
+    bool any = false;
+    for (int l = 0; l < listed && !any; l += 64) any = __any(l + lane < listed && list[min(l + lane, kDirectTokens - 1)] >> 16 == r);
+    if (!any) {
+      if (!a.add) {
+        Word* to = static_cast<Word*>(a.out) + static_cast<int64_t>(first + r) * a.words;
+        for (int i = lane; i < a.words; i += 64) to[i] = Word{};
+      }
+      continue;
+    }
+    for (int slice = 0; slice < a.slices; slice++) {
+      const int at      = slice * 64 + lane;
+      const bool inside = at < a.words;
+      float sum[P::kValues];
+#pragma unroll
+      for (int e = 0; e < P::kValues; e++) sum[e] = 0.f;
+      for (int l = 0; l < listed; l += 64) {
+        const int entry = l + lane < listed ? list[l + lane] : -1;
+        uint64_t same   = __ballot(entry >> 16 == r);
+        constexpr int kAhead = 8;
+        while (same != 0) {
+          Word w[kAhead];
+          int found = 0;
+#pragma unroll
+          for (int j = 0; j < kAhead; j++) {
+            if (same == 0) break;
+            const int place = __builtin_amdgcn_readlane(entry, __builtin_ctzll(same)) & 0xffff;
+            same &= same - 1;
+            found++;
+            if (inside) w[j] = static_cast<const Word*>(a.grad)[static_cast<int64_t>(place) * a.words + at];
+          }
+#pragma unroll
+          for (int j = 0; j < kAhead; j++) {
+            if (j >= found) break;
+            float x[P::kValues];
+            P::unpack(w[j], x);
+#pragma unroll
+            for (int e = 0; e < P::kValues; e++) sum[e] += x[e];
+          }
+        }
+      }
+      if (inside) write_row<kDtype, kBytes>(a, first + r, at, sum);
+    }
+  }
 }
 
 // ---- host -------------------------------------------------------------------------------------------
 
 constexpr int kCountSortTokens = 8192;  // at most this many are sorted by counting
+// Without sorting where one wave can add up all that is there, should it belong to one row.
+bool direct(int64_t n_tokens, int64_t row_bytes) { return n_tokens <= kDirectTokens && n_tokens * row_bytes <= (1 << 20); }
 
 int value_bytes(int dtype) { return dtype == LBT_F32 ? 4 : 2; }
 
@@ -445,10 +568,19 @@ int embed_gradient(hipStream_t s, const EmbedCall& c, const void* grad, const vo
                    void* out)
 {
   int at = 0;
+  RunArgs a{grad,  c.sorted[0], static_cast<int>(c.n_tokens), c.n_rows, c.words, c.chunk, c.slices, scale, out, add ? 1 : 0, 0,
+            c.part};
+  if (direct(c.n_tokens, static_cast<int64_t>(c.words) * kBytes)) {
+    int each = 64;  // rows of a workgroup: fewer where that gives too few workgroups
+    while (each > 4 && c.n_rows / each < 2048) each /= 2;
+    direct_rows_kernel<kDtype, kBytes><<<static_cast<unsigned>((static_cast<int64_t>(c.n_rows) + each - 1) / each), kRowThreads, 0, s>>>(
+      a, tokens, token_bytes, each);
+    LBT_HIP(hipGetLastError());
+    return LBT_OK;
+  }
   if (c.n_tokens <= kCountSortTokens) {
-    if (c.n_tokens > 0)
-      count_sort_kernel<<<static_cast<unsigned>((c.n_tokens + 63) / 64), kSortThreads, 0, s>>>(
-        tokens, token_bytes, static_cast<int>(c.n_tokens), c.n_rows, c.sorted[0]);
+    count_sort_kernel<<<static_cast<unsigned>((c.n_tokens + 63) / 64), kSortThreads, 0, s>>>(
+      tokens, token_bytes, static_cast<int>(c.n_tokens), c.n_rows, c.sorted[0]);
   } else {
     const int each = (c.bits + c.passes - 1) / c.passes;
     for (int p = 0; p < c.passes; p++) {
@@ -458,26 +590,19 @@ int embed_gradient(hipStream_t s, const EmbedCall& c, const void* grad, const vo
       const Sorted to     = c.sorted[1 - at];
       const unsigned grid = static_cast<unsigned>(c.blocks);
       digit_count_kernel<<<grid, kSortThreads, 0, s>>>(tokens, token_bytes, keys, c.n_tokens, c.n_rows, shift, 1 << bits,
-                                                       static_cast<int>(c.blocks), c.counts);
+                                                       c.counts);
       digit_offsets_kernel<<<1, kSortThreads, 0, s>>>(1 << bits, static_cast<int>(c.blocks), c.counts);
       digit_move_kernel<<<grid, kSortThreads, 0, s>>>(tokens, token_bytes, keys, from, c.n_tokens, c.n_rows, shift, bits,
-                                                      static_cast<int>(c.blocks), c.counts, to);
+                                                      c.counts, to);
       at = 1 - at;
     }
   }
   LBT_HIP(hipGetLastError());
-  if (!add) {
-    const int64_t groups = (static_cast<int64_t>(c.n_rows) + kClearRows - 1) / kClearRows;
-    clear_rows_kernel<kBytes><<<static_cast<unsigned>(groups), kRowThreads, 0, s>>>(c.sorted[at].key, static_cast<int>(c.n_tokens),
-                                                                                   c.n_rows, c.words, out);
-    LBT_HIP(hipGetLastError());
-  }
-  if (c.n_tokens == 0) return LBT_OK;
-  const RunArgs a{grad,     c.sorted[at], static_cast<int>(c.n_tokens), c.n_rows, c.words, c.chunk, c.slices, scale, out, add ? 1 : 0,
-                  c.part};
-  const int64_t grid = (c.chunks * c.slices + kRowThreads / 64 - 1) / (kRowThreads / 64);
-  LBT_REQUIRE(grid < (int64_t(1) << 31), "too many elements");
-  sum_runs_kernel<kDtype, kBytes><<<static_cast<unsigned>(grid), kRowThreads, 0, s>>>(a);
+  a.sorted = c.sorted[at];
+  if (!add) a.clears = static_cast<unsigned>((static_cast<int64_t>(c.n_rows) + kClearRows - 1) / kClearRows);
+  const int64_t grid = (c.chunks * c.slices + kRowWaves - 1) / kRowWaves;
+  LBT_REQUIRE(grid + a.clears < (int64_t(1) << 31), "too many elements");
+  sum_runs_kernel<kDtype, kBytes><<<static_cast<unsigned>(grid + a.clears), kRowThreads, 0, s>>>(a);
   LBT_HIP(hipGetLastError());
   if (c.chunks > 1) {
     join_runs_kernel<kDtype, kBytes><<<static_cast<unsigned>(grid), kRowThreads, 0, s>>>(a);
@@ -529,10 +654,18 @@ int lbt_embed_rows(void* stream, const void* table, int32_t dtype, int32_t n_row
   const lbt::EmbedCall c(n_tokens, n_features, n_rows, dtype);
   lbt::ProfScope ps(LBT_PROF_OTHER, s);
   return lbt::for_type(dtype, c.bytes, [&](auto type, auto bytes) -> int {
-    const int64_t blocks = (n_tokens * c.words + lbt::kRowThreads - 1) / lbt::kRowThreads;
-    LBT_REQUIRE(blocks < (int64_t(1) << 31), "too many elements");
-    lbt::embed_rows_kernel<decltype(type)::value, decltype(bytes)::value>
-      <<<static_cast<unsigned>(blocks), lbt::kRowThreads, 0, s>>>(table, n_rows, c.words, tokens, token_bytes, n_tokens, scale, out);
+    auto launch = [&](auto lanes) -> int {
+      constexpr int kLanes = decltype(lanes)::value, kRows = lbt::kRowThreads / kLanes;
+      const int64_t blocks = (n_tokens + kRows - 1) / kRows;
+      LBT_REQUIRE(blocks < (int64_t(1) << 31), "too many elements");
+      lbt::embed_rows_kernel<decltype(type)::value, decltype(bytes)::value, kLanes>
+        <<<static_cast<unsigned>(blocks), lbt::kRowThreads, 0, s>>>(table, n_rows, c.words, tokens, token_bytes, n_tokens, scale, out);
+      return LBT_OK;
+    };
+    // a wave takes a row, or a part of one a short row; 4 words of a lane at a time
+    if (c.words > 64) LBT_TRY(launch(std::integral_constant<int, 64>{}));
+    else if (c.words > 8) LBT_TRY(launch(std::integral_constant<int, 16>{}));
+    else LBT_TRY(launch(std::integral_constant<int, 4>{}));
     LBT_HIP(hipGetLastError());
     return LBT_OK;
   });
