@@ -159,13 +159,14 @@ __global__ void __launch_bounds__(kSortThreads)
 }
 
 // Many tokens: by digits of up to 10 bits, least significant first; each pass counts, adds up and moves.
-constexpr int kDigits = 1024, kSortEach = 4, kSortBlock = kSortThreads * kSortEach;
+constexpr int kDigits = 1024;  // at most; a block is kSortThreads * kSortEach entries
 
 __device__ __forceinline__ int sort_key(const void* tokens, int token_bytes, const int32_t* keys, int64_t i, int n_rows)
 {
   return keys != nullptr ? keys[i] : token_at(tokens, token_bytes, i, n_rows);
 }
 
+template <int kSortEach>
 __global__ void __launch_bounds__(kSortThreads)
   digit_count_kernel(const void* __restrict__ tokens, int token_bytes, const int32_t* __restrict__ keys, int64_t n, int n_rows,
                      int shift, int digits, int32_t* __restrict__ counts)
@@ -174,7 +175,7 @@ __global__ void __launch_bounds__(kSortThreads)
   count[threadIdx.x] = 0;
   __syncthreads();
   for (int e = 0; e < kSortEach; e++) {
-    const int64_t i = blockIdx.x * int64_t(kSortBlock) + e * kSortThreads + threadIdx.x;
+    const int64_t i = blockIdx.x * int64_t(kSortThreads * kSortEach) + e * kSortThreads + threadIdx.x;
     if (i < n) atomicAdd(&count[(sort_key(tokens, token_bytes, keys, i, n_rows) >> shift) & (digits - 1)], 1);
   }
   __syncthreads();
@@ -218,6 +219,7 @@ __global__ void __launch_bounds__(kSortThreads) digit_offsets_kernel(int digits,
 
 // A wave takes 256 consecutive entries, 64 at a time: the lanes of equal digits find one another by ballots, the first of
 // them moves the wave's count on. Ranks are then the block's offset, the waves before, and the place in the wave: stable.
+template <int kSortEach>
 __global__ void __launch_bounds__(kSortThreads)
   digit_move_kernel(const void* __restrict__ tokens, int token_bytes, const int32_t* __restrict__ keys,
                     const int32_t* __restrict__ places, int64_t n, int n_rows, int shift, int bits,
@@ -230,7 +232,7 @@ __global__ void __launch_bounds__(kSortThreads)
   for (int w = 0; w < kSortWaves; w++) count[w][threadIdx.x] = 0;
   if (static_cast<int>(threadIdx.x) < digits) first[threadIdx.x] = offsets[static_cast<int64_t>(blockIdx.x) * digits + threadIdx.x];
   __syncthreads();
-  const int64_t begin = blockIdx.x * int64_t(kSortBlock) + wave * (64 * kSortEach);
+  const int64_t begin = blockIdx.x * int64_t(kSortThreads * kSortEach) + wave * (64 * kSortEach);
   int key[kSortEach], digit[kSortEach], rank[kSortEach];
   for (int e = 0; e < kSortEach; e++) {
     const int64_t i = begin + e * 64 + lane;
@@ -531,7 +533,7 @@ int lane_bytes(int n_features, int dtype)
 struct EmbedCall {
   int64_t n_tokens;
   int n_features, n_rows, dtype;
-  int bytes, words, slices, chunk, bits, passes;
+  int bytes, words, slices, chunk, bits, passes, each;
   int64_t chunks, blocks;
   Sorted sorted[2];
   int32_t* counts;
@@ -546,7 +548,9 @@ struct EmbedCall {
     chunk = 64;
     while (chunk > 8 && (t / chunk) * slices < 4096) chunk /= 2;
     chunks = (t + chunk - 1) / chunk;
-    blocks = (t + kSortBlock - 1) / kSortBlock;
+    // entries of a thread of the sort: one while the blocks are few, as a block is a CU's work
+    each   = t <= 262144 ? 1 : 4;
+    blocks = (t + kSortThreads * each - 1) / (kSortThreads * each);
     bits   = 1;
     while ((int64_t(1) << bits) <= rows) bits++;  // keys go up to n_rows
     passes = (bits + 9) / 10;
@@ -582,18 +586,21 @@ int embed_gradient(hipStream_t s, const EmbedCall& c, const void* grad, const vo
     count_sort_kernel<<<static_cast<unsigned>((c.n_tokens + 63) / 64), kSortThreads, 0, s>>>(
       tokens, token_bytes, static_cast<int>(c.n_tokens), c.n_rows, c.sorted[0]);
   } else {
-    const int each = (c.bits + c.passes - 1) / c.passes;
+    const int width = (c.bits + c.passes - 1) / c.passes;  // bits of a digit
     for (int p = 0; p < c.passes; p++) {
-      const int shift     = p * each, bits = std::min(each, c.bits - shift);
+      const int shift     = p * width, bits = std::min(width, c.bits - shift);
       const int32_t* keys = p == 0 ? nullptr : c.sorted[at].key;
       const int32_t* from = p == 0 ? nullptr : c.sorted[at].place;
       const Sorted to     = c.sorted[1 - at];
       const unsigned grid = static_cast<unsigned>(c.blocks);
-      digit_count_kernel<<<grid, kSortThreads, 0, s>>>(tokens, token_bytes, keys, c.n_tokens, c.n_rows, shift, 1 << bits,
-                                                       c.counts);
-      digit_offsets_kernel<<<1, kSortThreads, 0, s>>>(1 << bits, static_cast<int>(c.blocks), c.counts);
-      digit_move_kernel<<<grid, kSortThreads, 0, s>>>(tokens, token_bytes, keys, from, c.n_tokens, c.n_rows, shift, bits,
-                                                      c.counts, to);
+      auto pass = [&](auto entries) {
+        constexpr int kEach = decltype(entries)::value;
+        digit_count_kernel<kEach><<<grid, kSortThreads, 0, s>>>(tokens, token_bytes, keys, c.n_tokens, c.n_rows, shift, 1 << bits, c.counts);
+        digit_offsets_kernel<<<1, kSortThreads, 0, s>>>(1 << bits, static_cast<int>(c.blocks), c.counts);
+        digit_move_kernel<kEach><<<grid, kSortThreads, 0, s>>>(tokens, token_bytes, keys, from, c.n_tokens, c.n_rows, shift, bits, c.counts, to);
+      };
+      if (c.each == 1) pass(std::integral_constant<int, 1>{});
+      else pass(std::integral_constant<int, 4>{});
       at = 1 - at;
     }
   }

@@ -87,6 +87,21 @@ __device__ __forceinline__ void store_value(void* p, int64_t i, float v)
     static_cast<uint16_t*>(p)[i] = narrow_value<kDtype>(v);
 }
 
+// Four values rounded to 16 bits, side by side.
+template <int kType>
+__device__ __forceinline__ uint2 narrow_four(const float (&v)[4])
+{
+  typedef __attribute__((ext_vector_type(4))) float Four;
+  const Four f = {v[0], v[1], v[2], v[3]};
+  if constexpr (kType == LBT_F16) {
+    typedef __attribute__((ext_vector_type(4))) _Float16 Half4;
+    return __builtin_bit_cast(uint2, __builtin_convertvector(f, Half4));
+  } else {
+    typedef __attribute__((ext_vector_type(4))) __bf16 Brain4;
+    return __builtin_bit_cast(uint2, __builtin_convertvector(f, Brain4));
+  }
+}
+
 // Four consecutive values of an output row of which `n` are inside.
 template <int kDtype>
 __device__ __forceinline__ void store_four(void* p, int64_t i, const float (&v)[4], int n, bool aligned)
@@ -95,9 +110,7 @@ __device__ __forceinline__ void store_four(void* p, int64_t i, const float (&v)[
     if constexpr (kDtype == LBT_F32) {
       *reinterpret_cast<float4*>(static_cast<float*>(p) + i) = make_float4(v[0], v[1], v[2], v[3]);
     } else {
-      const uint32_t a = narrow_value<kDtype>(v[0]) | static_cast<uint32_t>(narrow_value<kDtype>(v[1])) << 16;
-      const uint32_t b = narrow_value<kDtype>(v[2]) | static_cast<uint32_t>(narrow_value<kDtype>(v[3])) << 16;
-      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p) + i) = make_uint2(a, b);
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p) + i) = narrow_four<kDtype>(v);
     }
     return;
   }
@@ -206,16 +219,13 @@ __global__ void __launch_bounds__(256)
   const int col   = static_cast<int>(i % groups) * 8;
   const int64_t r = order != nullptr ? order[p] : (first_row + p < rows ? first_row + p : -1);
   uint16_t v[L::kPlanes][8];
-  const bool whole = r >= 0 && col + 8 <= cols && cols % 8 == 0 && (reinterpret_cast<uintptr_t>(from) & 15) == 0;
+  const bool whole = r >= 0 && col + 8 <= cols;
   float f[8];
-  if (whole) {
-    if constexpr (kDtype == LBT_F32) {
-      const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(from) + r * cols + col);
-      const float4 a = q[0], b = q[1];
-      f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-    } else {
-      *reinterpret_cast<uint4*>(v[0]) = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(from) + r * cols + col);
-    }
+  if (whole) {  // (rows of any length: the memory takes loads at any address)
+    if constexpr (kDtype == LBT_F32)
+      __builtin_memcpy(f, static_cast<const float*>(from) + r * cols + col, 32);
+    else
+      __builtin_memcpy(v[0], static_cast<const uint16_t*>(from) + r * cols + col, 16);
   } else {
 #pragma unroll
     for (int e = 0; e < 8; e++) {
@@ -267,19 +277,29 @@ __global__ void __launch_bounds__(256)
 
 __device__ __forceinline__ float exp_of(float d, bool exact) { return exact ? expf(d) : __expf(d); }
 
-// scores: m = classes, n = rows. Adds the bias; classes past the end count as masked.
+// scores: m = classes, n = rows. Adds the bias; classes past the end count as masked. Most tiles have neither.
 template <class Tile>
 __device__ __forceinline__ void add_bias(Float16v (&acc)[Tile::kMT][Tile::kNT], const float* bias, int class_first, int n_classes,
                                          int lane)
 {
+  if (bias != nullptr) {
+#pragma unroll
+    for (int i = 0; i < Tile::kMT; i++)
+#pragma unroll
+      for (int e = 0; e < 16; e++) {
+        const float b = bias[min(class_first + i * 32 + block_m(e, lane), n_classes - 1)];
+#pragma unroll
+        for (int j = 0; j < Tile::kNT; j++) acc[i][j][e] += b;
+      }
+  }
+  if (class_first + Tile::kWM <= n_classes) return;
 #pragma unroll
   for (int i = 0; i < Tile::kMT; i++)
 #pragma unroll
     for (int e = 0; e < 16; e++) {
-      const int c   = class_first + i * 32 + block_m(e, lane);
-      const float b = bias != nullptr && c < n_classes ? bias[c] : 0.f;
+      const bool in = class_first + i * 32 + block_m(e, lane) < n_classes;
 #pragma unroll
-      for (int j = 0; j < Tile::kNT; j++) acc[i][j][e] = c < n_classes ? acc[i][j][e] + b : -INFINITY;
+      for (int j = 0; j < Tile::kNT; j++) acc[i][j][e] = in ? acc[i][j][e] : -INFINITY;
     }
 }
 
@@ -311,11 +331,12 @@ struct LossEpilogue {
       const int64_t row = static_cast<int64_t>(tile_n) * Tile::kBN + wn * Tile::kWN + j * 32 + (lane & 31);
       const int label   = rows.label[row] - c0;
       if (__any(label >= 0 && label < Tile::kWM)) {
+        float at = 0.f;
 #pragma unroll
         for (int i = 0; i < Tile::kMT; i++)
 #pragma unroll
-          for (int e = 0; e < 16; e++)
-            if (i * 32 + block_m(e, lane) == label) rows.picked[row] = acc[i][j][e];
+          for (int e = 0; e < 16; e++) at = i * 32 + block_m(e, lane) == label ? acc[i][j][e] : at;
+        if (label >= 0 && label < Tile::kWM && ((label >> 2) & 1) == lane >> 5) rows.picked[row] = at;
       }
       float top = -INFINITY;
 #pragma unroll
@@ -515,36 +536,54 @@ __device__ __forceinline__ int64_t round_up_rows(int counted) { return (static_c
 
 // ---- joins ----------------------------------------------------------------------------------------
 
-constexpr int kJoinRows = 64, kJoinSlices = 16;
+constexpr int kJoinRows = 16, kJoinSlices = 64;
 
-// Top and total of each row from its shares by tile; its loss. 16 threads take the shares of a row between them, neighbours
-// in a wave are neighbouring rows.
+// Top and total of each row from its shares; its loss. 64 threads take the shares of a row between them, neighbours in a wave are
+// neighbouring rows.
 __global__ void __launch_bounds__(kJoinRows * kJoinSlices)
-  join_kernel(const float2* __restrict__ partial, int tiles, int64_t padded, LossRows rows, const RowCounts* __restrict__ counts,
+  join_kernel(const float2* __restrict__ partial, int shares, int64_t padded, LossRows rows, const RowCounts* __restrict__ counts,
               float* __restrict__ loss)
 {
-  __shared__ float2 share[kJoinSlices][kJoinRows];
+  __shared__ float tops[kJoinSlices][kJoinRows], totals[kJoinSlices][kJoinRows];
   const int n       = threadIdx.x % kJoinRows, slice = threadIdx.x / kJoinRows;
   const int64_t row = blockIdx.x * int64_t(kJoinRows) + n;
   const int counted = counts->rows;
   if (blockIdx.x * int64_t(kJoinRows) >= counted) return;
+  constexpr int kAhead = 8;  // shares asked for together
+  float2 s[kAhead];
+  auto load = [&](int first) {
+#pragma unroll
+    for (int e = 0; e < kAhead; e++) {
+      const int t = first + e * kJoinSlices;
+      s[e]        = t < shares ? partial[t * padded + row] : make_float2(-INFINITY, 0.f);
+    }
+  };
   float top = -INFINITY, total = 0.f;
-  for (int t = slice; t < tiles; t += kJoinSlices) {
-    const float2 s   = partial[t * padded + row];
-    const float next = fmaxf(top, s.x);
+  for (int first = slice; first < shares; first += kAhead * kJoinSlices) {
+    load(first);
+    float next = top;
+#pragma unroll
+    for (int e = 0; e < kAhead; e++) next = fmaxf(next, s[e].x);
     const float from = next == -INFINITY ? 0.f : next;
-    total            = total * expf(top - from) + s.y * expf(s.x - from);
-    top              = next;
+    total *= expf(top - from);
+#pragma unroll
+    for (int e = 0; e < kAhead; e++) total += s[e].y * expf(s[e].x - from);
+    top = next;
   }
-  share[slice][n] = make_float2(top, total);
+  tops[slice][n] = top;
+  __syncthreads();
+  float all = -INFINITY;
+#pragma unroll 8
+  for (int v = 0; v < kJoinSlices; v++) all = fmaxf(all, tops[v][n]);
+  const float from = all == -INFINITY ? 0.f : all;
+  totals[slice][n] = total * expf(top - from);
   __syncthreads();
   if (slice != 0 || row >= counted) return;
-  for (int s = 1; s < kJoinSlices; s++) top = fmaxf(top, share[s][n].x);
-  const float from = top == -INFINITY ? 0.f : top;
-  total            = 0.f;
-  for (int s = 0; s < kJoinSlices; s++) total += share[s][n].y * expf(share[s][n].x - from);
+  total = 0.f;
+#pragma unroll 8
+  for (int v = 0; v < kJoinSlices; v++) total += totals[v][n];
   // where every class is masked there is no probability: the loss is infinite and p is 0
-  const bool none = top == -INFINITY && total == 0.f;
+  const bool none = all == -INFINITY && total == 0.f;
   rows.top[row]     = from;
   rows.inverse[row] = none ? 0.f : 1.f / total;
   loss[rows.order[row]] = none ? INFINITY : (from - rows.picked[row]) + logf(total);
@@ -848,15 +887,25 @@ __global__ void __launch_bounds__(256)
   store_four<kDtype>(out, r * cols + col, v, cols - col, cols % 4 == 0);
 }
 
-__global__ void __launch_bounds__(256)
-  finish_bias_kernel(const float* __restrict__ sums, int n_classes, int tile_rows, const RowCounts* __restrict__ counts, int half,
+// grad_bias from its sums over blocks of rows; a class's blocks are shared out among 16 threads.
+__global__ void __launch_bounds__(kJoinRows * kJoinSlices)
+  finish_bias_kernel(const float* __restrict__ sums, int n_classes, int block_rows, const RowCounts* __restrict__ counts, int half,
                      float* __restrict__ out)
 {
-  const int c = blockIdx.x * 256 + threadIdx.x;
-  if (c >= n_classes) return;
-  const int tiles = (counts->rows + tile_rows - 1) / tile_rows;
-  float sum       = 0.f;
-  for (int t = 0; t < tiles; t++) sum += sums[static_cast<int64_t>(t) * n_classes + c];
+  __shared__ float share[kJoinSlices][kJoinRows];
+  const int n = threadIdx.x % kJoinRows, slice = threadIdx.x / kJoinRows;
+  const int c      = blockIdx.x * kJoinRows + n;
+  const int blocks = (counts->rows + block_rows - 1) / block_rows;
+  float sum        = 0.f;
+  if (c < n_classes) {
+#pragma unroll 8
+    for (int t = slice; t < blocks; t += kJoinSlices) sum += sums[static_cast<int64_t>(t) * n_classes + c];
+  }
+  share[slice][n] = sum;
+  __syncthreads();
+  if (slice != 0 || c >= n_classes) return;
+  sum = 0.f;
+  for (int s = 0; s < kJoinSlices; s++) sum += share[s][n];
   out[c] = half ? ldexpf(sum, counts->exponent - kHalfShift) : sum;
 }
 
@@ -870,7 +919,7 @@ __global__ void __launch_bounds__(256) clear_kernel(uint16_t* __restrict__ out, 
 
 using LargeTile  = ProductTile<256, 256, 2, 4, 2>;
 using MediumTile = ProductTile<128, 128, 2, 2, 2>;
-using SmallTile  = ProductTile<64, 64, 2, 2, 4>;
+using SmallTile  = ProductTile<64, 64, 2, 2, 5>;
 
 int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 int64_t tiles_of(int64_t v, int64_t by) { return (v + by - 1) / by; }
@@ -1131,7 +1180,7 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
                                                                            c.n_rows, c.features, c.rows, grad_X);
   LBT_HIP(hipGetLastError());
   if (grad_bias != nullptr) {
-    finish_bias_kernel<<<static_cast<unsigned>(tiles_of(c.classes, 256)), 256, 0, s>>>(c.bias_sums, c.classes,
+    finish_bias_kernel<<<static_cast<unsigned>(tiles_of(c.classes, kJoinRows)), kJoinRows * kJoinSlices, 0, s>>>(c.bias_sums, c.classes,
                                                                                        c.kept ? c.scale_rows : c.scores.tile, c.counts, kHalf,
                                                                                        grad_bias);
     LBT_HIP(hipGetLastError());
