@@ -597,7 +597,7 @@ __global__ void __launch_bounds__(kJoinRows * kJoinSlices)
 // for both operands, which is all a product asks of it. float goes to the float products of the matrix cores as it is. Rows are not
 // taken out: what a row that does not count holds stays in its own column.
 // kShared: the four waves of a workgroup share out k instead of taking 16 classes each, where the classes would give the CUs too
-// few waves to keep memory busy.
+// few waves to keep memory busy. More than 16 rows have two blocks of classes beside theirs, so that the rows are read less often.
 
 typedef __attribute__((ext_vector_type(4))) float Float4v;
 
@@ -632,49 +632,56 @@ struct FewStep {  // 16 bytes of a row: kValues of k
   }
 };
 
-template <int kDtype, int kBlocks, bool kShared>
+template <int kDtype, int kBlocks, int kClassBlocks, bool kShared>
 __global__ void __launch_bounds__(kFewThreads)
   few_rows_kernel(const void* __restrict__ X, const void* __restrict__ weight, const float* __restrict__ bias,
-                  const int64_t* __restrict__ y, int n_rows, int cols, int n_classes, int tiles, float2* __restrict__ partial,
+                  const int64_t* __restrict__ y, int n_rows, int cols, int n_classes, int shares, float2* __restrict__ partial,
                   float* __restrict__ picked)
 {
   using S = FewStep<kDtype>;
   using V = typename S::Value;
   constexpr bool kExact = kDtype == LBT_F32;
-  constexpr int kWaves = kFewThreads / 64, kUnroll = kBlocks >= 4 ? 2 : 4, kStep = 4 * S::kValues;  // k of a product
-  __shared__ float4 sums[kShared ? kWaves * kBlocks * 64 : 1];
-  __shared__ float2 share[kWaves][16 * kBlocks];
+  constexpr int kWaves = kFewThreads / 64, kUnroll = kBlocks >= 3 ? 2 : 4, kStep = 4 * S::kValues;  // k of a product
+  constexpr int kClasses = 16 * kClassBlocks;                                                       // of a wave
+  __shared__ float4 sums[kShared ? kWaves * kClassBlocks * kBlocks * 64 : 1];
+  __shared__ float2 share[kWaves][kClassBlocks][16 * kBlocks];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int c0 = blockIdx.x * (kShared ? 16 : 64) + (kShared ? 0 : wave * 16);  // of this wave
-  const V* w   = static_cast<const V*>(weight) + static_cast<int64_t>(min(c0 + (lane & 15), n_classes - 1)) * cols;
-  const V* x[kBlocks];
+  const int c0 = blockIdx.x * (kShared ? kClasses : kWaves * kClasses) + (kShared ? 0 : wave * kClasses);  // of this wave
+  const V *w[kClassBlocks], *x[kBlocks];
+#pragma unroll
+  for (int i = 0; i < kClassBlocks; i++)
+    w[i] = static_cast<const V*>(weight) + static_cast<int64_t>(min(c0 + i * 16 + (lane & 15), n_classes - 1)) * cols;
 #pragma unroll
   for (int b = 0; b < kBlocks; b++)
     x[b] = static_cast<const V*>(X) + static_cast<int64_t>(min(b * 16 + (lane & 15), n_rows - 1)) * cols;
   const int at  = (lane >> 4) * S::kValues;
   const int hop = kShared ? kWaves * kUnroll * kStep : kUnroll * kStep;  // k of a turn, from wave to wave
-  Float4v acc[kBlocks];
+  Float4v acc[kClassBlocks][kBlocks];
 #pragma unroll
-  for (int b = 0; b < kBlocks; b++) acc[b] = Float4v{0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < kClassBlocks; i++)
+#pragma unroll
+    for (int b = 0; b < kBlocks; b++) acc[i][b] = Float4v{0.f, 0.f, 0.f, 0.f};
   int k = kShared ? wave * kUnroll * kStep : 0;
-  S a[kUnroll], m[kBlocks][kUnroll];
+  S a[kUnroll][kClassBlocks], m[kUnroll][kBlocks];
   auto load = [&](int from) {
 #pragma unroll
     for (int u = 0; u < kUnroll; u++) {
-      a[u].load(w, from + u * kStep + at);
 #pragma unroll
-      for (int b = 0; b < kBlocks; b++) m[b][u].load(x[b], from + u * kStep + at);
+      for (int i = 0; i < kClassBlocks; i++) a[u][i].load(w[i], from + u * kStep + at);
+#pragma unroll
+      for (int b = 0; b < kBlocks; b++) m[u][b].load(x[b], from + u * kStep + at);
     }
   };
   bool whole = k + kUnroll * kStep <= cols;
   if (whole) load(k);
   while (whole) {  // the next turn is asked for before this one is multiplied
-    S a1[kUnroll], m1[kBlocks][kUnroll];
+    S a1[kUnroll][kClassBlocks], m1[kUnroll][kBlocks];
 #pragma unroll
     for (int u = 0; u < kUnroll; u++) {
-      a1[u] = a[u];
 #pragma unroll
-      for (int b = 0; b < kBlocks; b++) m1[b][u] = m[b][u];
+      for (int i = 0; i < kClassBlocks; i++) a1[u][i] = a[u][i];
+#pragma unroll
+      for (int b = 0; b < kBlocks; b++) m1[u][b] = m[u][b];
     }
     k += hop;
     whole = k + kUnroll * kStep <= cols;
@@ -682,68 +689,76 @@ __global__ void __launch_bounds__(kFewThreads)
 #pragma unroll
     for (int u = 0; u < kUnroll; u++)
 #pragma unroll
-      for (int b = 0; b < kBlocks; b++) acc[b] = S::multiply(a1[u], m1[b][u], acc[b]);
+      for (int i = 0; i < kClassBlocks; i++)
+#pragma unroll
+        for (int b = 0; b < kBlocks; b++) acc[i][b] = S::multiply(a1[u][i], m1[u][b], acc[i][b]);
   }
   for (int u = 0; u < kUnroll && k + u * kStep < cols; u++) {  // the end of the rows
-    S e, f;
-    e.load_end(w, k + u * kStep + at, cols);
+    S e[kClassBlocks], f;
+#pragma unroll
+    for (int i = 0; i < kClassBlocks; i++) e[i].load_end(w[i], k + u * kStep + at, cols);
 #pragma unroll
     for (int b = 0; b < kBlocks; b++) {
       f.load_end(x[b], k + u * kStep + at, cols);
-      acc[b] = S::multiply(e, f, acc[b]);
+#pragma unroll
+      for (int i = 0; i < kClassBlocks; i++) acc[i][b] = S::multiply(e[i], f, acc[i][b]);
     }
   }
   if constexpr (kShared) {
 #pragma unroll
-    for (int b = 0; b < kBlocks; b++) sums[(wave * kBlocks + b) * 64 + lane] = make_float4(acc[b][0], acc[b][1], acc[b][2], acc[b][3]);
+    for (int i = 0; i < kClassBlocks; i++)
+#pragma unroll
+      for (int b = 0; b < kBlocks; b++)
+        sums[((wave * kClassBlocks + i) * kBlocks + b) * 64 + lane] = make_float4(acc[i][b][0], acc[i][b][1], acc[i][b][2], acc[i][b][3]);
     __syncthreads();
   }
 #pragma unroll
-  for (int b = 0; b < kBlocks; b++) {  // lane: row lane % 16, classes 4 (lane / 16) ...
-    if constexpr (kShared) {
-      if (b % kWaves != wave) continue;
-      float4 t = sums[b * 64 + lane];
-      for (int v = 1; v < kWaves; v++) {
-        const float4 o = sums[(v * kBlocks + b) * 64 + lane];
-        t.x += o.x; t.y += o.y; t.z += o.z; t.w += o.w;
+  for (int i = 0; i < kClassBlocks; i++)
+#pragma unroll
+    for (int b = 0; b < kBlocks; b++) {  // lane: row lane % 16, classes 4 (lane / 16) ...
+      if constexpr (kShared) {
+        if ((i * kBlocks + b) % kWaves != wave) continue;
+        Float4v t = Float4v{0.f, 0.f, 0.f, 0.f};
+        for (int v = 0; v < kWaves; v++) t += __builtin_bit_cast(Float4v, sums[((v * kClassBlocks + i) * kBlocks + b) * 64 + lane]);
+        acc[i][b] = t;
       }
-      acc[b] = Float4v{t.x, t.y, t.z, t.w};
-    }
-    const int r     = b * 16 + (lane & 15);
-    const int first = c0 + 4 * (lane >> 4);
-    const int64_t label = r < n_rows ? y[r] : -1;
-    float top = -INFINITY;
+      const int r         = b * 16 + (lane & 15);
+      const int first     = c0 + i * 16 + 4 * (lane >> 4);
+      const int64_t label = r < n_rows ? y[r] : -1;
+      float top           = -INFINITY;
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
-      const int c = first + e;
-      acc[b][e]   = c < n_classes ? acc[b][e] + (bias != nullptr ? bias[c] : 0.f) : -INFINITY;
-      if (c == label && c < n_classes) picked[r] = acc[b][e];
-      top = fmaxf(top, acc[b][e]);
-    }
-    top = fmaxf(top, __shfl_xor(top, 16));
-    top = fmaxf(top, __shfl_xor(top, 32));
-    const float from = top == -INFINITY ? 0.f : top;
-    float total      = 0.f;
+      for (int e = 0; e < 4; e++) {
+        const int c  = first + e;
+        acc[i][b][e] = c < n_classes ? acc[i][b][e] + (bias != nullptr ? bias[c] : 0.f) : -INFINITY;
+        if (c == label && c < n_classes) picked[r] = acc[i][b][e];
+        top = fmaxf(top, acc[i][b][e]);
+      }
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      const float from = top == -INFINITY ? 0.f : top;
+      float total      = 0.f;
 #pragma unroll
-    for (int e = 0; e < 4; e++) total += exp_of(acc[b][e] - from, kExact);
-    total += __shfl_xor(total, 16);
-    total += __shfl_xor(total, 32);
-    if constexpr (kShared) {
-      if (lane < 16 && r < n_rows) partial[static_cast<int64_t>(r) * tiles + blockIdx.x] = make_float2(top, total);
-    } else {
-      if (lane < 16) share[wave][b * 16 + lane] = make_float2(top, total);
+      for (int e = 0; e < 4; e++) total += exp_of(acc[i][b][e] - from, kExact);
+      total += __shfl_xor(total, 16);
+      total += __shfl_xor(total, 32);
+      if constexpr (kShared) {
+        if (lane < 16 && r < n_rows) partial[static_cast<int64_t>(r) * shares + blockIdx.x * kClassBlocks + i] = make_float2(top, total);
+      } else {
+        if (lane < 16) share[wave][i][r] = make_float2(top, total);
+      }
     }
-  }
   if constexpr (!kShared) {
     __syncthreads();
-    const int r = threadIdx.x;
-    if (r >= n_rows || r >= 16 * kBlocks) return;
-    float top = share[0][r].x;
-    for (int v = 1; v < kWaves; v++) top = fmaxf(top, share[v][r].x);
-    const float from = top == -INFINITY ? 0.f : top;
-    float total      = 0.f;
-    for (int v = 0; v < kWaves; v++) total += share[v][r].y * exp_of(share[v][r].x - from, kExact);
-    partial[static_cast<int64_t>(r) * tiles + blockIdx.x] = make_float2(top, total);
+    for (int t = threadIdx.x; t < kClassBlocks * 16 * kBlocks; t += kFewThreads) {
+      const int i = t / (16 * kBlocks), r = t % (16 * kBlocks);
+      if (r >= n_rows) continue;
+      float top = share[0][i][r].x;
+      for (int v = 1; v < kWaves; v++) top = fmaxf(top, share[v][i][r].x);
+      const float from = top == -INFINITY ? 0.f : top;
+      float total      = 0.f;
+      for (int v = 0; v < kWaves; v++) total += share[v][i][r].y * exp_of(share[v][i][r].x - from, kExact);
+      partial[static_cast<int64_t>(r) * shares + blockIdx.x * kClassBlocks + i] = make_float2(top, total);
+    }
   }
 }
 
@@ -1188,17 +1203,19 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
   return LBT_OK;
 }
 
-// Workgroups of the scores of few rows; four waves share the classes of one where they would be fewer than four a CU.
+// Scores of few rows: four waves share the classes of a workgroup where they would be fewer than four a CU.
 bool few_shared(int classes) { return classes < 65536; }
-int64_t few_tiles(int classes) { return tiles_of(classes, few_shared(classes) ? 16 : 64); }
+int few_class_blocks(int64_t n_rows) { return n_rows <= 16 ? 1 : 2; }
+int64_t few_groups(int classes, int class_blocks) { return tiles_of(classes, 16 * class_blocks * (few_shared(classes) ? 1 : 4)); }
 
 struct FewCall {
   float2* partial;
   float* picked;
   void carve(Arena& arena, int64_t n_rows, int classes)
   {
-    partial = arena.take<float2>(n_rows * few_tiles(classes));
-    picked  = arena.take<float>(n_rows);
+    const int blocks = few_class_blocks(n_rows);
+    partial          = arena.take<float2>(n_rows * few_groups(classes, blocks) * blocks);
+    picked           = arena.take<float>(n_rows);
   }
 };
 
@@ -1206,14 +1223,15 @@ template <int kDtype, int kBlocks>
 int few_log_loss(hipStream_t s, const FewCall& c, const void* X, const void* weight, const float* bias, const int64_t* y, int n_rows,
                  int features, int classes, float* loss)
 {
-  const int tiles = static_cast<int>(few_tiles(classes));
+  constexpr int kClassBlocks = kBlocks == 1 ? 1 : 2;
+  const int groups = static_cast<int>(few_groups(classes, kClassBlocks)), shares = groups * kClassBlocks;
   if (few_shared(classes))
-    few_rows_kernel<kDtype, kBlocks, true>
-      <<<tiles, kFewThreads, 0, s>>>(X, weight, bias, y, n_rows, features, classes, tiles, c.partial, c.picked);
+    few_rows_kernel<kDtype, kBlocks, kClassBlocks, true>
+      <<<groups, kFewThreads, 0, s>>>(X, weight, bias, y, n_rows, features, classes, shares, c.partial, c.picked);
   else
-    few_rows_kernel<kDtype, kBlocks, false>
-      <<<tiles, kFewThreads, 0, s>>>(X, weight, bias, y, n_rows, features, classes, tiles, c.partial, c.picked);
-  join_few_kernel<<<n_rows, kFewThreads, 0, s>>>(c.partial, tiles, c.picked, y, classes, loss);
+    few_rows_kernel<kDtype, kBlocks, kClassBlocks, false>
+      <<<groups, kFewThreads, 0, s>>>(X, weight, bias, y, n_rows, features, classes, shares, c.partial, c.picked);
+  join_few_kernel<<<n_rows, kFewThreads, 0, s>>>(c.partial, shares, c.picked, y, classes, loss);
   LBT_HIP(hipGetLastError());
   return LBT_OK;
 }
@@ -1224,6 +1242,7 @@ int few_log_loss(hipStream_t s, const FewCall& c, const void* X, const void* wei
 {
   if (n_rows <= 16) return few_log_loss<kDtype, 1>(s, c, X, weight, bias, y, n_rows, features, classes, loss);
   if (n_rows <= 32) return few_log_loss<kDtype, 2>(s, c, X, weight, bias, y, n_rows, features, classes, loss);
+  if (n_rows <= 48) return few_log_loss<kDtype, 3>(s, c, X, weight, bias, y, n_rows, features, classes, loss);
   return few_log_loss<kDtype, 4>(s, c, X, weight, bias, y, n_rows, features, classes, loss);
 }
 

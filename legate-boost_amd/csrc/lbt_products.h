@@ -61,6 +61,8 @@ struct ProductTile {
   static constexpr int kWaves = kWaveM * kWaveN, kThreads = kWaves * 64;
   static constexpr int kMT = kWM / 32, kNT = kWN / 32;  // 32 x 32 blocks of a wave
   static constexpr int kStages = kDepth;                // of the LDS
+  // Steps of 16 of k whose fragments are read together: a wave of one block has too little to multiply in a step to cover a read.
+  static constexpr int kGroup = kMT == 1 ? kProductK / 16 : 1;
   static constexpr int kStageA = kM * kProductK * 2, kStageB = kN * kProductK * 2;  // bytes
   static constexpr int kLoads = (kM + kN) * kProductK / 8 / kThreads;               // of a lane for a stage
 };
@@ -101,12 +103,17 @@ __device__ __forceinline__ int turned(int row)
   return (row & (kTile >= 128 ? 3 : 1)) << 2;
 }
 
-// Where a lane's chunks of a stage lie in an operand, relative to the stage's first element.
+// One operand's way through the stages of a product: kTile of its m (or n) from `tile0` on, 64 of k at a time from `k_first`
+// to `k_end`, once for each plane that is multiplied. What a stage asks of the scalar unit is an addition and a comparison:
+// with small tiles that is what a stage takes.
 template <bool kRowsAreK, int kTile, int kWaves>
 struct StageLoader {
-  static constexpr int kEach = kTile * kProductK / 8 / (kWaves * 64);  // chunks of 16 bytes
+  static constexpr int kEach = kTile * kProductK / 8 / (kWaves * 64);  // chunks of 16 bytes of a lane
   static_assert(kEach * kWaves * 64 * 8 == kTile * kProductK, "every lane loads the same number of chunks");
-  uint32_t offset[kEach];
+  const uint16_t* at;       // first element of the next stage
+  int64_t step;             // from stage to stage
+  int whole;                // stages of a plane that lie inside the operand
+  uint32_t offset[kEach];   // of a lane's chunks, bytes
 
   static __device__ __forceinline__ void place(int j, int wave, int lane, int* row, int* col)
   {
@@ -120,8 +127,17 @@ struct StageLoader {
       *col = ((q & 7) ^ (*row & 7)) * 8;
     }
   }
-  __device__ __forceinline__ void init(const ProductOperand& op, int wave, int lane)
+  __device__ __forceinline__ void begin(const ProductOperand& op, int plane, int tile0, int k_first)
   {
+    at = op.base + plane * op.plane + (kRowsAreK ? static_cast<int64_t>(k_first) * op.ld + tile0 : static_cast<int64_t>(tile0) * op.ld + k_first);
+  }
+  __device__ __forceinline__ void init(const ProductOperand& op, int tile0, int k_first, int k_end, int wave, int lane)
+  {
+    const int limit = kRowsAreK ? op.rows : op.cols;  // of k
+    const bool edge = tile0 + kTile > (kRowsAreK ? op.cols : op.rows);
+    // (the last stage may reach past k_end: there the other operand, or this one, holds zeros)
+    whole = edge ? 0 : max(0, min((k_end - k_first + kProductK - 1) / kProductK, (limit - k_first) / kProductK));
+    step  = kRowsAreK ? kProductK * op.ld : kProductK;
 #pragma unroll
     for (int j = 0; j < kEach; j++) {
       int row, col;
@@ -129,27 +145,26 @@ struct StageLoader {
       offset[j] = (static_cast<uint32_t>(row) * static_cast<uint32_t>(op.ld) + col) * 2;
     }
   }
-  // Asks for kTile of its m (or n) from `tile0` on, 64 of its k from `k0` on; stages that reach past the operand, or past the
-  // product's end (not `live`), take zeros there.
-  __device__ __forceinline__ void load(const ProductOperand& op, const uint16_t* plane, int tile0, int k0, bool live,
-                                       const uint16_t* zeros, uint32_t lds, int wave, int lane) const
+  // Asks for stage `s` of a plane. One that reaches past the operand, or that there is none of (not `live`), has zeros there.
+  __device__ __forceinline__ void load(const ProductOperand& op, int tile0, int k_first, int s, bool live, const uint16_t* zeros,
+                                       uint32_t lds, int wave, int lane)
   {
-    const int row0 = kRowsAreK ? k0 : tile0, col0 = kRowsAreK ? tile0 : k0;
-    constexpr int kRows = kRowsAreK ? kProductK : kTile, kCols = kRowsAreK ? kTile : kProductK;
-    const uint16_t* base = plane + static_cast<int64_t>(row0) * op.ld + col0;
-    if (live && row0 + kRows <= op.rows && col0 + kCols <= op.cols) {
+    if (s < whole) {
 #pragma unroll
-      for (int j = 0; j < kEach; j++) load_to_lds(base, offset[j], lds + (j * kWaves + wave) * 1024);
+      for (int j = 0; j < kEach; j++) load_to_lds(at, offset[j], lds + (j * kWaves + wave) * 1024);
     } else {
+      const int k0   = k_first + s * kProductK;
+      const int row0 = kRowsAreK ? k0 : tile0, col0 = kRowsAreK ? tile0 : k0;
 #pragma unroll
       for (int j = 0; j < kEach; j++) {
         int row, col;
         place(j, wave, lane, &row, &col);
         const bool inside   = live && row0 + row < op.rows && col0 + col < op.cols;
-        const uint16_t* from = base + static_cast<int64_t>(row) * op.ld + col;
+        const uint16_t* from = at + static_cast<int64_t>(row) * op.ld + col;
         load_to_lds(inside ? from : zeros, lds + (j * kWaves + wave) * 1024);
       }
     }
+    at += step;
   }
 };
 
@@ -209,7 +224,7 @@ struct PlanePairs<3> {
 enum { kRowsN = 0, kRowsK = 1 };
 
 template <class Tile, int kType, int kPlanes, bool kAMajor, bool kBMajor, int kRowsSide, class Epilogue>
-__global__ void __launch_bounds__(Tile::kThreads, 1) product_kernel(const ProductArgs args, const Epilogue epilogue)
+__global__ void __launch_bounds__(Tile::kThreads, 2) product_kernel(const ProductArgs args, const Epilogue epilogue)
 {
   constexpr int kStage = Tile::kStageA + Tile::kStageB, kSteps = kProductK / 16;
   __shared__ __attribute__((aligned(1024))) char lds[Tile::kStages * kStage];
@@ -236,62 +251,105 @@ __global__ void __launch_bounds__(Tile::kThreads, 1) product_kernel(const Produc
   const int total = steps * PlanePairs<kPlanes>::kCount;
   StageLoader<kAMajor, Tile::kBM, Tile::kWaves> load_a;
   StageLoader<kBMajor, Tile::kBN, Tile::kWaves> load_b;
-  load_a.init(args.a, wave, lane);
-  load_b.init(args.b, wave, lane);
+  const int m0 = tile_m * Tile::kBM, n0 = tile_n * Tile::kBN;
+  load_a.init(args.a, m0, k_first, k_end, wave, lane);
+  load_b.init(args.b, n0, k_first, k_end, wave, lane);
+  load_a.begin(args.a, PlanePairs<kPlanes>::a(0), m0, k_first);
+  load_b.begin(args.b, PlanePairs<kPlanes>::b(0), n0, k_first);
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds));
-  // (one operand of stage t of the product, to where `stage` lies)
-  auto load = [&](int t, int stage, auto second) {
-    const int pair  = kPlanes == 1 ? 0 : t / max(steps, 1);
-    const int k0    = k_first + (kPlanes == 1 ? t : t % max(steps, 1)) * kProductK;
-    const bool live = t < total;
+  // Stages are asked for in order, the first operand's part before the second's: stage `asked` of the pair `pair` of planes.
+  int asked = 0, pair = 0;
+  bool live = total > 0;
+  if (!live) load_a.whole = load_b.whole = 0;
+  auto load = [&](int stage, auto second) {
     const uint32_t at = lds0 + stage * kStage;
-    if constexpr (decltype(second)::value)
-      load_b.load(args.b, args.b.base + PlanePairs<kPlanes>::b(pair) * args.b.plane, tile_n * Tile::kBN, k0, live, args.zeros,
-                  at + Tile::kStageA, wave, lane);
-    else
-      load_a.load(args.a, args.a.base + PlanePairs<kPlanes>::a(pair) * args.a.plane, tile_m * Tile::kBM, k0, live, args.zeros,
-                  at, wave, lane);
+    if constexpr (!decltype(second)::value) {
+      load_a.load(args.a, m0, k_first, asked, live, args.zeros, at, wave, lane);
+    } else {
+      load_b.load(args.b, n0, k_first, asked, live, args.zeros, at + Tile::kStageA, wave, lane);
+      if (++asked < steps) return;
+      asked = 0;
+      pair++;
+      if (pair < PlanePairs<kPlanes>::kCount && steps > 0) {
+        load_a.begin(args.a, PlanePairs<kPlanes>::a(pair), m0, k_first);
+        load_b.begin(args.b, PlanePairs<kPlanes>::b(pair), n0, k_first);
+      } else {
+        live         = false;
+        load_a.whole = load_b.whole = 0;
+      }
+    }
   };
   constexpr std::false_type kA{};
   constexpr std::true_type kB{};
-  Short8 a[2][Tile::kMT], b[2][Tile::kNT];
+  // A group of steps' fragments are read while those of the group before are multiplied.
+  constexpr int kGroup = Tile::kGroup, kGroups = kSteps / kGroup;
+  Short8 a[2][kGroup][Tile::kMT], b[2][kGroup][Tile::kNT];
   // The i-th part of the fragments of a step: one of each operand.
   auto read = [&](const char* at, int kk, int to, int i) {
-    if (i < Tile::kMT) a[to][i] = fragment<kAMajor, Tile::kBM>(at, wm * Tile::kWM + i * 32, kk, lane);
-    if (i < Tile::kNT) b[to][i] = fragment<kBMajor, Tile::kBN>(at + Tile::kStageA, wn * Tile::kWN + i * 32, kk, lane);
+    if (i < Tile::kMT) a[to][kk % kGroup][i] = fragment<kAMajor, Tile::kBM>(at, wm * Tile::kWM + i * 32, kk, lane);
+    if (i < Tile::kNT) b[to][kk % kGroup][i] = fragment<kBMajor, Tile::kBN>(at + Tile::kStageA, wn * Tile::kWN + i * 32, kk, lane);
   };
-  // Stages are asked for kStages ahead. The fragments of a step are read while the step before is multiplied; those of a stage's
-  // first step while the last one of the stage before is, after all waves have met: then that stage has been read by all,
-  // and is filled again, and the next has arrived. Reads and loads are dealt out between the multiplications.
+  // Stages are asked for kStages ahead. The fragments of a stage's first group are read while the last one of the stage before is
+  // multiplied, after all waves have met: then that stage has been read by all, and is filled again, and the next has arrived.
+  // Reads and loads are dealt out between the multiplications.
 #pragma unroll
   for (int s = 0; s < Tile::kStages; s++) {
-    load(s, s, kA);
-    load(s, s, kB);
+    load(s, kA);
+    load(s, kB);
   }
   wait_and_meet<(Tile::kStages - 1) * Tile::kLoads>();
   static_assert(Tile::kMT >= Tile::kNT, "the parts of a step are those of the first operand");
 #pragma unroll
-  for (int i = 0; i < Tile::kMT; i++) read(lds, 0, 0, i);
+  for (int kk = 0; kk < kGroup; kk++)
+#pragma unroll
+    for (int i = 0; i < Tile::kMT; i++) read(lds, kk, 0, i);
   int stage = 0;
-  for (int t = 0; t < total; t++) {
+  // `own`: which half of the fragments holds the stage's first group
+  auto multiply_stage = [&](auto own) {
     const int next = stage + 1 == Tile::kStages ? 0 : stage + 1;
 #pragma unroll
-    for (int kk = 0; kk < kSteps; kk++) {
-      const bool last = kk + 1 == kSteps;
+    for (int group = 0; group < kGroups; group++) {
+      const int from  = (decltype(own)::value + group) & 1;
+      const bool last = group + 1 == kGroups;
       if (last) wait_and_meet<(Tile::kStages - 2) * Tile::kLoads>();
 #pragma unroll
-      for (int i = 0; i < Tile::kMT; i++) {
-        if (last) read(lds + next * kStage, 0, 0, i);
-        else read(lds + stage * kStage, kk + 1, (kk + 1) & 1, i);
+      for (int kk = 0; kk < kGroup; kk++)
+#pragma unroll
+        for (int i = 0; i < Tile::kMT; i++) {
+          if (last) read(lds + next * kStage, kk, 1 - from, i);
+          else read(lds + stage * kStage, (group + 1) * kGroup + kk, 1 - from, i);
+          if constexpr (kGroup > 1) continue;  // (all reads of a group of several steps come first)
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int j = 0; j < Tile::kNT; j++) acc[i][j] = mfma_32x32x16<kType>(a[from][kk][i], b[from][kk][j], acc[i][j]);
+          __builtin_amdgcn_sched_barrier(0);
+          if (last && i == 0) load(stage, kA);
+          if (last && i == Tile::kMT / 2) load(stage, kB);
+        }
+      if constexpr (kGroup > 1) {
+        if (last) {
+          load(stage, kA);
+          load(stage, kB);
+        }
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int j = 0; j < Tile::kNT; j++) acc[i][j] = mfma_32x32x16<kType>(a[kk & 1][i], b[kk & 1][j], acc[i][j]);
+        for (int kk = 0; kk < kGroup; kk++)
+#pragma unroll
+          for (int i = 0; i < Tile::kMT; i++)
+#pragma unroll
+            for (int j = 0; j < Tile::kNT; j++) acc[i][j] = mfma_32x32x16<kType>(a[from][kk][i], b[from][kk][j], acc[i][j]);
         __builtin_amdgcn_sched_barrier(0);
-        if (last && i == 0) load(t + Tile::kStages, stage, kA);
-        if (last && i == Tile::kMT / 2) load(t + Tile::kStages, stage, kB);
       }
     }
     stage = next;
+  };
+  if constexpr (kGroups % 2 == 0) {
+    for (int t = 0; t < total; t++) multiply_stage(std::integral_constant<int, 0>{});
+  } else {
+    for (int t = 0; t < total; t += 2) {
+      multiply_stage(std::integral_constant<int, 0>{});
+      if (t + 1 < total) multiply_stage(std::integral_constant<int, 1>{});
+    }
   }
   wait_and_meet<0>();  // the LDS is free for what follows
   epilogue.template store<Tile>(acc, tile_m, tile_n, wm, wn, lane, rows, args.counts, lds);
