@@ -217,20 +217,54 @@ __global__ void __launch_bounds__(kSortThreads) digit_offsets_kernel(int digits,
   }
 }
 
+// Where a block's entries of each digit begin, from the counts of all blocks, by every block of the move itself: while the blocks are
+// few that takes less than a launch. Thread d has digit d.
+__device__ __forceinline__ int digit_offset(const int32_t* __restrict__ counts, int digits, int blocks, int block, int* wave_sum)
+{
+  constexpr int kAhead = 16;
+  const int d = threadIdx.x, lane = d & 63, wave = d >> 6;
+  int all = 0, before = 0;
+  for (int b0 = 0; b0 < blocks; b0 += kAhead) {
+    int c[kAhead];
+#pragma unroll
+    for (int e = 0; e < kAhead; e++) c[e] = d < digits && b0 + e < blocks ? counts[static_cast<int64_t>(b0 + e) * digits + d] : 0;
+#pragma unroll
+    for (int e = 0; e < kAhead; e++) {
+      all += c[e];
+      before += b0 + e < block ? c[e] : 0;
+    }
+  }
+  int upto = all;
+  for (int s = 1; s < 64; s <<= 1) {
+    const int other = __shfl_up(upto, s);
+    if (lane >= s) upto += other;
+  }
+  if (lane == 63) wave_sum[wave] = upto;
+  __syncthreads();
+  int at = upto - all + before;
+  for (int w = 0; w < wave; w++) at += wave_sum[w];
+  return at;
+}
+
 // A wave takes 256 consecutive entries, 64 at a time: the lanes of equal digits find one another by ballots, the first of
 // them moves the wave's count on. Ranks are then the block's offset, the waves before, and the place in the wave: stable.
 template <int kSortEach>
 __global__ void __launch_bounds__(kSortThreads)
   digit_move_kernel(const void* __restrict__ tokens, int token_bytes, const int32_t* __restrict__ keys,
                     const int32_t* __restrict__ places, int64_t n, int n_rows, int shift, int bits,
-                    const int32_t* __restrict__ offsets, Sorted out)
+                    const int32_t* __restrict__ offsets, int blocks, Sorted out)
 {
+  __shared__ int wave_sum[kSortWaves];
   __shared__ uint16_t count[kSortWaves][kDigits];
   __shared__ int first[kDigits];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int digits = 1 << bits;
   for (int w = 0; w < kSortWaves; w++) count[w][threadIdx.x] = 0;
-  if (static_cast<int>(threadIdx.x) < digits) first[threadIdx.x] = offsets[static_cast<int64_t>(blockIdx.x) * digits + threadIdx.x];
+  if (blocks > 0) {  // `offsets` are counts still
+    first[threadIdx.x] = digit_offset(offsets, digits, blocks, blockIdx.x, wave_sum);
+  } else if (static_cast<int>(threadIdx.x) < digits) {
+    first[threadIdx.x] = offsets[static_cast<int64_t>(blockIdx.x) * digits + threadIdx.x];
+  }
   __syncthreads();
   const int64_t begin = blockIdx.x * int64_t(kSortThreads * kSortEach) + wave * (64 * kSortEach);
   int key[kSortEach], digit[kSortEach], rank[kSortEach];
@@ -596,8 +630,10 @@ int embed_gradient(hipStream_t s, const EmbedCall& c, const void* grad, const vo
       auto pass = [&](auto entries) {
         constexpr int kEach = decltype(entries)::value;
         digit_count_kernel<kEach><<<grid, kSortThreads, 0, s>>>(tokens, token_bytes, keys, c.n_tokens, c.n_rows, shift, 1 << bits, c.counts);
-        digit_offsets_kernel<<<1, kSortThreads, 0, s>>>(1 << bits, static_cast<int>(c.blocks), c.counts);
-        digit_move_kernel<kEach><<<grid, kSortThreads, 0, s>>>(tokens, token_bytes, keys, from, c.n_tokens, c.n_rows, shift, bits, c.counts, to);
+        const bool own = c.blocks <= 128;  // each block adds up the counts for itself
+        if (!own) digit_offsets_kernel<<<1, kSortThreads, 0, s>>>(1 << bits, static_cast<int>(c.blocks), c.counts);
+        digit_move_kernel<kEach><<<grid, kSortThreads, 0, s>>>(tokens, token_bytes, keys, from, c.n_tokens, c.n_rows, shift, bits, c.counts,
+                                                               own ? static_cast<int>(c.blocks) : 0, to);
       };
       if (c.each == 1) pass(std::integral_constant<int, 1>{});
       else pass(std::integral_constant<int, 4>{});

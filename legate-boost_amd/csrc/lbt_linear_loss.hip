@@ -258,9 +258,14 @@ __global__ void __launch_bounds__(256)
           if (x != 0.f) reach = max(reach, own - 1 + exponent[p]);
         }
       for (int s = 32; s > 0; s >>= 1) reach = max(reach, __shfl_xor(reach, s));
-      // (most waves find a larger one there already: they need not wait their turn for the atomic)
-      if ((threadIdx.x & 63) == 0 && reach > __hip_atomic_load(&counts->reach, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT))
-        atomicMax(&counts->reach, reach);
+      __shared__ int by_wave[4];
+      if ((threadIdx.x & 63) == 0) by_wave[threadIdx.x >> 6] = reach;
+      __syncthreads();
+      // (most workgroups find a larger one there already: they need not wait their turn for the atomic)
+      if (threadIdx.x == 0) {
+        reach = max(max(by_wave[0], by_wave[1]), max(by_wave[2], by_wave[3]));
+        if (reach > __hip_atomic_load(&counts->reach, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) atomicMax(&counts->reach, reach);
+      }
     } else if (mode == kScale) {
       const int shift = exponent[p] + kReach - counts->reach;
 #pragma unroll
@@ -536,6 +541,12 @@ __device__ __forceinline__ int64_t round_up_rows(int counted) { return (static_c
 
 // ---- joins ----------------------------------------------------------------------------------------
 
+__device__ __forceinline__ float loss_of(float2 s, float picked)
+{
+  if (s.x == -INFINITY && s.y == 0.f) return INFINITY;  // every class is masked
+  return ((s.x == -INFINITY ? 0.f : s.x) - picked) + logf(s.y);
+}
+
 constexpr int kJoinRows = 16, kJoinSlices = 64;
 
 // Top and total of each row from its shares; its loss. 64 threads take the shares of a row between them, neighbours in a wave are
@@ -583,10 +594,9 @@ __global__ void __launch_bounds__(kJoinRows * kJoinSlices)
 #pragma unroll 8
   for (int v = 0; v < kJoinSlices; v++) total += totals[v][n];
   // where every class is masked there is no probability: the loss is infinite and p is 0
-  const bool none = all == -INFINITY && total == 0.f;
-  rows.top[row]     = from;
-  rows.inverse[row] = none ? 0.f : 1.f / total;
-  loss[rows.order[row]] = none ? INFINITY : (from - rows.picked[row]) + logf(total);
+  rows.top[row]         = from;
+  rows.inverse[row]     = all == -INFINITY && total == 0.f ? 0.f : 1.f / total;
+  loss[rows.order[row]] = loss_of(make_float2(all, total), rows.picked[row]);
 }
 
 // ---- few rows -----------------------------------------------------------------------------------------
@@ -784,12 +794,6 @@ __device__ __forceinline__ float2 join_row(const float2* __restrict__ shares, in
   return make_float2(top, total);
 }
 
-__device__ __forceinline__ float loss_of(float2 s, float picked)
-{
-  if (s.x == -INFINITY && s.y == 0.f) return INFINITY;  // every class is masked
-  return ((s.x == -INFINITY ? 0.f : s.x) - picked) + logf(s.y);
-}
-
 __global__ void __launch_bounds__(kFewThreads)
   join_few_kernel(const float2* __restrict__ partial, int tiles, const float* __restrict__ picked, const int64_t* __restrict__ y,
                   int n_classes, float* __restrict__ loss)
@@ -802,20 +806,48 @@ __global__ void __launch_bounds__(kFewThreads)
 
 // G from what LossEpilogue kept, once the rows' tops and totals are known: p = u exp(top of the share - top) / total. A workgroup
 // takes 16 rows and 2048 classes; bound by memory, each value is read and written once (bfloat16: in the same place).
-// The sums of G over the workgroup's rows are those of floats. Where 16 rows each would be too few workgroups they take 4.
+// The sums of G over the workgroup's rows are those of floats. Where 16 rows each would be too few workgroups they take 4; a wave
+// of such a workgroup joins the shares of one of them itself (join_shares of them), which saves a launch while they are few.
 constexpr int kScaleClasses = 2048;
 template <int kDtype, bool kKeptAsHalf, int kRows>
 __global__ void __launch_bounds__(256)
   scale_kernel(const void* kept, const float2* __restrict__ partial, int share_classes, int64_t padded, LossRows rows,
-               const RowCounts* __restrict__ counts, int n_classes, int piece, int64_t plane, uint16_t* g, float* bias_sums)
+               const RowCounts* __restrict__ counts, int n_classes, int piece, int64_t plane, uint16_t* g, float* bias_sums,
+               int join_shares, float* __restrict__ loss)
 {
   using L = LossType<kDtype>;
   __shared__ float factor[kRows][kScaleClasses / 32 + 1];
+  __shared__ float row_top[kRows], row_inverse[kRows];
   const int wides       = (piece + kScaleClasses - 1) / kScaleClasses;
   const int64_t block   = blockIdx.x / wides;
   const int64_t row0    = block * kRows;
   const int counted     = counts->rows;
   if (row0 >= round_up_rows(counted)) return;
+  if constexpr (kRows == 4) {
+    if (join_shares > 0) {
+      const int lane    = threadIdx.x & 63, r = threadIdx.x >> 6;
+      const int64_t row = row0 + r;
+      float top = -INFINITY, total = 0.f;
+      for (int t = lane; t < join_shares; t += 64) top = fmaxf(top, partial[t * padded + row].x);
+      for (int s = 32; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor(top, s));
+      const float from = top == -INFINITY ? 0.f : top;
+      for (int t = lane; t < join_shares; t += 64) {
+        const float2 s = partial[t * padded + row];
+        total += s.y * expf(s.x - from);
+      }
+      for (int s = 32; s > 0; s >>= 1) total += __shfl_xor(total, s);
+      if (lane == 0) {
+        row_top[r]     = from;
+        row_inverse[r] = top == -INFINITY && total == 0.f ? 0.f : 1.f / total;
+        if (blockIdx.x % wides == 0 && row < counted) loss[rows.order[row]] = loss_of(make_float2(top, total), rows.picked[row]);
+      }
+    }
+  }
+  if (join_shares == 0 && threadIdx.x < kRows) {
+    row_top[threadIdx.x]     = rows.top[row0 + threadIdx.x];
+    row_inverse[threadIdx.x] = rows.inverse[row0 + threadIdx.x];
+  }
+  __syncthreads();
   const int class0 = static_cast<int>(blockIdx.x % wides) * kScaleClasses, shares = kScaleClasses / share_classes, first = class0 / share_classes;
   for (int i = threadIdx.x; i < kRows * shares; i += 256) {
     const int64_t row = row0 + i % kRows;
@@ -823,7 +855,7 @@ __global__ void __launch_bounds__(256)
     float f           = 0.f;
     if (row < counted && class0 + s * share_classes < piece) {
       const float top = partial[(first + s) * padded + row].x;
-      f = top == -INFINITY ? 0.f : exp_of(top - rows.top[row], kDtype == LBT_F32) * rows.inverse[row] * (kKeptAsHalf ? 1.f / kKeptScale : 1.f);
+      f = top == -INFINITY ? 0.f : exp_of(top - row_top[i % kRows], kDtype == LBT_F32) * row_inverse[i % kRows] * (kKeptAsHalf ? 1.f / kKeptScale : 1.f);
     }
     factor[i % kRows][s] = f;
   }
@@ -1133,9 +1165,13 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
       }
     LBT_TRY(c.kept == kNotKept ? scores(std::integral_constant<int, kNotKept>{}) : scores(std::integral_constant<int, kKeptFloat>{}));
   }
-  join_kernel<<<static_cast<unsigned>(tiles_of(c.n_rows, kJoinRows)), kJoinRows * kJoinSlices, 0, s>>>(
-    c.partial, 2 * static_cast<int>(tiles), c.padded, c.rows, c.counts, loss);
-  LBT_HIP(hipGetLastError());
+  const int shares    = 2 * static_cast<int>(tiles);
+  const int join_here = c.kept != kNotKept && c.scale_rows == 4 && shares <= 256 ? shares : 0;  // in scale_kernel
+  if (join_here == 0) {
+    join_kernel<<<static_cast<unsigned>(tiles_of(c.n_rows, kJoinRows)), kJoinRows * kJoinSlices, 0, s>>>(c.partial, shares, c.padded, c.rows,
+                                                                                                       c.counts, loss);
+    LBT_HIP(hipGetLastError());
+  }
   if (!c.gradient) return LBT_OK;
 
   if (scaled)
@@ -1154,7 +1190,7 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
         scale_kernel<kDtype, decltype(half)::value, kRows>
           <<<static_cast<unsigned>(tiles_of(c.piece, kScaleClasses) * tiles_of(c.padded, kRows)), 256, 0, s>>>(
             decltype(half)::value ? static_cast<const void*>(c.g) : c.exps, c.partial, c.all_scores.tile / 2, c.padded, c.rows, c.counts,
-            c.classes, static_cast<int>(c.piece), c.padded * c.piece, c.g, grad_bias != nullptr ? c.bias_sums : nullptr);
+            c.classes, static_cast<int>(c.piece), c.padded * c.piece, c.g, grad_bias != nullptr ? c.bias_sums : nullptr, join_here, loss);
       };
       auto scale_by = [&](auto half) {
         if (c.scale_rows == 16) scale(half, std::integral_constant<int, 16>{});

@@ -90,6 +90,8 @@ _NATIVE = _lib._host if _lib._host is not None and _raw_stream is not None else 
 _BUILD, _BUILD_BYTES = _address(_lib.lib.lbt_build_tree_async), _address(_lib.lib.lbt_build_tree_workspace_bytes)
 _GRADIENT, _ADD_LEAVES = _address(_lib.lib.lbt_weighted_gradient), _address(_lib.lib.lbt_add_leaf_values)
 _NEXT_GRADIENT = _address(_lib.lib.lbt_next_gradient)
+_EMBED, _EMBED_GRADIENT = _address(_lib.lib.lbt_embed_rows), _address(_lib.lib.lbt_embed_rows_gradient)
+_EMBED_BYTES = _address(_lib.lib.lbt_embed_rows_gradient_workspace_bytes)
 
 
 def feature_mask(mask, device):
@@ -624,6 +626,21 @@ def _ptr(a):
     return None if a is None else a.data_ptr()
 
 
+class _On:
+    """torch.cuda.device, which costs 2 us, where another device than the current one is meant."""
+
+    def __init__(self, device):
+        self.other = torch.cuda.device(device) if device.index != torch.cuda.current_device() else None
+
+    def __enter__(self):
+        if self.other is not None:
+            self.other.__enter__()
+
+    def __exit__(self, *error):
+        if self.other is not None:
+            self.other.__exit__(*error)
+
+
 def linear_log_loss(X, weight, y, bias=None):
     """Log loss per row of the linear scores X @ weight.T + bias over many classes, without the scores in memory: float32
     [n_rows]. X [n_rows, n_features] and weight [n_classes, n_features]: both float32, bfloat16 or float16; y: whole numbers, a
@@ -632,7 +649,7 @@ def linear_log_loss(X, weight, y, bias=None):
     X, weight, y, bias = _loss_arguments(X, weight, y, bias)
     n, f = X.shape
     k, dt = weight.shape[0], _DT_NARROW[X.dtype]
-    with torch.cuda.device(X.device):
+    with _On(X.device):
         loss = torch.empty(n, dtype=torch.float32, device=X.device)
         ws = _scratch(_lib.lib.lbt_linear_log_loss_workspace_bytes(n, f, k, dt, 0), X.device)
         _lib.check(_lib.lib.lbt_linear_log_loss(_stream(), X.data_ptr(), weight.data_ptr(), dt, n, f, k, _ptr(bias), y.data_ptr(),
@@ -652,7 +669,7 @@ def linear_log_loss_gradient(X, weight, y, sample_weight=None, bias=None):
         w = _beside(as_device(sample_weight, torch.float32), X.device, "sample_weight")
         if w.numel() != n:
             raise _lib.LbtError("sample_weight must have one entry per row")
-    with torch.cuda.device(X.device):
+    with _On(X.device):
         loss = torch.empty(n, dtype=torch.float32, device=X.device)
         grad_X, grad_weight = torch.empty_like(X), torch.empty_like(weight)
         grad_bias = None if bias is None else torch.empty(k, dtype=torch.float32, device=X.device)
@@ -672,9 +689,16 @@ def embed_rows(table, tokens, scale=1.0):
     """scale * table[tokens] for whole numbers `tokens` of any shape: [*tokens.shape, n_features] of the table's type (float32,
     bfloat16 or float16), multiplied in float32 and rounded once. A token that is no row of the table gives zeros. tokens may be
     a tree's row_leaf (build_tree(row_leaf=True))."""
+    if _NATIVE is not None and torch.cuda.is_initialized():
+        device = torch.cuda.current_device()
+        got = _NATIVE.embed_rows(table, tokens, _EMBED, _raw_stream(device), device, scale)
+        if got is not None:
+            if not isinstance(got, torch.Tensor):
+                _lib.check(got)
+            return got
     table = _narrow(table, 2, "table")
     tokens = _tokens(tokens, table.device)
-    with torch.cuda.device(table.device):
+    with _On(table.device):
         out = torch.empty(tuple(tokens.shape) + (table.shape[1],), dtype=table.dtype, device=table.device)
         _lib.check(_lib.lib.lbt_embed_rows(_stream(), table.data_ptr(), _DT_NARROW[table.dtype], table.shape[0], table.shape[1],
                                            tokens.data_ptr(), tokens.element_size(), tokens.numel(), float(scale), out.data_ptr()))
@@ -686,6 +710,13 @@ def embed_rows_gradient(grad, tokens, n_rows, scale=1.0, add_to=None):
     tokens[t] = v, in float32 and in a fixed order. grad: [*tokens.shape, n_features]. add_to: a contiguous [n_rows, n_features]
     tensor of grad's type that the sums are added to in place, and which is returned, instead of a new one (a table that is also
     the weight of linear_log_loss_gradient)."""
+    if _NATIVE is not None and add_to is None and torch.cuda.is_initialized():
+        device = torch.cuda.current_device()
+        got = _NATIVE.embed_rows_gradient(grad, tokens, _scratch, _EMBED_GRADIENT, _EMBED_BYTES, _raw_stream(device), device, n_rows, scale)
+        if got is not None:
+            if not isinstance(got, torch.Tensor):
+                _lib.check(got)
+            return got
     grad = _narrow(grad, None, "grad")
     tokens = _tokens(tokens, grad.device)
     if grad.dim() == 0 or grad.shape[:-1] != tokens.shape:
@@ -695,7 +726,7 @@ def embed_rows_gradient(grad, tokens, n_rows, scale=1.0, add_to=None):
     if add_to is not None and not (isinstance(add_to, torch.Tensor) and add_to.shape == (n_rows, f) and add_to.dtype == grad.dtype
                                    and add_to.device == grad.device and add_to.is_contiguous() and add_to.data_ptr() % 16 == 0):
         raise _lib.LbtError("add_to must be a contiguous, 16-byte aligned [%d, %d] tensor of %s beside grad" % (n_rows, f, grad.dtype))
-    with torch.cuda.device(grad.device):
+    with _On(grad.device):
         if out is None:
             out = torch.empty((max(n_rows, 0), f), dtype=grad.dtype, device=grad.device)
         ws = _scratch(_lib.lib.lbt_embed_rows_gradient_workspace_bytes(tokens.numel(), f, n_rows, dt), grad.device)

@@ -256,7 +256,10 @@ def test_calls_repeat_bit_for_bit_and_leave_their_inputs():
     b = ops.linear_log_loss_gradient(x, w, y, bias=torch.zeros(3000, device="cuda"))
     assert all(torch.equal(p, q) for p, q in zip(a, b))
     assert all(torch.equal(p, q) for p, q in zip(keep, (x, w, y)))
-    assert torch.equal(ops.linear_log_loss(x, w, y), a[0])
+    # The call without gradients may join the shares of a row in another order: of 3000 classes at most 94, of 32 each. Each order is
+    # off by at most 94 u of the total and the exponentials by 2^-22, so the two differ by 2 (94 u + 2^-22) before the logarithm,
+    # whose value and the sum with the top are rounded to u of sizes below 32.
+    assert (ops.linear_log_loss(x, w, y) - a[0]).abs().max() <= 2 * (94 * U + 2.0 ** -22) + 4 * 32 * U
 
 
 def test_strided_and_unaligned_inputs():
