@@ -548,7 +548,8 @@ int lbt_gather_rows(void* stream, const void* X, int32_t x_dtype, int64_t row_of
  *   loss    device float [n_rows]
  *   workspace  at least lbt_linear_log_loss_workspace_bytes(..., gradient = 0), 256-byte aligned. `gradient`: 0 for this
  *              call, 1 for lbt_linear_log_loss_gradient, 2 for that with grad_bias; 0 bytes for invalid arguments
- * Enqueues on the stream and does not wait. All results are the same from call to call.
+ * Enqueues on the stream and does not wait. All results are the same from call to call. What is written (and the workspace) may
+ * not overlap what is read, or one another: LBT_ERR_INVALID, here and in the calls below.
  */
 size_t lbt_linear_log_loss_workspace_bytes(int64_t n_rows, int32_t n_features, int32_t n_outputs, int32_t dtype, int32_t gradient);
 int lbt_linear_log_loss(void* stream, const void* X, const void* weight, int32_t dtype, int64_t n_rows, int32_t n_features,

@@ -693,6 +693,9 @@ int lbt_embed_rows(void* stream, const void* table, int32_t dtype, int32_t n_row
   LBT_REQUIRE(table && tokens && out, "null pointer");
   LBT_REQUIRE(((reinterpret_cast<uintptr_t>(table) | reinterpret_cast<uintptr_t>(out)) & 15) == 0,
               "table and out must be 16-byte aligned");
+  const int64_t row                = static_cast<int64_t>(n_features) * lbt::value_bytes(dtype);
+  const lbt::MemoryRange ranges[] = {{out, n_tokens * row}, {table, n_rows * row}, {tokens, n_tokens * token_bytes}};
+  LBT_REQUIRE(lbt::ranges_apart(ranges, 1, 3), "out may not overlap the table or the tokens");
   hipStream_t s = static_cast<hipStream_t>(stream);
   const lbt::EmbedCall c(n_tokens, n_features, n_rows, dtype);
   lbt::ProfScope ps(LBT_PROF_OTHER, s);
@@ -735,6 +738,10 @@ int lbt_embed_rows_gradient(void* stream, const void* grad, int32_t dtype, const
   LBT_REQUIRE(grad_table && (n_tokens == 0 || (grad && tokens)), "null pointer");
   LBT_REQUIRE(((reinterpret_cast<uintptr_t>(grad) | reinterpret_cast<uintptr_t>(grad_table)) & 15) == 0,
               "grad and grad_table must be 16-byte aligned");
+  const int64_t row                = static_cast<int64_t>(n_features) * lbt::value_bytes(dtype);
+  const lbt::MemoryRange ranges[] = {{workspace, static_cast<int64_t>(workspace_bytes)}, {grad_table, n_rows * row}, {grad, n_tokens * row},
+                                     {tokens, n_tokens * token_bytes}};
+  LBT_REQUIRE(lbt::ranges_apart(ranges, 2, 4), "grad_table and workspace may not overlap the inputs or one another");
   if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0) {
     lbt::set_error("a workspace aligned to 16 bytes is needed");
     return LBT_ERR_WORKSPACE;

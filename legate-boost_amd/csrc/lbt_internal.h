@@ -42,6 +42,22 @@ void set_error(const char* fmt, ...);
     if (rc__ != LBT_OK) return rc__; \
   } while (0)
 
+// What a call reads or writes; null: nothing.
+struct MemoryRange {
+  const void* begin;
+  int64_t bytes;
+};
+// Whether none of the first `written` ranges overlaps another of the `all`.
+inline bool ranges_apart(const MemoryRange* ranges, int written, int all)
+{
+  for (int i = 0; i < written; i++)
+    for (int j = i + 1; j < all; j++) {
+      const char *a = static_cast<const char*>(ranges[i].begin), *b = static_cast<const char*>(ranges[j].begin);
+      if (a != nullptr && b != nullptr && a < b + ranges[j].bytes && b < a + ranges[i].bytes) return false;
+    }
+  return true;
+}
+
 // ---------------------------------------------------------------- workspace
 
 // Bump allocator over the caller's scratch buffer. In "measure" mode it only

@@ -132,57 +132,69 @@ struct LossRows {
 
 constexpr int kPrepareThreads = 1024;
 
-// One workgroup goes through the labels: the rows that count, in order. Their weights' largest exponent is found on the way.
-// 8192 rows take 3 us and the work grows with the rows only; it runs beside nothing, as all that follows needs it.
+// One workgroup goes through the labels, 4096 at a time: the rows that count, in order. Their weights' largest exponent is found
+// on the way. It runs beside nothing, as all that follows needs it: what it takes is the latency of its loads and two meetings a turn.
 __global__ void __launch_bounds__(kPrepareThreads)
   prepare_rows_kernel(const int64_t* __restrict__ y, const float* __restrict__ weight, int64_t n_rows, int64_t padded,
                       int n_classes, int half, LossRows out, float* __restrict__ loss, RowCounts* counts, uint16_t* zeros)
 {
-  __shared__ int wave_sum[kPrepareThreads / 64];
+  constexpr int kEach = 4, kWaves = kPrepareThreads / 64;
+  __shared__ int wave_sum[kEach][kWaves];
   __shared__ int largest;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if (threadIdx.x < 8) zeros[threadIdx.x] = 0;
   if (threadIdx.x == 0) largest = -1000;
   int at = 0;  // rows that count so far
-  for (int64_t first = 0; first < n_rows; first += kPrepareThreads) {
-    const int64_t r     = first + threadIdx.x;
-    const int64_t label = r < n_rows ? y[r] : -1;
-    const bool in       = label >= 0 && label < n_classes;
-    const uint64_t set  = __ballot(in);
-    __syncthreads();
-    if (lane == 0) wave_sum[wave] = __popcll(set);
-    __syncthreads();
-    int before = at, all = 0;
-    for (int w = 0; w < kPrepareThreads / 64; w++) {
-      const int s = wave_sum[w];
-      before += w < wave ? s : 0;
-      all += s;
+  for (int64_t first = 0; first < n_rows; first += kEach * kPrepareThreads) {
+    int64_t label[kEach];
+    float w[kEach];
+    uint64_t set[kEach];
+#pragma unroll
+    for (int e = 0; e < kEach; e++) {
+      const int64_t r = first + e * kPrepareThreads + threadIdx.x;
+      label[e]        = r < n_rows ? y[r] : -1;
+      w[e]            = weight != nullptr && r < n_rows ? weight[r] : 1.f;
     }
-    at += all;
-    if (in) {
-      const int p  = before + __popcll(set & ((uint64_t(1) << lane) - 1));
-      float w      = weight != nullptr ? weight[r] : 1.f;
-      int exponent = 0;
-      if (half) {
-        if (w != 0.f && fabsf(w) < INFINITY) {
-          w = 2.f * frexpf(w, &exponent);  // 1 <= |w| < 2
-          exponent -= 1;
-          atomicMax(&largest, exponent);
-        } else {
-          exponent = -1000;  // adds nothing to grad_weight where the weight is 0
-          if (w != 0.f) { exponent = 0; atomicMax(&largest, 0); }
-        }
-        w *= 1 << kHalfShift;
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < kEach; e++) {
+      set[e] = __ballot(label[e] >= 0 && label[e] < n_classes);
+      if (lane == 0) wave_sum[e][wave] = __popcll(set[e]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < kEach; e++) {
+      int before = at;
+      for (int v = 0; v < kWaves; v++) {
+        const int s = wave_sum[e][v];
+        before += v < wave ? s : 0;
+        at += s;
       }
-      out.order[p]    = static_cast<int32_t>(r);
-      out.place[r]    = p;
-      out.label[p]    = static_cast<int32_t>(label);
-      out.factor[p]   = w;
-      out.exponent[p] = exponent;
-      out.picked[p]   = -INFINITY;
-    } else if (r < n_rows) {
-      out.place[r] = -1;
-      loss[r]      = 0.f;
+      const int64_t r = first + e * kPrepareThreads + threadIdx.x;
+      if ((set[e] >> lane) & 1) {
+        const int p  = before + __popcll(set[e] & ((uint64_t(1) << lane) - 1));
+        int exponent = 0;
+        if (half) {
+          if (w[e] != 0.f && fabsf(w[e]) < INFINITY) {
+            w[e] = 2.f * frexpf(w[e], &exponent);  // 1 <= |w| < 2
+            exponent -= 1;
+            atomicMax(&largest, exponent);
+          } else {
+            exponent = -1000;  // adds nothing to grad_weight where the weight is 0
+            if (w[e] != 0.f) { exponent = 0; atomicMax(&largest, 0); }
+          }
+          w[e] *= 1 << kHalfShift;
+        }
+        out.order[p]    = static_cast<int32_t>(r);
+        out.place[r]    = p;
+        out.label[p]    = static_cast<int32_t>(label[e]);
+        out.factor[p]   = w[e];
+        out.exponent[p] = exponent;
+        out.picked[p]   = -INFINITY;
+      } else if (r < n_rows) {
+        out.place[r] = -1;
+        loss[r]      = 0.f;
+      }
     }
   }
   __syncthreads();
@@ -191,8 +203,10 @@ __global__ void __launch_bounds__(kPrepareThreads)
     counts->exponent = largest > -1000 ? largest : 0;
     counts->reach    = -1000;
   }
+  // (past the tiles that rows which count are in, nothing is looked at but `order`)
   for (int64_t p = at + threadIdx.x; p < padded; p += kPrepareThreads) {
-    out.order[p]    = -1;
+    out.order[p] = -1;
+    if (p >= at + 256) continue;
     out.label[p]    = -1;
     out.factor[p]   = 0.f;
     out.exponent[p] = -1000;
@@ -471,12 +485,14 @@ struct GradientEpilogue {
   }
 };
 
-// grad_X: m = features, n = rows. Adds to (or begins) the sums of this split of the classes, [split][rows][padded_cols].
+// grad_X: m = features, n = rows. Adds to (or begins) the sums of this split of the classes, [split][rows][padded_cols]. The same for
+// grad_weight where the rows are split, n = classes of the piece.
 struct RowsEpilogue {
   float* sums;
   int64_t split;  // values of a split
   int padded_cols;
   bool begin;
+  int classes;  // n ends here; 0: at the rows that count
 
   template <class Tile>
   __device__ __forceinline__ void store(Float16v (&acc)[Tile::kMT][Tile::kNT], int tile_m, int tile_n, int wm, int wn, int lane,
@@ -485,7 +501,7 @@ struct RowsEpilogue {
 #pragma unroll
     for (int j = 0; j < Tile::kNT; j++) {
       const int64_t row = static_cast<int64_t>(tile_n) * Tile::kBN + wn * Tile::kWN + j * 32 + (lane & 31);
-      if (row >= counted) continue;
+      if (row >= (classes > 0 ? classes : counted)) continue;
 #pragma unroll
       for (int i = 0; i < Tile::kMT; i++)
 #pragma unroll
@@ -934,6 +950,27 @@ __global__ void __launch_bounds__(256)
   store_four<kDtype>(out, r * cols + col, v, cols - col, cols % 4 == 0);
 }
 
+// grad_weight of a piece of the classes from its sums over the splits of the rows.
+template <int kDtype>
+__global__ void __launch_bounds__(256)
+  finish_classes_kernel(const float* __restrict__ sums, int splits, int64_t split, int padded_cols, int64_t first, int64_t classes, int cols,
+                        const RowCounts* __restrict__ counts, bool scaled, void* __restrict__ out)
+{
+  const int groups = (cols + 3) / 4;
+  const int64_t i  = blockIdx.x * int64_t(256) + threadIdx.x;
+  if (i >= classes * groups) return;
+  const int64_t c = i / groups;
+  const int col   = static_cast<int>(i % groups) * 4;
+  float v[4]      = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < splits; s++) {
+    const float4 a = *reinterpret_cast<const float4*>(sums + s * split + c * padded_cols + col);
+    v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+  }
+  if (kDtype == LBT_F16)
+    for (int q = 0; q < 4; q++) v[q] = ldexpf(v[q], (scaled ? counts->reach - kReach : 0) - kHalfShift);
+  store_four<kDtype>(out, (first + c) * cols + col, v, cols - col, cols % 4 == 0);
+}
+
 // grad_bias from its sums over blocks of rows; a class's blocks are shared out among 16 threads.
 __global__ void __launch_bounds__(kJoinRows * kJoinSlices)
   finish_bias_kernel(const float* __restrict__ sums, int n_classes, int block_rows, const RowCounts* __restrict__ counts, int half,
@@ -1013,7 +1050,7 @@ struct LossCall {
   RowCounts* counts;
   uint16_t *zeros, *x, *x_scaled, *weight, *g;
   float2* partial;
-  float *row_sums, *bias_sums, *exps;
+  float *row_sums, *class_sums, *bias_sums, *exps;
 
   LossCall(int64_t n, int f, int k, int type, int grad)
     : n_rows(n), features(f), classes(k), dtype(type), gradient(grad != 0), with_bias(grad > 1)
@@ -1036,7 +1073,7 @@ struct LossCall {
     all_scores  = packed ? scores : cut_product(k, n, pairs * cols / kProductK, 1);
     scale_rows  = tiles_of(padded, 16) * tiles_of(piece, kScaleClasses) >= 1024 ? 16 : 4;
     row_product = cut_product(f, n, pairs * piece / kProductK, 16);
-    class_product = cut_product(f, std::min<int64_t>(piece, k), pairs * padded / kProductK, 1);
+    class_product = cut_product(f, std::min<int64_t>(piece, k), pairs * tiles_of(n, kProductK), 16);
   }
 
   template <typename A>
@@ -1055,13 +1092,14 @@ struct LossCall {
     x             = arena.template take<uint16_t>(planes * padded * cols);
     partial       = arena.template take<float2>(2 * (tiles_of(round_up(classes, 256), all_scores.tile) + tiles_of(classes, piece)) * padded);
     weight = x_scaled = g = nullptr;
-    row_sums = bias_sums = exps = nullptr;
+    row_sums = class_sums = bias_sums = exps = nullptr;
     if (packed) weight = arena.template take<uint16_t>(planes * piece * cols);
     if (!gradient) return;
     if (dtype == LBT_F16) x_scaled = arena.template take<uint16_t>(padded * cols);
     g         = arena.template take<uint16_t>(planes * padded * piece);
     if (kept == kKeptFloat) exps = arena.template take<float>(padded * piece);
     row_sums  = arena.template take<float>(row_product.splits * padded * cols);
+    if (class_product.splits > 1) class_sums = arena.template take<float>(class_product.splits * piece * cols);
     if (with_bias) bias_sums = arena.template take<float>(tiles_of(padded, kept ? scale_rows : scores.tile) * classes);
   }
 };
@@ -1217,13 +1255,22 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
     args.b        = g;
     args.k_extent = static_cast<int32_t>(c.piece);
     args.k_split  = static_cast<int32_t>(round_up(tiles_of(c.piece, c.row_product.splits), kProductK));
-    const RowsEpilogue re{c.row_sums, c.padded * c.cols, c.cols, first == 0};
+    const RowsEpilogue re{c.row_sums, c.padded * c.cols, c.cols, first == 0, 0};
     LBT_TRY((launch_product<L, true, false, kRowsN>(s, args, c.features, c.n_rows, c.row_product, re)));
     args.a        = x_scaled;
     args.b        = g;
-    args.k_extent = args.k_split = static_cast<int32_t>(c.padded);
-    const ClassesEpilogue<kDtype> ce{grad_weight, static_cast<int>(first), c.classes, c.features, scaled};
-    LBT_TRY((launch_product<L, true, true, kRowsK>(s, args, c.features, classes, c.class_product, ce)));
+    args.k_extent = static_cast<int32_t>(c.padded);
+    args.k_split  = static_cast<int32_t>(round_up(tiles_of(c.padded, c.class_product.splits), kProductK));
+    if (c.class_product.splits > 1) {
+      const RowsEpilogue ce{c.class_sums, c.piece * c.cols, c.cols, true, static_cast<int>(classes)};
+      LBT_TRY((launch_product<L, true, true, kRowsK>(s, args, c.features, classes, c.class_product, ce)));
+      finish_classes_kernel<kDtype><<<static_cast<unsigned>(tiles_of(classes * ((c.features + 3) / 4), 256)), 256, 0, s>>>(
+        c.class_sums, c.class_product.splits, c.piece * c.cols, c.cols, first, classes, c.features, c.counts, scaled, grad_weight);
+      LBT_HIP(hipGetLastError());
+    } else {
+      const ClassesEpilogue<kDtype> ce{grad_weight, static_cast<int>(first), c.classes, c.features, scaled};
+      LBT_TRY((launch_product<L, true, true, kRowsK>(s, args, c.features, classes, c.class_product, ce)));
+    }
   }
   const int64_t blocks = tiles_of(c.n_rows * ((c.features + 3) / 4), 256);
   LBT_REQUIRE(blocks < (int64_t(1) << 31), "too many values");
@@ -1304,6 +1351,11 @@ int run_loss(void* stream, const void* X, const void* weight, int32_t dtype, int
   const uintptr_t places = reinterpret_cast<uintptr_t>(X) | reinterpret_cast<uintptr_t>(weight) |
                            reinterpret_cast<uintptr_t>(grad_X) | reinterpret_cast<uintptr_t>(grad_weight);
   LBT_REQUIRE((places & 15) == 0, "X, weight and their gradients must be 16-byte aligned");
+  const int64_t size = dtype == LBT_F32 ? 4 : 2, rows = size * n_rows * n_features, classes = size * n_outputs * n_features;
+  const MemoryRange ranges[] = {{workspace, static_cast<int64_t>(workspace_bytes)}, {loss, 4 * n_rows}, {grad_X, rows}, {grad_weight, classes},
+                                {grad_bias, 4 * int64_t(n_outputs)}, {X, rows}, {weight, classes}, {bias, 4 * int64_t(n_outputs)}, {y, 8 * n_rows},
+                                {sample_weight, 4 * n_rows}};
+  LBT_REQUIRE(ranges_apart(ranges, 5, 10), "outputs and workspace may not overlap the inputs or one another");
   if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0) {
     set_error("a workspace aligned to 256 bytes is needed");
     return LBT_ERR_WORKSPACE;

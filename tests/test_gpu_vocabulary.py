@@ -436,6 +436,58 @@ def test_embed_gradient_against_differences():
     assert abs(value[0] - value[1] - float((g * step.double()).sum())) <= 12000 * 18 * 5 * 4 * U
 
 
+def test_lookups_from_native_code_and_from_python_are_the_same(monkeypatch):
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    table = torch.randn((50, 24), generator=gen, device="cuda").to(torch.bfloat16).requires_grad_()
+    tokens = torch.randint(-2, 52, (7, 300), generator=gen, device="cuda")
+    grad = torch.randn((7, 300, 24), generator=gen, device="cuda").to(torch.bfloat16)
+    assert ops._NATIVE is not None
+    got = ops.embed_rows(table, tokens, 3.0), ops.embed_rows_gradient(grad, tokens, 50, 3.0)
+    assert not got[0].requires_grad
+    monkeypatch.setattr(ops, "_NATIVE", None)
+    want = ops.embed_rows(table, tokens, 3.0), ops.embed_rows_gradient(grad, tokens, 50, 3.0)
+    assert all(torch.equal(a, b) and a.shape == b.shape and a.dtype == b.dtype for a, b in zip(got, want))
+
+
+def test_an_exception_of_the_library_is_left_to_python():
+    import ctypes as C
+
+    thrower = C.cast(C.CDLL("libstdc++.so.6")._ZSt17__throw_bad_allocv, C.c_void_p).value
+    table, tokens = torch.zeros((4, 8), device="cuda"), torch.zeros(3, dtype=torch.int64, device="cuda")
+    device = torch.cuda.current_device()
+    for _ in range(3):
+        assert _lib._host.embed_rows(table, tokens, thrower, 0, device, 1.0) is None
+        assert _lib._host.embed_rows_gradient(table[:3], tokens, ops._scratch, thrower, ops._EMBED_BYTES, 0, device, 4, 1.0) is None
+    assert C.pythonapi.PyGILState_Check() == 1
+
+
+def test_threads_on_streams_of_their_own():
+    """Four threads at once, each with its stream and so with its scratch."""
+    import threading
+
+    cases = [inputs(150 + 40 * i, 64 + 8 * i, 700 + 300 * i, "bf16", seed=60 + i) for i in range(4)]
+    tokens = [torch.randint(0, 500, (9000 + i,), device="cuda") for i in range(4)]
+    grads = [torch.randn((9000 + i, 16), device="cuda") for i in range(4)]
+    want = [ops.linear_log_loss_gradient(*c) + (ops.embed_rows_gradient(g, t, 500),) for c, t, g in zip(cases, tokens, grads)]
+    torch.cuda.synchronize()
+    got = [None] * 4
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(5):
+                got[i] = ops.linear_log_loss_gradient(*cases[i]) + (ops.embed_rows_gradient(grads[i], tokens[i], 500),)
+        stream.synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for a, b in zip(got, want):
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
 # ---- together ------------------------------------------------------------------------------------------
 
 

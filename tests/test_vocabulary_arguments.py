@@ -6,16 +6,17 @@ import pytest
 from lbtree import _lib
 
 L = _lib.lib
-AT = C.c_void_p(4096)  # never followed: the checks come first
-ODD = C.c_void_p(4096 + 8)
+# addresses far apart, never followed: the checks come first
+AT, W, Y, OUT, GX, GW, GB, WS = (C.c_void_p((i + 1) << 50) for i in range(8))
+ODD = C.c_void_p((9 << 50) + 8)
 BIG = 1 << 40
 
 
-def loss(stream=None, X=AT, weight=AT, dtype=_lib.LBT_BF16, n=10, f=8, k=100, bias=None, y=AT, out=AT, ws=None, size=0):
+def loss(stream=None, X=AT, weight=W, dtype=_lib.LBT_BF16, n=10, f=8, k=100, bias=None, y=Y, out=OUT, ws=None, size=0):
     return L.lbt_linear_log_loss(stream, X, weight, dtype, n, f, k, bias, y, out, ws, size)
 
 
-def gradient(X=AT, weight=AT, dtype=_lib.LBT_BF16, n=10, f=8, k=100, bias=None, y=AT, w=None, out=AT, gx=AT, gw=AT, gb=None,
+def gradient(X=AT, weight=W, dtype=_lib.LBT_BF16, n=10, f=8, k=100, bias=None, y=Y, w=None, out=OUT, gx=GX, gw=GW, gb=None,
              ws=None, size=0):
     return L.lbt_linear_log_loss_gradient(None, X, weight, dtype, n, f, k, bias, y, w, out, gx, gw, gb, ws, size)
 
@@ -35,7 +36,7 @@ def test_loss_refuses(arguments, message):
 
 @pytest.mark.parametrize("arguments,message", [
     (dict(gx=None), b"null"), (dict(gw=None), b"null"), (dict(gx=ODD), b"aligned"), (dict(gw=ODD), b"aligned"),
-    (dict(gb=AT), b"without a bias"),
+    (dict(gb=GB), b"without a bias"),
 ])
 def test_gradient_refuses(arguments, message):
     assert gradient(**arguments) == -1
@@ -47,7 +48,7 @@ def test_workspaces_are_checked():
         need = L.lbt_linear_log_loss_workspace_bytes(10, 8, 100, _lib.LBT_BF16, grad)
         assert need > 0
         assert call(ws=None) == -3 and b"workspace" in L.lbt_last_error()
-        assert call(ws=AT, size=need - 1) == -3 and str(need).encode() in L.lbt_last_error()
+        assert call(ws=WS, size=need - 1) == -3 and str(need).encode() in L.lbt_last_error()
         assert call(ws=ODD, size=BIG) == -3 and b"aligned" in L.lbt_last_error()
 
 
@@ -72,10 +73,10 @@ def test_no_rows_no_work():
 
 
 def test_embed_refuses():
-    def rows(table=AT, dtype=_lib.LBT_F32, n=10, f=8, tokens=AT, width=8, t=5, out=AT):
+    def rows(table=AT, dtype=_lib.LBT_F32, n=10, f=8, tokens=Y, width=8, t=5, out=OUT):
         return L.lbt_embed_rows(None, table, dtype, n, f, tokens, width, t, 1.0, out)
 
-    def grad(g=AT, dtype=_lib.LBT_F32, tokens=AT, width=8, t=5, f=8, n=10, add=0, out=AT, ws=AT, size=BIG):
+    def grad(g=AT, dtype=_lib.LBT_F32, tokens=Y, width=8, t=5, f=8, n=10, add=0, out=OUT, ws=WS, size=BIG):
         return L.lbt_embed_rows_gradient(None, g, dtype, tokens, width, t, f, n, 1.0, add, out, ws, size)
 
     for call in (rows, grad):
@@ -93,3 +94,39 @@ def test_embed_refuses():
     assert need > 0 and grad(size=need - 1) == -3 and grad(ws=None) == -3 and grad(ws=ODD) == -3
     assert L.lbt_embed_rows_gradient_workspace_bytes(5, 8, 10, _lib.LBT_F64) == 0
     assert L.lbt_embed_rows_gradient_workspace_bytes(0, 8, 10, _lib.LBT_F32) > 0
+
+
+def inside(a, by=16):
+    return C.c_void_p(a.value + by)
+
+
+def test_overlaps_are_refused():
+    """Ten rows of 8 values of 2 bytes: 160 bytes of X, 1600 of weight, 40 of the loss."""
+    for call, arguments in ((loss, dict(out=inside(AT, 156))), (loss, dict(out=inside(Y, 64))), (loss, dict(ws=inside(W, 256), size=BIG)),
+                            (loss, dict(bias=inside(OUT))), (gradient, dict(gx=AT)), (gradient, dict(gw=inside(W, 1584))),
+                            (gradient, dict(gx=inside(GW))), (gradient, dict(out=inside(GX, 144))), (gradient, dict(w=inside(OUT, 36))),
+                            (gradient, dict(bias=GB, gb=GB))):
+        assert call(**arguments) == -1 and b"overlap" in L.lbt_last_error(), arguments
+    # side by side is apart: the next check, that of the workspace, is reached
+    assert gradient(gx=inside(AT, 160), gw=inside(W, 1600)) == -3
+    rows, grad = L.lbt_embed_rows, L.lbt_embed_rows_gradient
+    assert rows(None, AT, _lib.LBT_F32, 10, 8, Y, 8, 5, 1.0, inside(AT, 304)) == -1 and b"overlap" in L.lbt_last_error()
+    assert grad(None, AT, _lib.LBT_F32, Y, 8, 5, 8, 10, 1.0, 1, AT, WS, BIG) == -1 and b"overlap" in L.lbt_last_error()
+    assert grad(None, AT, _lib.LBT_F32, Y, 8, 5, 8, 10, 1.0, 1, OUT, inside(OUT), BIG) == -1 and b"overlap" in L.lbt_last_error()
+
+
+def test_native_calls_leave_what_they_do_not_take():
+    """No tensor, one on the host, a type or a shape of another kind: None, and the Python form says what is wrong."""
+    import torch
+
+    host = _lib._host
+    table, tokens = torch.zeros(4, 8), torch.zeros(3, dtype=torch.int64)
+    for a, b in ((table, tokens), (table.numpy(), tokens), (table, [1, 2]), (None, None)):
+        assert host.embed_rows(a, b, 0, 0, 0, 1.0) is None
+        assert host.embed_rows_gradient(a, b, None, 0, 0, 0, 0, 4, 1.0) is None
+    for scale in ("1", None, [1]):
+        assert host.embed_rows(table, tokens, 0, 0, 0, scale) is None
+    with pytest.raises(TypeError):
+        host.embed_rows(table, tokens)
+    with pytest.raises(TypeError):
+        host.embed_rows_gradient(table, tokens)
