@@ -102,15 +102,17 @@ __device__ __forceinline__ uint2 narrow_four(const float (&v)[4])
   }
 }
 
-// Four consecutive values of an output row of which `n` are inside.
+// Four consecutive values of an output row of which `n` are inside. (The memory takes stores at any address: rows of an odd
+// length need no others. One value at a time, grad_weight of 2519 features took twice the time of its product.)
 template <int kDtype>
-__device__ __forceinline__ void store_four(void* p, int64_t i, const float (&v)[4], int n, bool aligned)
+__device__ __forceinline__ void store_four(void* p, int64_t i, const float (&v)[4], int n)
 {
-  if (n >= 4 && aligned) {
+  if (n >= 4) {
     if constexpr (kDtype == LBT_F32) {
-      *reinterpret_cast<float4*>(static_cast<float*>(p) + i) = make_float4(v[0], v[1], v[2], v[3]);
+      __builtin_memcpy(static_cast<float*>(p) + i, v, 16);
     } else {
-      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p) + i) = narrow_four<kDtype>(v);
+      const uint2 w = narrow_four<kDtype>(v);
+      __builtin_memcpy(static_cast<uint16_t*>(p) + i, &w, 8);
     }
     return;
   }
@@ -144,7 +146,7 @@ __global__ void __launch_bounds__(kPrepareThreads)
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if (threadIdx.x < 8) zeros[threadIdx.x] = 0;
   if (threadIdx.x == 0) largest = -1000;
-  int at = 0;  // rows that count so far
+  int at = 0, top_exponent = -1000;  // rows that count so far, their weights' largest exponent in this lane
   for (int64_t first = 0; first < n_rows; first += kEach * kPrepareThreads) {
     int64_t label[kEach];
     float w[kEach];
@@ -178,11 +180,10 @@ __global__ void __launch_bounds__(kPrepareThreads)
           if (w[e] != 0.f && fabsf(w[e]) < INFINITY) {
             w[e] = 2.f * frexpf(w[e], &exponent);  // 1 <= |w| < 2
             exponent -= 1;
-            atomicMax(&largest, exponent);
           } else {
-            exponent = -1000;  // adds nothing to grad_weight where the weight is 0
-            if (w[e] != 0.f) { exponent = 0; atomicMax(&largest, 0); }
+            exponent = w[e] == 0.f ? -1000 : 0;  // (a weight of 0 adds nothing to grad_weight)
           }
+          top_exponent = max(top_exponent, exponent);
           w[e] *= 1 << kHalfShift;
         }
         out.order[p]    = static_cast<int32_t>(r);
@@ -196,6 +197,11 @@ __global__ void __launch_bounds__(kPrepareThreads)
         loss[r]      = 0.f;
       }
     }
+  }
+  if (half) {
+    for (int s = 32; s > 0; s >>= 1) top_exponent = max(top_exponent, __shfl_xor(top_exponent, s));
+    __syncthreads();  // `largest` is there
+    if (lane == 0) atomicMax(&largest, top_exponent);
   }
   __syncthreads();
   if (threadIdx.x == 0) {
@@ -382,7 +388,7 @@ struct LossEpilogue {
             } else {
 #pragma unroll
               for (int e = 0; e < 4; e++) u[e] *= kKeptScale;
-              store_four<LBT_F16>(kept, at, u, 4, true);
+              store_four<LBT_F16>(kept, at, u, 4);
             }
           }
         }
@@ -532,7 +538,6 @@ struct ClassesEpilogue {
                                         int, const RowCounts* counts, char*) const
   {
     const int shift    = (scaled ? counts->reach - kReach : 0) - kHalfShift;
-    const bool aligned = cols % 4 == 0;
 #pragma unroll
     for (int j = 0; j < Tile::kNT; j++) {
       const int c = class_first + tile_n * Tile::kBN + wn * Tile::kWN + j * 32 + (lane & 31);
@@ -546,14 +551,12 @@ struct ClassesEpilogue {
           float v[4];
 #pragma unroll
           for (int e = 0; e < 4; e++) v[e] = kDtype == LBT_F16 ? ldexpf(acc[i][j][q * 4 + e], shift) : acc[i][j][q * 4 + e];
-          store_four<kDtype>(out, static_cast<int64_t>(c) * cols + col, v, cols - col, aligned);
+          store_four<kDtype>(out, static_cast<int64_t>(c) * cols + col, v, cols - col);
         }
     }
   }
 };
 
-// The rows that tiles of rows reach: those that count, filled up.
-__device__ __forceinline__ int64_t round_up_rows(int counted) { return (static_cast<int64_t>(counted) + 255) / 256 * 256; }
 
 // ---- joins ----------------------------------------------------------------------------------------
 
@@ -623,11 +626,12 @@ __global__ void __launch_bounds__(kJoinRows * kJoinSlices)
 // for both operands, which is all a product asks of it. float goes to the float products of the matrix cores as it is. Rows are not
 // taken out: what a row that does not count holds stays in its own column.
 // kShared: the four waves of a workgroup share out k instead of taking 16 classes each, where the classes would give the CUs too
-// few waves to keep memory busy. More than 16 rows have two blocks of classes beside theirs, so that the rows are read less often.
+// few waves to keep memory busy. More than 16 rows have two blocks of classes beside
+// theirs where there are classes enough, so that the rows are read less often.
 
 typedef __attribute__((ext_vector_type(4))) float Float4v;
 
-constexpr int kFewThreads = 256, kFewRows = 64;
+constexpr int kFewThreads = 256, kFewBlock = 64;  // rows of a workgroup, at most
 
 template <int kDtype>
 struct FewStep {  // 16 bytes of a row: kValues of k
@@ -658,17 +662,33 @@ struct FewStep {  // 16 bytes of a row: kValues of k
   }
 };
 
-template <int kDtype, int kBlocks, int kClassBlocks, bool kShared>
-__global__ void __launch_bounds__(kFewThreads)
-  few_rows_kernel(const void* __restrict__ X, const void* __restrict__ weight, const float* __restrict__ bias,
-                  const int64_t* __restrict__ y, int n_rows, int cols, int n_classes, int shares, float2* __restrict__ partial,
-                  float* __restrict__ picked)
+// For the gradient the rows are those that count, `order` names them, and u is left for scale_kernel as LossEpilogue does.
+struct FewRowsArgs {
+  const void *x, *weight;
+  const float* bias;
+  const int64_t* y;   // labels, where order is null
+  int n_rows, cols, n_classes;
+  int64_t share_step, row_step;  // of `partial`
+  float2* partial;
+  float* picked;
+  const int32_t *order, *label;
+  const RowCounts* counts;
+  void* kept;
+  int piece;
+};
+
+template <int kDtype, int kBlocks, int kClassBlocks, int kWaves, bool kShared, int kKeep>
+__global__ void __launch_bounds__(kWaves * 64, 3)
+  few_rows_kernel(const FewRowsArgs args)
 {
   using S = FewStep<kDtype>;
   using V = typename S::Value;
   constexpr bool kExact = kDtype == LBT_F32;
-  constexpr int kWaves = kFewThreads / 64, kUnroll = kBlocks >= 3 ? 2 : 4, kStep = 4 * S::kValues;  // k of a product
-  constexpr int kClasses = 16 * kClassBlocks;                                                       // of a wave
+  constexpr int kUnroll = kBlocks >= 3 ? 2 : 4, kStep = 4 * S::kValues;  // k of a product
+  constexpr int kClasses = 16 * kClassBlocks;                            // of a wave
+  const int row0 = blockIdx.y * kFewBlock, cols = args.cols, n_classes = args.n_classes;
+  const int n_rows = args.order != nullptr ? args.counts->rows : args.n_rows;
+  if (row0 >= n_rows) return;
   __shared__ float4 sums[kShared ? kWaves * kClassBlocks * kBlocks * 64 : 1];
   __shared__ float2 share[kWaves][kClassBlocks][16 * kBlocks];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -676,10 +696,12 @@ __global__ void __launch_bounds__(kFewThreads)
   const V *w[kClassBlocks], *x[kBlocks];
 #pragma unroll
   for (int i = 0; i < kClassBlocks; i++)
-    w[i] = static_cast<const V*>(weight) + static_cast<int64_t>(min(c0 + i * 16 + (lane & 15), n_classes - 1)) * cols;
+    w[i] = static_cast<const V*>(args.weight) + static_cast<int64_t>(min(c0 + i * 16 + (lane & 15), n_classes - 1)) * cols;
 #pragma unroll
-  for (int b = 0; b < kBlocks; b++)
-    x[b] = static_cast<const V*>(X) + static_cast<int64_t>(min(b * 16 + (lane & 15), n_rows - 1)) * cols;
+  for (int b = 0; b < kBlocks; b++) {
+    const int r = min(row0 + b * 16 + (lane & 15), n_rows - 1);
+    x[b]        = static_cast<const V*>(args.x) + static_cast<int64_t>(args.order != nullptr ? args.order[r] : r) * cols;
+  }
   const int at  = (lane >> 4) * S::kValues;
   const int hop = kShared ? kWaves * kUnroll * kStep : kUnroll * kStep;  // k of a turn, from wave to wave
   Float4v acc[kClassBlocks][kBlocks];
@@ -748,42 +770,56 @@ __global__ void __launch_bounds__(kFewThreads)
         for (int v = 0; v < kWaves; v++) t += __builtin_bit_cast(Float4v, sums[((v * kClassBlocks + i) * kBlocks + b) * 64 + lane]);
         acc[i][b] = t;
       }
-      const int r         = b * 16 + (lane & 15);
+      const int r         = row0 + b * 16 + (lane & 15);
       const int first     = c0 + i * 16 + 4 * (lane >> 4);
-      const int64_t label = r < n_rows ? y[r] : -1;
+      const int64_t label = r >= n_rows ? -1 : args.order != nullptr ? args.label[r] : args.y[r];
       float top           = -INFINITY;
 #pragma unroll
       for (int e = 0; e < 4; e++) {
         const int c  = first + e;
-        acc[i][b][e] = c < n_classes ? acc[i][b][e] + (bias != nullptr ? bias[c] : 0.f) : -INFINITY;
-        if (c == label && c < n_classes) picked[r] = acc[i][b][e];
+        acc[i][b][e] = c < n_classes ? acc[i][b][e] + (args.bias != nullptr ? args.bias[c] : 0.f) : -INFINITY;
+        if (c == label && c < n_classes) args.picked[r] = acc[i][b][e];
         top = fmaxf(top, acc[i][b][e]);
       }
       top = fmaxf(top, __shfl_xor(top, 16));
       top = fmaxf(top, __shfl_xor(top, 32));
       const float from = top == -INFINITY ? 0.f : top;
-      float total      = 0.f;
+      float total      = 0.f, u[4];
 #pragma unroll
-      for (int e = 0; e < 4; e++) total += exp_of(acc[i][b][e] - from, kExact);
+      for (int e = 0; e < 4; e++) {
+        u[e] = exp_of(acc[i][b][e] - from, kExact);
+        total += u[e];
+      }
+      if (kKeep != kNotKept && r < n_rows && first < args.piece) {
+        const int64_t at = static_cast<int64_t>(r) * args.piece + first;
+        if constexpr (kKeep == kKeptFloat) {
+          *reinterpret_cast<float4*>(static_cast<float*>(args.kept) + at) = make_float4(u[0], u[1], u[2], u[3]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; e++) u[e] *= kKeptScale;
+          store_four<LBT_F16>(args.kept, at, u, 4);
+        }
+      }
       total += __shfl_xor(total, 16);
       total += __shfl_xor(total, 32);
       if constexpr (kShared) {
-        if (lane < 16 && r < n_rows) partial[static_cast<int64_t>(r) * shares + blockIdx.x * kClassBlocks + i] = make_float2(top, total);
+        if (lane < 16 && r < n_rows)
+          args.partial[r * args.row_step + (blockIdx.x * kClassBlocks + i) * args.share_step] = make_float2(top, total);
       } else {
-        if (lane < 16) share[wave][i][r] = make_float2(top, total);
+        if (lane < 16) share[wave][i][r - row0] = make_float2(top, total);
       }
     }
   if constexpr (!kShared) {
     __syncthreads();
-    for (int t = threadIdx.x; t < kClassBlocks * 16 * kBlocks; t += kFewThreads) {
+    for (int t = threadIdx.x; t < kClassBlocks * 16 * kBlocks; t += kWaves * 64) {
       const int i = t / (16 * kBlocks), r = t % (16 * kBlocks);
-      if (r >= n_rows) continue;
+      if (row0 + r >= n_rows) continue;
       float top = share[0][i][r].x;
       for (int v = 1; v < kWaves; v++) top = fmaxf(top, share[v][i][r].x);
       const float from = top == -INFINITY ? 0.f : top;
       float total      = 0.f;
       for (int v = 0; v < kWaves; v++) total += share[v][i][r].y * exp_of(share[v][i][r].x - from, kExact);
-      partial[static_cast<int64_t>(r) * shares + blockIdx.x * kClassBlocks + i] = make_float2(top, total);
+      args.partial[(row0 + r) * args.row_step + (blockIdx.x * kClassBlocks + i) * args.share_step] = make_float2(top, total);
     }
   }
 }
@@ -820,6 +856,20 @@ __global__ void __launch_bounds__(kFewThreads)
   if (threadIdx.x == 0) loss[r] = l >= 0 && l < n_classes ? loss_of(s, picked[r]) : 0.f;
 }
 
+// The same among the rows of a gradient, for scale_kernel.
+__global__ void __launch_bounds__(kFewThreads)
+  join_few_rows_kernel(const float2* __restrict__ partial, int shares, LossRows rows, const RowCounts* __restrict__ counts,
+                       float* __restrict__ loss)
+{
+  const int r = blockIdx.x;
+  if (r >= counts->rows) return;
+  const float2 s = join_row(partial + static_cast<int64_t>(r) * shares, shares);
+  if (threadIdx.x != 0) return;
+  rows.top[r]           = s.x == -INFINITY ? 0.f : s.x;
+  rows.inverse[r]       = s.x == -INFINITY && s.y == 0.f ? 0.f : 1.f / s.y;
+  loss[rows.order[r]]   = loss_of(s, rows.picked[r]);
+}
+
 // G from what LossEpilogue kept, once the rows' tops and totals are known: p = u exp(top of the share - top) / total. A workgroup
 // takes 16 rows and 2048 classes; bound by memory, each value is read and written once (bfloat16: in the same place).
 // The sums of G over the workgroup's rows are those of floats. Where 16 rows each would be too few workgroups they take 4; a wave
@@ -827,28 +877,29 @@ __global__ void __launch_bounds__(kFewThreads)
 constexpr int kScaleClasses = 2048;
 template <int kDtype, bool kKeptAsHalf, int kRows>
 __global__ void __launch_bounds__(256)
-  scale_kernel(const void* kept, const float2* __restrict__ partial, int share_classes, int64_t padded, LossRows rows,
+  scale_kernel(const void* kept, const float2* __restrict__ partial, int share_classes, int64_t share_step, int64_t row_step, int row_tile, LossRows rows,
                const RowCounts* __restrict__ counts, int n_classes, int piece, int64_t plane, uint16_t* g, float* bias_sums,
                int join_shares, float* __restrict__ loss)
 {
   using L = LossType<kDtype>;
-  __shared__ float factor[kRows][kScaleClasses / 32 + 1];
+  __shared__ float factor[kRows][kScaleClasses / 16 + 1];
   __shared__ float row_top[kRows], row_inverse[kRows];
   const int wides       = (piece + kScaleClasses - 1) / kScaleClasses;
   const int64_t block   = blockIdx.x / wides;
   const int64_t row0    = block * kRows;
   const int counted     = counts->rows;
-  if (row0 >= round_up_rows(counted)) return;
+  // (the products reach as far as their last tile of rows: up to there G is zeros)
+  if (row0 >= (static_cast<int64_t>(counted) + row_tile - 1) / row_tile * row_tile) return;
   if constexpr (kRows == 4) {
     if (join_shares > 0) {
       const int lane    = threadIdx.x & 63, r = threadIdx.x >> 6;
       const int64_t row = row0 + r;
       float top = -INFINITY, total = 0.f;
-      for (int t = lane; t < join_shares; t += 64) top = fmaxf(top, partial[t * padded + row].x);
+      for (int t = lane; t < join_shares; t += 64) top = fmaxf(top, partial[t * share_step + row * row_step].x);
       for (int s = 32; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor(top, s));
       const float from = top == -INFINITY ? 0.f : top;
       for (int t = lane; t < join_shares; t += 64) {
-        const float2 s = partial[t * padded + row];
+        const float2 s = partial[t * share_step + row * row_step];
         total += s.y * expf(s.x - from);
       }
       for (int s = 32; s > 0; s >>= 1) total += __shfl_xor(total, s);
@@ -870,7 +921,7 @@ __global__ void __launch_bounds__(256)
     const int s       = i / kRows;
     float f           = 0.f;
     if (row < counted && class0 + s * share_classes < piece) {
-      const float top = partial[(first + s) * padded + row].x;
+      const float top = partial[(first + s) * share_step + row * row_step].x;
       f = top == -INFINITY ? 0.f : exp_of(top - row_top[i % kRows], kDtype == LBT_F32) * row_inverse[i % kRows] * (kKeptAsHalf ? 1.f / kKeptScale : 1.f);
     }
     factor[i % kRows][s] = f;
@@ -947,7 +998,7 @@ __global__ void __launch_bounds__(256)
       for (int q = 0; q < 4; q++) v[q] = e <= -1000 ? v[q] * 0.f : ldexpf(v[q], e - kHalfShift);
     }
   }
-  store_four<kDtype>(out, r * cols + col, v, cols - col, cols % 4 == 0);
+  store_four<kDtype>(out, r * cols + col, v, cols - col);
 }
 
 // grad_weight of a piece of the classes from its sums over the splits of the rows.
@@ -968,7 +1019,7 @@ __global__ void __launch_bounds__(256)
   }
   if (kDtype == LBT_F16)
     for (int q = 0; q < 4; q++) v[q] = ldexpf(v[q], (scaled ? counts->reach - kReach : 0) - kHalfShift);
-  store_four<kDtype>(out, (first + c) * cols + col, v, cols - col, cols % 4 == 0);
+  store_four<kDtype>(out, (first + c) * cols + col, v, cols - col);
 }
 
 // grad_bias from its sums over blocks of rows; a class's blocks are shared out among 16 threads.
@@ -1021,8 +1072,8 @@ Cut cut_product(int64_t m, int64_t n, int64_t stages, int64_t most_splits)
   Cut best{256, 1};
   double least = 1e30;
   for (const auto& t : kTiles)
-    for (int splits = 1; splits <= 16; splits++) {
-      if (splits > 1 && (splits > most_splits || stages / splits < 4)) break;
+    for (int splits = 1; splits <= most_splits; splits++) {
+      if (splits > 1 && stages / splits < 4) break;
       const int64_t each = tiles_of(tiles_of(m, t.tile) * tiles_of(n, t.tile) * splits, kCus);
       const double time  = each * (tiles_of(stages, splits) * (each == 1 ? t.lone : t.stage) + t.ends) +
                           (splits - 1) * (1.0 + m * n * 8e-6 / 4.0);
@@ -1032,6 +1083,69 @@ Cut cut_product(int64_t m, int64_t n, int64_t stages, int64_t most_splits)
       }
     }
   return best;
+}
+
+// Scores of few rows: the waves share the classes of a workgroup where they would be fewer than four a CU, and always where they
+// leave u, whose shares are then 16 classes each. Blocks of 64 rows: one of them for 16-bit types, whose weights the tiles take as
+// they are; up to four for float, which the tiles would first lay out in planes.
+bool few_shared(int classes) { return classes < 65536; }
+bool few_rows(int64_t n_rows, int dtype) { return n_rows <= (dtype == LBT_F32 ? 4 * kFewBlock : kFewBlock); }
+int few_class_blocks(int64_t n_rows, int classes) { return n_rows <= 16 || classes < 32768 ? 1 : 2; }
+int64_t few_groups(int classes, int class_blocks, bool shared) { return tiles_of(classes, 16 * class_blocks * (shared ? 1 : 4)); }
+
+struct FewCall {
+  float2* partial;
+  float* picked;
+  void carve(Arena& arena, int64_t n_rows, int classes)
+  {
+    const int blocks = few_class_blocks(n_rows, classes);
+    partial          = arena.take<float2>(n_rows * few_groups(classes, blocks, few_shared(classes)) * blocks);
+    picked           = arena.take<float>(n_rows);
+  }
+};
+
+template <int kDtype, int kKeep, int kBlocks, int kClassBlocks>
+int launch_few(hipStream_t s, const FewRowsArgs& args, int64_t classes, bool shared)
+{
+  constexpr int kWaves = kFewThreads / 64;
+  const dim3 grid(static_cast<unsigned>(few_groups(static_cast<int>(classes), kClassBlocks, shared)),
+                  static_cast<unsigned>(tiles_of(args.n_rows, kFewBlock)));
+  if (shared || kKeep != kNotKept)
+    few_rows_kernel<kDtype, kBlocks, kClassBlocks, kWaves, true, kKeep><<<grid, kFewThreads, 0, s>>>(args);
+  else
+    few_rows_kernel<kDtype, kBlocks, kClassBlocks, kWaves, false, kNotKept><<<grid, kFewThreads, 0, s>>>(args);
+  LBT_HIP(hipGetLastError());
+  return LBT_OK;
+}
+
+template <int kDtype, int kKeep, int kBlocks>
+int launch_few(hipStream_t s, const FewRowsArgs& args, int64_t classes, bool shared)
+{
+  if constexpr (kBlocks > 1)
+    if (few_class_blocks(args.n_rows, static_cast<int>(classes)) == 2) return launch_few<kDtype, kKeep, kBlocks, 2>(s, args, classes, shared);
+  return launch_few<kDtype, kKeep, kBlocks, 1>(s, args, classes, shared);
+}
+
+template <int kDtype, int kKeep>
+int launch_few(hipStream_t s, const FewRowsArgs& args, int64_t classes, bool shared)
+{
+  if (args.n_rows <= 16) return launch_few<kDtype, kKeep, 1>(s, args, classes, shared);
+  if (args.n_rows <= 32) return launch_few<kDtype, kKeep, 2>(s, args, classes, shared);
+  if (args.n_rows <= 48) return launch_few<kDtype, kKeep, 3>(s, args, classes, shared);
+  return launch_few<kDtype, kKeep, 4>(s, args, classes, shared);
+}
+
+template <int kDtype>
+int few_log_loss(hipStream_t s, const FewCall& c, const void* X, const void* weight, const float* bias, const int64_t* y, int n_rows,
+                 int features, int classes, float* loss)
+{
+  const bool shared = few_shared(classes);
+  const int blocks  = few_class_blocks(n_rows, classes), shares = static_cast<int>(few_groups(classes, blocks, shared)) * blocks;
+  const FewRowsArgs args{X, weight, bias, y, n_rows, features, classes, 1, shares, c.partial, c.picked, nullptr, nullptr, nullptr, nullptr, 0};
+  LBT_TRY((launch_few<kDtype, kNotKept>(s, args, classes, shared)));
+  join_few_kernel<<<n_rows, kFewThreads, 0, s>>>(c.partial, shares, c.picked, y, classes, loss);
+  LBT_HIP(hipGetLastError());
+  return LBT_OK;
 }
 
 struct LossCall {
@@ -1045,6 +1159,7 @@ struct LossCall {
   int64_t piece;    // classes at a time
   int kept;         // all classes are one piece: G is made from the scores' exponentials instead of the scores once more
   int scale_rows;   // of a workgroup of scale_kernel
+  bool few;         // the scores are those of few_rows_kernel
   Cut all_scores, scores, row_product, class_product;
   LossRows rows;
   RowCounts* counts;
@@ -1071,9 +1186,10 @@ struct LossCall {
     const int64_t pairs = type == LBT_F32 ? 6 : 1;
     scores      = cut_product(std::min<int64_t>(piece, k), n, pairs * cols / kProductK, 1);
     all_scores  = packed ? scores : cut_product(k, n, pairs * cols / kProductK, 1);
+    few         = kept != kNotKept && few_rows(n, type);
     scale_rows  = tiles_of(padded, 16) * tiles_of(piece, kScaleClasses) >= 1024 ? 16 : 4;
-    row_product = cut_product(f, n, pairs * piece / kProductK, 16);
-    class_product = cut_product(f, std::min<int64_t>(piece, k), pairs * tiles_of(n, kProductK), 16);
+    row_product = cut_product(f, n, pairs * piece / kProductK, 64);
+    class_product = cut_product(f, std::min<int64_t>(piece, k), pairs * tiles_of(n, kProductK), 64);
   }
 
   template <typename A>
@@ -1090,7 +1206,7 @@ struct LossCall {
     rows.top      = arena.template take<float>(padded);
     rows.inverse  = arena.template take<float>(padded);
     x             = arena.template take<uint16_t>(planes * padded * cols);
-    partial       = arena.template take<float2>(2 * (tiles_of(round_up(classes, 256), all_scores.tile) + tiles_of(classes, piece)) * padded);
+    partial       = arena.template take<float2>(std::max(few ? 2 * tiles_of(piece, 32) : 0, 2 * (tiles_of(round_up(classes, 256), all_scores.tile) + tiles_of(classes, piece))) * padded);
     weight = x_scaled = g = nullptr;
     row_sums = class_sums = bias_sums = exps = nullptr;
     if (packed) weight = arena.template take<uint16_t>(planes * piece * cols);
@@ -1180,7 +1296,16 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
   // top and total of each row; weights that are multiplied where they lie need no pieces here
   const int64_t step = c.packed ? c.piece : c.classes;
   int64_t tiles      = 0;
-  for (int64_t first = 0; first < c.classes; first += step) {
+  if (c.few) {
+    const FewRowsArgs few{X, weight, bias, nullptr, static_cast<int>(c.n_rows), c.features, c.classes, 1, c.piece / 16, c.partial, c.rows.picked,
+                          c.rows.order, c.rows.label, c.counts, c.kept == kKeptFloat ? static_cast<void*>(c.exps) : c.g,
+                          static_cast<int>(c.piece)};
+    if constexpr (kDtype == LBT_BF16)
+      LBT_TRY((c.kept == kKeptHalf ? launch_few<kDtype, kKeptHalf>(s, few, c.piece, true) : launch_few<kDtype, kKeptFloat>(s, few, c.piece, true)));
+    else
+      LBT_TRY((launch_few<kDtype, kKeptFloat>(s, few, c.piece, true)));
+  }
+  for (int64_t first = 0; first < c.classes && !c.few; first += step) {
     const int64_t classes = std::min<int64_t>(step, c.classes - first);
     LBT_TRY(lay_out(first));
     args.a = weights(first, classes);
@@ -1203,9 +1328,13 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
       }
     LBT_TRY(c.kept == kNotKept ? scores(std::integral_constant<int, kNotKept>{}) : scores(std::integral_constant<int, kKeptFloat>{}));
   }
-  const int shares    = 2 * static_cast<int>(tiles);
+  const int share_classes = c.few ? 16 : c.all_scores.tile / 2;
+  const int shares    = c.few ? static_cast<int>(c.piece / 16) : 2 * static_cast<int>(tiles);
   const int join_here = c.kept != kNotKept && c.scale_rows == 4 && shares <= 256 ? shares : 0;  // in scale_kernel
-  if (join_here == 0) {
+  if (c.few && join_here == 0) {
+    join_few_rows_kernel<<<static_cast<unsigned>(c.n_rows), kFewThreads, 0, s>>>(c.partial, shares, c.rows, c.counts, loss);
+    LBT_HIP(hipGetLastError());
+  } else if (join_here == 0) {
     join_kernel<<<static_cast<unsigned>(tiles_of(c.n_rows, kJoinRows)), kJoinRows * kJoinSlices, 0, s>>>(c.partial, shares, c.padded, c.rows,
                                                                                                        c.counts, loss);
     LBT_HIP(hipGetLastError());
@@ -1220,14 +1349,14 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
   const ProductOperand g{c.g, c.piece, c.padded * c.piece, static_cast<int32_t>(c.padded), static_cast<int32_t>(c.piece)};
   for (int64_t first = 0; first < c.classes; first += c.piece) {
     const int64_t classes = std::min<int64_t>(c.piece, c.classes - first);
-    if (first > 0 || c.piece < c.classes) LBT_TRY(lay_out(first));
+    if (first > 0 || c.piece < c.classes || c.few) LBT_TRY(lay_out(first));
     const ProductOperand w = weights(first, classes);
     if (c.kept != kNotKept) {
       auto scale = [&](auto half, auto each) {
         constexpr int kRows = decltype(each)::value;
         scale_kernel<kDtype, decltype(half)::value, kRows>
           <<<static_cast<unsigned>(tiles_of(c.piece, kScaleClasses) * tiles_of(c.padded, kRows)), 256, 0, s>>>(
-            decltype(half)::value ? static_cast<const void*>(c.g) : c.exps, c.partial, c.all_scores.tile / 2, c.padded, c.rows, c.counts,
+            decltype(half)::value ? static_cast<const void*>(c.g) : c.exps, c.partial, share_classes, c.few ? 1 : c.padded, c.few ? shares : 1, std::max(c.row_product.tile, kProductK), c.rows, c.counts,
             c.classes, static_cast<int>(c.piece), c.padded * c.piece, c.g, grad_bias != nullptr ? c.bias_sums : nullptr, join_here, loss);
       };
       auto scale_by = [&](auto half) {
@@ -1286,49 +1415,6 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
   return LBT_OK;
 }
 
-// Scores of few rows: four waves share the classes of a workgroup where they would be fewer than four a CU.
-bool few_shared(int classes) { return classes < 65536; }
-int few_class_blocks(int64_t n_rows) { return n_rows <= 16 ? 1 : 2; }
-int64_t few_groups(int classes, int class_blocks) { return tiles_of(classes, 16 * class_blocks * (few_shared(classes) ? 1 : 4)); }
-
-struct FewCall {
-  float2* partial;
-  float* picked;
-  void carve(Arena& arena, int64_t n_rows, int classes)
-  {
-    const int blocks = few_class_blocks(n_rows);
-    partial          = arena.take<float2>(n_rows * few_groups(classes, blocks) * blocks);
-    picked           = arena.take<float>(n_rows);
-  }
-};
-
-template <int kDtype, int kBlocks>
-int few_log_loss(hipStream_t s, const FewCall& c, const void* X, const void* weight, const float* bias, const int64_t* y, int n_rows,
-                 int features, int classes, float* loss)
-{
-  constexpr int kClassBlocks = kBlocks == 1 ? 1 : 2;
-  const int groups = static_cast<int>(few_groups(classes, kClassBlocks)), shares = groups * kClassBlocks;
-  if (few_shared(classes))
-    few_rows_kernel<kDtype, kBlocks, kClassBlocks, true>
-      <<<groups, kFewThreads, 0, s>>>(X, weight, bias, y, n_rows, features, classes, shares, c.partial, c.picked);
-  else
-    few_rows_kernel<kDtype, kBlocks, kClassBlocks, false>
-      <<<groups, kFewThreads, 0, s>>>(X, weight, bias, y, n_rows, features, classes, shares, c.partial, c.picked);
-  join_few_kernel<<<n_rows, kFewThreads, 0, s>>>(c.partial, shares, c.picked, y, classes, loss);
-  LBT_HIP(hipGetLastError());
-  return LBT_OK;
-}
-
-template <int kDtype>
-int few_log_loss(hipStream_t s, const FewCall& c, const void* X, const void* weight, const float* bias, const int64_t* y, int n_rows,
-                 int features, int classes, float* loss)
-{
-  if (n_rows <= 16) return few_log_loss<kDtype, 1>(s, c, X, weight, bias, y, n_rows, features, classes, loss);
-  if (n_rows <= 32) return few_log_loss<kDtype, 2>(s, c, X, weight, bias, y, n_rows, features, classes, loss);
-  if (n_rows <= 48) return few_log_loss<kDtype, 3>(s, c, X, weight, bias, y, n_rows, features, classes, loss);
-  return few_log_loss<kDtype, 4>(s, c, X, weight, bias, y, n_rows, features, classes, loss);
-}
-
 bool loss_shape(int64_t n_rows, int32_t n_features, int32_t n_outputs, int32_t dtype)
 {
   return (dtype == LBT_F32 || dtype == LBT_BF16 || dtype == LBT_F16) && n_rows >= 0 && n_features >= 1 && n_outputs >= 1 &&
@@ -1362,7 +1448,7 @@ int run_loss(void* stream, const void* X, const void* weight, int32_t dtype, int
   }
   LossCall c(std::max<int64_t>(n_rows, 1), n_features, n_outputs, dtype, !gradient ? 0 : grad_bias == nullptr ? 1 : 2);
   c.n_rows       = n_rows;
-  const bool few = !gradient && n_rows <= kFewRows;
+  const bool few = !gradient && few_rows(n_rows, dtype);
   FewCall f;
   Arena arena;
   arena.base = static_cast<char*>(workspace);
@@ -1401,7 +1487,7 @@ size_t lbt_linear_log_loss_workspace_bytes(int64_t n_rows, int32_t n_features, i
   lbt::LossCall c(std::max<int64_t>(n_rows, 1), n_features, n_outputs, dtype, gradient);
   lbt::Arena arena;
   arena.measure = true;
-  if (gradient == 0 && n_rows <= lbt::kFewRows) {
+  if (gradient == 0 && lbt::few_rows(n_rows, dtype)) {
     lbt::FewCall f;
     f.carve(arena, n_rows, n_outputs);
     return std::max<size_t>(arena.used, 256);

@@ -100,7 +100,7 @@ def check(x, w, y, dtype, bias=None, weight=None):
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("n,f,k", [(1, 1, 1), (1, 64, 1000), (2, 3, 2), (5, 7, 9), (16, 129, 255), (17, 8, 257), (64, 256, 1000),
-                                   (130, 72, 300), (257, 200, 1031), (33, 1000, 517), (511, 65, 64)])
+                                   (130, 72, 300), (257, 200, 1031), (33, 1000, 517), (511, 65, 64), (48, 90, 70001), (63, 2049, 3000), (250, 136, 9000)])
 def test_loss_and_gradients(n, f, k, dtype):
     check(*inputs(n, f, k, dtype, seed=n + f + k), dtype)
 
@@ -123,7 +123,7 @@ def test_several_pieces_of_the_classes(dtype, n, f, k, biased):
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("n,f,k", [(1, 1024, 5000), (16, 40, 33), (17, 1000, 700), (32, 2053, 70001), (33, 7, 90000), (64, 130, 66000),
-                                   (65, 130, 66000), (3, 4096, 10)])
+                                   (65, 130, 66000), (3, 4096, 10), (200, 520, 3000), (256, 70, 70000), (257, 33, 3000)])
 def test_loss_of_few_rows(n, f, k, dtype):
     x, w, y = inputs(n, f, k, dtype, seed=n * f)
     rs = np.random.RandomState(k)
