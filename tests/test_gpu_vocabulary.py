@@ -111,12 +111,13 @@ def test_tiles_of_256(dtype):
     check(*inputs(3900, {"bf16": 4104, "f16": 4099, "f32": 4100}[dtype], 5100, dtype, seed=3), dtype)
 
 
-@pytest.mark.parametrize("dtype,n,f,k,biased", [("bf16", 4100, 64, 250000, False), ("f16", 4100, 40, 85000, True),
-                                                ("f32", 4100, 24, 50000, False), ("bf16", 40, 2050, 131001, True)])
+@pytest.mark.parametrize("dtype,n,f,k,biased", [("f16", 4100, 40, 170000, True), ("f16", 4100, 24, 165000, False),
+                                                ("f32", 4100, 24, 100000, False), ("bf16", 40, 2050, 131001, True),
+                                                ("bf16", 300, 1030, 261000, False)])
 def test_several_pieces_of_the_classes(dtype, n, f, k, biased):
-    """G of a piece takes 2 GiB, with float exponentials beside it but for bfloat16; weights that are laid out first 512 MiB."""
+    """G of a piece takes 4 GiB, with float exponentials beside it but for bfloat16; weights that are laid out first 512 MiB."""
     entry = {"bf16": 2, "f16": 6, "f32": 10}[dtype]
-    assert entry * ((n + 255) // 256 * 256) * k > 2 << 30 or 2 * 2112 * k > 512 << 20
+    assert entry * ((n + 255) // 256 * 256) * k > 4 << 30 or 2 * ((f + 63) // 64 * 64) * k > 512 << 20
     bias = torch.randn(k, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda") if biased else None
     check(*inputs(n, f, k, dtype, seed=5), dtype, bias=bias)
 
