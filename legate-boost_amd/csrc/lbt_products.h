@@ -150,8 +150,12 @@ struct StageLoader {
                                        uint32_t lds, int wave, int lane)
   {
     if (s < whole) {
+      const uint64_t bits  = reinterpret_cast<uint64_t>(at);  // (the same in all lanes, which the compiler loses sight of)
+      const void* const to = reinterpret_cast<const void*>(
+        static_cast<uint64_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(bits >> 32))) << 32 |
+        static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(bits))));
 #pragma unroll
-      for (int j = 0; j < kEach; j++) load_to_lds(at, offset[j], lds + (j * kWaves + wave) * 1024);
+      for (int j = 0; j < kEach; j++) load_to_lds(to, offset[j], lds + (j * kWaves + wave) * 1024);
     } else {
       const int k0   = k_first + s * kProductK;
       const int row0 = kRowsAreK ? k0 : tile0, col0 = kRowsAreK ? tile0 : k0;
@@ -284,10 +288,14 @@ __global__ void __launch_bounds__(Tile::kThreads, 2) product_kernel(const Produc
   // A group of steps' fragments are read while those of the group before are multiplied.
   constexpr int kGroup = Tile::kGroup, kGroups = kSteps / kGroup;
   Short8 a[2][kGroup][Tile::kMT], b[2][kGroup][Tile::kNT];
-  // The i-th part of the fragments of a step: one of each operand.
+  // The i-th part of the fragments of a step: the second operand's first, all of which the next step begins with.
   auto read = [&](const char* at, int kk, int to, int i) {
-    if (i < Tile::kMT) a[to][kk % kGroup][i] = fragment<kAMajor, Tile::kBM>(at, wm * Tile::kWM + i * 32, kk, lane);
-    if (i < Tile::kNT) b[to][kk % kGroup][i] = fragment<kBMajor, Tile::kBN>(at + Tile::kStageA, wn * Tile::kWN + i * 32, kk, lane);
+    constexpr int kAll = Tile::kMT + Tile::kNT;
+#pragma unroll
+    for (int p = i * kAll / Tile::kMT; p < (i + 1) * kAll / Tile::kMT; p++) {
+      if (p < Tile::kNT) b[to][kk % kGroup][p] = fragment<kBMajor, Tile::kBN>(at + Tile::kStageA, wn * Tile::kWN + p * 32, kk, lane);
+      else a[to][kk % kGroup][p - Tile::kNT] = fragment<kAMajor, Tile::kBM>(at, wm * Tile::kWM + (p - Tile::kNT) * 32, kk, lane);
+    }
   };
   // Stages are asked for kStages ahead. The fragments of a stage's first group are read while the last one of the stage before is
   // multiplied, after all waves have met: then that stage has been read by all, and is filled again, and the next has arrived.
@@ -298,7 +306,6 @@ __global__ void __launch_bounds__(Tile::kThreads, 2) product_kernel(const Produc
     load(s, kB);
   }
   wait_and_meet<(Tile::kStages - 1) * Tile::kLoads>();
-  static_assert(Tile::kMT >= Tile::kNT, "the parts of a step are those of the first operand");
 #pragma unroll
   for (int kk = 0; kk < kGroup; kk++)
 #pragma unroll
