@@ -124,7 +124,7 @@ struct StageLoader {
       *col = ((q % kRow) ^ turned<kTile>(*row)) * 8;
     } else {
       *row = q >> 3;
-      *col = ((q & 7) ^ (*row & 7)) * 8;
+      *col = ((q & 7) ^ ((*row >> 1) & 7)) * 8;
     }
   }
   __device__ __forceinline__ void begin(const ProductOperand& op, int plane, int tile0, int k_first)
@@ -187,7 +187,7 @@ __device__ __forceinline__ Short8 fragment(const char* lds, int first, int kk, i
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
   } else {
     const int row   = first + (lane & 31);
-    const int chunk = (kk * 2 + (lane >> 5)) ^ (row & 7);
+    const int chunk = (kk * 2 + (lane >> 5)) ^ ((row >> 1) & 7);
     return *reinterpret_cast<const Short8*>(lds + row * (kProductK * 2) + chunk * 16);
   }
 }
