@@ -470,6 +470,36 @@ int token_bytes(const at::Tensor& t, int64_t device)
   return t.scalar_type() == at::kLong ? 8 : t.scalar_type() == at::kInt ? 4 : 0;
 }
 
+// A dense, contiguous tensor of `n` numbers of `type` on device `device`; null: something else
+const at::Tensor* numbers_of(PyObject* o, at::ScalarType type, int64_t n, int64_t device)
+{
+  if (!THPVariable_CheckExact(o)) return nullptr;
+  const at::Tensor& t = THPVariable_Unpack(o);
+  if (!t.defined() || t.layout() != at::kStrided || !t.is_cuda() || t.get_device() != device || !t.is_contiguous() || t.scalar_type() != type ||
+      t.numel() != n)
+    return nullptr;
+  return &t;
+}
+
+// workspace(bytes, device of `beside`): a new reference to a dense tensor; null: an error is set, or (with none set) it is something else
+PyObject* scratch_of(PyObject* workspace, size_t bytes, const at::Tensor& beside)
+{
+  PyObject* size   = PyLong_FromSize_t(bytes);
+  PyObject* device = size != nullptr ? THPDevice_New(beside.device()) : nullptr;
+  PyObject* held   = device != nullptr ? PyObject_CallFunctionObjArgs(workspace, size, device, nullptr) : nullptr;
+  Py_XDECREF(size);
+  Py_XDECREF(device);
+  if (held != nullptr && !THPVariable_CheckExact(held)) {
+    Py_DECREF(held);
+    held = nullptr;
+  }
+  return held;
+}
+struct Reference {
+  PyObject* o;
+  ~Reference() { Py_DECREF(o); }
+};
+
 // embed_rows(table, tokens, entry, stream, device, scale): lbt_embed_rows for tensors as they have to be on `device`, the current one. Returns the
 // rows, the status where that is not 0, or None as above. A lookup of 16 tokens took its host 10.9 us in Python.
 PyObject* embed_rows(PyObject*, PyObject* const* args, Py_ssize_t n_args)
@@ -527,17 +557,12 @@ PyObject* embed_rows_gradient(PyObject*, PyObject* const* args, Py_ssize_t n_arg
     const int32_t cols = static_cast<int32_t>(grad.size(dims - 1));
     const size_t need  = reinterpret_cast<decltype(&lbt_embed_rows_gradient_workspace_bytes)>(v[1])(n, cols, static_cast<int32_t>(rows), type);
     if (need == 0) Py_RETURN_NONE;
-    PyObject* size   = PyLong_FromSize_t(need);
-    PyObject* device = size != nullptr ? THPDevice_New(grad.device()) : nullptr;
-    PyObject* held   = device != nullptr ? PyObject_CallFunctionObjArgs(args[2], size, device, nullptr) : nullptr;
-    Py_XDECREF(size);
-    Py_XDECREF(device);
-    if (held == nullptr) return nullptr;  // (no memory, say: as it would be raised in Python)
-    struct Held {
-      PyObject* o;
-      ~Held() { Py_DECREF(o); }
-    } keep{held};
-    if (!THPVariable_CheckExact(held)) Py_RETURN_NONE;
+    PyObject* held = scratch_of(args[2], need, grad);
+    if (held == nullptr) {
+      if (PyErr_Occurred()) return nullptr;  // (no memory, say: as it would be raised in Python)
+      Py_RETURN_NONE;
+    }
+    const Reference keep{held};
     const at::Tensor& scratch = THPVariable_Unpack(held);
     at::Tensor out            = at::empty({rows, grad.size(dims - 1)}, grad.options().requires_grad(false));
     const void *const from = grad.const_data_ptr(), *const at = tokens.const_data_ptr();
@@ -554,6 +579,88 @@ PyObject* embed_rows_gradient(PyObject*, PyObject* const* args, Py_ssize_t n_arg
   }
 }
 
+// linear_log_loss(X, weight, y, bias, workspace, entry, size_entry, stream, device): lbt_linear_log_loss for tensors as they have to be on `device`, the
+// current one; bias: a tensor or None. Returns the losses, or as above. linear_log_loss_gradient(X, weight, y, bias, workspace, entry, size_entry,
+// stream, device, sample_weight): lbt_linear_log_loss_gradient, a tuple.
+PyObject* log_loss(PyObject* const* args, PyObject* sample_weight, bool gradient)
+{
+  int64_t v[4];
+  if (!integers(args + 5, 4, v)) return not_a_number();
+  try {
+    if (listened_to() || !THPVariable_CheckExact(args[0]) || !THPVariable_CheckExact(args[1])) Py_RETURN_NONE;
+    const at::Tensor &x = THPVariable_Unpack(args[0]), &weight = THPVariable_Unpack(args[1]);
+    const int type = narrow_type(x, v[3]);
+    if (type < 0 || narrow_type(weight, v[3]) != type || x.dim() != 2 || weight.dim() != 2 || x.size(1) != weight.size(1) || x.size(1) < 1 ||
+        weight.size(0) < 1 || x.size(1) > INT32_MAX || weight.size(0) > INT32_MAX)
+      Py_RETURN_NONE;
+    const int64_t n = x.size(0);
+    const int32_t f = static_cast<int32_t>(x.size(1)), k = static_cast<int32_t>(weight.size(0));
+    const at::Tensor *y = numbers_of(args[2], at::kLong, n, v[3]), *bias = nullptr, *w = nullptr;
+    if (y == nullptr) Py_RETURN_NONE;
+    if (args[3] != Py_None && (bias = numbers_of(args[3], at::kFloat, k, v[3])) == nullptr) Py_RETURN_NONE;
+    if (sample_weight != Py_None && (w = numbers_of(sample_weight, at::kFloat, n, v[3])) == nullptr) Py_RETURN_NONE;
+    const size_t need =
+      reinterpret_cast<decltype(&lbt_linear_log_loss_workspace_bytes)>(v[1])(n, f, k, type, gradient ? (bias != nullptr ? 2 : 1) : 0);
+    if (need == 0) Py_RETURN_NONE;
+    PyObject* held = scratch_of(args[4], need, x);
+    if (held == nullptr) {
+      if (PyErr_Occurred()) return nullptr;  // (no memory, say: as it would be raised in Python)
+      Py_RETURN_NONE;
+    }
+    const Reference keep{held};
+    const at::Tensor& scratch = THPVariable_Unpack(held);
+    const auto like  = x.options().requires_grad(false);
+    at::Tensor loss  = at::empty({n}, like.dtype(at::kFloat)), grad_x, grad_weight, grad_bias;
+    if (gradient) {
+      grad_x      = at::empty({n, f}, like);
+      grad_weight = at::empty({k, f}, like);
+      if (bias != nullptr) grad_bias = at::empty({k}, like.dtype(at::kFloat));
+    }
+    const void *const from = x.const_data_ptr(), *const rows = weight.const_data_ptr();
+    const int64_t* const labels = y->const_data_ptr<int64_t>();
+    const float *const b = bias != nullptr ? bias->const_data_ptr<float>() : nullptr, *const each = w != nullptr ? w->const_data_ptr<float>() : nullptr;
+    float* const to = loss.mutable_data_ptr<float>();
+    void *const ws = scratch.mutable_data_ptr(), *const gx = gradient ? grad_x.mutable_data_ptr() : nullptr,
+               *const gw = gradient ? grad_weight.mutable_data_ptr() : nullptr;
+    float* const gb       = grad_bias.defined() ? grad_bias.mutable_data_ptr<float>() : nullptr;
+    const size_t ws_bytes = static_cast<size_t>(scratch.nbytes());
+    void* const stream    = reinterpret_cast<void*>(v[2]);
+    const int status      = unlocked([&] {
+      if (gradient)
+        return reinterpret_cast<decltype(&lbt_linear_log_loss_gradient)>(v[0])(stream, from, rows, type, n, f, k, b, labels, each, to, gx, gw, gb, ws,
+                                                                               ws_bytes);
+      return reinterpret_cast<decltype(&lbt_linear_log_loss)>(v[0])(stream, from, rows, type, n, f, k, b, labels, to, ws, ws_bytes);
+    });
+    if (status != 0) return PyLong_FromLong(status);
+    if (!gradient) return THPVariable_Wrap(std::move(loss));
+    PyObject* out = PyTuple_New(bias != nullptr ? 4 : 3);
+    if (out == nullptr) return nullptr;
+    PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(std::move(loss)));
+    PyTuple_SET_ITEM(out, 1, THPVariable_Wrap(std::move(grad_x)));
+    PyTuple_SET_ITEM(out, 2, THPVariable_Wrap(std::move(grad_weight)));
+    if (bias != nullptr) PyTuple_SET_ITEM(out, 3, THPVariable_Wrap(std::move(grad_bias)));
+    return out;
+  } catch (const std::exception&) {
+    Py_RETURN_NONE;
+  }
+}
+PyObject* linear_log_loss(PyObject*, PyObject* const* args, Py_ssize_t n_args)
+{
+  if (n_args != 9) {
+    PyErr_SetString(PyExc_TypeError, "linear_log_loss takes nine arguments");
+    return nullptr;
+  }
+  return log_loss(args, Py_None, false);
+}
+PyObject* linear_log_loss_gradient(PyObject*, PyObject* const* args, Py_ssize_t n_args)
+{
+  if (n_args != 10) {
+    PyErr_SetString(PyExc_TypeError, "linear_log_loss_gradient takes ten arguments");
+    return nullptr;
+  }
+  return log_loss(args, args[9], true);
+}
+
 PyMethodDef methods[] = {{"tree_arrays", tree_arrays, METH_VARARGS, "addresses and node counts of an ensemble's arrays"},
                          {"model_arrays", model_arrays, METH_VARARGS, "the same from the attributes of an ensemble's models"},
                          {"predict_packed", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(predict_packed)), METH_FASTCALL,
@@ -568,6 +675,10 @@ PyMethodDef methods[] = {{"tree_arrays", tree_arrays, METH_VARARGS, "addresses a
                          {"embed_rows", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(embed_rows)), METH_FASTCALL, "rows of a table"},
                          {"embed_rows_gradient", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(embed_rows_gradient)), METH_FASTCALL,
                           "gradient of the rows of a table"},
+                         {"linear_log_loss", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(linear_log_loss)), METH_FASTCALL,
+                          "log loss of linear scores"},
+                         {"linear_log_loss_gradient", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(linear_log_loss_gradient)),
+                          METH_FASTCALL, "its gradients"},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -91,6 +91,8 @@ _BUILD, _BUILD_BYTES = _address(_lib.lib.lbt_build_tree_async), _address(_lib.li
 _GRADIENT, _ADD_LEAVES = _address(_lib.lib.lbt_weighted_gradient), _address(_lib.lib.lbt_add_leaf_values)
 _NEXT_GRADIENT = _address(_lib.lib.lbt_next_gradient)
 _EMBED, _EMBED_GRADIENT = _address(_lib.lib.lbt_embed_rows), _address(_lib.lib.lbt_embed_rows_gradient)
+_LOG_LOSS, _LOG_LOSS_GRADIENT = _address(_lib.lib.lbt_linear_log_loss), _address(_lib.lib.lbt_linear_log_loss_gradient)
+_LOG_LOSS_BYTES = _address(_lib.lib.lbt_linear_log_loss_workspace_bytes)
 _EMBED_BYTES = _address(_lib.lib.lbt_embed_rows_gradient_workspace_bytes)
 
 
@@ -646,6 +648,13 @@ def linear_log_loss(X, weight, y, bias=None):
     [n_rows]. X [n_rows, n_features] and weight [n_classes, n_features]: both float32, bfloat16 or float16; y: whole numbers, a
     row whose label is not in [0, n_classes) does not count and has loss 0; bias: float32 [n_classes], -inf masks a class.
     No autograd graph is recorded: linear_log_loss_gradient returns the gradients."""
+    if _NATIVE is not None and torch.cuda.is_initialized():
+        device = torch.cuda.current_device()
+        got = _NATIVE.linear_log_loss(X, weight, y, bias, _scratch, _LOG_LOSS, _LOG_LOSS_BYTES, _raw_stream(device), device)
+        if got is not None:
+            if not isinstance(got, torch.Tensor):
+                _lib.check(got)
+            return got
     X, weight, y, bias = _loss_arguments(X, weight, y, bias)
     n, f = X.shape
     k, dt = weight.shape[0], _DT_NARROW[X.dtype]
@@ -661,6 +670,14 @@ def linear_log_loss_gradient(X, weight, y, sample_weight=None, bias=None):
     """linear_log_loss with the gradients of sum_r sample_weight[r] * loss[r]: (loss, grad_X, grad_weight), and grad_bias (float32)
     behind them where a bias is given. grad_X and grad_weight have the types of X and weight. sample_weight: [n_rows], all ones
     where it is not given (1 / n_rows makes it the mean); the loss that is returned is not weighted."""
+    if _NATIVE is not None and torch.cuda.is_initialized():
+        device = torch.cuda.current_device()
+        got = _NATIVE.linear_log_loss_gradient(X, weight, y, bias, _scratch, _LOG_LOSS_GRADIENT, _LOG_LOSS_BYTES, _raw_stream(device), device,
+                                               sample_weight)
+        if got is not None:
+            if not isinstance(got, tuple):
+                _lib.check(got)
+            return got
     X, weight, y, bias = _loss_arguments(X, weight, y, bias)
     n, f = X.shape
     k, dt = weight.shape[0], _DT_NARROW[X.dtype]

@@ -437,6 +437,23 @@ def test_embed_gradient_against_differences():
     assert abs(value[0] - value[1] - float((g * step.double()).sum())) <= 12000 * 18 * 5 * 4 * U
 
 
+@pytest.mark.parametrize("n", [20, 200])
+def test_losses_from_native_code_and_from_python_are_the_same(monkeypatch, n):
+    x, w, y = inputs(n, 40, 600, "bf16", seed=47)
+    w.requires_grad_()
+    bias, weight = torch.randn(600, device="cuda"), torch.rand(n, device="cuda")
+
+    def calls():
+        return ((ops.linear_log_loss(x, w, y), ops.linear_log_loss(x, w, y, bias)) + ops.linear_log_loss_gradient(x, w, y)
+                + ops.linear_log_loss_gradient(x, w, y, weight, bias) + ops.linear_log_loss_gradient(x, w, y, bias=bias))
+
+    got = calls()
+    assert not any(t.requires_grad for t in got)
+    monkeypatch.setattr(ops, "_NATIVE", None)
+    want = calls()
+    assert len(got) == len(want) and all(torch.equal(a, b) and a.dtype == b.dtype and a.shape == b.shape for a, b in zip(got, want))
+
+
 def test_lookups_from_native_code_and_from_python_are_the_same(monkeypatch):
     gen = torch.Generator(device="cuda").manual_seed(4)
     table = torch.randn((50, 24), generator=gen, device="cuda").to(torch.bfloat16).requires_grad_()
@@ -459,6 +476,8 @@ def test_an_exception_of_the_library_is_left_to_python():
     for _ in range(3):
         assert _lib._host.embed_rows(table, tokens, thrower, 0, device, 1.0) is None
         assert _lib._host.embed_rows_gradient(table[:3], tokens, ops._scratch, thrower, ops._EMBED_BYTES, 0, device, 4, 1.0) is None
+        for call, more in ((_lib._host.linear_log_loss, ()), (_lib._host.linear_log_loss_gradient, (None,))):
+            assert call(table[:3], table, tokens, None, ops._scratch, thrower, ops._LOG_LOSS_BYTES, 0, device, *more) is None
     assert C.pythonapi.PyGILState_Check() == 1
 
 

@@ -124,9 +124,12 @@ def test_native_calls_leave_what_they_do_not_take():
     for a, b in ((table, tokens), (table.numpy(), tokens), (table, [1, 2]), (None, None)):
         assert host.embed_rows(a, b, 0, 0, 0, 1.0) is None
         assert host.embed_rows_gradient(a, b, None, 0, 0, 0, 0, 4, 1.0) is None
+        assert host.linear_log_loss(a, a, b, None, None, 0, 0, 0, 0) is None
+        assert host.linear_log_loss_gradient(a, a, b, None, None, 0, 0, 0, 0, None) is None
     for scale in ("1", None, [1]):
         assert host.embed_rows(table, tokens, 0, 0, 0, scale) is None
     with pytest.raises(TypeError):
         host.embed_rows(table, tokens)
-    with pytest.raises(TypeError):
-        host.embed_rows_gradient(table, tokens)
+    for call in (host.embed_rows_gradient, host.linear_log_loss, host.linear_log_loss_gradient):
+        with pytest.raises(TypeError):
+            call(table, tokens)
