@@ -220,25 +220,11 @@ __global__ void __launch_bounds__(kPrepareThreads)
   }
 }
 
-// Rows of an array as rows of an operand: in `order` where that is given, -1 and what lies past the end as zeros, columns
-// padded with zeros to `padded_cols`, floats as three planes. A thread takes 8 columns. Bound by the copy: it reads and writes
-// each value once. Half precision with weights: kMeasure finds counts->reach, kScale multiplies row p by 2^(exponent[p] + 14 - reach).
-enum { kCopy = 0, kMeasure = 1, kScale = 2 };
-constexpr int kReach = 14;
+// Columns col .. col + 7 of row r as they lie in an operand: zeros where r < 0 or past the row's end, a float as three planes.
 template <int kDtype>
-__global__ void __launch_bounds__(256)
-  pack_rows_kernel(const void* __restrict__ from, int64_t first_row, int64_t rows, int cols, const int32_t* __restrict__ order,
-                   int mode, const int32_t* __restrict__ exponent, RowCounts* counts, int64_t out_rows, int padded_cols,
-                   int64_t plane, uint16_t* __restrict__ out)
+__device__ __forceinline__ void take_eight(const void* __restrict__ from, int64_t r, int col, int cols,
+                                           uint16_t (&v)[LossType<kDtype>::kPlanes][8])
 {
-  using L          = LossType<kDtype>;
-  const int groups = padded_cols / 8;
-  const int64_t i  = blockIdx.x * int64_t(256) + threadIdx.x;
-  if (i >= out_rows * groups) return;
-  const int64_t p = i / groups;
-  const int col   = static_cast<int>(i % groups) * 8;
-  const int64_t r = order != nullptr ? order[p] : (first_row + p < rows ? first_row + p : -1);
-  uint16_t v[L::kPlanes][8];
   const bool whole = r >= 0 && col + 8 <= cols;
   float f[8];
   if (whole) {  // (rows of any length: the memory takes loads at any address)
@@ -266,6 +252,28 @@ __global__ void __launch_bounds__(256)
       v[2][e] = s[2];
     }
   }
+}
+
+// Rows of an array as rows of an operand: in `order` where that is given, -1 and what lies past the end as zeros, columns
+// padded with zeros to `padded_cols`, floats as three planes. A thread takes 8 columns. Bound by the copy: it reads and writes
+// each value once. Half precision with weights: kMeasure finds counts->reach, kScale multiplies row p by 2^(exponent[p] + 14 - reach).
+enum { kCopy = 0, kMeasure = 1, kScale = 2 };
+constexpr int kReach = 14;
+template <int kDtype>
+__global__ void __launch_bounds__(256)
+  pack_rows_kernel(const void* __restrict__ from, int64_t first_row, int64_t rows, int cols, const int32_t* __restrict__ order,
+                   int mode, const int32_t* __restrict__ exponent, RowCounts* counts, int64_t out_rows, int padded_cols,
+                   int64_t plane, uint16_t* __restrict__ out)
+{
+  using L          = LossType<kDtype>;
+  const int groups = padded_cols / 8;
+  const int64_t i  = blockIdx.x * int64_t(256) + threadIdx.x;
+  if (i >= out_rows * groups) return;
+  const int64_t p = i / groups;
+  const int col   = static_cast<int>(i % groups) * 8;
+  const int64_t r = order != nullptr ? order[p] : (first_row + p < rows ? first_row + p : -1);
+  uint16_t v[L::kPlanes][8];
+  take_eight<kDtype>(from, r, col, cols, v);
   if constexpr (kDtype == LBT_F16) {
     if (mode == kMeasure) {
       int reach = -1000;
@@ -296,6 +304,107 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
   for (int q = 0; q < L::kPlanes; q++)
     *reinterpret_cast<uint4*>(out + q * plane + p * padded_cols + col) = *reinterpret_cast<const uint4*>(v[q]);
+}
+
+// prepare_rows_kernel and the laying out of X, and of the weights where they are laid out, in one launch for up to 1024 rows: a workgroup
+// goes through all labels for itself and lays out 16 of the rows that count; others lay out the weights. Not for weighted rows in half
+// precision, whose weights' exponents have to be known first.
+constexpr int kFusedRows = 1024, kFusedEach = 16;
+struct FusedArgs {
+  const int64_t* y;
+  const float* row_weight;
+  int n_rows, padded, n_classes;
+  float* loss;
+  RowCounts* counts;
+  uint16_t* zeros;
+  const void *x, *weight;
+  int cols, padded_cols;
+  uint16_t *x_out, *weight_out;  // (the second: null where the weights are not laid out)
+  int64_t weight_rows;           // of weight_out
+};
+
+template <int kDtype>
+__global__ void __launch_bounds__(256) prepare_pack_kernel(const FusedArgs a, const LossRows out)
+{
+  using L          = LossType<kDtype>;
+  const int groups = a.padded_cols / 8, x_blocks = a.padded / kFusedEach;
+  uint16_t v[L::kPlanes][8];
+  if (static_cast<int>(blockIdx.x) >= x_blocks) {
+    const int64_t i = (static_cast<int64_t>(blockIdx.x) - x_blocks) * 256 + threadIdx.x;
+    if (i >= a.weight_rows * groups) return;
+    const int64_t c = i / groups;
+    const int col   = static_cast<int>(i % groups) * 8;
+    take_eight<kDtype>(a.weight, c < a.n_classes ? c : -1, col, a.cols, v);
+#pragma unroll
+    for (int q = 0; q < L::kPlanes; q++)
+      *reinterpret_cast<uint4*>(a.weight_out + (q * a.weight_rows + c) * a.padded_cols + col) = *reinterpret_cast<const uint4*>(v[q]);
+    return;
+  }
+  constexpr int kEach = kFusedRows / 256;
+  __shared__ int wave_sum[kEach][4], from[kFusedEach];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int p0 = blockIdx.x * kFusedEach;
+  const bool first = blockIdx.x == 0;
+  if (first && threadIdx.x < 8) a.zeros[threadIdx.x] = 0;
+  if (threadIdx.x < kFusedEach) from[threadIdx.x] = -1;
+  int64_t label[kEach];
+  uint64_t set[kEach];
+#pragma unroll
+  for (int e = 0; e < kEach; e++) {
+    const int r = e * 256 + threadIdx.x;
+    label[e]    = r < a.n_rows ? a.y[r] : -1;
+  }
+#pragma unroll
+  for (int e = 0; e < kEach; e++) {
+    set[e] = __ballot(label[e] >= 0 && label[e] < a.n_classes);
+    if (lane == 0) wave_sum[e][wave] = __popcll(set[e]);
+  }
+  __syncthreads();
+  int at = 0;
+#pragma unroll
+  for (int e = 0; e < kEach; e++) {
+    int before = at;
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+      const int s = wave_sum[e][w];
+      before += w < wave ? s : 0;
+      at += s;
+    }
+    const int r = e * 256 + threadIdx.x;
+    if ((set[e] >> lane) & 1) {
+      const int p = before + __popcll(set[e] & ((uint64_t(1) << lane) - 1));
+      if (first) out.place[r] = p;
+      if (p >= p0 && p < p0 + kFusedEach) {
+        const float w   = a.row_weight != nullptr ? a.row_weight[r] : 1.f;
+        from[p - p0]    = r;
+        out.order[p]    = r;
+        out.label[p]    = static_cast<int32_t>(label[e]);
+        out.factor[p]   = kDtype == LBT_F16 ? w * (1 << kHalfShift) : w;
+        out.exponent[p] = 0;
+        out.picked[p]   = -INFINITY;
+      }
+    } else if (first && r < a.n_rows) {
+      out.place[r] = -1;
+      a.loss[r]    = 0.f;
+    }
+  }
+  if (first && threadIdx.x == 0) *a.counts = RowCounts{at, 0, -1000};
+  __syncthreads();
+  if (threadIdx.x < kFusedEach && p0 + static_cast<int>(threadIdx.x) >= at) {
+    const int p     = p0 + threadIdx.x;
+    out.order[p]    = -1;
+    out.label[p]    = -1;
+    out.factor[p]   = 0.f;
+    out.exponent[p] = -1000;
+    out.picked[p]   = 0.f;
+  }
+  for (int i = threadIdx.x; i < kFusedEach * groups; i += 256) {
+    const int p = i / groups, col = (i % groups) * 8;
+    take_eight<kDtype>(a.x, from[p], col, a.cols, v);
+#pragma unroll
+    for (int q = 0; q < L::kPlanes; q++)
+      *reinterpret_cast<uint4*>(a.x_out + (static_cast<int64_t>(q) * a.padded + p0 + p) * a.padded_cols + col) = *reinterpret_cast<const uint4*>(v[q]);
+  }
 }
 
 // ---- what the products end in -------------------------------------------------------------------
@@ -338,7 +447,7 @@ __device__ __forceinline__ void turn_rows(char* lds, int wave, int lane, Value v
 {
   constexpr int kBlocks = Tile::kMT * 32 * kSize <= 256 ? Tile::kMT : 256 / (32 * kSize);
   constexpr int kRow = kBlocks * 32 * kSize, kStride = kRow + 16, kLanes = kRow / 16, kRows = 64 / kLanes;
-  static_assert(Tile::kWaves * 32 * kStride <= Tile::kStages * (Tile::kStageA + Tile::kStageB), "each wave has its part of the LDS");
+  static_assert(Tile::kWaves * 32 * kStride <= Tile::kLds, "each wave has its part of the LDS");
   char* own = lds + wave * (32 * kStride);
 #pragma unroll
   for (int group = 0; group < Tile::kMT / kBlocks; group++) {
@@ -380,7 +489,7 @@ struct LossEpilogue {
 
   template <class Tile>
   __device__ __forceinline__ void store(Float16v (&acc)[Tile::kMT][Tile::kNT], int tile_m, int tile_n, int wm, int wn, int lane,
-                                        int, const RowCounts*, char* lds) const
+                                        int, int, const RowCounts*, char* lds) const
   {
     const int in_piece = tile_m * Tile::kBM + wm * Tile::kWM;
     const int c0       = class_first + in_piece;
@@ -466,7 +575,7 @@ struct GradientEpilogue {
 
   template <class Tile>
   __device__ __forceinline__ void store(Float16v (&acc)[Tile::kMT][Tile::kNT], int tile_m, int tile_n, int wm, int wn, int lane,
-                                        int counted, const RowCounts* counts, char* lds) const
+                                        int counted, int, const RowCounts* counts, char* lds) const
   {
     const int in_piece = tile_m * Tile::kBM + wm * Tile::kWM;
     const int c0       = class_first + in_piece;
@@ -543,7 +652,7 @@ struct RowsEpilogue {
 
   template <class Tile>
   __device__ __forceinline__ void store(Float16v (&acc)[Tile::kMT][Tile::kNT], int tile_m, int tile_n, int wm, int wn, int lane,
-                                        int counted, const RowCounts*, char*) const
+                                        int counted, int part, const RowCounts*, char*) const
   {
 #pragma unroll
     for (int j = 0; j < Tile::kNT; j++) {
@@ -555,7 +664,7 @@ struct RowsEpilogue {
         for (int q = 0; q < 4; q++) {
           const int col = tile_m * Tile::kBM + wm * Tile::kWM + i * 32 + q * 8 + 4 * (lane >> 5);
           if (col >= padded_cols) continue;
-          float4* at = reinterpret_cast<float4*>(sums + blockIdx.y * split + row * padded_cols + col);
+          float4* at = reinterpret_cast<float4*>(sums + part * split + row * padded_cols + col);
           float4 v   = make_float4(acc[i][j][q * 4], acc[i][j][q * 4 + 1], acc[i][j][q * 4 + 2], acc[i][j][q * 4 + 3]);
           if (!begin) {
             const float4 o = *at;
@@ -576,7 +685,7 @@ struct ClassesEpilogue {
 
   template <class Tile>
   __device__ __forceinline__ void store(Float16v (&acc)[Tile::kMT][Tile::kNT], int tile_m, int tile_n, int wm, int wn, int lane,
-                                        int, const RowCounts* counts, char* lds) const
+                                        int, int, const RowCounts* counts, char* lds) const
   {
     const int shift    = (scaled ? counts->reach - kReach : 0) - kHalfShift;
     constexpr int kSize = kDtype == LBT_F32 ? 4 : 2;
@@ -1313,9 +1422,6 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
   using L              = LossType<kDtype>;
   constexpr bool kFine = kDtype == LBT_F32;
   constexpr bool kHalf = kDtype == LBT_F16;
-  prepare_rows_kernel<<<1, kPrepareThreads, 0, s>>>(y, sample_weight, c.n_rows, c.padded, c.classes, kHalf, c.rows, loss,
-                                                    c.counts, c.zeros);
-  LBT_HIP(hipGetLastError());
   if (c.n_rows == 0) {  // no row: the gradients are zeros
     const int64_t halves = int64_t(c.classes) * c.features * sizeof(typename L::Value) / 2;
     LBT_REQUIRE(tiles_of(halves, 256) < (int64_t(1) << 31), "too many values");
@@ -1327,8 +1433,20 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
     return LBT_OK;
   }
   const bool scaled = kHalf && sample_weight != nullptr;  // (without weights every exponent is 0)
-  LBT_TRY(launch_pack<kDtype>(s, X, 0, c.n_rows, c.features, c.rows.order, scaled ? kMeasure : kCopy, c.rows.exponent, c.counts, c.padded, c.cols,
-                              c.padded * c.cols, c.x));
+  const bool fused  = c.n_rows <= kFusedRows && !scaled;
+  if (fused) {
+    const FusedArgs a{y,         sample_weight, static_cast<int>(c.n_rows), static_cast<int>(c.padded), c.classes, loss, c.counts, c.zeros, X, weight,
+                      c.features, c.cols,        c.x,                        c.packed ? c.weight : nullptr, c.packed ? c.piece : 0};
+    const int64_t blocks = c.padded / kFusedEach + tiles_of(a.weight_rows * (c.cols / 8), 256);
+    LBT_REQUIRE(blocks < (int64_t(1) << 31), "too many values to lay out");
+    prepare_pack_kernel<kDtype><<<static_cast<unsigned>(blocks), 256, 0, s>>>(a, c.rows);
+    LBT_HIP(hipGetLastError());
+  } else {
+    prepare_rows_kernel<<<1, kPrepareThreads, 0, s>>>(y, sample_weight, c.n_rows, c.padded, c.classes, kHalf, c.rows, loss, c.counts, c.zeros);
+    LBT_HIP(hipGetLastError());
+    LBT_TRY(launch_pack<kDtype>(s, X, 0, c.n_rows, c.features, c.rows.order, scaled ? kMeasure : kCopy, c.rows.exponent, c.counts, c.padded,
+                                c.cols, c.padded * c.cols, c.x));
+  }
 
   // (rows that do not count are not there: x holds them side by side)
   const ProductOperand x{c.x, c.cols, c.padded * c.cols, static_cast<int32_t>(c.padded), c.cols};
@@ -1360,7 +1478,7 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
   }
   for (int64_t first = 0; first < c.classes && !c.few; first += step) {
     const int64_t classes = std::min<int64_t>(step, c.classes - first);
-    LBT_TRY(lay_out(first));
+    if (first > 0 || !fused) LBT_TRY(lay_out(first));  // (the first piece is there)
     args.a = weights(first, classes);
     args.b = x;
     args.k_extent = args.k_split = c.cols;
@@ -1402,7 +1520,7 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
   const ProductOperand g{c.g, c.piece, c.padded * c.piece, static_cast<int32_t>(c.padded), static_cast<int32_t>(c.piece)};
   for (int64_t first = 0; first < c.classes; first += c.piece) {
     const int64_t classes = std::min<int64_t>(c.piece, c.classes - first);
-    if (first > 0 || c.piece < c.classes || c.few) LBT_TRY(lay_out(first));
+    if (first > 0 || c.piece < c.classes || (c.few && !fused)) LBT_TRY(lay_out(first));
     const ProductOperand w = weights(first, classes);
     if (c.kept != kNotKept) {
       auto scale = [&](auto half, auto each) {
@@ -1438,20 +1556,33 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
     args.k_extent = static_cast<int32_t>(c.piece);
     args.k_split  = static_cast<int32_t>(round_up(tiles_of(c.piece, c.row_product.splits), kProductK));
     const RowsEpilogue re{c.row_sums, c.padded * c.cols, c.cols, first == 0, 0};
-    LBT_TRY((launch_product<L, true, false, kRowsN>(s, args, c.features, c.n_rows, c.row_product, re)));
-    args.a        = x_scaled;
-    args.b        = g;
-    args.k_extent = static_cast<int32_t>(c.padded);
-    args.k_split  = static_cast<int32_t>(round_up(tiles_of(c.padded, c.class_product.splits), kProductK));
+    ProductArgs more = args;
+    more.a           = x_scaled;
+    more.k_extent    = static_cast<int32_t>(c.padded);
+    more.k_split     = static_cast<int32_t>(round_up(tiles_of(c.padded, c.class_product.splits), kProductK));
+    auto products    = [&](const auto& ce) -> int {
+      if (c.row_product.tile == SmallTile::kBM && c.class_product.tile == SmallTile::kBM) {
+        args.tiles_m = more.tiles_m = static_cast<int>(tiles_of(c.features, SmallTile::kBM));
+        args.tiles_n = static_cast<int>(tiles_of(c.n_rows, SmallTile::kBN));
+        more.tiles_n = static_cast<int>(tiles_of(classes, SmallTile::kBN));
+        const int64_t blocks = static_cast<int64_t>(args.tiles_m) * args.tiles_n * c.row_product.splits;
+        const int64_t all    = blocks + static_cast<int64_t>(more.tiles_m) * more.tiles_n * c.class_product.splits;
+        LBT_REQUIRE(all < (int64_t(1) << 31), "too many tiles");
+        two_products_kernel<SmallTile, L::kProduct, L::kPlanes>
+          <<<static_cast<unsigned>(all), SmallTile::kThreads, 0, s>>>(args, re, static_cast<unsigned>(blocks), more, ce);
+        LBT_HIP(hipGetLastError());
+        return LBT_OK;
+      }
+      LBT_TRY((launch_product<L, true, false, kRowsN>(s, args, c.features, c.n_rows, c.row_product, re)));
+      return launch_product<L, true, true, kRowsK>(s, more, c.features, classes, c.class_product, ce);
+    };
     if (c.class_product.splits > 1) {
-      const RowsEpilogue ce{c.class_sums, c.piece * c.cols, c.cols, true, static_cast<int>(classes)};
-      LBT_TRY((launch_product<L, true, true, kRowsK>(s, args, c.features, classes, c.class_product, ce)));
+      LBT_TRY(products(RowsEpilogue{c.class_sums, c.piece * c.cols, c.cols, true, static_cast<int>(classes)}));
       finish_classes_kernel<kDtype><<<static_cast<unsigned>(tiles_of(classes * ((c.features + 3) / 4), 256)), 256, 0, s>>>(
         c.class_sums, c.class_product.splits, c.piece * c.cols, c.cols, first, classes, c.features, c.counts, scaled, grad_weight);
       LBT_HIP(hipGetLastError());
     } else {
-      const ClassesEpilogue<kDtype> ce{grad_weight, static_cast<int>(first), c.classes, c.features, scaled};
-      LBT_TRY((launch_product<L, true, true, kRowsK>(s, args, c.features, classes, c.class_product, ce)));
+      LBT_TRY(products(ClassesEpilogue<kDtype>{grad_weight, static_cast<int>(first), c.classes, c.features, scaled}));
     }
   }
   const int64_t blocks = tiles_of(c.n_rows * ((c.features + 3) / 4), 256);

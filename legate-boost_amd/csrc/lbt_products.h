@@ -64,6 +64,7 @@ struct ProductTile {
   // Steps of 16 of k whose fragments are read together: a wave of one block has too little to multiply in a step to cover a read.
   static constexpr int kGroup = kMT == 1 ? kProductK / 16 : 1;
   static constexpr int kStageA = kM * kProductK * 2, kStageB = kN * kProductK * 2;  // bytes
+  static constexpr int kLds = kStages * (kStageA + kStageB);
   static constexpr int kLoads = (kM + kN) * kProductK / 8 / kThreads;               // of a lane for a stage
 };
 
@@ -227,19 +228,19 @@ struct PlanePairs<3> {
 // kRowsSide: which direction of the product is the call's rows: 0 n, 1 k, 2 m
 enum { kRowsN = 0, kRowsK = 1 };
 
+// Tile `block` of split `split`, in an LDS of Tile::kLds bytes.
 template <class Tile, int kType, int kPlanes, bool kAMajor, bool kBMajor, int kRowsSide, class Epilogue>
-__global__ void __launch_bounds__(Tile::kThreads, 2) product_kernel(const ProductArgs args, const Epilogue epilogue)
+__device__ __forceinline__ void product_tile(const ProductArgs& args, const Epilogue& epilogue, int block, int split, char* lds)
 {
   constexpr int kStage = Tile::kStageA + Tile::kStageB, kSteps = kProductK / 16;
-  __shared__ __attribute__((aligned(1024))) char lds[Tile::kStages * kStage];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   int tile_m, tile_n;
-  tile_of_block(blockIdx.x, args.tiles_m, args.tiles_n, &tile_m, &tile_n);
+  tile_of_block(block, args.tiles_m, args.tiles_n, &tile_m, &tile_n);
   const int rows = args.counts->rows;
   int k_end      = args.k_extent;
   if (kRowsSide == kRowsN && tile_n * Tile::kBN >= rows) return;
   if (kRowsSide == kRowsK) k_end = min(k_end, rows);
-  const int k_first = blockIdx.y * args.k_split;
+  const int k_first = split * args.k_split;
   k_end             = min(k_end, k_first + args.k_split);
   const int steps   = k_end > k_first ? (k_end - k_first + kProductK - 1) / kProductK : 0;
 
@@ -359,7 +360,30 @@ __global__ void __launch_bounds__(Tile::kThreads, 2) product_kernel(const Produc
     }
   }
   wait_and_meet<0>();  // the LDS is free for what follows
-  epilogue.template store<Tile>(acc, tile_m, tile_n, wm, wn, lane, rows, args.counts, lds);
+  epilogue.template store<Tile>(acc, tile_m, tile_n, wm, wn, lane, rows, split, args.counts, lds);
+}
+
+template <class Tile, int kType, int kPlanes, bool kAMajor, bool kBMajor, int kRowsSide, class Epilogue>
+__global__ void __launch_bounds__(Tile::kThreads, 2) product_kernel(const ProductArgs args, const Epilogue epilogue)
+{
+  __shared__ __attribute__((aligned(1024))) char lds[Tile::kLds];
+  product_tile<Tile, kType, kPlanes, kAMajor, kBMajor, kRowsSide>(args, epilogue, blockIdx.x, blockIdx.y, lds);
+}
+
+// Two products that need nothing of one another in one launch: both operands' k in rows for the second, the first operand's for the
+// first. What they take alone is mostly their beginning and end where both are in small tiles.
+template <class Tile, int kType, int kPlanes, class First, class Second>
+__global__ void __launch_bounds__(Tile::kThreads, 2)
+  two_products_kernel(const ProductArgs args, const First first, unsigned blocks, const ProductArgs more, const Second second)
+{
+  __shared__ __attribute__((aligned(1024))) char lds[Tile::kLds];
+  if (blockIdx.x < blocks) {
+    const int tiles = args.tiles_m * args.tiles_n;
+    product_tile<Tile, kType, kPlanes, true, false, kRowsN>(args, first, blockIdx.x % tiles, blockIdx.x / tiles, lds);
+  } else {
+    const int tiles = more.tiles_m * more.tiles_n, block = blockIdx.x - blocks;
+    product_tile<Tile, kType, kPlanes, true, true, kRowsK>(more, second, block % tiles, block / tiles, lds);
+  }
 }
 
 // Element e of a 32 x 32 block: its m within the block; its n is lane % 32.
