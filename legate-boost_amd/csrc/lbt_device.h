@@ -72,6 +72,14 @@ __device__ __forceinline__ int64_t wave_read_lane(int64_t v, int src)
   return static_cast<int64_t>((static_cast<uint64_t>(hi) << 32) | lo);
 }
 
+// What a wave's lanes have written to the LDS is there for its other lanes: the LDS takes a wave's accesses in order, so this is no
+// instruction; it keeps the compiler from moving accesses past it.
+__device__ __forceinline__ void meet_in_wave()
+{
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 __device__ __forceinline__ uint32_t wave_read_lane32(uint32_t v, int src)
 {
   return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), src));

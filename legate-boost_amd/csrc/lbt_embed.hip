@@ -12,6 +12,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "lbt_device.h"
 #include "lbt_internal.h"
 
 namespace lbt {
@@ -281,9 +282,9 @@ __global__ void __launch_bounds__(kSortThreads)
     const int ahead = __popcll(same & ((uint64_t(1) << lane) - 1));
     const int so_far = in ? count[wave][digit[e]] : 0;
     rank[e]         = so_far + ahead;
-    __builtin_amdgcn_wave_barrier();
+    meet_in_wave();
     if (in && ahead == 0) count[wave][digit[e]] = static_cast<uint16_t>(so_far + __popcll(same));
-    __builtin_amdgcn_wave_barrier();
+    meet_in_wave();
   }
   __syncthreads();
   if (static_cast<int>(threadIdx.x) < digits) {
@@ -424,56 +425,99 @@ __global__ void __launch_bounds__(kRowThreads) sum_runs_kernel(const RunArgs a)
   }
 }
 
-// Runs that cross the end of a chunk: the wave of the chunk in which one begins adds up its parts.
+// Runs that cross the end of a chunk: the wave of the chunk in which one begins adds up its parts, one that reaches over 64 chunks
+// and more the 16 waves of its workgroup together. (65536 places of 64 floats that are all alike: 359 us for one wave.)
+constexpr int kJoinThreads = 1024, kJoinWaves = kJoinThreads / 64;
 template <int kDtype, int kBytes>
-__global__ void __launch_bounds__(kRowThreads) join_runs_kernel(const RunArgs a)
+__global__ void __launch_bounds__(kJoinThreads) join_runs_kernel(const RunArgs a)
 {
   using P = Pack<kDtype, kBytes>;
-  const int64_t task  = static_cast<int64_t>(blockIdx.x) * kRowWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t chunk = task / a.slices;
-  const int at        = static_cast<int>(task % a.slices) * 64 + (threadIdx.x & 63);
-  const int64_t p0    = chunk * a.chunk, p1 = p0 + a.chunk;
-  if (p1 >= a.n_tokens) return;
-  const int row = a.sorted.key[p1 - 1];
-  if (row >= a.n_rows || a.sorted.key[p1] != row) return;
-  if (p0 > 0 && a.sorted.key[p0 - 1] == row) return;  // it began earlier
+  __shared__ int64_t heads_of[kJoinWaves];
+  __shared__ float part[kJoinWaves][P::kValues][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t stride = static_cast<int64_t>(a.words) * P::kValues;
-  const float* from    = a.part + (chunk * 2 + 1) * stride + static_cast<int64_t>(at) * P::kValues;
   float sum[P::kValues];
-#pragma unroll
-  for (int e = 0; e < P::kValues; e++) sum[e] = at < a.words ? from[e] : 0.f;
-  from += stride;  // the part at the head of the next chunk
-  // 64 chunks at a time: how many of them begin with this token
-  for (int64_t p = p1;; p += 64 * static_cast<int64_t>(a.chunk)) {
-    const int64_t own   = p + static_cast<int64_t>(threadIdx.x & 63) * a.chunk;
-    const uint64_t same = __ballot(own < a.n_tokens && a.sorted.key[min(own, static_cast<int64_t>(a.n_tokens) - 1)] == row);
-    const int parts     = same == ~uint64_t(0) ? 64 : __builtin_ctzll(~same);
+  // adds the heads begin .. end - 1 of the chunks after `chunk`
+  auto add_heads = [&](int64_t chunk, int at, int64_t begin, int64_t end) {
+    const float* from = a.part + (chunk + 1 + begin) * 2 * stride + static_cast<int64_t>(min(at, a.words - 1)) * P::kValues;
     constexpr int kAhead = 8;
-    for (int i = 0; i < parts; i += kAhead) {
+    for (int64_t i = begin; i < end; i += kAhead, from += kAhead * 2 * stride) {
       float x[kAhead][P::kValues];
 #pragma unroll
       for (int j = 0; j < kAhead; j++)
-        if (at < a.words && i + j < parts)
 #pragma unroll
-          for (int e = 0; e < P::kValues; e++) x[j][e] = from[(i + j) * 2 * stride + e];
+        for (int e = 0; e < P::kValues; e++) x[j][e] = from[min(static_cast<int64_t>(j), end - 1 - i) * 2 * stride + e];
 #pragma unroll
       for (int j = 0; j < kAhead; j++)
-        if (i + j < parts)
 #pragma unroll
-          for (int e = 0; e < P::kValues; e++) sum[e] += x[j][e];
+        for (int e = 0; e < P::kValues; e++) sum[e] += i + j < end ? x[j][e] : 0.f;
     }
-    if (parts < 64) break;
-    from += 64 * 2 * stride;
+  };
+  auto begin_sum = [&](int64_t chunk, int at, bool tail) {  // with the part at the tail of the chunk, where the run begins
+#pragma unroll
+    for (int e = 0; e < P::kValues; e++)
+      sum[e] = tail && at < a.words ? a.part[(chunk * 2 + 1) * stride + static_cast<int64_t>(at) * P::kValues + e] : 0.f;
+  };
+  const int64_t first_task = static_cast<int64_t>(blockIdx.x) * kJoinWaves;
+  const int64_t chunk = (first_task + wave) / a.slices, p0 = chunk * a.chunk, p1 = p0 + a.chunk;
+  int64_t heads = 0;
+  if (p1 < a.n_tokens) {
+    const int row = a.sorted.key[p1 - 1];
+    // (a run that began earlier is another chunk's)
+    if (row < a.n_rows && a.sorted.key[p1] == row && !(p0 > 0 && a.sorted.key[p0 - 1] == row)) {
+      // how many chunks begin with this token, found 64 at a time from steps of `step` chunks down to single ones
+      auto in_run = [&](int64_t head) {
+        const int64_t p = p1 + head * a.chunk;
+        return p < a.n_tokens && a.sorted.key[min(p, static_cast<int64_t>(a.n_tokens) - 1)] == row;
+      };
+      auto reach = [&](int64_t from, int64_t step) {  // the lanes' first that is no longer in the run
+        const uint64_t same = __ballot(in_run(from + lane * step));
+        return same == ~uint64_t(0) ? 64 : __builtin_ctzll(~same);
+      };
+      heads = reach(0, 1);
+      if (heads < 64) {
+        const int at = static_cast<int>((first_task + wave) % a.slices) * 64 + lane;
+        begin_sum(chunk, at, true);
+        add_heads(chunk, at, 0, heads);
+        if (at < a.words) write_row<kDtype, kBytes>(a, row, at, sum);
+        heads = 0;
+      } else {
+        int64_t step = 64;
+        while (step * 64 * a.chunk < a.n_tokens) step *= 64;
+        heads = 0;
+        for (; step > 0; step /= 64) heads += (reach(heads, step) - 1) * step;  // (head `heads` is in the run)
+        heads += 1;
+      }
+    }
   }
-  if (at >= a.words) return;
-  write_row<kDtype, kBytes>(a, row, at, sum);
+  if (lane == 0) heads_of[wave] = heads;
+  if (!__syncthreads_or(heads != 0)) return;
+  for (int w = 0; w < kJoinWaves; w++) {
+    const int64_t all = heads_of[w];
+    if (all == 0) continue;
+    const int64_t of = (first_task + w) / a.slices;
+    const int at     = static_cast<int>((first_task + w) % a.slices) * 64 + lane;
+    const int64_t share = (all + kJoinWaves - 1) / kJoinWaves;
+    begin_sum(of, at, wave == 0);
+    add_heads(of, at, min(wave * share, all), min((wave + 1) * share, all));
+#pragma unroll
+    for (int e = 0; e < P::kValues; e++) part[wave][e][lane] = sum[e];
+    __syncthreads();
+    if (wave == 0) {
+      for (int v = 1; v < kJoinWaves; v++)
+#pragma unroll
+        for (int e = 0; e < P::kValues; e++) sum[e] += part[v][e][lane];
+      if (at < a.words) write_row<kDtype, kBytes>(a, a.sorted.key[(of + 1) * a.chunk], at, sum);
+    }
+    __syncthreads();
+  }
 }
 
 // ---- few places -----------------------------------------------------------------------------------------
 
 // Few tokens need no sorting: a workgroup takes some rows of the table, lists the places that name one of them in ascending order,
-// and its waves add up a row each. One launch.
-constexpr int kDirectTokens = 2048;
+// and its waves add up a row each; a long one, or one that more than 32 places name, is shared out among them afterwards. One launch.
+constexpr int kDirectTokens = 2048, kDirectShared = 32, kDirectRows = 64;
 
 template <int kDtype, int kBytes>
 __global__ void __launch_bounds__(kRowThreads)
@@ -483,6 +527,9 @@ __global__ void __launch_bounds__(kRowThreads)
   using Word = typename P::Word;
   __shared__ int list[kDirectTokens];  // row of the workgroup << 16 | place
   __shared__ int count[kRowWaves];
+  enum { kAlone = 0, kBySlices = 1, kByPlaces = 2 };  // a row is one wave's; its slices, or the places that name it, are shared out
+  __shared__ uint8_t shared[kDirectRows];
+  __shared__ float part[kRowWaves][P::kValues][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int first = blockIdx.x * rows_each;
   int listed = 0;
@@ -503,48 +550,88 @@ __global__ void __launch_bounds__(kRowThreads)
     __syncthreads();
   }
   listed = __builtin_amdgcn_readfirstlane(listed);
+  if (listed == 0) {
+    if (a.add) return;
+    Word* to          = static_cast<Word*>(a.out) + static_cast<int64_t>(first) * a.words;
+    const int64_t all = static_cast<int64_t>(min(rows_each, a.n_rows - first)) * a.words;
+    for (int64_t i = threadIdx.x; i < all; i += kRowThreads) to[i] = Word{};
+    return;
+  }
+  // adds the rows of the places l .. l_end - 1 of the list that name row r
+  auto add_up = [&](int r, int l, int l_end, int at, float(&sum)[P::kValues]) {
+    constexpr int kAhead = 8;
+#pragma unroll
+    for (int e = 0; e < P::kValues; e++) sum[e] = 0.f;
+    for (; l < l_end; l += 64) {
+      const int entry = l + lane < l_end ? list[l + lane] : -1;
+      uint64_t same   = __ballot(entry >> 16 == r);
+      while (same != 0) {
+        // (the last one again where there are no more: behind a branch the loads would be waited for one by one)
+        Word w[kAhead];
+        int found = 0, place = 0;
+#pragma unroll
+        for (int j = 0; j < kAhead; j++) {
+          if (same != 0) {
+            place = __builtin_amdgcn_readlane(entry, __builtin_ctzll(same)) & 0xffff;
+            found++;
+          }
+          same &= same - 1;
+          w[j] = static_cast<const Word*>(a.grad)[static_cast<int64_t>(place) * a.words + min(at, a.words - 1)];
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < kAhead; j++) {
+          float x[P::kValues];
+          P::unpack(w[j], x);
+#pragma unroll
+          for (int e = 0; e < P::kValues; e++) sum[e] += j < found ? x[e] : 0.f;
+        }
+      }
+    }
+  };
   for (int r = wave; r < rows_each && first + r < a.n_rows; r += kRowWaves) {
-    bool any = false;
-    for (int l = 0; l < listed && !any; l += 64) any = __any(l + lane < listed && list[min(l + lane, kDirectTokens - 1)] >> 16 == r);
-    if (!any) {
+    int named = 0;
+    for (int l = 0; l < listed; l += 64) named += __popcll(__ballot(l + lane < listed && list[min(l + lane, kDirectTokens - 1)] >> 16 == r));
+    const int how = named == 0                                            ? kAlone
+                    : named > kDirectShared && a.slices < kRowWaves ? kByPlaces
+                    : a.slices > 1                                        ? kBySlices
+                                                                          : kAlone;
+    if (lane == 0) shared[r] = static_cast<uint8_t>(how);
+    if (how != kAlone) continue;
+    if (named == 0) {
       if (!a.add) {
         Word* to = static_cast<Word*>(a.out) + static_cast<int64_t>(first + r) * a.words;
         for (int i = lane; i < a.words; i += 64) to[i] = Word{};
       }
       continue;
     }
-    for (int slice = 0; slice < a.slices; slice++) {
-      const int at      = slice * 64 + lane;
-      const bool inside = at < a.words;
+    float sum[P::kValues];
+    add_up(r, 0, listed, lane, sum);
+    if (lane < a.words) write_row<kDtype, kBytes>(a, first + r, lane, sum);
+  }
+  __syncthreads();
+  const int share = ((listed + 63) / 64 + kRowWaves - 1) / kRowWaves * 64;
+  const int begin = min(wave * share, listed), end = min(begin + share, listed);
+  for (int r = 0; r < rows_each && first + r < a.n_rows; r++) {
+    const int how = __builtin_amdgcn_readfirstlane(shared[r]);
+    if (how == kAlone) continue;
+    for (int slice = how == kBySlices ? wave : 0; slice < a.slices; slice += how == kBySlices ? kRowWaves : 1) {
+      const int at = slice * 64 + lane;
       float sum[P::kValues];
+      add_up(r, how == kBySlices ? 0 : begin, how == kBySlices ? listed : end, at, sum);
+      if (how == kByPlaces) {
 #pragma unroll
-      for (int e = 0; e < P::kValues; e++) sum[e] = 0.f;
-      for (int l = 0; l < listed; l += 64) {
-        const int entry = l + lane < listed ? list[l + lane] : -1;
-        uint64_t same   = __ballot(entry >> 16 == r);
-        constexpr int kAhead = 8;
-        while (same != 0) {
-          Word w[kAhead];
-          int found = 0;
+        for (int e = 0; e < P::kValues; e++) part[wave][e][lane] = sum[e];
+        __syncthreads();
+        if (wave == 0) {
 #pragma unroll
-          for (int j = 0; j < kAhead; j++) {
-            if (same == 0) break;
-            const int place = __builtin_amdgcn_readlane(entry, __builtin_ctzll(same)) & 0xffff;
-            same &= same - 1;
-            found++;
-            if (inside) w[j] = static_cast<const Word*>(a.grad)[static_cast<int64_t>(place) * a.words + at];
-          }
+          for (int w = 1; w < kRowWaves; w++)
 #pragma unroll
-          for (int j = 0; j < kAhead; j++) {
-            if (j >= found) break;
-            float x[P::kValues];
-            P::unpack(w[j], x);
-#pragma unroll
-            for (int e = 0; e < P::kValues; e++) sum[e] += x[e];
-          }
+            for (int e = 0; e < P::kValues; e++) sum[e] += part[w][e][lane];
         }
+        __syncthreads();
       }
-      if (inside) write_row<kDtype, kBytes>(a, first + r, at, sum);
+      if ((how == kBySlices || wave == 0) && at < a.words) write_row<kDtype, kBytes>(a, first + r, at, sum);
     }
   }
 }
@@ -609,7 +696,7 @@ int embed_gradient(hipStream_t s, const EmbedCall& c, const void* grad, const vo
   RunArgs a{grad,  c.sorted[0], static_cast<int>(c.n_tokens), c.n_rows, c.words, c.chunk, c.slices, scale, out, add ? 1 : 0, 0,
             c.part};
   if (direct(c.n_tokens, static_cast<int64_t>(c.words) * kBytes)) {
-    int each = 64;  // rows of a workgroup: fewer where that gives too few workgroups
+    int each = kDirectRows;  // rows of a workgroup: fewer where that gives too few workgroups
     while (each > 4 && c.n_rows / each < 2048) each /= 2;
     direct_rows_kernel<kDtype, kBytes><<<static_cast<unsigned>((static_cast<int64_t>(c.n_rows) + each - 1) / each), kRowThreads, 0, s>>>(
       a, tokens, token_bytes, each);
@@ -648,7 +735,7 @@ int embed_gradient(hipStream_t s, const EmbedCall& c, const void* grad, const vo
   sum_runs_kernel<kDtype, kBytes><<<static_cast<unsigned>(grid + a.clears), kRowThreads, 0, s>>>(a);
   LBT_HIP(hipGetLastError());
   if (c.chunks > 1) {
-    join_runs_kernel<kDtype, kBytes><<<static_cast<unsigned>(grid), kRowThreads, 0, s>>>(a);
+    join_runs_kernel<kDtype, kBytes><<<static_cast<unsigned>((c.chunks * c.slices + kJoinWaves - 1) / kJoinWaves), kJoinThreads, 0, s>>>(a);
     LBT_HIP(hipGetLastError());
   }
   return LBT_OK;

@@ -17,6 +17,7 @@
 // theirs. bfloat16 and float hold G as it is: their exponents reach far enough.
 #include <algorithm>
 
+#include "lbt_device.h"
 #include "lbt_products.h"
 
 namespace lbt {
@@ -461,13 +462,13 @@ __device__ __forceinline__ void turn_rows(char* lds, int wave, int lane, Value v
         if constexpr (kSize == 4) *reinterpret_cast<float4*>(at) = make_float4(v[0], v[1], v[2], v[3]);
         else *reinterpret_cast<uint2*>(at) = *reinterpret_cast<const uint2*>(v);  // (`value` has packed them)
       }
-    __builtin_amdgcn_wave_barrier();
+    meet_in_wave();
 #pragma unroll
     for (int pass = 0; pass < 32 / kRows; pass++) {
       const int n = pass * kRows + lane / kLanes, c = lane % kLanes;
       sink(n, group * kBlocks * 32 + c * (16 / kSize), *reinterpret_cast<const uint4*>(own + n * kStride + c * 16));
     }
-    __builtin_amdgcn_wave_barrier();
+    meet_in_wave();
   }
 }
 

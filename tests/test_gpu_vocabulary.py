@@ -406,6 +406,30 @@ def test_embed_rows_gradient(t, f, rows, kind, dtype):
     assert to.cpu()[~named].isnan().all()
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("lengths,f", [
+    ((33, 32, 1, 0, 64, 700, 31, 1100), 130),  # at once: rows that one wave, and rows that four waves add up
+    ((2048,), 40),
+    ((3, 505, 512, 0, 520, 529, 1, 1040, 513), 24),  # 63, 64 and more chunks of 8
+    ((5, 4096 * 8, 1, 20000, 4000, 3), 7),  # over 4096 of them
+    ((1, 40000, 0, 25000, 7), 1030),
+])
+def test_embed_rows_gradient_of_rows_that_many_places_name(lengths, f, dtype):
+    gen = torch.Generator(device="cuda").manual_seed(len(lengths) + f)
+    tokens = torch.repeat_interleave(torch.arange(len(lengths)), torch.tensor(lengths)).cuda()
+    tokens = tokens[torch.randperm(tokens.numel(), generator=gen, device="cuda")]
+    grad = torch.randn((tokens.numel(), f), generator=gen, device="cuda").to(TYPES[dtype])
+    got = ops.embed_rows_gradient(grad, tokens, len(lengths), scale=0.3)
+    want, bound, named = embed_reference(grad, tokens, len(lengths), 0.3, dtype)
+    assert_within(got.cpu(), want, bound, "grad_table")
+    assert not got.cpu()[~named].any()
+    assert torch.equal(ops.embed_rows_gradient(grad, tokens, len(lengths), scale=0.3), got)
+    # one place more, that names no row and has no number: nothing changes but the order of the sums
+    grad = torch.cat([torch.full((1, f), float("nan"), dtype=grad.dtype, device="cuda"), grad])
+    tokens = torch.cat([torch.tensor([-100], device="cuda"), tokens])
+    assert_within(ops.embed_rows_gradient(grad, tokens, len(lengths), scale=0.3).cpu(), want, bound, "grad_table")
+
+
 def test_embed_gradient_shapes_and_places_that_name_no_row():
     grad = torch.randn((4, 6, 16), device="cuda")
     tokens = torch.randint(0, 9, (4, 6), device="cuda")
