@@ -255,6 +255,12 @@ __device__ __forceinline__ void take_eight(const void* __restrict__ from, int64_
   }
 }
 
+// Where an operand's values are: plane q of row p begins at q * plane + p * row, every 32 columns are `block` further on.
+struct Layout {
+  int64_t plane, row, block;
+  __device__ __forceinline__ int64_t at(int q, int64_t p, int col) const { return q * plane + p * row + (col >> 5) * block + (col & 31); }
+};
+
 // Rows of an array as rows of an operand: in `order` where that is given, -1 and what lies past the end as zeros, columns
 // padded with zeros to `padded_cols`, floats as three planes. A thread takes 8 columns. Bound by the copy: it reads and writes
 // each value once. Half precision with weights: kMeasure finds counts->reach, kScale multiplies row p by 2^(exponent[p] + 14 - reach).
@@ -264,7 +270,7 @@ template <int kDtype>
 __global__ void __launch_bounds__(256)
   pack_rows_kernel(const void* __restrict__ from, int64_t first_row, int64_t rows, int cols, const int32_t* __restrict__ order,
                    int mode, const int32_t* __restrict__ exponent, RowCounts* counts, int64_t out_rows, int padded_cols,
-                   int64_t plane, uint16_t* __restrict__ out)
+                   Layout layout, uint16_t* __restrict__ out)
 {
   using L          = LossType<kDtype>;
   const int groups = padded_cols / 8;
@@ -304,13 +310,13 @@ __global__ void __launch_bounds__(256)
   }
 #pragma unroll
   for (int q = 0; q < L::kPlanes; q++)
-    *reinterpret_cast<uint4*>(out + q * plane + p * padded_cols + col) = *reinterpret_cast<const uint4*>(v[q]);
+    *reinterpret_cast<uint4*>(out + layout.at(q, p, col)) = *reinterpret_cast<const uint4*>(v[q]);
 }
 
 // prepare_rows_kernel and the laying out of X, and of the weights where they are laid out, in one launch for up to 1024 rows: a workgroup
-// goes through all labels for itself and lays out 16 of the rows that count; others lay out the weights. Not for weighted rows in half
+// goes through all labels for itself and lays out up to 512 columns of 16 of the rows that count; others lay out the weights. Not for weighted rows in half
 // precision, whose weights' exponents have to be known first.
-constexpr int kFusedRows = 1024, kFusedEach = 16;
+constexpr int kFusedRows = 1024, kFusedEach = 16, kFusedGroups = 64;
 struct FusedArgs {
   const int64_t* y;
   const float* row_weight;
@@ -322,13 +328,14 @@ struct FusedArgs {
   int cols, padded_cols;
   uint16_t *x_out, *weight_out;  // (the second: null where the weights are not laid out)
   int64_t weight_rows;           // of weight_out
+  Layout x_layout;
 };
 
 template <int kDtype>
 __global__ void __launch_bounds__(256) prepare_pack_kernel(const FusedArgs a, const LossRows out)
 {
   using L          = LossType<kDtype>;
-  const int groups = a.padded_cols / 8, x_blocks = a.padded / kFusedEach;
+  const int groups = a.padded_cols / 8, slices = (groups + kFusedGroups - 1) / kFusedGroups, x_blocks = a.padded / kFusedEach * slices;
   uint16_t v[L::kPlanes][8];
   if (static_cast<int>(blockIdx.x) >= x_blocks) {
     const int64_t i = (static_cast<int64_t>(blockIdx.x) - x_blocks) * 256 + threadIdx.x;
@@ -344,7 +351,7 @@ __global__ void __launch_bounds__(256) prepare_pack_kernel(const FusedArgs a, co
   constexpr int kEach = kFusedRows / 256;
   __shared__ int wave_sum[kEach][4], from[kFusedEach];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int p0 = blockIdx.x * kFusedEach;
+  const int p0 = blockIdx.x / slices * kFusedEach, group0 = blockIdx.x % slices * kFusedGroups, own = min(kFusedGroups, groups - group0);
   const bool first = blockIdx.x == 0;
   if (first && threadIdx.x < 8) a.zeros[threadIdx.x] = 0;
   if (threadIdx.x < kFusedEach) from[threadIdx.x] = -1;
@@ -376,8 +383,9 @@ __global__ void __launch_bounds__(256) prepare_pack_kernel(const FusedArgs a, co
       const int p = before + __popcll(set[e] & ((uint64_t(1) << lane) - 1));
       if (first) out.place[r] = p;
       if (p >= p0 && p < p0 + kFusedEach) {
+        from[p - p0] = r;
+        if (group0 > 0) continue;
         const float w   = a.row_weight != nullptr ? a.row_weight[r] : 1.f;
-        from[p - p0]    = r;
         out.order[p]    = r;
         out.label[p]    = static_cast<int32_t>(label[e]);
         out.factor[p]   = kDtype == LBT_F16 ? w * (1 << kHalfShift) : w;
@@ -391,7 +399,7 @@ __global__ void __launch_bounds__(256) prepare_pack_kernel(const FusedArgs a, co
   }
   if (first && threadIdx.x == 0) *a.counts = RowCounts{at, 0, -1000};
   __syncthreads();
-  if (threadIdx.x < kFusedEach && p0 + static_cast<int>(threadIdx.x) >= at) {
+  if (group0 == 0 && threadIdx.x < kFusedEach && p0 + static_cast<int>(threadIdx.x) >= at) {
     const int p     = p0 + threadIdx.x;
     out.order[p]    = -1;
     out.label[p]    = -1;
@@ -399,12 +407,12 @@ __global__ void __launch_bounds__(256) prepare_pack_kernel(const FusedArgs a, co
     out.exponent[p] = -1000;
     out.picked[p]   = 0.f;
   }
-  for (int i = threadIdx.x; i < kFusedEach * groups; i += 256) {
-    const int p = i / groups, col = (i % groups) * 8;
+  for (int i = threadIdx.x; i < kFusedEach * own; i += 256) {
+    const int p = i / own, col = (group0 + i % own) * 8;
     take_eight<kDtype>(a.x, from[p], col, a.cols, v);
 #pragma unroll
     for (int q = 0; q < L::kPlanes; q++)
-      *reinterpret_cast<uint4*>(a.x_out + (static_cast<int64_t>(q) * a.padded + p0 + p) * a.padded_cols + col) = *reinterpret_cast<const uint4*>(v[q]);
+      *reinterpret_cast<uint4*>(a.x_out + a.x_layout.at(q, p0 + p, col)) = *reinterpret_cast<const uint4*>(v[q]);
   }
 }
 
@@ -1218,6 +1226,8 @@ __global__ void __launch_bounds__(256) clear_kernel(uint16_t* __restrict__ out, 
 using LargeTile  = ProductTile<256, 256, 2, 4, 2>;
 using MediumTile = ProductTile<128, 128, 2, 2, 2>;
 using SmallTile  = ProductTile<64, 64, 2, 2, 5>;
+using FloatLarge = FloatTile<128, 128, 2, 2, 1, 2>;
+using FloatSmall = FloatTile<64, 64, 2, 2, 2, 4>;
 
 int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 int64_t tiles_of(int64_t v, int64_t by) { return (v + by - 1) / by; }
@@ -1227,34 +1237,58 @@ int64_t tiles_of(int64_t v, int64_t by) { return (v + by - 1) / by; }
 // then waits for memory), and a tile 8, 3 and 2 us to begin and end. Each split adds a pass over the sums.
 struct Cut {
   int tile, splits;
+  double time;  // us, roughly
 };
 Cut cut_product(int64_t m, int64_t n, int64_t stages, int64_t most_splits)
 {
   constexpr int kCus = 256;
   constexpr struct { int tile; double stage, lone, ends; } kTiles[3] = {{256, 1.72, 1.72, 8.0}, {128, 0.5, 0.7, 3.0}, {64, 0.2, 0.35, 2.0}};
-  Cut best{256, 1};
-  double least = 1e30;
+  Cut best{256, 1, 1e30};
   for (const auto& t : kTiles)
     for (int splits = 1; splits <= most_splits; splits++) {
       if (splits > 1 && stages / splits < 4) break;
       const int64_t each = tiles_of(tiles_of(m, t.tile) * tiles_of(n, t.tile) * splits, kCus);
       const double time  = each * (tiles_of(stages, splits) * (each == 1 ? t.lone : t.stage) + t.ends) +
                           (splits - 1) * (1.0 + m * n * 8e-6 / 4.0);
-      if (time < least) {
-        least = time;
-        best  = {t.tile, splits};
-      }
+      if (time < best.time) best = {t.tile, splits, time};
     }
   return best;
 }
 
 // Scores of few rows: the waves share the classes of a workgroup where they would be fewer than four a CU, and always where they
-// leave u, whose shares are then 16 classes each. Blocks of 64 rows: one of them for 16-bit types, whose weights the tiles take as
-// they are; up to four for float, which the tiles would first lay out in planes.
+// leave u, whose shares are then 16 classes each. Blocks of 64 rows: one of them for 16-bit types, up to four for float.
 bool few_shared(int classes) { return classes < 65536; }
-bool few_rows(int64_t n_rows, int dtype) { return n_rows <= (dtype == LBT_F32 ? 4 * kFewBlock : kFewBlock); }
+constexpr int kFewFloatRows = 4 * kFewBlock;
 int few_class_blocks(int64_t n_rows, int classes) { return n_rows <= 16 || classes < 32768 ? 1 : 2; }
 int64_t few_groups(int classes, int class_blocks, bool shared) { return tiles_of(classes, 16 * class_blocks * (shared ? 1 : 4)); }
+
+// The same for float_product_kernel over `stages` of 32 of k: a stage takes a CU 0.5 and 1.4 us. (3000 classes of 4000 features: 256
+// rows 75 us in tiles of 64, 168 in those of 128; 4096 rows 665 and 537.)
+Cut cut_floats(int64_t m, int64_t n, int64_t stages)
+{
+  constexpr int kCus = 256;
+  constexpr struct { int tile; double stage, ends; } kTiles[2] = {{128, 1.4, 4.0}, {64, 0.5, 2.0}};
+  Cut best{128, 1, 1e30};
+  for (const auto& t : kTiles) {
+    const double time = tiles_of(tiles_of(m, t.tile) * tiles_of(n, t.tile), kCus) * (stages * t.stage + t.ends);
+    if (time < best.time) best = {t.tile, 1, time};
+  }
+  return best;
+}
+
+// us of few_rows_kernel for float, whose products it forms at 50 TFLOP/s, and of the join.
+double few_float_time(int64_t n_rows, int64_t features, int64_t classes)
+{
+  return 6.0 + 4e-8 * static_cast<double>(round_up(n_rows, 16)) * features * classes;
+}
+// Whether the loss alone takes few_rows_kernel. (float, 1000 features: 33 rows 25.7 us and 32.1 in tiles over 10007 classes, 61 and 44 over
+// 30000; 4000 features, 3000 classes: 64 rows 42 and 72 us, 256 rows 115 and 75.)
+bool few_loss(int64_t n_rows, int64_t features, int64_t classes, int dtype)
+{
+  if (dtype != LBT_F32) return n_rows <= kFewBlock;
+  return n_rows <= 16 || (n_rows <= kFewFloatRows && few_float_time(n_rows, features, classes) <
+                                                       11.0 + cut_floats(classes, n_rows, tiles_of(features, FloatLarge::kK)).time);
+}
 
 struct FewCall {
   float2* partial;
@@ -1323,6 +1357,7 @@ struct LossCall {
   int kept;         // all classes are one piece: G is made from the scores' exponentials instead of the scores once more
   int scale_rows;   // of a workgroup of scale_kernel
   bool few;         // the scores are those of few_rows_kernel
+  bool floats;      // of float_product_kernel
   Cut all_scores, scores, row_product, class_product;
   LossRows rows;
   RowCounts* counts;
@@ -1336,7 +1371,8 @@ struct LossCall {
     planes = type == LBT_F32 ? 3 : 1;
     padded = round_up(n, 256);
     cols   = static_cast<int>(round_up(f, kProductK));
-    packed = type == LBT_F32 || f % 8 != 0;
+    floats = type == LBT_F32 && grad == 0;
+    packed = !floats && (type == LBT_F32 || f % 8 != 0);
     // a piece's G and its packed weights within their bounds; pieces of one size
     int64_t most = round_up(k, 256);
     kept                = type == LBT_BF16 && !with_bias ? kKeptHalf : kKeptFloat;  // (the sums for the bias are those of floats)
@@ -1349,7 +1385,8 @@ struct LossCall {
     const int64_t pairs = type == LBT_F32 ? 6 : 1;
     scores      = cut_product(std::min<int64_t>(piece, k), n, pairs * cols / kProductK, 1);
     all_scores  = packed ? scores : cut_product(k, n, pairs * cols / kProductK, 1);
-    few         = kept != kNotKept && few_rows(n, type);
+    if (floats) all_scores = cut_floats(k, n, tiles_of(f, FloatLarge::kK));
+    few         = kept != kNotKept && (type == LBT_F32 ? n <= kFewFloatRows && few_float_time(n, f, k) < 6.0 + scores.time : n <= kFewBlock);
     scale_rows  = tiles_of(padded, 16) * tiles_of(piece, kScaleClasses) >= 1024 ? 16 : 4;
     row_product = cut_product(f, n, pairs * piece / kProductK, 64);
     class_product = cut_product(f, std::min<int64_t>(piece, k), pairs * tiles_of(n, kProductK), 64);
@@ -1404,14 +1441,26 @@ int launch_product(hipStream_t s, const ProductArgs& args, int64_t m, int64_t n,
   return launch_tiles<SmallTile, L, kAMajor, kBMajor, kRowsSide>(s, args, m, n, cut.splits, e);
 }
 
+template <class Tile, class Epilogue>
+int launch_floats(hipStream_t s, FloatArgs args, int64_t n, const Epilogue& e)
+{
+  args.tiles_m = static_cast<int>(tiles_of(args.m, Tile::kBM));
+  args.tiles_n = static_cast<int>(tiles_of(n, Tile::kBN));
+  const int64_t blocks = static_cast<int64_t>(args.tiles_m) * args.tiles_n;
+  LBT_REQUIRE(blocks < (int64_t(1) << 31), "too many tiles");
+  float_product_kernel<Tile, Epilogue><<<static_cast<unsigned>(blocks), Tile::kThreads, 0, s>>>(args, e);
+  LBT_HIP(hipGetLastError());
+  return LBT_OK;
+}
+
 template <int kDtype>
 int launch_pack(hipStream_t s, const void* from, int64_t first_row, int64_t rows, int cols, const int32_t* order,
-                int mode, const int32_t* exponent, RowCounts* counts, int64_t out_rows, int padded_cols, int64_t plane, uint16_t* out)
+                int mode, const int32_t* exponent, RowCounts* counts, int64_t out_rows, int padded_cols, Layout layout, uint16_t* out)
 {
   const int64_t blocks = tiles_of(out_rows * (padded_cols / 8), 256);
   LBT_REQUIRE(blocks < (int64_t(1) << 31), "too many values to lay out");
   pack_rows_kernel<kDtype><<<static_cast<unsigned>(blocks), 256, 0, s>>>(from, first_row, rows, cols, order, mode, exponent, counts,
-                                                                         out_rows, padded_cols, plane, out);
+                                                                         out_rows, padded_cols, layout, out);
   LBT_HIP(hipGetLastError());
   return LBT_OK;
 }
@@ -1435,10 +1484,11 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
   }
   const bool scaled = kHalf && sample_weight != nullptr;  // (without weights every exponent is 0)
   const bool fused  = c.n_rows <= kFusedRows && !scaled;
+  const Layout x_layout = c.floats ? Layout{32, 96, 96 * c.padded} : Layout{c.padded * c.cols, c.cols, 32};
   if (fused) {
     const FusedArgs a{y,         sample_weight, static_cast<int>(c.n_rows), static_cast<int>(c.padded), c.classes, loss, c.counts, c.zeros, X, weight,
-                      c.features, c.cols,        c.x,                        c.packed ? c.weight : nullptr, c.packed ? c.piece : 0};
-    const int64_t blocks = c.padded / kFusedEach + tiles_of(a.weight_rows * (c.cols / 8), 256);
+                      c.features, c.cols,        c.x,                        c.packed ? c.weight : nullptr, c.packed ? c.piece : 0, x_layout};
+    const int64_t blocks = c.padded / kFusedEach * tiles_of(c.cols / 8, kFusedGroups) + tiles_of(a.weight_rows * (c.cols / 8), 256);
     LBT_REQUIRE(blocks < (int64_t(1) << 31), "too many values to lay out");
     prepare_pack_kernel<kDtype><<<static_cast<unsigned>(blocks), 256, 0, s>>>(a, c.rows);
     LBT_HIP(hipGetLastError());
@@ -1446,7 +1496,7 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
     prepare_rows_kernel<<<1, kPrepareThreads, 0, s>>>(y, sample_weight, c.n_rows, c.padded, c.classes, kHalf, c.rows, loss, c.counts, c.zeros);
     LBT_HIP(hipGetLastError());
     LBT_TRY(launch_pack<kDtype>(s, X, 0, c.n_rows, c.features, c.rows.order, scaled ? kMeasure : kCopy, c.rows.exponent, c.counts, c.padded,
-                                c.cols, c.padded * c.cols, c.x));
+                                c.cols, x_layout, c.x));
   }
 
   // (rows that do not count are not there: x holds them side by side)
@@ -1459,7 +1509,7 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
   auto lay_out = [&](int64_t first) {
     if (!c.packed) return LBT_OK;
     return launch_pack<kDtype>(s, weight, first, c.classes, c.features, nullptr, kCopy, nullptr, c.counts, c.piece, c.cols,
-                               c.piece * c.cols, c.weight);
+                               Layout{c.piece * c.cols, c.cols, 32}, c.weight);
   };
   ProductArgs args{};
   args.zeros  = c.zeros;
@@ -1480,7 +1530,7 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
   for (int64_t first = 0; first < c.classes && !c.few; first += step) {
     const int64_t classes = std::min<int64_t>(step, c.classes - first);
     if (first > 0 || !fused) LBT_TRY(lay_out(first));  // (the first piece is there)
-    args.a = weights(first, classes);
+    if (!c.floats) args.a = weights(first, classes);
     args.b = x;
     args.k_extent = args.k_split = c.cols;
     const int share = 2 * static_cast<int>(tiles);  // (all tiles are two waves high)
@@ -1491,6 +1541,11 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
       const LossEpilogue<kFine, kKind> e{bias, static_cast<int>(first), c.classes, share, c.padded, c.rows, c.partial,
                                          kKind == kKeptFloat ? static_cast<void*>(c.exps) : c.g, static_cast<int>(c.piece)};
       tiles += tiles_of(m, c.all_scores.tile);
+      if constexpr (kFine && kKind == kNotKept)
+        if (c.floats) {
+          const FloatArgs fa{static_cast<const float*>(weight), c.classes, c.features, c.x, c.padded, 0, 0, c.zeros, c.counts};
+          return c.all_scores.tile == FloatLarge::kBM ? launch_floats<FloatLarge>(s, fa, c.n_rows, e) : launch_floats<FloatSmall>(s, fa, c.n_rows, e);
+        }
       return launch_product<L, false, false, kRowsN>(s, args, m, c.n_rows, c.all_scores, e);
     };
     if constexpr (kDtype == LBT_BF16)
@@ -1515,7 +1570,7 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
 
   if (scaled)
     LBT_TRY(launch_pack<kDtype>(s, X, 0, c.n_rows, c.features, c.rows.order, kScale, c.rows.exponent, c.counts, c.padded, c.cols,
-                                c.padded * c.cols, c.x_scaled));
+                                x_layout, c.x_scaled));
   ProductOperand x_scaled = x;
   if (scaled) x_scaled.base = c.x_scaled;
   const ProductOperand g{c.g, c.piece, c.padded * c.piece, static_cast<int32_t>(c.padded), static_cast<int32_t>(c.piece)};
@@ -1633,7 +1688,7 @@ int run_loss(void* stream, const void* X, const void* weight, int32_t dtype, int
   }
   LossCall c(std::max<int64_t>(n_rows, 1), n_features, n_outputs, dtype, !gradient ? 0 : grad_bias == nullptr ? 1 : 2);
   c.n_rows       = n_rows;
-  const bool few = !gradient && few_rows(n_rows, dtype);
+  const bool few = !gradient && few_loss(n_rows, n_features, n_outputs, dtype);
   FewCall f;
   Arena arena;
   arena.base = static_cast<char*>(workspace);
@@ -1672,7 +1727,7 @@ size_t lbt_linear_log_loss_workspace_bytes(int64_t n_rows, int32_t n_features, i
   lbt::LossCall c(std::max<int64_t>(n_rows, 1), n_features, n_outputs, dtype, gradient);
   lbt::Arena arena;
   arena.measure = true;
-  if (gradient == 0 && lbt::few_rows(n_rows, dtype)) {
+  if (gradient == 0 && lbt::few_loss(n_rows, n_features, n_outputs, dtype)) {
     lbt::FewCall f;
     f.carve(arena, n_rows, n_outputs);
     return std::max<size_t>(arena.used, 256);

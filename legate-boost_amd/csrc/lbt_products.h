@@ -386,6 +386,242 @@ __global__ void __launch_bounds__(Tile::kThreads, 2)
   }
 }
 
+// ---- float by planes: the first operand as it lies in memory ----------------------------------------
+//
+// C[m][n] = sum_k A(m, k) B(n, k) for an A of floats that is read once, k contiguous, rows of any length, and a B laid out in planes.
+// A goes into the LDS as floats and becomes three planes on its way from the registers to the matrix cores: hi is the float's upper
+// half, what is left goes on exactly and is rounded, v = hi + mid + lo. The six products of a step follow one another, so a value is
+// read from memory and from the LDS once where operands of planes are read up to six times, and nothing is laid out first. The eight
+// values of a fragment take 44 instructions to split while its 6 products with each fragment of B take 192 cycles.
+template <int kM, int kN, int kWaveM, int kWaveN, int kWaveK, int kDepth>
+struct FloatTile {
+  static constexpr int kBM = kM, kBN = kN, kWM = kM / kWaveM, kWN = kN / kWaveN;
+  static constexpr int kWavesM = kWaveM, kWavesN = kWaveN, kWavesK = kWaveK;
+  static constexpr int kWaves = kWaveM * kWaveN * kWaveK, kThreads = kWaves * 64;
+  static constexpr int kMT = kWM / 32, kNT = kWN / 32, kStages = kDepth;
+  static constexpr int kK = 32;  // of a stage
+  static constexpr int kStageA = kM * kK * 4, kRowB = 3 * kK * 2, kStage = kStageA + kN * kRowB, kLds = kStages * kStage;  // bytes
+  // loads of a wave for a stage; the first kMore waves have one of B more where they do not come out even
+  static constexpr int kLoadsA = kM * kK / 4 / kThreads, kPartsB = 3 * kN * kK / 8 / 64, kLoadsB = kPartsB / kWaves, kMore = kPartsB % kWaves;
+  static constexpr int kEachB = kLoadsB + (kMore > 0), kLoads = kLoadsA + kLoadsB;
+  static_assert(kLoadsA * 4 * kThreads == kM * kK && kPartsB * 512 == 3 * kN * kK, "a stage is whole loads");
+};
+
+struct FloatArgs {
+  const float* a;  // [m][cols]
+  int32_t m, cols;
+  const uint16_t* b;  // [k / kK][b_rows][3][kK], padded with zeros
+  int64_t b_rows;     // a multiple of the tile
+  int32_t tiles_m, tiles_n;
+  const uint16_t* zeros;
+  const RowCounts* counts;
+};
+
+// 4 bytes a lane from memory into the LDS.
+__device__ __forceinline__ void load_word_to_lds(const void* from, uint32_t lds)
+{
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(lds), "v"(from) : "memory");
+}
+
+// (infinities leave NaN in the second plane: their product with a plane that is 0 is NaN in any case)
+__device__ __forceinline__ void split_eight(const float4& low, const float4& high, Short8 (&out)[3])
+{
+  typedef __attribute__((ext_vector_type(2))) float Float2v;
+  typedef __attribute__((ext_vector_type(2))) __bf16 Bf16x2;
+  const float v[8] = {low.x, low.y, low.z, low.w, high.x, high.y, high.z, high.w};
+  uint32_t w[3][4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const uint32_t b0 = __builtin_bit_cast(uint32_t, v[2 * i]), b1 = __builtin_bit_cast(uint32_t, v[2 * i + 1]);
+    w[0][i]        = __builtin_amdgcn_perm(b1, b0, 0x07060302u);
+    const float r0 = v[2 * i] - __builtin_bit_cast(float, b0 & 0xffff0000u), r1 = v[2 * i + 1] - __builtin_bit_cast(float, b1 & 0xffff0000u);
+    w[1][i]        = __builtin_bit_cast(uint32_t, __builtin_convertvector(Float2v{r0, r1}, Bf16x2));
+    const float s0 = r0 - __builtin_bit_cast(float, w[1][i] << 16), s1 = r1 - __builtin_bit_cast(float, w[1][i] & 0xffff0000u);
+    w[2][i]        = __builtin_bit_cast(uint32_t, __builtin_convertvector(Float2v{s0, s1}, Bf16x2));
+  }
+#pragma unroll
+  for (int q = 0; q < 3; q++) out[q] = __builtin_bit_cast(Short8, make_uint4(w[q][0], w[q][1], w[q][2], w[q][3]));
+}
+
+template <class Tile, class Epilogue>
+__global__ void __launch_bounds__(Tile::kThreads, 2) float_product_kernel(const FloatArgs args, const Epilogue epilogue)
+{
+  __shared__ __attribute__((aligned(1024))) char lds[Tile::kLds];
+  constexpr int kK = Tile::kK, kSteps = kK / 16 / Tile::kWavesK;  // of 16 of k, of a wave for a stage
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  int tile_m, tile_n;
+  tile_of_block(blockIdx.x, args.tiles_m, args.tiles_n, &tile_m, &tile_n);
+  const int rows = args.counts->rows;
+  if (tile_n * Tile::kBN >= rows) return;
+  const int m0 = tile_m * Tile::kBM, n0 = tile_n * Tile::kBN;
+  const int wk = wave / (Tile::kWavesM * Tile::kWavesN), wm = wave / Tile::kWavesN % Tile::kWavesM, wn = wave % Tile::kWavesN;
+  const int whole = args.cols / kK, steps = (args.cols + kK - 1) / kK;
+  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds));
+  const float* const a0 = args.a + static_cast<int64_t>(m0) * args.cols;
+  const uint16_t* const b0 = args.b + static_cast<int64_t>(n0) * (3 * kK);
+  // A: 8 chunks of 16 bytes of a row, their order turned by pairs of rows; rows past the last are the last one once more
+  uint32_t from_a[Tile::kLoadsA], from_b[Tile::kEachB];
+#pragma unroll
+  for (int j = 0; j < Tile::kLoadsA; j++) {
+    const int q = (j * Tile::kWaves + wave) * 64 + lane, row = q >> 3, chunk = (q & 7) ^ ((row >> 1) & 7);
+    from_a[j]   = (static_cast<uint32_t>(min(row, args.m - 1 - m0)) * static_cast<uint32_t>(args.cols) + chunk * 4) * 4;
+  }
+  // B: 3 planes of 4 chunks of a row, turned by fours of rows
+#pragma unroll
+  for (int j = 0; j < Tile::kEachB; j++) {
+    const int q = (j * Tile::kWaves + wave) * 64 + lane;
+    from_b[j]   = (q ^ ((q / 12 >> 2) & 3)) * 16;
+  }
+  const bool more_loads = wave < Tile::kMore;
+  auto meet = [&](auto stages) {  // wait_and_meet with the loads of so many stages on their way
+    constexpr int kLater = decltype(stages)::value;
+    if (Tile::kMore > 0 && more_loads) wait_and_meet<kLater * (Tile::kLoads + 1)>();
+    else wait_and_meet<kLater * Tile::kLoads>();
+  };
+  auto uniform = [](const void* p) {
+    const uint64_t bits = reinterpret_cast<uint64_t>(p);
+    return reinterpret_cast<const void*>(static_cast<uint64_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(bits >> 32))) << 32 |
+                                         static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(bits))));
+  };
+  // Stage `s` into its place: kLoads of them at least, whether there is such a stage or not, as the waits count them.
+  auto load = [&](int s, int place) {
+    const uint32_t at = lds0 + place * Tile::kStage;
+    if (s < whole) {
+      const void* const a = uniform(a0 + s * kK);
+#pragma unroll
+      for (int j = 0; j < Tile::kLoadsA; j++) load_to_lds(a, from_a[j], at + (j * Tile::kWaves + wave) * 1024);
+    } else if (s < steps) {  // the rows' ends, by single floats
+      for (int j = 0; j < Tile::kLoadsA * 4; j++) {
+        const int q = (j * Tile::kWaves + wave) * 64 + lane, row = q >> 5;
+        const int k = s * kK + ((((q >> 2) & 7) ^ ((row >> 1) & 7)) * 4 + (q & 3));
+        const float* from = a0 + static_cast<int64_t>(min(row, args.m - 1 - m0)) * args.cols + k;
+        load_word_to_lds(k < args.cols ? static_cast<const void*>(from) : args.zeros, at + (j * Tile::kWaves + wave) * 256);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < Tile::kLoadsA; j++) load_to_lds(args.zeros, at + (j * Tile::kWaves + wave) * 1024);
+    }
+    if (s < steps) {
+      const void* const b = uniform(b0 + s * args.b_rows * (3 * kK));
+#pragma unroll
+      for (int j = 0; j < Tile::kEachB; j++) {
+        if (j == Tile::kLoadsB && !more_loads) continue;
+        load_to_lds(b, from_b[j], at + Tile::kStageA + (j * Tile::kWaves + wave) * 1024);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < Tile::kEachB; j++)
+        if (j < Tile::kLoadsB || more_loads) load_to_lds(args.zeros, at + Tile::kStageA + (j * Tile::kWaves + wave) * 1024);
+    }
+  };
+  Float16v acc[Tile::kMT][Tile::kNT];
+#pragma unroll
+  for (int i = 0; i < Tile::kMT; i++)
+#pragma unroll
+    for (int j = 0; j < Tile::kNT; j++)
+#pragma unroll
+      for (int e = 0; e < 16; e++) acc[i][j][e] = 0.f;
+  // a wave of one block has two sums of it, that a product does not wait for the one before
+  constexpr int kSums = Tile::kMT * Tile::kNT == 1 ? 2 : 1;
+  Float16v more[kSums == 2 ? 1 : Tile::kMT][kSums == 2 ? 1 : Tile::kNT];
+#pragma unroll
+  for (int e = 0; kSums == 2 && e < 16; e++) more[0][0][e] = 0.f;
+  float4 raw[Tile::kMT][2];
+  Short8 a[2][Tile::kMT][3], b[2][Tile::kNT][3];
+  auto read = [&](const char* at, int step, int to) {
+    const int kk = wk * kSteps + step;
+#pragma unroll
+    for (int i = 0; i < Tile::kMT; i++)
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const int row = wm * Tile::kWM + i * 32 + (lane & 31), chunk = (kk * 4 + (lane >> 5) * 2 + h) ^ ((row >> 1) & 7);
+        raw[i][h]     = *reinterpret_cast<const float4*>(at + row * (kK * 4) + chunk * 16);
+      }
+#pragma unroll
+    for (int j = 0; j < Tile::kNT; j++)
+#pragma unroll
+      for (int q = 0; q < 3; q++) {
+        const int row = wn * Tile::kWN + j * 32 + (lane & 31), chunk = (kk * 2 + (lane >> 5)) ^ ((row >> 2) & 3);
+        b[to][j][q] = *reinterpret_cast<const Short8*>(at + Tile::kStageA + row * Tile::kRowB + (q * 4 + chunk) * 16);
+      }
+  };
+  auto multiply = [&](int from, int first, int last) {  // products first .. last - 1 of a step
+    constexpr int kA[6] = {2, 1, 0, 1, 0, 0}, kB[6] = {0, 1, 2, 0, 1, 0};  // the small ones first
+#pragma unroll
+    for (int p = first; p < last; p++)
+#pragma unroll
+      for (int i = 0; i < Tile::kMT; i++)
+#pragma unroll
+        for (int j = 0; j < Tile::kNT; j++) {
+          Float16v& to = kSums == 2 && p % 2 == 0 ? more[i][j] : acc[i][j];
+          to           = mfma_32x32x16<LBT_BF16>(a[from][i][kA[p]], b[from][j][kB[p]], to);
+        }
+  };
+  // As in product_tile: what a step multiplies has been read during the one before; all waves meet before a stage's last step, when
+  // that stage has been read by all and the next has arrived. The next step's planes are made between the second half of the
+  // products: a wave's own instructions fill the matrix cores' time only where they stand between theirs.
+#pragma unroll
+  for (int s = 0; s < Tile::kStages; s++) load(s, s);
+  meet(std::integral_constant<int, Tile::kStages - 1>{});
+  read(lds, 0, 0);
+#pragma unroll
+  for (int i = 0; i < Tile::kMT; i++) split_eight(raw[i][0], raw[i][1], a[0][i]);
+  int place = 0;
+  auto multiply_stage = [&](int s, auto own) {  // `own`: which half of the fragments holds the stage's first step
+    const int next = place + 1 == Tile::kStages ? 0 : place + 1;
+#pragma unroll
+    for (int kk = 0; kk < kSteps; kk++) {
+      const bool last = kk + 1 == kSteps;
+      const int from = (decltype(own)::value + kk) & 1, to = 1 - from;
+      if (last) meet(std::integral_constant<int, Tile::kStages - 2>{});
+      read(lds + (last ? next : place) * Tile::kStage, last ? 0 : kk + 1, to);
+      __builtin_amdgcn_sched_barrier(0);
+      if (last) load(s + Tile::kStages, place);
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(from, 0, 3);
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(from, 3, 6);
+#pragma unroll
+      for (int i = 0; i < Tile::kMT; i++) split_eight(raw[i][0], raw[i][1], a[to][i]);
+      constexpr int kHalf = 3 * Tile::kMT * Tile::kNT, kBetween = (Tile::kMT * 52 + kHalf - 1) / kHalf;
+#pragma unroll
+      for (int p = 0; p < kHalf; p++) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x2, kBetween, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    place = next;
+  };
+  if constexpr (kSteps % 2 == 0) {
+    for (int s = 0; s < steps; s++) multiply_stage(s, std::integral_constant<int, 0>{});
+  } else {
+    for (int s = 0; s < steps; s += 2) {
+      multiply_stage(s, std::integral_constant<int, 0>{});
+      if (s + 1 < steps) multiply_stage(s + 1, std::integral_constant<int, 1>{});
+    }
+  }
+  if (kSums == 2) acc[0][0] += more[0][0];
+  wait_and_meet<0>();  // the LDS is free for what follows
+  if constexpr (Tile::kWavesK == 2) {
+    static_assert(Tile::kMT * Tile::kNT == 1 && Tile::kThreads / 2 * 64 <= Tile::kLds, "a half's sums have room in the LDS");
+    float4* const sums = reinterpret_cast<float4*>(lds) + (wm * Tile::kWavesN + wn) * 256 + lane;
+#pragma unroll
+    for (int q = 0; wk == 1 && q < 4; q++) sums[q * 64] = make_float4(acc[0][0][4 * q], acc[0][0][4 * q + 1], acc[0][0][4 * q + 2], acc[0][0][4 * q + 3]);
+    __syncthreads();
+    if (wk == 1) return;
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+      const float4 v = sums[q * 64];
+      acc[0][0][4 * q] += v.x;
+      acc[0][0][4 * q + 1] += v.y;
+      acc[0][0][4 * q + 2] += v.z;
+      acc[0][0][4 * q + 3] += v.w;
+    }
+  }
+  epilogue.template store<Tile>(acc, tile_m, tile_n, wm, wn, lane, rows, 0, args.counts, lds);
+}
+
 // Element e of a 32 x 32 block: its m within the block; its n is lane % 32.
 __device__ __forceinline__ int block_m(int e, int lane) { return 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3); }
 
