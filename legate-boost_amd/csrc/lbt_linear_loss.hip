@@ -328,7 +328,8 @@ struct FusedArgs {
   int cols, padded_cols;
   uint16_t *x_out, *weight_out;  // (the second: null where the weights are not laid out)
   int64_t weight_rows;           // of weight_out
-  Layout x_layout;
+  uint16_t* x_blocks;            // where X goes for float_product_kernel; x_out: for the others; null: not there
+  Layout blocks;
 };
 
 template <int kDtype>
@@ -411,8 +412,11 @@ __global__ void __launch_bounds__(256) prepare_pack_kernel(const FusedArgs a, co
     const int p = i / own, col = (group0 + i % own) * 8;
     take_eight<kDtype>(a.x, from[p], col, a.cols, v);
 #pragma unroll
-    for (int q = 0; q < L::kPlanes; q++)
-      *reinterpret_cast<uint4*>(a.x_out + a.x_layout.at(q, p0 + p, col)) = *reinterpret_cast<const uint4*>(v[q]);
+    for (int q = 0; q < L::kPlanes; q++) {
+      const uint4 w = *reinterpret_cast<const uint4*>(v[q]);
+      if (a.x_out != nullptr) *reinterpret_cast<uint4*>(a.x_out + (static_cast<int64_t>(q) * a.padded + p0 + p) * a.padded_cols + col) = w;
+      if (a.x_blocks != nullptr) *reinterpret_cast<uint4*>(a.x_blocks + a.blocks.at(q, p0 + p, col)) = w;
+    }
   }
 }
 
@@ -456,7 +460,7 @@ __device__ __forceinline__ void turn_rows(char* lds, int wave, int lane, Value v
 {
   constexpr int kBlocks = Tile::kMT * 32 * kSize <= 256 ? Tile::kMT : 256 / (32 * kSize);
   constexpr int kRow = kBlocks * 32 * kSize, kStride = kRow + 16, kLanes = kRow / 16, kRows = 64 / kLanes;
-  static_assert(Tile::kWaves * 32 * kStride <= Tile::kLds, "each wave has its part of the LDS");
+  static_assert(Tile::kWavesM * Tile::kWavesN * 32 * kStride <= Tile::kLds, "each wave has its part of the LDS");
   char* own = lds + wave * (32 * kStride);
 #pragma unroll
   for (int group = 0; group < Tile::kMT / kBlocks; group++) {
@@ -1361,7 +1365,7 @@ struct LossCall {
   Cut all_scores, scores, row_product, class_product;
   LossRows rows;
   RowCounts* counts;
-  uint16_t *zeros, *x, *x_scaled, *weight, *g;
+  uint16_t *zeros, *x, *x_blocks, *x_scaled, *weight, *g;  // x_blocks: of float_product_kernel; x: of the other products
   float2* partial;
   float *row_sums, *class_sums, *bias_sums, *exps;
 
@@ -1371,8 +1375,7 @@ struct LossCall {
     planes = type == LBT_F32 ? 3 : 1;
     padded = round_up(n, 256);
     cols   = static_cast<int>(round_up(f, kProductK));
-    floats = type == LBT_F32 && grad == 0;
-    packed = !floats && (type == LBT_F32 || f % 8 != 0);
+    packed = type == LBT_F32 ? gradient : f % 8 != 0;
     // a piece's G and its packed weights within their bounds; pieces of one size
     int64_t most = round_up(k, 256);
     kept                = type == LBT_BF16 && !with_bias ? kKeptHalf : kKeptFloat;  // (the sums for the bias are those of floats)
@@ -1384,9 +1387,11 @@ struct LossCall {
     if (!gradient || piece < k) kept = kNotKept;
     const int64_t pairs = type == LBT_F32 ? 6 : 1;
     scores      = cut_product(std::min<int64_t>(piece, k), n, pairs * cols / kProductK, 1);
-    all_scores  = packed ? scores : cut_product(k, n, pairs * cols / kProductK, 1);
-    if (floats) all_scores = cut_floats(k, n, tiles_of(f, FloatLarge::kK));
-    few         = kept != kNotKept && (type == LBT_F32 ? n <= kFewFloatRows && few_float_time(n, f, k) < 6.0 + scores.time : n <= kFewBlock);
+    all_scores  = type == LBT_F32 ? cut_floats(k, n, tiles_of(f, FloatLarge::kK))
+                  : packed        ? scores
+                                  : cut_product(k, n, pairs * cols / kProductK, 1);
+    few         = kept != kNotKept && (type == LBT_F32 ? n <= kFewFloatRows && few_float_time(n, f, k) < 6.0 + all_scores.time : n <= kFewBlock);
+    floats      = type == LBT_F32 && !few;
     scale_rows  = tiles_of(padded, 16) * tiles_of(piece, kScaleClasses) >= 1024 ? 16 : 4;
     row_product = cut_product(f, n, pairs * piece / kProductK, 64);
     class_product = cut_product(f, std::min<int64_t>(piece, k), pairs * tiles_of(n, kProductK), 64);
@@ -1405,7 +1410,9 @@ struct LossCall {
     rows.picked   = arena.template take<float>(padded);
     rows.top      = arena.template take<float>(padded);
     rows.inverse  = arena.template take<float>(padded);
-    x             = arena.template take<uint16_t>(planes * padded * cols);
+    x = x_blocks = nullptr;
+    if (!floats || gradient) x = arena.template take<uint16_t>(planes * padded * cols);
+    if (floats) x_blocks = arena.template take<uint16_t>(planes * padded * cols);
     partial       = arena.template take<float2>(std::max(few ? 2 * tiles_of(piece, 32) : 0, 2 * (tiles_of(round_up(classes, 256), all_scores.tile) + tiles_of(classes, piece))) * padded);
     weight = x_scaled = g = nullptr;
     row_sums = class_sums = bias_sums = exps = nullptr;
@@ -1442,9 +1449,9 @@ int launch_product(hipStream_t s, const ProductArgs& args, int64_t m, int64_t n,
 }
 
 template <class Tile, class Epilogue>
-int launch_floats(hipStream_t s, FloatArgs args, int64_t n, const Epilogue& e)
+int launch_floats(hipStream_t s, FloatArgs args, int64_t m, int64_t n, const Epilogue& e)
 {
-  args.tiles_m = static_cast<int>(tiles_of(args.m, Tile::kBM));
+  args.tiles_m = static_cast<int>(tiles_of(m, Tile::kBM));
   args.tiles_n = static_cast<int>(tiles_of(n, Tile::kBN));
   const int64_t blocks = static_cast<int64_t>(args.tiles_m) * args.tiles_n;
   LBT_REQUIRE(blocks < (int64_t(1) << 31), "too many tiles");
@@ -1484,19 +1491,23 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
   }
   const bool scaled = kHalf && sample_weight != nullptr;  // (without weights every exponent is 0)
   const bool fused  = c.n_rows <= kFusedRows && !scaled;
-  const Layout x_layout = c.floats ? Layout{32, 96, 96 * c.padded} : Layout{c.padded * c.cols, c.cols, 32};
+  const Layout x_layout{c.padded * c.cols, c.cols, 32}, x_blocks{32, 96, 96 * c.padded};
   if (fused) {
     const FusedArgs a{y,         sample_weight, static_cast<int>(c.n_rows), static_cast<int>(c.padded), c.classes, loss, c.counts, c.zeros, X, weight,
-                      c.features, c.cols,        c.x,                        c.packed ? c.weight : nullptr, c.packed ? c.piece : 0, x_layout};
-    const int64_t blocks = c.padded / kFusedEach * tiles_of(c.cols / 8, kFusedGroups) + tiles_of(a.weight_rows * (c.cols / 8), 256);
-    LBT_REQUIRE(blocks < (int64_t(1) << 31), "too many values to lay out");
-    prepare_pack_kernel<kDtype><<<static_cast<unsigned>(blocks), 256, 0, s>>>(a, c.rows);
+                      c.features, c.cols,        c.x,                        c.packed ? c.weight : nullptr, c.packed ? c.piece : 0, c.x_blocks, x_blocks};
+    const int64_t groups = c.padded / kFusedEach * tiles_of(c.cols / 8, kFusedGroups) + tiles_of(a.weight_rows * (c.cols / 8), 256);
+    LBT_REQUIRE(groups < (int64_t(1) << 31), "too many values to lay out");
+    prepare_pack_kernel<kDtype><<<static_cast<unsigned>(groups), 256, 0, s>>>(a, c.rows);
     LBT_HIP(hipGetLastError());
   } else {
     prepare_rows_kernel<<<1, kPrepareThreads, 0, s>>>(y, sample_weight, c.n_rows, c.padded, c.classes, kHalf, c.rows, loss, c.counts, c.zeros);
     LBT_HIP(hipGetLastError());
-    LBT_TRY(launch_pack<kDtype>(s, X, 0, c.n_rows, c.features, c.rows.order, scaled ? kMeasure : kCopy, c.rows.exponent, c.counts, c.padded,
-                                c.cols, x_layout, c.x));
+    if (c.x != nullptr)
+      LBT_TRY(launch_pack<kDtype>(s, X, 0, c.n_rows, c.features, c.rows.order, scaled ? kMeasure : kCopy, c.rows.exponent, c.counts, c.padded,
+                                  c.cols, x_layout, c.x));
+    if (c.x_blocks != nullptr)
+      LBT_TRY(launch_pack<kDtype>(s, X, 0, c.n_rows, c.features, c.rows.order, kCopy, c.rows.exponent, c.counts, c.padded, c.cols, x_blocks,
+                                  c.x_blocks));
   }
 
   // (rows that do not count are not there: x holds them side by side)
@@ -1516,7 +1527,7 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
   args.counts = c.counts;
 
   // top and total of each row; weights that are multiplied where they lie need no pieces here
-  const int64_t step = c.packed ? c.piece : c.classes;
+  const int64_t step = c.packed && !c.floats ? c.piece : c.classes;
   int64_t tiles      = 0;
   if (c.few) {
     const FewRowsArgs few{X, weight, bias, nullptr, static_cast<int>(c.n_rows), c.features, c.classes, 1, c.piece / 16, c.partial, c.rows.picked,
@@ -1529,8 +1540,8 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
   }
   for (int64_t first = 0; first < c.classes && !c.few; first += step) {
     const int64_t classes = std::min<int64_t>(step, c.classes - first);
-    if (first > 0 || !fused) LBT_TRY(lay_out(first));  // (the first piece is there)
-    if (!c.floats) args.a = weights(first, classes);
+    if (!c.floats && (first > 0 || !fused)) LBT_TRY(lay_out(first));  // (the first piece is there)
+    args.a = weights(first, classes);
     args.b = x;
     args.k_extent = args.k_split = c.cols;
     const int share = 2 * static_cast<int>(tiles);  // (all tiles are two waves high)
@@ -1541,12 +1552,12 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
       const LossEpilogue<kFine, kKind> e{bias, static_cast<int>(first), c.classes, share, c.padded, c.rows, c.partial,
                                          kKind == kKeptFloat ? static_cast<void*>(c.exps) : c.g, static_cast<int>(c.piece)};
       tiles += tiles_of(m, c.all_scores.tile);
-      if constexpr (kFine && kKind == kNotKept)
-        if (c.floats) {
-          const FloatArgs fa{static_cast<const float*>(weight), c.classes, c.features, c.x, c.padded, 0, 0, c.zeros, c.counts};
-          return c.all_scores.tile == FloatLarge::kBM ? launch_floats<FloatLarge>(s, fa, c.n_rows, e) : launch_floats<FloatSmall>(s, fa, c.n_rows, e);
-        }
-      return launch_product<L, false, false, kRowsN>(s, args, m, c.n_rows, c.all_scores, e);
+      if constexpr (kFine) {
+        const FloatArgs fa{static_cast<const float*>(weight), c.classes, c.features, c.x_blocks, c.padded, 0, 0, c.zeros, c.counts};
+        return c.all_scores.tile == FloatLarge::kBM ? launch_floats<FloatLarge>(s, fa, m, c.n_rows, e) : launch_floats<FloatSmall>(s, fa, m, c.n_rows, e);
+      } else {
+        return launch_product<L, false, false, kRowsN>(s, args, m, c.n_rows, c.all_scores, e);
+      }
     };
     if constexpr (kDtype == LBT_BF16)
       if (c.kept == kKeptHalf) {
@@ -1574,9 +1585,11 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
   ProductOperand x_scaled = x;
   if (scaled) x_scaled.base = c.x_scaled;
   const ProductOperand g{c.g, c.piece, c.padded * c.piece, static_cast<int32_t>(c.padded), static_cast<int32_t>(c.piece)};
+  // (whether the first piece of the weights is there still, or already)
+  const bool laid_out = c.few || c.floats ? fused : c.piece >= c.classes;
   for (int64_t first = 0; first < c.classes; first += c.piece) {
     const int64_t classes = std::min<int64_t>(c.piece, c.classes - first);
-    if (first > 0 || c.piece < c.classes || (c.few && !fused)) LBT_TRY(lay_out(first));
+    if (first > 0 || !laid_out) LBT_TRY(lay_out(first));
     const ProductOperand w = weights(first, classes);
     if (c.kept != kNotKept) {
       auto scale = [&](auto half, auto each) {

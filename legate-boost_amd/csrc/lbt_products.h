@@ -457,14 +457,15 @@ __global__ void __launch_bounds__(Tile::kThreads, 2) float_product_kernel(const 
   const int wk = wave / (Tile::kWavesM * Tile::kWavesN), wm = wave / Tile::kWavesN % Tile::kWavesM, wn = wave % Tile::kWavesN;
   const int whole = args.cols / kK, steps = (args.cols + kK - 1) / kK;
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds));
-  const float* const a0 = args.a + static_cast<int64_t>(m0) * args.cols;
+  const int a_first = min(m0, args.m - 1), a_last = args.m - 1 - a_first;  // (tiles may lie past the last row)
+  const float* const a0 = args.a + static_cast<int64_t>(a_first) * args.cols;
   const uint16_t* const b0 = args.b + static_cast<int64_t>(n0) * (3 * kK);
   // A: 8 chunks of 16 bytes of a row, their order turned by pairs of rows; rows past the last are the last one once more
   uint32_t from_a[Tile::kLoadsA], from_b[Tile::kEachB];
 #pragma unroll
   for (int j = 0; j < Tile::kLoadsA; j++) {
     const int q = (j * Tile::kWaves + wave) * 64 + lane, row = q >> 3, chunk = (q & 7) ^ ((row >> 1) & 7);
-    from_a[j]   = (static_cast<uint32_t>(min(row, args.m - 1 - m0)) * static_cast<uint32_t>(args.cols) + chunk * 4) * 4;
+    from_a[j]   = (static_cast<uint32_t>(min(row, a_last)) * static_cast<uint32_t>(args.cols) + chunk * 4) * 4;
   }
   // B: 3 planes of 4 chunks of a row, turned by fours of rows
 #pragma unroll
@@ -494,7 +495,7 @@ __global__ void __launch_bounds__(Tile::kThreads, 2) float_product_kernel(const 
       for (int j = 0; j < Tile::kLoadsA * 4; j++) {
         const int q = (j * Tile::kWaves + wave) * 64 + lane, row = q >> 5;
         const int k = s * kK + ((((q >> 2) & 7) ^ ((row >> 1) & 7)) * 4 + (q & 3));
-        const float* from = a0 + static_cast<int64_t>(min(row, args.m - 1 - m0)) * args.cols + k;
+        const float* from = a0 + static_cast<int64_t>(min(row, a_last)) * args.cols + k;
         load_word_to_lds(k < args.cols ? static_cast<const void*>(from) : args.zeros, at + (j * Tile::kWaves + wave) * 256);
       }
     } else {
@@ -604,8 +605,10 @@ __global__ void __launch_bounds__(Tile::kThreads, 2) float_product_kernel(const 
   if (kSums == 2) acc[0][0] += more[0][0];
   wait_and_meet<0>();  // the LDS is free for what follows
   if constexpr (Tile::kWavesK == 2) {
-    static_assert(Tile::kMT * Tile::kNT == 1 && Tile::kThreads / 2 * 64 <= Tile::kLds, "a half's sums have room in the LDS");
-    float4* const sums = reinterpret_cast<float4*>(lds) + (wm * Tile::kWavesN + wn) * 256 + lane;
+    static_assert(Tile::kMT * Tile::kNT == 1 && Tile::kThreads / 2 * 64 <= Tile::kLds / 2 && Tile::kWaves / 2 * 32 * 272 <= Tile::kLds / 2,
+                  "a half's sums have room in the LDS");
+    // (in its upper half: what follows begins to write in the lower one while another wave reads here)
+    float4* const sums = reinterpret_cast<float4*>(lds + Tile::kLds / 2) + (wm * Tile::kWavesN + wn) * 256 + lane;
 #pragma unroll
     for (int q = 0; wk == 1 && q < 4; q++) sums[q * 64] = make_float4(acc[0][0][4 * q], acc[0][0][4 * q + 1], acc[0][0][4 * q + 2], acc[0][0][4 * q + 3]);
     __syncthreads();
