@@ -1259,11 +1259,13 @@ Cut cut_product(int64_t m, int64_t n, int64_t stages, int64_t most_splits)
   return best;
 }
 
-// Scores of few rows: the waves share the classes of a workgroup where they would be fewer than four a CU, and always where they
-// leave u, whose shares are then 16 classes each. Blocks of 64 rows: one of them for 16-bit types, up to four for float.
-bool few_shared(int classes) { return classes < 65536; }
-constexpr int kFewFloatRows = 4 * kFewBlock;
-int few_class_blocks(int64_t n_rows, int classes) { return n_rows <= 16 || classes < 32768 ? 1 : 2; }
+// Scores of few rows: the waves share the classes of a workgroup where they would be fewer than two a SIMD, and always where they
+// leave u, whose shares are then 16 classes each. (One row of bfloat16: 512 features, 65000 classes 21.1 us shared, 16.3 not; 33 rows,
+// 20000 classes 14.8 and 18.3.) Two blocks of classes beside more than 16 rows: 64 rows of 1024 features, 10000 classes 17.7 us, with one
+// 20.0; 50000 classes 48 and 78.
+constexpr int kFewRows = kFewBlock, kFewFloatRows = 4 * kFewBlock;
+bool few_shared(int classes) { return classes < 32768; }
+int few_class_blocks(int64_t n_rows, int classes, int dtype) { return n_rows <= 16 || classes < (dtype == LBT_F32 ? 32768 : 8192) ? 1 : 2; }
 int64_t few_groups(int classes, int class_blocks, bool shared) { return tiles_of(classes, 16 * class_blocks * (shared ? 1 : 4)); }
 
 // The same for float_product_kernel over `stages` of 32 of k: a stage takes a CU 0.5 and 1.4 us. (3000 classes of 4000 features: 256
@@ -1280,26 +1282,32 @@ Cut cut_floats(int64_t m, int64_t n, int64_t stages)
   return best;
 }
 
-// us of few_rows_kernel for float, whose products it forms at 50 TFLOP/s, and of the join.
-double few_float_time(int64_t n_rows, int64_t features, int64_t classes)
+// Whether the scores are those of few_rows_kernel and not of tiles, whose product takes `tiles` us: its own products come at 50 TFLOP/s
+// for float and 130 for 16 bits. (bfloat16, 64 rows of 1024 features: 10000 classes 18 us and 20 in tiles, 50000 classes 48 and 31.
+// float, 1000 features: 33 rows 25.7 us and 32.1 in tiles over 10007 classes, 61 and 44 over 30000; 4000 features, 3000 classes: 64
+// rows 42 and 72 us, 256 rows 115 and 75.)
+bool few_rows(int64_t n_rows, int64_t features, int64_t classes, int dtype, double tiles)
 {
-  return 6.0 + 4e-8 * static_cast<double>(round_up(n_rows, 16)) * features * classes;
+  if (n_rows <= 16) return true;
+  const double rate = dtype == LBT_F32 ? 4e-8 : 1.5e-8;  // us a product
+  return n_rows <= (dtype == LBT_F32 ? kFewFloatRows : kFewRows) &&
+         6.0 + rate * static_cast<double>(round_up(n_rows, 16)) * features * classes < 10.0 + tiles;
 }
-// Whether the loss alone takes few_rows_kernel. (float, 1000 features: 33 rows 25.7 us and 32.1 in tiles over 10007 classes, 61 and 44 over
-// 30000; 4000 features, 3000 classes: 64 rows 42 and 72 us, 256 rows 115 and 75.)
+// Of the loss alone. (Weights of 16 bits in rows that are no whole chunks are laid out for tiles, at 5 TB/s.)
 bool few_loss(int64_t n_rows, int64_t features, int64_t classes, int dtype)
 {
-  if (dtype != LBT_F32) return n_rows <= kFewBlock;
-  return n_rows <= 16 || (n_rows <= kFewFloatRows && few_float_time(n_rows, features, classes) <
-                                                       11.0 + cut_floats(classes, n_rows, tiles_of(features, FloatLarge::kK)).time);
+  const double tiles = dtype == LBT_F32 ? cut_floats(classes, n_rows, tiles_of(features, FloatLarge::kK)).time
+                                        : cut_product(classes, n_rows, tiles_of(features, kProductK), 1).time +
+                                            (features % 8 != 0 ? 4.0 * features * classes / 5e6 : 0.0);
+  return few_rows(n_rows, features, classes, dtype, tiles);
 }
 
 struct FewCall {
   float2* partial;
   float* picked;
-  void carve(Arena& arena, int64_t n_rows, int classes)
+  void carve(Arena& arena, int64_t n_rows, int classes, int dtype)
   {
-    const int blocks = few_class_blocks(n_rows, classes);
+    const int blocks = few_class_blocks(n_rows, classes, dtype);
     partial          = arena.take<float2>(n_rows * few_groups(classes, blocks, few_shared(classes)) * blocks);
     picked           = arena.take<float>(n_rows);
   }
@@ -1323,7 +1331,7 @@ template <int kDtype, int kKeep, int kBlocks>
 int launch_few(hipStream_t s, const FewRowsArgs& args, int64_t classes, bool shared)
 {
   if constexpr (kBlocks > 1)
-    if (few_class_blocks(args.n_rows, static_cast<int>(classes)) == 2) return launch_few<kDtype, kKeep, kBlocks, 2>(s, args, classes, shared);
+    if (few_class_blocks(args.n_rows, static_cast<int>(classes), kDtype) == 2) return launch_few<kDtype, kKeep, kBlocks, 2>(s, args, classes, shared);
   return launch_few<kDtype, kKeep, kBlocks, 1>(s, args, classes, shared);
 }
 
@@ -1341,7 +1349,7 @@ int few_log_loss(hipStream_t s, const FewCall& c, const void* X, const void* wei
                  int features, int classes, float* loss)
 {
   const bool shared = few_shared(classes);
-  const int blocks  = few_class_blocks(n_rows, classes), shares = static_cast<int>(few_groups(classes, blocks, shared)) * blocks;
+  const int blocks  = few_class_blocks(n_rows, classes, kDtype), shares = static_cast<int>(few_groups(classes, blocks, shared)) * blocks;
   const FewRowsArgs args{X, weight, bias, y, n_rows, features, classes, 1, shares, c.partial, c.picked, nullptr, nullptr, nullptr, nullptr, 0};
   LBT_TRY((launch_few<kDtype, kNotKept>(s, args, classes, shared)));
   join_few_kernel<<<n_rows, kFewThreads, 0, s>>>(c.partial, shares, c.picked, y, classes, loss);
@@ -1390,7 +1398,7 @@ struct LossCall {
     all_scores  = type == LBT_F32 ? cut_floats(k, n, tiles_of(f, FloatLarge::kK))
                   : packed        ? scores
                                   : cut_product(k, n, pairs * cols / kProductK, 1);
-    few         = kept != kNotKept && (type == LBT_F32 ? n <= kFewFloatRows && few_float_time(n, f, k) < 6.0 + all_scores.time : n <= kFewBlock);
+    few         = kept != kNotKept && few_rows(n, f, k, type, all_scores.time - 4.0);  // (X is laid out in either case)
     floats      = type == LBT_F32 && !few;
     scale_rows  = tiles_of(padded, 16) * tiles_of(piece, kScaleClasses) >= 1024 ? 16 : 4;
     row_product = cut_product(f, n, pairs * piece / kProductK, 64);
@@ -1706,7 +1714,7 @@ int run_loss(void* stream, const void* X, const void* weight, int32_t dtype, int
   Arena arena;
   arena.base = static_cast<char*>(workspace);
   arena.cap  = workspace_bytes;
-  if (few) f.carve(arena, n_rows, n_outputs);
+  if (few) f.carve(arena, n_rows, n_outputs, dtype);
   else c.carve(arena);
   if (arena.failed) {
     set_error("workspace of %zu bytes, %zu needed", workspace_bytes, arena.used);
@@ -1742,7 +1750,7 @@ size_t lbt_linear_log_loss_workspace_bytes(int64_t n_rows, int32_t n_features, i
   arena.measure = true;
   if (gradient == 0 && lbt::few_loss(n_rows, n_features, n_outputs, dtype)) {
     lbt::FewCall f;
-    f.carve(arena, n_rows, n_outputs);
+    f.carve(arena, n_rows, n_outputs, dtype);
     return std::max<size_t>(arena.used, 256);
   }
   c.carve(arena);
