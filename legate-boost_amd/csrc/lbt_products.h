@@ -10,8 +10,13 @@
 // lane, so the loop has no edges. The LDS holds 16-byte chunks in an order (an exclusive or with the row's number) in which
 // the 32 rows that a fragment reads lie on all banks.
 //
+// A large product of 16 bits runs at 1210 to 1310 TFLOP/s, where the card's library reaches 1240: the matrix cores are busy 57 to 63 % of
+// the cycles and the clock is at 1.85 GHz then, which is what bounds both. Measured and not better: stages of 32 of k four and five deep, waves
+// of 128 x 128, waves of raised priority.
+//
 // float operands are sums of three bfloat16 planes (8 + 8 + 8 significant bits, exact); of the nine products of planes the
-// six that reach above 2^-24 of the result are added up, one walk over k each.
+// six that reach above 2^-24 of the result are added up, one walk over k each. (The scores, whose first operand lies in memory as floats, have
+// a product of their own below.)
 #pragma once
 
 #include <type_traits>
@@ -225,7 +230,7 @@ struct PlanePairs<3> {
   __device__ static int b(int i) { return (0x010210 >> (4 * i)) & 15; }
 };
 
-// kRowsSide: which direction of the product is the call's rows: 0 n, 1 k, 2 m
+// kRowsSide: which direction of the product is the call's rows
 enum { kRowsN = 0, kRowsK = 1 };
 
 // Tile `block` of split `split`, in an LDS of Tile::kLds bytes.
@@ -371,7 +376,8 @@ __global__ void __launch_bounds__(Tile::kThreads, 2) product_kernel(const Produc
 }
 
 // Two products that need nothing of one another in one launch: both operands' k in rows for the second, the first operand's for the
-// first. What they take alone is mostly their beginning and end where both are in small tiles.
+// first. What they take alone is mostly their beginning and end where both are in small tiles (64 rows of 256 floats, 1000 classes:
+// 10 us, 17 as two launches).
 template <class Tile, int kType, int kPlanes, class First, class Second>
 __global__ void __launch_bounds__(Tile::kThreads, 2)
   two_products_kernel(const ProductArgs args, const First first, unsigned blocks, const ProductArgs more, const Second second)
@@ -392,7 +398,10 @@ __global__ void __launch_bounds__(Tile::kThreads, 2)
 // A goes into the LDS as floats and becomes three planes on its way from the registers to the matrix cores: hi is the float's upper
 // half, what is left goes on exactly and is rounded, v = hi + mid + lo. The six products of a step follow one another, so a value is
 // read from memory and from the LDS once where operands of planes are read up to six times, and nothing is laid out first. The eight
-// values of a fragment take 44 instructions to split while its 6 products with each fragment of B take 192 cycles.
+// values of a fragment take 44 instructions to split while its 6 products with each fragment of B take 192 cycles. Large sizes are
+// bound as the products of 16 bits are (4096 rows, 30000 classes of 1000: 1.25 ms, 1200 TFLOP/s of bfloat16), few tiles by what a wave does
+// between two stages: a tile of 64 is therefore two waves a SIMD, each with half of a stage's k (256 rows, 3000 classes of 4000: 75 us, 100 by
+// four waves), and has two sums of a block.
 template <int kM, int kN, int kWaveM, int kWaveN, int kWaveK, int kDepth>
 struct FloatTile {
   static constexpr int kBM = kM, kBN = kN, kWM = kM / kWaveM, kWN = kN / kWaveN;
