@@ -211,6 +211,36 @@ def test_nan_and_infinity_in_rows_that_count_stay_in_their_rows():
     assert torch.equal(loss[rest], clean[0]) and torch.equal(gx[rest], clean[1])
 
 
+@pytest.mark.parametrize("n,f,k", [(70, 1, 200), (300, 31, 129), (300, 33, 64), (100, 4001, 500), (1100, 95, 1000), (1030, 64, 3000),
+                                   (2000, 129, 20000), (600, 36, 24001)])
+def test_float_tiles(n, f, k):
+    """Sizes beyond few rows: rows of the weights that end inside a stage and inside 16 bytes, tiles that lie past the last class."""
+    x, w, y = inputs(n, f, k, "f32", seed=n + k)
+    rs = np.random.RandomState(f)
+    y[torch.from_numpy(rs.rand(n) < 0.2).cuda()] = -100
+    bias = torch.from_numpy(rs.normal(0, 1, k)).float().cuda()
+    check(x, w, y, "f32")
+    check(x, w, y, "f32", bias=bias, weight=torch.from_numpy(rs.rand(n) + 0.1).float().cuda())
+    # the weights as a part of a larger array: what lies behind them is not looked at
+    wide = torch.full((k * f + 64,), float("nan"), device="cuda")
+    wide[:k * f] = w.reshape(-1)
+    assert torch.equal(ops.linear_log_loss(x, wide[:k * f].view(k, f), y, bias=bias), ops.linear_log_loss(x, w, y, bias=bias))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("n,f,k", [(1024, 520, 300), (1025, 520, 300), (1024, 7, 4000), (600, 1033, 77)])
+def test_rows_counted_and_laid_out_together_or_apart(n, f, k, dtype):
+    x, w, y = inputs(n, f, k, dtype, seed=n + f)
+    rs = np.random.RandomState(n)
+    out = torch.from_numpy(rs.rand(n) < 0.4).cuda()
+    y[out] = k
+    x[out] = float("nan")
+    got = check(x, w, y, dtype)
+    assert not got[0][out].any() and not got[1][out].any()
+    check(x, w, y, dtype, weight=torch.from_numpy(rs.rand(n) + 0.1).float().cuda())
+    assert torch.equal(ops.linear_log_loss(x, w, torch.full_like(y, -1)), torch.zeros(n, device="cuda"))
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_large_scores(dtype):
     """Scores of some hundreds: tops are taken off before the exponentials."""
