@@ -266,7 +266,7 @@ __device__ __forceinline__ void take_eight(const void* __restrict__ from, int64_
 // Where an operand's values are: plane q of row p begins at q * plane + p * row, every 32 columns are `block` further on.
 struct Layout {
   int64_t plane, row, block;
-  __device__ __forceinline__ int64_t at(int q, int64_t p, int col) const { return q * plane + p * row + (col >> 5) * block + (col & 31); }
+  __host__ __device__ __forceinline__ int64_t at(int q, int64_t p, int col) const { return q * plane + p * row + (col >> 5) * block + (col & 31); }
 };
 
 // Rows of an array as rows of an operand: in `order` where that is given, -1 and what lies past the end as zeros, columns
@@ -1067,7 +1067,7 @@ constexpr int kScaleClasses = 2048;
 template <int kDtype, bool kKeptAsHalf, int kRows>
 __global__ void __launch_bounds__(256)
   scale_kernel(const void* kept, const float2* __restrict__ partial, int share_classes, int64_t share_step, int64_t row_step, int row_tile, LossRows rows,
-               const RowCounts* __restrict__ counts, int n_classes, int piece, int64_t plane, uint16_t* g, float* bias_sums,
+               const RowCounts* __restrict__ counts, int n_classes, int piece, int64_t plane, uint16_t* g, uint16_t* g_blocks, int64_t padded, float* bias_sums,
                int join_shares, float* __restrict__ loss)
 {
   using L = LossType<kDtype>;
@@ -1157,6 +1157,11 @@ __global__ void __launch_bounds__(256)
     }
 #pragma unroll
     for (int l = 0; l < L::kPlanes; l++) *reinterpret_cast<uint4*>(g + l * plane + at) = *reinterpret_cast<const uint4*>(v[l]);
+    if constexpr (L::kPlanes == 3)
+      if (g_blocks != nullptr)
+#pragma unroll
+        for (int l = 0; l < 3; l++)
+          *reinterpret_cast<uint4*>(g_blocks + Layout{32, 96, 96 * padded}.at(l, row, c)) = *reinterpret_cast<const uint4*>(v[l]);
   }
   if (bias_sums == nullptr) return;
 #pragma unroll
@@ -1286,15 +1291,18 @@ int64_t few_groups(int classes, int class_blocks, bool shared) { return tiles_of
 
 // The same for float_product_kernel over `stages` of 32 of k: a stage takes a CU 0.5 and 1.4 us. (3000 classes of 4000 features: 256
 // rows 75 us in tiles of 64, 168 in those of 128; 4096 rows 665 and 537.)
-Cut cut_floats(int64_t m, int64_t n, int64_t stages)
+Cut cut_floats(int64_t m, int64_t n, int64_t stages, int64_t most_splits)
 {
   constexpr int kCus = 256;
   constexpr struct { int tile; double stage, ends; } kTiles[2] = {{128, 1.4, 4.0}, {64, 0.5, 2.0}};
   Cut best{128, 1, 1e30};
-  for (const auto& t : kTiles) {
-    const double time = tiles_of(tiles_of(m, t.tile) * tiles_of(n, t.tile), kCus) * (stages * t.stage + t.ends);
-    if (time < best.time) best = {t.tile, 1, time};
-  }
+  for (const auto& t : kTiles)
+    for (int splits = 1; splits <= most_splits; splits++) {
+      if (splits > 1 && stages / splits < 8) break;
+      const double time = tiles_of(tiles_of(m, t.tile) * tiles_of(n, t.tile) * splits, kCus) * (tiles_of(stages, splits) * t.stage + t.ends) +
+                          (splits - 1) * (1.0 + m * n * 8e-6 / 4.0);
+      if (time < best.time) best = {t.tile, splits, time};
+    }
   return best;
 }
 
@@ -1312,7 +1320,7 @@ bool few_rows(int64_t n_rows, int64_t features, int64_t classes, int dtype, doub
 // Of the loss alone. (Weights of 16 bits in rows that are no whole chunks are laid out for tiles, at 5 TB/s.)
 bool few_loss(int64_t n_rows, int64_t features, int64_t classes, int dtype)
 {
-  const double tiles = dtype == LBT_F32 ? cut_floats(classes, n_rows, tiles_of(features, FloatLarge::kK)).time
+  const double tiles = dtype == LBT_F32 ? cut_floats(classes, n_rows, tiles_of(features, FloatLarge::kK), 1).time
                                         : cut_product(classes, n_rows, tiles_of(features, kProductK), 1).time +
                                             (features % 8 != 0 ? 4.0 * features * classes / 5e6 : 0.0);
   return few_rows(n_rows, features, classes, dtype, tiles);
@@ -1386,10 +1394,11 @@ struct LossCall {
   int scale_rows;   // of a workgroup of scale_kernel
   bool few;         // the scores are those of few_rows_kernel
   bool floats;      // of float_product_kernel
+  bool floats_back; // grad_X too: the weights are not laid out, G is, in both orders
   Cut all_scores, scores, row_product, class_product;
   LossRows rows;
   RowCounts* counts;
-  uint16_t *zeros, *x, *x_blocks, *x_scaled, *weight, *g;  // x_blocks: of float_product_kernel; x: of the other products
+  uint16_t *zeros, *x, *x_blocks, *x_scaled, *weight, *g, *g_blocks;  // blocks: of float_product_kernel; x and g: of the other products
   float2* partial;
   float *row_sums, *class_sums, *bias_sums, *exps;
 
@@ -1399,7 +1408,11 @@ struct LossCall {
     planes = type == LBT_F32 ? 3 : 1;
     padded = round_up(n, 256);
     cols   = static_cast<int>(round_up(f, kProductK));
-    packed = type == LBT_F32 ? gradient : f % 8 != 0;
+    // Where rows are few beside the features, laying out the weights and reading their planes up to six times costs more than G once more
+    // in the other order. (1000 floats, 30000 classes: 17 rows 150 us, 271 with the weights laid out; 256 rows 372 and 458; 1024 rows 1213
+    // and 1155.) Below 8 us of it the products of small gradients share a launch instead.
+    floats_back = type == LBT_F32 && gradient && 10.0 * (f - n) * k / 5e6 > 8.0 && 16 * padded * round_up(k, 256) <= kScoresBytes;
+    packed = type == LBT_F32 ? gradient && !floats_back : f % 8 != 0;
     // a piece's G and its packed weights within their bounds; pieces of one size
     int64_t most = round_up(k, 256);
     kept                = type == LBT_BF16 && !with_bias ? kKeptHalf : kKeptFloat;  // (the sums for the bias are those of floats)
@@ -1411,13 +1424,13 @@ struct LossCall {
     if (!gradient || piece < k) kept = kNotKept;
     const int64_t pairs = type == LBT_F32 ? 6 : 1;
     scores      = cut_product(std::min<int64_t>(piece, k), n, pairs * cols / kProductK, 1);
-    all_scores  = type == LBT_F32 ? cut_floats(k, n, tiles_of(f, FloatLarge::kK))
+    all_scores  = type == LBT_F32 ? cut_floats(k, n, tiles_of(f, FloatLarge::kK), 1)
                   : packed        ? scores
                                   : cut_product(k, n, pairs * cols / kProductK, 1);
     few         = kept != kNotKept && few_rows(n, f, k, type, all_scores.time - 4.0);  // (X is laid out in either case)
     floats      = type == LBT_F32 && !few;
     scale_rows  = tiles_of(padded, 16) * tiles_of(piece, kScaleClasses) >= 1024 ? 16 : 4;
-    row_product = cut_product(f, n, pairs * piece / kProductK, 64);
+    row_product = floats_back ? cut_floats(f, n, piece / FloatLarge::kK, 64) : cut_product(f, n, pairs * piece / kProductK, 64);
     class_product = cut_product(f, std::min<int64_t>(piece, k), pairs * tiles_of(n, kProductK), 64);
   }
 
@@ -1438,12 +1451,13 @@ struct LossCall {
     if (!floats || gradient) x = arena.template take<uint16_t>(planes * padded * cols);
     if (floats) x_blocks = arena.template take<uint16_t>(planes * padded * cols);
     partial       = arena.template take<float2>(std::max(few ? 2 * tiles_of(piece, 32) : 0, 2 * (tiles_of(round_up(classes, 256), all_scores.tile) + tiles_of(classes, piece))) * padded);
-    weight = x_scaled = g = nullptr;
+    weight = x_scaled = g = g_blocks = nullptr;
     row_sums = class_sums = bias_sums = exps = nullptr;
     if (packed) weight = arena.template take<uint16_t>(planes * piece * cols);
     if (!gradient) return;
     if (dtype == LBT_F16) x_scaled = arena.template take<uint16_t>(padded * cols);
     g         = arena.template take<uint16_t>(planes * padded * piece);
+    if (floats_back) g_blocks = arena.template take<uint16_t>(planes * padded * piece);
     if (kept == kKeptFloat) exps = arena.template take<float>(padded * piece);
     row_sums  = arena.template take<float>(row_product.splits * padded * cols);
     if (class_product.splits > 1) class_sums = arena.template take<float>(class_product.splits * piece * cols);
@@ -1472,16 +1486,24 @@ int launch_product(hipStream_t s, const ProductArgs& args, int64_t m, int64_t n,
   return launch_tiles<SmallTile, L, kAMajor, kBMajor, kRowsSide>(s, args, m, n, cut.splits, e);
 }
 
-template <class Tile, class Epilogue>
-int launch_floats(hipStream_t s, FloatArgs args, int64_t m, int64_t n, const Epilogue& e)
+template <class Tile, bool kAMajor, class Epilogue>
+int launch_float_tiles(hipStream_t s, FloatArgs args, int64_t m, int64_t n, int splits, const Epilogue& e)
 {
   args.tiles_m = static_cast<int>(tiles_of(m, Tile::kBM));
   args.tiles_n = static_cast<int>(tiles_of(n, Tile::kBN));
+  args.k_split = static_cast<int32_t>(round_up(tiles_of(kAMajor ? args.rows : args.cols, splits), Tile::kK));
   const int64_t blocks = static_cast<int64_t>(args.tiles_m) * args.tiles_n;
   LBT_REQUIRE(blocks < (int64_t(1) << 31), "too many tiles");
-  float_product_kernel<Tile, Epilogue><<<static_cast<unsigned>(blocks), Tile::kThreads, 0, s>>>(args, e);
+  float_product_kernel<Tile, kAMajor, Epilogue><<<dim3(static_cast<unsigned>(blocks), splits), Tile::kThreads, 0, s>>>(args, e);
   LBT_HIP(hipGetLastError());
   return LBT_OK;
+}
+
+template <bool kAMajor, class Epilogue>
+int launch_floats(hipStream_t s, const FloatArgs& args, int64_t m, int64_t n, Cut cut, const Epilogue& e)
+{
+  if (cut.tile == FloatLarge::kBM) return launch_float_tiles<FloatLarge, kAMajor>(s, args, m, n, cut.splits, e);
+  return launch_float_tiles<FloatSmall, kAMajor>(s, args, m, n, cut.splits, e);
 }
 
 template <int kDtype>
@@ -1577,8 +1599,8 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
                                          kKind == kKeptFloat ? static_cast<void*>(c.exps) : c.g, static_cast<int>(c.piece)};
       tiles += tiles_of(m, c.all_scores.tile);
       if constexpr (kFine) {
-        const FloatArgs fa{static_cast<const float*>(weight), c.classes, c.features, c.x_blocks, c.padded, 0, 0, c.zeros, c.counts};
-        return c.all_scores.tile == FloatLarge::kBM ? launch_floats<FloatLarge>(s, fa, m, c.n_rows, e) : launch_floats<FloatSmall>(s, fa, m, c.n_rows, e);
+        const FloatArgs fa{static_cast<const float*>(weight), c.classes, c.features, 0, c.x_blocks, c.padded, 0, 0, c.zeros, c.counts};
+        return launch_floats<false>(s, fa, m, c.n_rows, c.all_scores, e);
       } else {
         return launch_product<L, false, false, kRowsN>(s, args, m, c.n_rows, c.all_scores, e);
       }
@@ -1621,7 +1643,7 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
         scale_kernel<kDtype, decltype(half)::value, kRows>
           <<<static_cast<unsigned>(tiles_of(c.piece, kScaleClasses) * tiles_of(c.padded, kRows)), 256, 0, s>>>(
             decltype(half)::value ? static_cast<const void*>(c.g) : c.exps, c.partial, share_classes, c.few ? 1 : c.padded, c.few ? shares : 1, std::max(c.row_product.tile, kProductK), c.rows, c.counts,
-            c.classes, static_cast<int>(c.piece), c.padded * c.piece, c.g, grad_bias != nullptr ? c.bias_sums : nullptr, join_here, loss);
+            c.classes, static_cast<int>(c.piece), c.padded * c.piece, c.g, c.g_blocks, c.padded, grad_bias != nullptr ? c.bias_sums : nullptr, join_here, loss);
       };
       auto scale_by = [&](auto half) {
         if (c.scale_rows == 16) scale(half, std::integral_constant<int, 16>{});
@@ -1654,6 +1676,12 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
     more.k_extent    = static_cast<int32_t>(c.padded);
     more.k_split     = static_cast<int32_t>(round_up(tiles_of(c.padded, c.class_product.splits), kProductK));
     auto products    = [&](const auto& ce) -> int {
+      if constexpr (kFine)
+        if (c.floats_back) {
+          const FloatArgs fa{static_cast<const float*>(weight), c.classes, c.features, 0, c.g_blocks, c.padded, 0, 0, c.zeros, c.counts};
+          LBT_TRY((launch_floats<true>(s, fa, c.features, c.n_rows, c.row_product, re)));
+          return launch_product<L, true, true, kRowsK>(s, more, c.features, classes, c.class_product, ce);
+        }
       if (c.row_product.tile == SmallTile::kBM && c.class_product.tile == SmallTile::kBM) {
         args.tiles_m = more.tiles_m = static_cast<int>(tiles_of(c.features, SmallTile::kBM));
         args.tiles_n = static_cast<int>(tiles_of(c.n_rows, SmallTile::kBN));

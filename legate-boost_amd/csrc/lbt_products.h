@@ -15,8 +15,8 @@
 // of 128 x 128, waves of raised priority.
 //
 // float operands are sums of three bfloat16 planes (8 + 8 + 8 significant bits, exact); of the nine products of planes the
-// six that reach above 2^-24 of the result are added up, one walk over k each. (The scores, whose first operand lies in memory as floats, have
-// a product of their own below.)
+// six that reach above 2^-24 of the result are added up, one walk over k each. (The scores, and grad_X of few rows, whose
+// first operand lies in memory as floats, have a product of their own below.)
 #pragma once
 
 #include <type_traits>
@@ -394,7 +394,7 @@ __global__ void __launch_bounds__(Tile::kThreads, 2)
 
 // ---- float by planes: the first operand as it lies in memory ----------------------------------------
 //
-// C[m][n] = sum_k A(m, k) B(n, k) for an A of floats that is read once, k contiguous, rows of any length, and a B laid out in planes.
+// C[m][n] = sum_k A(m, k) B(n, k) for an A of floats that is read once, in rows of any length of k or (kAMajor) of m, and a B laid out in planes.
 // A goes into the LDS as floats and becomes three planes on its way from the registers to the matrix cores: hi is the float's upper
 // half, what is left goes on exactly and is rounded, v = hi + mid + lo. The six products of a step follow one another, so a value is
 // read from memory and from the LDS once where operands of planes are read up to six times, and nothing is laid out first. The eight
@@ -417,8 +417,9 @@ struct FloatTile {
 };
 
 struct FloatArgs {
-  const float* a;  // [m][cols]
-  int32_t m, cols;
+  const float* a;        // [rows][cols]
+  int32_t rows, cols;
+  int32_t k_split;       // values of k of one split, a multiple of kK
   const uint16_t* b;  // [k / kK][b_rows][3][kK], padded with zeros
   int64_t b_rows;     // a multiple of the tile
   int32_t tiles_m, tiles_n;
@@ -452,7 +453,9 @@ __device__ __forceinline__ void split_eight(const float4& low, const float4& hig
   for (int q = 0; q < 3; q++) out[q] = __builtin_bit_cast(Short8, make_uint4(w[q][0], w[q][1], w[q][2], w[q][3]));
 }
 
-template <class Tile, class Epilogue>
+// kAMajor: A's rows are its k, its columns the product's m; a fragment's eight values are then eight reads of 4 bytes, each of 32 values
+// of m beside one another, and in every second eight of k 32 values of m have changed places, which puts the lanes on all banks.
+template <class Tile, bool kAMajor, class Epilogue>
 __global__ void __launch_bounds__(Tile::kThreads, 2) float_product_kernel(const FloatArgs args, const Epilogue epilogue)
 {
   __shared__ __attribute__((aligned(1024))) char lds[Tile::kLds];
@@ -464,17 +467,30 @@ __global__ void __launch_bounds__(Tile::kThreads, 2) float_product_kernel(const 
   if (tile_n * Tile::kBN >= rows) return;
   const int m0 = tile_m * Tile::kBM, n0 = tile_n * Tile::kBN;
   const int wk = wave / (Tile::kWavesM * Tile::kWavesN), wm = wave / Tile::kWavesN % Tile::kWavesM, wn = wave % Tile::kWavesN;
-  const int whole = args.cols / kK, steps = (args.cols + kK - 1) / kK;
+  const int k_extent = kAMajor ? args.rows : args.cols, k_first = blockIdx.y * args.k_split;
+  const int steps    = (min(args.k_split, max(k_extent - k_first, 0)) + kK - 1) / kK;
+  // Stages of A that are read in whole chunks: those within its rows; with k in rows, those that end, with what follows the last row of
+  // the tile, within the array.
+  int whole = (k_extent - k_first) / kK;
+  if constexpr (kAMajor) {
+    const int64_t room = static_cast<int64_t>(args.rows) * args.cols - m0 - Tile::kBM;  // for the first column of a stage's last row
+    const int last     = static_cast<int>(room < 0 ? -1 : room / args.cols) - (kK - 1);  // first row of the last such stage
+    whole              = min(whole, last < k_first ? 0 : (last - k_first) / kK + 1);
+  }
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds));
-  const int a_first = min(m0, args.m - 1), a_last = args.m - 1 - a_first;  // (tiles may lie past the last row)
-  const float* const a0 = args.a + static_cast<int64_t>(a_first) * args.cols;
-  const uint16_t* const b0 = args.b + static_cast<int64_t>(n0) * (3 * kK);
-  // A: 8 chunks of 16 bytes of a row, their order turned by pairs of rows; rows past the last are the last one once more
+  const int a_first = min(m0, args.rows - 1), a_last = args.rows - 1 - a_first;  // (tiles may lie past the last row)
+  const float* const a0 = args.a + (kAMajor ? static_cast<int64_t>(k_first) * args.cols + m0 : static_cast<int64_t>(a_first) * args.cols);
+  const uint16_t* const b0 = args.b + (static_cast<int64_t>(k_first / kK) * args.b_rows + n0) * (3 * kK);
+  // A: 8 chunks of 16 bytes of a row, their order turned by pairs of rows; rows past the last are the last one once more. k in rows: the
+  // chunks of a row, turned by eights of rows.
   uint32_t from_a[Tile::kLoadsA], from_b[Tile::kEachB];
 #pragma unroll
   for (int j = 0; j < Tile::kLoadsA; j++) {
-    const int q = (j * Tile::kWaves + wave) * 64 + lane, row = q >> 3, chunk = (q & 7) ^ ((row >> 1) & 7);
-    from_a[j]   = (static_cast<uint32_t>(min(row, a_last)) * static_cast<uint32_t>(args.cols) + chunk * 4) * 4;
+    const int q = (j * Tile::kWaves + wave) * 64 + lane;
+    constexpr int kRow = Tile::kBM / 4;  // chunks of a row of k
+    const int row   = kAMajor ? q / kRow : min(q >> 3, a_last);
+    const int chunk = kAMajor ? (q % kRow) ^ (((row >> 3) & 1) << 3) : (q & 7) ^ ((q >> 4) & 7);
+    from_a[j]       = (static_cast<uint32_t>(row) * static_cast<uint32_t>(args.cols) + chunk * 4) * 4;
   }
   // B: 3 planes of 4 chunks of a row, turned by fours of rows
 #pragma unroll
@@ -497,15 +513,24 @@ __global__ void __launch_bounds__(Tile::kThreads, 2) float_product_kernel(const 
   auto load = [&](int s, int place) {
     const uint32_t at = lds0 + place * Tile::kStage;
     if (s < whole) {
-      const void* const a = uniform(a0 + s * kK);
+      const void* const a = uniform(a0 + (kAMajor ? static_cast<int64_t>(s) * kK * args.cols : s * kK));
 #pragma unroll
       for (int j = 0; j < Tile::kLoadsA; j++) load_to_lds(a, from_a[j], at + (j * Tile::kWaves + wave) * 1024);
-    } else if (s < steps) {  // the rows' ends, by single floats
+    } else if (s < steps) {  // the ends, by single floats
       for (int j = 0; j < Tile::kLoadsA * 4; j++) {
-        const int q = (j * Tile::kWaves + wave) * 64 + lane, row = q >> 5;
-        const int k = s * kK + ((((q >> 2) & 7) ^ ((row >> 1) & 7)) * 4 + (q & 3));
-        const float* from = a0 + static_cast<int64_t>(min(row, a_last)) * args.cols + k;
-        load_word_to_lds(k < args.cols ? static_cast<const void*>(from) : args.zeros, at + (j * Tile::kWaves + wave) * 256);
+        const int q = (j * Tile::kWaves + wave) * 64 + lane;
+        const float* from;
+        bool inside;
+        if constexpr (kAMajor) {
+          const int row = s * kK + q / Tile::kBM, col = (q % Tile::kBM) ^ (((row >> 3) & 1) << 5);
+          inside        = k_first + row < args.rows && m0 + col < args.cols;
+          from          = a0 + static_cast<int64_t>(row) * args.cols + col;
+        } else {
+          const int row = q >> 5, k = s * kK + ((((q >> 2) & 7) ^ ((row >> 1) & 7)) * 4 + (q & 3));
+          inside        = k < args.cols;
+          from          = a0 + static_cast<int64_t>(min(row, a_last)) * args.cols + k;
+        }
+        load_word_to_lds(inside ? static_cast<const void*>(from) : args.zeros, at + (j * Tile::kWaves + wave) * 256);
       }
     } else {
 #pragma unroll
@@ -544,8 +569,14 @@ __global__ void __launch_bounds__(Tile::kThreads, 2) float_product_kernel(const 
     for (int i = 0; i < Tile::kMT; i++)
 #pragma unroll
       for (int h = 0; h < 2; h++) {
-        const int row = wm * Tile::kWM + i * 32 + (lane & 31), chunk = (kk * 4 + (lane >> 5) * 2 + h) ^ ((row >> 1) & 7);
-        raw[i][h]     = *reinterpret_cast<const float4*>(at + row * (kK * 4) + chunk * 16);
+        if constexpr (kAMajor) {
+          const int m      = (wm * Tile::kWM + i * 32 + (lane & 31)) ^ ((lane >> 5) << 5);
+          const float* row = reinterpret_cast<const float*>(at) + (kk * 16 + (lane >> 5) * 8 + h * 4) * Tile::kBM + m;
+          raw[i][h]        = make_float4(row[0], row[Tile::kBM], row[2 * Tile::kBM], row[3 * Tile::kBM]);
+        } else {
+          const int row = wm * Tile::kWM + i * 32 + (lane & 31), chunk = (kk * 4 + (lane >> 5) * 2 + h) ^ ((row >> 1) & 7);
+          raw[i][h]     = *reinterpret_cast<const float4*>(at + row * (kK * 4) + chunk * 16);
+        }
       }
 #pragma unroll
     for (int j = 0; j < Tile::kNT; j++)
@@ -631,7 +662,7 @@ __global__ void __launch_bounds__(Tile::kThreads, 2) float_product_kernel(const 
       acc[0][0][4 * q + 3] += v.w;
     }
   }
-  epilogue.template store<Tile>(acc, tile_m, tile_n, wm, wn, lane, rows, 0, args.counts, lds);
+  epilogue.template store<Tile>(acc, tile_m, tile_n, wm, wn, lane, rows, blockIdx.y, args.counts, lds);
 }
 
 // Element e of a 32 x 32 block: its m within the block; its n is lane % 32.

@@ -212,7 +212,8 @@ def test_nan_and_infinity_in_rows_that_count_stay_in_their_rows():
 
 
 @pytest.mark.parametrize("n,f,k", [(70, 1, 200), (300, 31, 129), (300, 33, 64), (100, 4001, 500), (1100, 95, 1000), (1030, 64, 3000),
-                                   (2000, 129, 20000), (600, 36, 24001)])
+                                   (2000, 129, 20000), (600, 36, 24001), (20, 1003, 9001), (130, 2050, 3001), (700, 65, 130000),
+                                   (257, 4001, 1003)])
 def test_float_tiles(n, f, k):
     """Sizes beyond few rows: rows of the weights that end inside a stage and inside 16 bytes, tiles that lie past the last class."""
     x, w, y = inputs(n, f, k, "f32", seed=n + k)
