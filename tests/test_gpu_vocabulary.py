@@ -563,6 +563,49 @@ def test_threads_on_streams_of_their_own():
         assert all(torch.equal(p, q) for p, q in zip(a, b))
 
 
+@pytest.mark.parametrize("n,f,k", [(20, 1003, 9001), (300, 70, 900), (1500, 64, 2000)])
+def test_float_captured_and_replayed(n, f, k):
+    x, w, y = inputs(n, f, k, "f32", seed=n)
+    bias = torch.randn(k, device="cuda")
+    ops.linear_log_loss_gradient(x, w, y, bias=bias)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = ops.linear_log_loss_gradient(x, w, y, bias=bias) + (ops.linear_log_loss(x, w, y, bias=bias),)
+    for turn in range(4):
+        y.copy_((y + 7 * turn) % (k + 3))  # some that are no class
+        w.mul_(0.9)
+        graph.replay()
+        want = ops.linear_log_loss_gradient(x, w, y, bias=bias) + (ops.linear_log_loss(x, w, y, bias=bias),)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_offsets_beyond_32_bits():
+    """Weights and a table of 4.9 GB whose last rows differ from 0: 600000 rows of 4096 bfloat16."""
+    rows, f = 600000, 4096
+    w = torch.zeros((rows, f), dtype=torch.bfloat16, device="cuda")
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    w[-300:] = torch.randn((300, f), generator=gen, device="cuda").to(w.dtype) * 0.02
+    tokens = torch.tensor([rows - 1, 0, rows - 300, rows - 7, rows], device="cuda")
+    got = ops.embed_rows(w, tokens, 0.5)
+    assert torch.equal(got[:4], (w[tokens[:4]].float() * 0.5).to(w.dtype)) and not got[4].any()
+    for n in (1, 70):
+        x = torch.randn((n, f), generator=gen, device="cuda").to(w.dtype)
+        y = torch.randint(rows - 300, rows, (n,), generator=gen, device="cuda")
+        y[0] = 5
+        s = x.double() @ w[-300:].double().t()
+        label = torch.where(y >= rows - 300, s[torch.arange(n, device="cuda"), (y - (rows - 300)).clamp(min=0)], 0.0)
+        want = torch.log(torch.exp(s).sum(1) + (rows - 300)) - label
+        size = (x.double().abs() @ w[-300:].double().abs().t()).max(1).values
+        loss = ops.linear_log_loss(x, w, y)
+        # as in `reference`: 2 d + e, and the logarithm
+        assert ((loss - want).abs() <= 2 * ((f + 8) * U + 2.0 ** -22) * size + 1e-4 + 8 * U * 20).all()
+    g = torch.ones((3, f), dtype=torch.bfloat16, device="cuda")
+    to = ops.embed_rows_gradient(g, torch.tensor([rows - 1, 3, rows - 1], device="cuda"), rows)
+    assert torch.equal(to[-1], torch.full((f,), 2.0, dtype=to.dtype, device="cuda")) and (to[3] == 1).all()
+    assert not to[-100:-1].any() and not to[:3].any() and not to[4:100].any() and not to[299990:300010].any()
+
+
 # ---- together ------------------------------------------------------------------------------------------
 
 
