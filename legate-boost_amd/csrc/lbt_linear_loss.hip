@@ -807,7 +807,7 @@ __global__ void __launch_bounds__(kJoinRows * kJoinSlices)
 //
 // A score of few rows is bound by reading the weights once. Each wave takes 16 classes, 16 bytes of a class a lane, straight from
 // memory into the operand of a 16 x 16 product, with up to four blocks of 16 rows beside it (they are read over and over, from the
-// L1): there is no stage in the LDS to wait for and nothing is laid out first. (One row of 1024 bfloat16, 32768 classes: 67 MB at 5.2
+// L1): there is no stage in the LDS to wait for and nothing is laid out first. (One row of 1024 bfloat16, 32768 classes: 67 MB at 4.8
 // TB/s. 33 rows of 1000 floats, 10007 classes: 24 us, 40 TFLOP/s of padded rows, bound by the float products and their operands' loads.) The order of k within 16 lanes' chunks is the same
 // for both operands, which is all a product asks of it. float goes to the float products of the matrix cores as it is. Rows are not
 // taken out: what a row that does not count holds stays in its own column.
