@@ -665,18 +665,28 @@ struct GradientEpilogue {
 };
 
 // grad_X: m = features, n = rows. Adds to (or begins) the sums of this split of the classes, [split][rows][padded_cols]. The same for
-// grad_weight where the rows are split, n = classes of the piece.
+// grad_weight where the rows are split or come in parts, n = classes of the piece.
 struct RowsEpilogue {
   float* sums;
   int64_t split;  // values of a split
   int padded_cols;
   bool begin;
   int classes;  // n ends here; 0: at the rows that count
+  bool scaled;  // the rows were multiplied by a power of two that is taken out here: each part of the rows has its own
 
   template <class Tile>
   __device__ __forceinline__ void store(Float16v (&acc)[Tile::kMT][Tile::kNT], int tile_m, int tile_n, int wm, int wn, int lane,
-                                        int counted, int part, const RowCounts*, char*) const
+                                        int counted, int part, const RowCounts* counts, char*) const
   {
+    if (scaled) {
+      const int shift = counts->reach - kReach;
+#pragma unroll
+      for (int i = 0; i < Tile::kMT; i++)
+#pragma unroll
+        for (int j = 0; j < Tile::kNT; j++)
+#pragma unroll
+          for (int e = 0; e < 16; e++) acc[i][j][e] = ldexpf(acc[i][j][e], shift);
+    }
 #pragma unroll
     for (int j = 0; j < Tile::kNT; j++) {
       const int64_t row = static_cast<int64_t>(tile_n) * Tile::kBN + wn * Tile::kWN + j * 32 + (lane & 31);
@@ -1216,9 +1226,9 @@ __global__ void __launch_bounds__(256)
   store_four<kDtype>(out, (first + c) * cols + col, v, cols - col);
 }
 
-// grad_bias from its sums over blocks of rows; a class's blocks are shared out among 16 threads.
+// grad_bias from its sums over blocks of rows; a class's blocks are shared out among 64 threads. `add`: to that of the rows before.
 __global__ void __launch_bounds__(kJoinRows * kJoinSlices)
-  finish_bias_kernel(const float* __restrict__ sums, int n_classes, int block_rows, const RowCounts* __restrict__ counts, int half,
+  finish_bias_kernel(const float* __restrict__ sums, int n_classes, int block_rows, const RowCounts* __restrict__ counts, int half, bool add,
                      float* __restrict__ out)
 {
   __shared__ float share[kJoinSlices][kJoinRows];
@@ -1235,7 +1245,8 @@ __global__ void __launch_bounds__(kJoinRows * kJoinSlices)
   if (slice != 0 || c >= n_classes) return;
   sum = 0.f;
   for (int s = 0; s < kJoinSlices; s++) sum += share[s][n];
-  out[c] = half ? ldexpf(sum, counts->exponent - kHalfShift) : sum;
+  if (half) sum = ldexpf(sum, counts->exponent - kHalfShift);
+  out[c] = add ? out[c] + sum : sum;
 }
 
 __global__ void __launch_bounds__(256) clear_kernel(uint16_t* __restrict__ out, int64_t n)
@@ -1381,8 +1392,21 @@ int few_log_loss(hipStream_t s, const FewCall& c, const void* X, const void* wei
   return LBT_OK;
 }
 
+// Rows are taken in parts where they are many: what a call lays out and keeps for a row does not depend on how many there are. At most
+// 131072 at a time, 2^30 values of their planes, and 2^34 rows times classes, which is 1 GiB of the rows' tops and totals: calls of up
+// to 8192 rows are one part up to two million classes and 131072 features (43690 of float). (With gradients, 2,000,000 rows of 200
+// floats, 8 classes: 0.8 GiB and 11.9 ms, in one part 12.6 GiB and 11.6 ms; 262144 rows of 1024 bfloat16, 32000 classes: 63.9 and 65.1 ms.)
+int64_t rows_at_once(int64_t n, int f, int k, int dtype)
+{
+  const int64_t planes = dtype == LBT_F32 ? 3 : 1;
+  int64_t most         = std::min<int64_t>({1 << 17, (int64_t(1) << 30) / (planes * round_up(f, kProductK)), (int64_t(1) << 34) / k});
+  most                 = std::max<int64_t>(most / 256 * 256, 256);
+  return n <= most ? n : round_up(tiles_of(n, tiles_of(n, most)), 256);
+}
+
 struct LossCall {
-  int64_t n_rows;
+  int64_t n_rows;   // of this part
+  bool parts;       // the call's rows are several
   int features, classes, dtype;
   bool gradient, with_bias;
   int planes;
@@ -1402,9 +1426,10 @@ struct LossCall {
   float2* partial;
   float *row_sums, *class_sums, *bias_sums, *exps;
 
-  LossCall(int64_t n, int f, int k, int type, int grad)
-    : n_rows(n), features(f), classes(k), dtype(type), gradient(grad != 0), with_bias(grad > 1)
+  LossCall(int64_t all_rows, int f, int k, int type, int grad) : features(f), classes(k), dtype(type), gradient(grad != 0), with_bias(grad > 1)
   {
+    const int64_t n = n_rows = rows_at_once(all_rows, f, k, type);
+    parts                    = n < all_rows;
     planes = type == LBT_F32 ? 3 : 1;
     padded = round_up(n, 256);
     cols   = static_cast<int>(round_up(f, kProductK));
@@ -1460,7 +1485,9 @@ struct LossCall {
     if (floats_back) g_blocks = arena.template take<uint16_t>(planes * padded * piece);
     if (kept == kKeptFloat) exps = arena.template take<float>(padded * piece);
     row_sums  = arena.template take<float>(row_product.splits * padded * cols);
-    if (class_product.splits > 1) class_sums = arena.template take<float>(class_product.splits * piece * cols);
+    // (of all classes where the rows come in parts: each part adds to them)
+    if (parts) class_sums = arena.template take<float>(class_product.splits * static_cast<int64_t>(classes) * cols);
+    else if (class_product.splits > 1) class_sums = arena.template take<float>(class_product.splits * piece * cols);
     if (with_bias) bias_sums = arena.template take<float>(tiles_of(padded, kept ? scale_rows : scores.tile) * classes);
   }
 };
@@ -1518,9 +1545,10 @@ int launch_pack(hipStream_t s, const void* from, int64_t first_row, int64_t rows
   return LBT_OK;
 }
 
+// Of one part of the rows; `begins` and `ends`: whether it is the first one and the last.
 template <int kDtype>
 int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void* weight, const float* bias, const int64_t* y,
-                    const float* sample_weight, float* loss, void* grad_X, void* grad_weight, float* grad_bias)
+                    const float* sample_weight, float* loss, void* grad_X, void* grad_weight, float* grad_bias, bool begins, bool ends)
 {
   using L              = LossType<kDtype>;
   constexpr bool kFine = kDtype == LBT_F32;
@@ -1536,7 +1564,7 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
     return LBT_OK;
   }
   const bool scaled = kHalf && sample_weight != nullptr;  // (without weights every exponent is 0)
-  const bool fused  = c.n_rows <= kFusedRows && !scaled;
+  const bool fused  = c.padded <= kFusedRows && !scaled;
   const Layout x_layout{c.padded * c.cols, c.cols, 32}, x_blocks{32, 96, 96 * c.padded};
   if (fused) {
     const FusedArgs a{y,         sample_weight, static_cast<int>(c.n_rows), static_cast<int>(c.padded), c.classes, loss, c.counts, c.zeros, X, weight,
@@ -1564,7 +1592,7 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
                           c.features};
   };
   auto lay_out = [&](int64_t first) {
-    if (!c.packed) return LBT_OK;
+    if (!c.packed || (!begins && c.piece >= c.classes)) return LBT_OK;  // (all of them are there from the rows before)
     return launch_pack<kDtype>(s, weight, first, c.classes, c.features, nullptr, kCopy, nullptr, c.counts, c.piece, c.cols,
                                Layout{c.piece * c.cols, c.cols, 32}, c.weight);
   };
@@ -1670,7 +1698,7 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
     args.b        = g;
     args.k_extent = static_cast<int32_t>(c.piece);
     args.k_split  = static_cast<int32_t>(round_up(tiles_of(c.piece, c.row_product.splits), kProductK));
-    const RowsEpilogue re{c.row_sums, c.padded * c.cols, c.cols, first == 0, 0};
+    const RowsEpilogue re{c.row_sums, c.padded * c.cols, c.cols, first == 0, 0, false};
     ProductArgs more = args;
     more.a           = x_scaled;
     more.k_extent    = static_cast<int32_t>(c.padded);
@@ -1697,14 +1725,25 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
       LBT_TRY((launch_product<L, true, false, kRowsN>(s, args, c.features, c.n_rows, c.row_product, re)));
       return launch_product<L, true, true, kRowsK>(s, more, c.features, classes, c.class_product, ce);
     };
-    if (c.class_product.splits > 1) {
-      LBT_TRY(products(RowsEpilogue{c.class_sums, c.piece * c.cols, c.cols, true, static_cast<int>(classes)}));
+    if (c.parts) {
+      LBT_TRY(products(RowsEpilogue{c.class_sums + first * c.cols, static_cast<int64_t>(c.classes) * c.cols, c.cols, begins,
+                                    static_cast<int>(classes), scaled}));
+    } else if (c.class_product.splits > 1) {
+      LBT_TRY(products(RowsEpilogue{c.class_sums, c.piece * c.cols, c.cols, true, static_cast<int>(classes), false}));
       finish_classes_kernel<kDtype><<<static_cast<unsigned>(tiles_of(classes * ((c.features + 3) / 4), 256)), 256, 0, s>>>(
         c.class_sums, c.class_product.splits, c.piece * c.cols, c.cols, first, classes, c.features, c.counts, scaled, grad_weight);
       LBT_HIP(hipGetLastError());
     } else {
       LBT_TRY(products(ClassesEpilogue<kDtype>{grad_weight, static_cast<int>(first), c.classes, c.features, scaled}));
     }
+  }
+  if (c.parts && ends) {
+    const int64_t blocks = tiles_of(static_cast<int64_t>(c.classes) * ((c.features + 3) / 4), 256);
+    LBT_REQUIRE(blocks < (int64_t(1) << 24), "too many values");
+    finish_classes_kernel<kDtype><<<static_cast<unsigned>(blocks), 256, 0, s>>>(c.class_sums, c.class_product.splits,
+                                                                                static_cast<int64_t>(c.classes) * c.cols, c.cols, 0, c.classes,
+                                                                                c.features, c.counts, false, grad_weight);
+    LBT_HIP(hipGetLastError());
   }
   const int64_t blocks = tiles_of(c.n_rows * ((c.features + 3) / 4), 256);
   LBT_REQUIRE(blocks < (int64_t(1) << 31), "too many values");
@@ -1714,7 +1753,7 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
   if (grad_bias != nullptr) {
     finish_bias_kernel<<<static_cast<unsigned>(tiles_of(c.classes, kJoinRows)), kJoinRows * kJoinSlices, 0, s>>>(c.bias_sums, c.classes,
                                                                                        c.kept ? c.scale_rows : c.scores.tile, c.counts, kHalf,
-                                                                                       grad_bias);
+                                                                                       !begins, grad_bias);
     LBT_HIP(hipGetLastError());
   }
   return LBT_OK;
@@ -1752,7 +1791,6 @@ int run_loss(void* stream, const void* X, const void* weight, int32_t dtype, int
     return LBT_ERR_WORKSPACE;
   }
   LossCall c(std::max<int64_t>(n_rows, 1), n_features, n_outputs, dtype, !gradient ? 0 : grad_bias == nullptr ? 1 : 2);
-  c.n_rows       = n_rows;
   const bool few = !gradient && few_loss(n_rows, n_features, n_outputs, dtype);
   FewCall f;
   Arena arena;
@@ -1771,14 +1809,28 @@ int run_loss(void* stream, const void* X, const void* weight, int32_t dtype, int
     if (dtype == LBT_F16) return few_log_loss<LBT_F16>(s, f, X, weight, bias, y, n, n_features, n_outputs, loss);
     return few_log_loss<LBT_F32>(s, f, X, weight, bias, y, n, n_features, n_outputs, loss);
   }
-  switch (dtype) {
-    case LBT_BF16:
-      return linear_log_loss<LBT_BF16>(s, c, X, weight, bias, y, sample_weight, loss, grad_X, grad_weight, grad_bias);
-    case LBT_F16:
-      return linear_log_loss<LBT_F16>(s, c, X, weight, bias, y, sample_weight, loss, grad_X, grad_weight, grad_bias);
-    default:
-      return linear_log_loss<LBT_F32>(s, c, X, weight, bias, y, sample_weight, loss, grad_X, grad_weight, grad_bias);
-  }
+  const int64_t at_once = c.n_rows;
+  int64_t first         = 0;
+  do {
+    c.n_rows              = std::min(at_once, n_rows - first);
+    const int64_t value   = size * first * n_features;  // bytes before this part's rows
+    const void* const x   = static_cast<const char*>(X) + value;
+    void* const gx        = grad_X == nullptr ? nullptr : static_cast<char*>(grad_X) + value;
+    const float* const sw = sample_weight == nullptr ? nullptr : sample_weight + first;
+    const bool begins = first == 0, ends = first + at_once >= n_rows;
+    switch (dtype) {
+      case LBT_BF16:
+        LBT_TRY(linear_log_loss<LBT_BF16>(s, c, x, weight, bias, y + first, sw, loss + first, gx, grad_weight, grad_bias, begins, ends));
+        break;
+      case LBT_F16:
+        LBT_TRY(linear_log_loss<LBT_F16>(s, c, x, weight, bias, y + first, sw, loss + first, gx, grad_weight, grad_bias, begins, ends));
+        break;
+      default:
+        LBT_TRY(linear_log_loss<LBT_F32>(s, c, x, weight, bias, y + first, sw, loss + first, gx, grad_weight, grad_bias, begins, ends));
+    }
+    first += at_once;
+  } while (first < n_rows);
+  return LBT_OK;
 }
 
 }  // namespace

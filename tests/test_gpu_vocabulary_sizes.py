@@ -1,0 +1,109 @@
+"""The operators for vocabularies at sizes where a call is cut up: rows in parts, long sorts.
+
+The bounds are those of test_gpu_vocabulary.py. Where a sum goes over hundreds of thousands of rows its worst case is a few hundredths of
+the sum of sizes; the values here have one sign for half of the classes, so that a part left out, or added twice, is far more than that."""
+import pytest
+import torch
+
+from lbtree import ops
+from test_gpu_vocabulary import ENTRY, LEAST, STEP, TYPES, U, assert_within
+
+pytestmark = pytest.mark.gpu
+
+
+def reference_by_rows(x, w, y, bias, weight, t, step):
+    """test_gpu_vocabulary.reference for many rows, `step` at a time: outputs in 64 bits and what they may be off by."""
+    n, f = x.shape
+    k = w.shape[0]
+    W = w.double()
+    kinds = dict(dtype=torch.float64, device=x.device)
+    loss, gx, gw, gb = torch.zeros(n, **kinds), torch.zeros(n, f, **kinds), torch.zeros(k, f, **kinds), torch.zeros(k, **kinds)
+    bl, bx, bw, bb = (torch.zeros_like(a) for a in (loss, gx, gw, gb))
+    sw, sb = torch.zeros_like(gw), torch.zeros_like(gb)  # sums of sizes
+    counted = 0
+    for i in range(0, n, step):
+        rows = ((y[i:i + step] >= 0) & (y[i:i + step] < k)).nonzero()[:, 0] + i
+        X, lab, here = x[rows].double(), y[rows], torch.arange(rows.numel(), device=x.device)
+        s, size = X @ W.t(), X.abs() @ W.abs().t()
+        if bias is not None:
+            s, size = s + bias.double(), size + bias.double().abs()
+        d = ((f + 8) * U + 2.0 ** -22) * (size.max(dim=1).values if rows.numel() else size.sum(dim=1))
+        rel = 2 * d + 1e-4
+        lse = torch.logsumexp(s, dim=1)
+        loss[rows], bl[rows] = lse - s[here, lab], rel + 8 * U * (lse.abs() + 1.0)
+        p = torch.exp(s - lse[:, None])
+        g = p.clone()
+        g[here, lab] -= 1.0
+        wt = torch.ones(rows.numel(), **kinds) if weight is None else weight.double()[rows]
+        g = g * wt[:, None]
+        off = g.abs() * 4 * U + p * rel[:, None] * wt.abs()[:, None]
+        # an entry of G is rounded once; where bfloat16 has no bias the exponential is held as half before, half a step of which is 2^-11
+        entry = off + g.abs() * (ENTRY[t] + (2.0 ** -11 if t == "bf16" and bias is None else 0.0))
+        gx[rows] = g @ W
+        bx[rows] = (entry @ W.abs() + (k + 64) * U * (g.abs() @ W.abs())) * (1 + STEP[t]) + gx[rows].abs() * STEP[t] + LEAST[t]
+        gw += g.t() @ X
+        gb += g.sum(dim=0)
+        bw += entry.t() @ X.abs()
+        bb += off.sum(dim=0)
+        sw += g.abs().t() @ X.abs()
+        sb += g.abs().sum(dim=0)
+        counted += rows.numel()
+    bw = (bw + (counted + 64) * U * sw) * (1 + STEP[t]) + gw.abs() * STEP[t] + LEAST[t]
+    return (loss, gx, gw, gb), (bl, bx, bw, bb + (counted + 64) * U * sb + gb.abs() * U)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("n,f,k,masked", [(300000, 20, 40, "some"), (131073, 100, 9, "none"), (280000, 7, 300, "first")])
+def test_rows_in_parts(n, f, k, masked, dtype):
+    """At most 131072 rows are one part."""
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    x = (torch.rand((n, f), generator=gen, device="cuda") * 0.5).to(TYPES[dtype])
+    w = (torch.randn((k, f), generator=gen, device="cuda") * 0.3).to(TYPES[dtype])
+    y = torch.randint(0, k // 2, (n,), generator=gen, device="cuda")  # the other classes' entries of G are all positive
+    if masked == "some":
+        y[torch.rand(n, generator=gen, device="cuda") < 0.2] = k
+    if masked == "first":  # not one row of the first part, and of the last one, counts
+        y[:140001] = -1
+        y[279000:] = -1
+    x[(y < 0) | (y >= k)] = float("nan")
+    # (weights far apart from part to part: half precision has a power of two for each)
+    weight = (torch.rand(n, generator=gen, device="cuda") + 0.5) * torch.where(torch.arange(n, device="cuda") < n // 2, 2e-3, 1e-2)
+    bias = torch.randn(k, generator=gen, device="cuda")
+    for b, wt in ((None, None), (bias, weight), (None, weight)):
+        if wt is None and dtype == "f16":
+            wt = torch.full((n,), 2.0 ** -6, device="cuda")  # (the sums of 300000 rows pass the largest number)
+        want, bound = reference_by_rows(x, w, y, b, wt, dtype, 50000)
+        got = ops.linear_log_loss_gradient(x, w, y, sample_weight=wt, bias=b)
+        for i, name in enumerate(("loss", "grad_X", "grad_weight", "grad_bias")[:len(got)]):
+            assert_within(got[i], want[i], bound[i], name)
+        again = ops.linear_log_loss_gradient(x, w, y, sample_weight=wt, bias=b)
+        assert all(torch.equal(p, q) for p, q in zip(got, again))
+        assert_within(ops.linear_log_loss(x, w, y, bias=b), want[0], bound[0], "loss alone")
+
+
+def test_rows_in_parts_and_classes_in_pieces():
+    """Two parts of 65792 rows: 4 GiB of G and its exponentials are 6400 classes of float."""
+    n, f, k = 131100, 8, 6600
+    assert 10 * 65792 * k > 4 << 30
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    x = torch.rand((n, f), generator=gen, device="cuda") * 0.5
+    w = torch.randn((k, f), generator=gen, device="cuda") * 0.3
+    y = torch.randint(0, k // 2, (n,), generator=gen, device="cuda")
+    want, bound = reference_by_rows(x, w, y, None, None, "f32", 20000)
+    for i, got in enumerate(ops.linear_log_loss_gradient(x, w, y)):
+        assert_within(got, want[i], bound[i], ("loss", "grad_X", "grad_weight")[i])
+    assert_within(ops.linear_log_loss(x, w, y), want[0], bound[0], "loss alone")
+
+
+@pytest.mark.parametrize("dtype,n,f", [("f32", 9000, 66000), ("f16", 8300, 132000), ("bf16", 8300, 131073)])
+def test_parts_of_long_rows(dtype, n, f):
+    """At most 2^30 values of planes are one part."""
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    k = 20
+    x = torch.rand((n, f), generator=gen, device="cuda").mul_(0.5).to(TYPES[dtype])
+    w = (torch.randn((k, f), generator=gen, device="cuda") * 0.005).to(TYPES[dtype])
+    y = torch.randint(0, k // 2, (n,), generator=gen, device="cuda")
+    weight = torch.full((n,), 2.0 ** -4, device="cuda")
+    want, bound = reference_by_rows(x, w, y, None, weight, dtype, 1500)
+    for i, got in enumerate(ops.linear_log_loss_gradient(x, w, y, sample_weight=weight)):
+        assert_within(got, want[i], bound[i], ("loss", "grad_X", "grad_weight")[i])

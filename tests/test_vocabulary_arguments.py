@@ -133,3 +133,17 @@ def test_native_calls_leave_what_they_do_not_take():
     for call in (host.embed_rows_gradient, host.linear_log_loss, host.linear_log_loss_gradient):
         with pytest.raises(TypeError):
             call(table, tokens)
+
+
+def test_workspaces_of_many_rows():
+    """Rows come in parts: millions of them take the scratch of one part, and no piece of the gradient passes 4 GiB."""
+    q = L.lbt_linear_log_loss_workspace_bytes
+    for dtype, size in ((_lib.LBT_BF16, 2), (_lib.LBT_F16, 2), (_lib.LBT_F32, 4)):
+        for gradient in (0, 1, 2):
+            for n, f, k in ((10000000, 100, 8), (2000000, 200, 8), (1 << 24, 28, 2), (1 << 30, 1, 1)):
+                assert 0 < q(n, f, k, dtype, gradient) < (1 << 30), (n, f, k, dtype, gradient)
+            # ten times the rows: the same but for what the parts' sizes differ by
+            assert q(10000000, 100, 8, dtype, gradient) <= q(1000000, 100, 8, dtype, gradient) * 1.2
+            # G and its exponentials, the tops and totals, X in planes twice and the sums of its gradient, and those of grad_weight
+            weights = 4 * 131072 * 1024
+            assert q(4000000, 1024, 131072, dtype, gradient) < (4 << 30) + (1 << 31) + 2 * (2 << 30) + (4 << 30) + (1 << 29) + weights
