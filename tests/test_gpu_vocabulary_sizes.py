@@ -107,3 +107,34 @@ def test_parts_of_long_rows(dtype, n, f):
     want, bound = reference_by_rows(x, w, y, None, weight, dtype, 1500)
     for i, got in enumerate(ops.linear_log_loss_gradient(x, w, y, sample_weight=weight)):
         assert_within(got, want[i], bound[i], ("loss", "grad_X", "grad_weight")[i])
+
+
+# ---- rows of a table ---------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("kind", ["uniform", "one", "few"])
+@pytest.mark.parametrize("rows", [1, 700, 60000, 1500000])  # one, one, two and three digits of the sort
+@pytest.mark.parametrize("t", [131073, 135201, 524288, 524289, 700003])
+def test_long_sorts(t, rows, kind):
+    """Beyond 131072 places a thread of the sort has four entries, beyond 524288 the blocks' offsets have a launch of their own. Whole
+    numbers below 8 are summed exactly: any place that is lost, doubled or misplaced is seen."""
+    gen = torch.Generator(device="cuda").manual_seed(t + rows)
+    if kind == "uniform":
+        tokens = torch.randint(-1, rows + 1, (t,), generator=gen, device="cuda")  # some name no row
+    elif kind == "one":
+        tokens = torch.full((t,), rows - 1, device="cuda")
+    else:
+        tokens = torch.randint(0, 5, (t,), generator=gen, device="cuda") * (rows // 5)
+    grad = torch.randint(-8, 9, (t, 4), generator=gen, device="cuda").float()
+    inside = (tokens >= 0) & (tokens < rows)
+    # (on the host: atomic sums of equal tokens would wait for one another)
+    want = torch.zeros((rows, 4), dtype=torch.float64).index_add_(0, tokens[inside].cpu(), grad[inside].double().cpu()).cuda()
+    assert 8 * t < 1 << 24
+    got = ops.embed_rows_gradient(grad, tokens, rows)
+    assert torch.equal(got.double(), want)
+    assert torch.equal(ops.embed_rows_gradient(grad, tokens.to(torch.int32), rows), got)
+    old = torch.randint(-8, 9, (rows, 4), generator=gen, device="cuda").float()
+    assert torch.equal(ops.embed_rows_gradient(grad, tokens, rows, add_to=old.clone()).double(), want + old.double())
+    # numbers that round: the same bits from call to call
+    grad = torch.randn((t, 4), generator=gen, device="cuda").to(torch.bfloat16)
+    assert torch.equal(ops.embed_rows_gradient(grad, tokens, rows, scale=1.3), ops.embed_rows_gradient(grad, tokens, rows, scale=1.3))
