@@ -550,7 +550,8 @@ int lbt_gather_rows(void* stream, const void* X, int32_t x_dtype, int64_t row_of
  *   workspace  at least lbt_linear_log_loss_workspace_bytes(..., gradient = 0), 256-byte aligned. `gradient`: 0 for this
  *              call, 1 for lbt_linear_log_loss_gradient, 2 for that with grad_bias; 0 bytes for invalid arguments
  * Enqueues on the stream and does not wait. All results are the same from call to call. What is written (and the workspace) may
- * not overlap what is read, or one another: LBT_ERR_INVALID, here and in the calls below.
+ * not overlap what is read, or one another: LBT_ERR_INVALID, here and in the calls below. Up to 2^30 rows, 2^30 - 64 classes, 2^20
+ * features and 2^38 values of X or weight.
  */
 size_t lbt_linear_log_loss_workspace_bytes(int64_t n_rows, int32_t n_features, int32_t n_outputs, int32_t dtype, int32_t gradient);
 int lbt_linear_log_loss(void* stream, const void* X, const void* weight, int32_t dtype, int64_t n_rows, int32_t n_features,
@@ -582,7 +583,7 @@ int lbt_linear_log_loss_gradient(void* stream, const void* X, const void* weight
  *   table   device [n_rows][n_features], dtype LBT_F32, LBT_BF16 or LBT_F16, 16-byte aligned
  *   tokens  device int32 (token_bytes 4) or int64 (8) [n_tokens]. A token not in [0, n_rows) gives a row of zeros
  *   out     device [n_tokens][n_features], dtype of the table, 16-byte aligned; may not overlap the table
- * Enqueues on the stream and does not wait.
+ * Enqueues on the stream and does not wait. Up to 2^30 tokens, 2^30 - 64 rows, 2^24 features and 2^38 values, here and below.
  */
 int lbt_embed_rows(void* stream, const void* table, int32_t dtype, int32_t n_rows, int32_t n_features, const void* tokens,
                    int32_t token_bytes, int64_t n_tokens, float scale, void* out);

@@ -739,7 +739,12 @@ int embed_gradient(hipStream_t s, const EmbedCall& c, const void* grad, const vo
   a.sorted = c.sorted[at];
   if (!add) a.clears = static_cast<unsigned>((static_cast<int64_t>(c.n_rows) + kClearRows - 1) / kClearRows);
   const int64_t grid = (c.chunks * c.slices + kRowWaves - 1) / kRowWaves;
-  LBT_REQUIRE(grid + a.clears < (int64_t(1) << 31), "too many elements");
+  LBT_REQUIRE(grid <= most_groups(kRowThreads), "too many elements");
+  if (grid + a.clears > most_groups(kRowThreads)) {  // (only with a thousand million rows) the clears have a launch of their own
+    sum_runs_kernel<kDtype, kBytes><<<a.clears, kRowThreads, 0, s>>>(a);
+    LBT_HIP(hipGetLastError());
+    a.clears = 0;
+  }
   sum_runs_kernel<kDtype, kBytes><<<static_cast<unsigned>(grid + a.clears), kRowThreads, 0, s>>>(a);
   LBT_HIP(hipGetLastError());
   if (c.chunks > 1) {
@@ -752,7 +757,7 @@ int embed_gradient(hipStream_t s, const EmbedCall& c, const void* grad, const vo
 bool embed_shape(int64_t n_tokens, int32_t n_features, int32_t n_rows, int32_t dtype)
 {
   return (dtype == LBT_F32 || dtype == LBT_BF16 || dtype == LBT_F16) && n_tokens >= 0 && n_tokens <= (1 << 30) &&
-         n_features >= 1 && n_features <= (1 << 24) && n_rows >= 1 && n_rows <= (1 << 30) &&
+         n_features >= 1 && n_features <= (1 << 24) && n_rows >= 1 && n_rows <= (1 << 30) - 64 &&
          n_tokens * n_features < (int64_t(1) << 38) && int64_t(n_rows) * n_features < (int64_t(1) << 38);
 }
 
@@ -797,10 +802,14 @@ int lbt_embed_rows(void* stream, const void* table, int32_t dtype, int32_t n_row
   return lbt::for_type(dtype, c.bytes, [&](auto type, auto bytes) -> int {
     auto launch = [&](auto lanes) -> int {
       constexpr int kLanes = decltype(lanes)::value, kRows = lbt::kRowThreads / kLanes;
-      const int64_t blocks = (n_tokens + kRows - 1) / kRows;
-      LBT_REQUIRE(blocks < (int64_t(1) << 31), "too many elements");
-      lbt::embed_rows_kernel<decltype(type)::value, decltype(bytes)::value, kLanes>
-        <<<static_cast<unsigned>(blocks), lbt::kRowThreads, 0, s>>>(table, n_rows, c.words, tokens, token_bytes, n_tokens, scale, out);
+      constexpr int64_t kMost = int64_t(1) << 22;  // workgroups of a launch: 2^24 of them would be too many threads
+      for (int64_t t = 0; t < n_tokens; t += kMost * kRows) {
+        const int64_t some = std::min(n_tokens - t, kMost * kRows);
+        lbt::embed_rows_kernel<decltype(type)::value, decltype(bytes)::value, kLanes>
+          <<<static_cast<unsigned>((some + kRows - 1) / kRows), lbt::kRowThreads, 0, s>>>(
+            table, n_rows, c.words, static_cast<const char*>(tokens) + t * token_bytes, token_bytes, some, scale, static_cast<char*>(out) + t * row);
+        LBT_HIP(hipGetLastError());
+      }
       return LBT_OK;
     };
     // a wave takes a row, or a part of one a short row; 4 words of a lane at a time (200000 rows of 32 bfloat16: 5.3 us, by whole waves 34;
@@ -808,7 +817,6 @@ int lbt_embed_rows(void* stream, const void* table, int32_t dtype, int32_t n_row
     if (c.words > 64) LBT_TRY(launch(std::integral_constant<int, 64>{}));
     else if (c.words > 8) LBT_TRY(launch(std::integral_constant<int, 16>{}));
     else LBT_TRY(launch(std::integral_constant<int, 4>{}));
-    LBT_HIP(hipGetLastError());
     return LBT_OK;
   });
 }

@@ -42,6 +42,9 @@ void set_error(const char* fmt, ...);
     if (rc__ != LBT_OK) return rc__; \
   } while (0)
 
+// Workgroups that a launch may have along x: the runtime takes their threads modulo 2^32, and runs that many without an error.
+constexpr int64_t most_groups(int threads) { return (int64_t(1) << 32) / threads - 1; }
+
 // What a call reads or writes; null: nothing.
 struct MemoryRange {
   const void* begin;

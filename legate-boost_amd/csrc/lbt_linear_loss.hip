@@ -1228,12 +1228,12 @@ __global__ void __launch_bounds__(256)
 
 // grad_bias from its sums over blocks of rows; a class's blocks are shared out among 64 threads. `add`: to that of the rows before.
 __global__ void __launch_bounds__(kJoinRows * kJoinSlices)
-  finish_bias_kernel(const float* __restrict__ sums, int n_classes, int block_rows, const RowCounts* __restrict__ counts, int half, bool add,
-                     float* __restrict__ out)
+  finish_bias_kernel(const float* __restrict__ sums, int first_class, int n_classes, int block_rows, const RowCounts* __restrict__ counts, int half,
+                     bool add, float* __restrict__ out)
 {
   __shared__ float share[kJoinSlices][kJoinRows];
   const int n = threadIdx.x % kJoinRows, slice = threadIdx.x / kJoinRows;
-  const int c      = blockIdx.x * kJoinRows + n;
+  const int c      = first_class + blockIdx.x * kJoinRows + n;
   const int blocks = (counts->rows + block_rows - 1) / block_rows;
   float sum        = 0.f;
   if (c < n_classes) {
@@ -1251,8 +1251,7 @@ __global__ void __launch_bounds__(kJoinRows * kJoinSlices)
 
 __global__ void __launch_bounds__(256) clear_kernel(uint16_t* __restrict__ out, int64_t n)
 {
-  const int64_t i = blockIdx.x * int64_t(256) + threadIdx.x;
-  if (i < n) out[i] = 0;
+  for (int64_t i = blockIdx.x * int64_t(256) + threadIdx.x; i < n; i += gridDim.x * int64_t(256)) out[i] = 0;
 }
 
 // ---- host -----------------------------------------------------------------------------------------
@@ -1498,7 +1497,7 @@ int launch_tiles(hipStream_t s, ProductArgs args, int64_t m, int64_t n, int spli
   args.tiles_m = static_cast<int>(tiles_of(m, Tile::kBM));
   args.tiles_n = static_cast<int>(tiles_of(n, Tile::kBN));
   const int64_t blocks = static_cast<int64_t>(args.tiles_m) * args.tiles_n;
-  LBT_REQUIRE(blocks < (int64_t(1) << 31), "too many tiles");
+  LBT_REQUIRE(blocks <= most_groups(Tile::kThreads), "too many tiles");
   product_kernel<Tile, L::kProduct, L::kPlanes, kAMajor, kBMajor, kRowsSide, Epilogue>
     <<<dim3(static_cast<unsigned>(blocks), splits), Tile::kThreads, 0, s>>>(args, e);
   LBT_HIP(hipGetLastError());
@@ -1520,7 +1519,7 @@ int launch_float_tiles(hipStream_t s, FloatArgs args, int64_t m, int64_t n, int 
   args.tiles_n = static_cast<int>(tiles_of(n, Tile::kBN));
   args.k_split = static_cast<int32_t>(round_up(tiles_of(kAMajor ? args.rows : args.cols, splits), Tile::kK));
   const int64_t blocks = static_cast<int64_t>(args.tiles_m) * args.tiles_n;
-  LBT_REQUIRE(blocks < (int64_t(1) << 31), "too many tiles");
+  LBT_REQUIRE(blocks <= most_groups(Tile::kThreads), "too many tiles");
   float_product_kernel<Tile, kAMajor, Epilogue><<<dim3(static_cast<unsigned>(blocks), splits), Tile::kThreads, 0, s>>>(args, e);
   LBT_HIP(hipGetLastError());
   return LBT_OK;
@@ -1538,10 +1537,24 @@ int launch_pack(hipStream_t s, const void* from, int64_t first_row, int64_t rows
                 int mode, const int32_t* exponent, RowCounts* counts, int64_t out_rows, int padded_cols, Layout layout, uint16_t* out)
 {
   const int64_t blocks = tiles_of(out_rows * (padded_cols / 8), 256);
-  LBT_REQUIRE(blocks < (int64_t(1) << 31), "too many values to lay out");
+  LBT_REQUIRE(blocks <= most_groups(256), "too many values to lay out");
   pack_rows_kernel<kDtype><<<static_cast<unsigned>(blocks), 256, 0, s>>>(from, first_row, rows, cols, order, mode, exponent, counts,
                                                                          out_rows, padded_cols, layout, out);
   LBT_HIP(hipGetLastError());
+  return LBT_OK;
+}
+
+// grad_weight of the classes first .. first + classes - 1 from their sums, as many at a time as a launch may take.
+template <int kDtype>
+int launch_finish_classes(hipStream_t s, const LossCall& c, const float* sums, int64_t split, int64_t first, int64_t classes, bool scaled, void* out)
+{
+  const int64_t groups = (c.features + 3) / 4, most = (int64_t(1) << 30) / groups;
+  for (int64_t at = 0; at < classes; at += most) {
+    const int64_t some = std::min(most, classes - at);
+    finish_classes_kernel<kDtype><<<static_cast<unsigned>(tiles_of(some * groups, 256)), 256, 0, s>>>(
+      sums + at * c.cols, c.class_product.splits, split, c.cols, first + at, some, c.features, c.counts, scaled, out);
+    LBT_HIP(hipGetLastError());
+  }
   return LBT_OK;
 }
 
@@ -1554,12 +1567,11 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
   constexpr bool kFine = kDtype == LBT_F32;
   constexpr bool kHalf = kDtype == LBT_F16;
   if (c.n_rows == 0) {  // no row: the gradients are zeros
-    const int64_t halves = int64_t(c.classes) * c.features * sizeof(typename L::Value) / 2;
-    LBT_REQUIRE(tiles_of(halves, 256) < (int64_t(1) << 31), "too many values");
-    clear_kernel<<<static_cast<unsigned>(tiles_of(halves, 256)), 256, 0, s>>>(static_cast<uint16_t*>(grad_weight), halves);
-    if (grad_bias != nullptr)
-      clear_kernel<<<static_cast<unsigned>(tiles_of(2 * int64_t(c.classes), 256)), 256, 0, s>>>(
-        reinterpret_cast<uint16_t*>(grad_bias), 2 * int64_t(c.classes));
+    auto clear = [&](void* out, int64_t halves) {
+      clear_kernel<<<static_cast<unsigned>(std::min<int64_t>(tiles_of(halves, 256), 1 << 20)), 256, 0, s>>>(static_cast<uint16_t*>(out), halves);
+    };
+    clear(grad_weight, int64_t(c.classes) * c.features * sizeof(typename L::Value) / 2);
+    if (grad_bias != nullptr) clear(grad_bias, 2 * int64_t(c.classes));
     LBT_HIP(hipGetLastError());
     return LBT_OK;
   }
@@ -1570,7 +1582,7 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
     const FusedArgs a{y,         sample_weight, static_cast<int>(c.n_rows), static_cast<int>(c.padded), c.classes, loss, c.counts, c.zeros, X, weight,
                       c.features, c.cols,        c.x,                        c.packed ? c.weight : nullptr, c.packed ? c.piece : 0, c.x_blocks, x_blocks};
     const int64_t groups = c.padded / kFusedEach * tiles_of(c.cols / 8, kFusedGroups) + tiles_of(a.weight_rows * (c.cols / 8), 256);
-    LBT_REQUIRE(groups < (int64_t(1) << 31), "too many values to lay out");
+    LBT_REQUIRE(groups <= most_groups(256), "too many values to lay out");
     prepare_pack_kernel<kDtype><<<static_cast<unsigned>(groups), 256, 0, s>>>(a, c.rows);
     LBT_HIP(hipGetLastError());
   } else {
@@ -1601,7 +1613,8 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
   args.counts = c.counts;
 
   // top and total of each row; weights that are multiplied where they lie need no pieces here
-  const int64_t step = c.packed && !c.floats ? c.piece : c.classes;
+  // (but launches their bound: 2^26 classes at a time where the tiles of more might be too many)
+  const int64_t step = c.packed && !c.floats ? c.piece : c.kept != kNotKept ? c.classes : std::min<int64_t>(c.classes, 1 << 26);
   int64_t tiles      = 0;
   if (c.few) {
     const FewRowsArgs few{X, weight, bias, nullptr, static_cast<int>(c.n_rows), c.features, c.classes, 1, c.piece / 16, c.partial, c.rows.picked,
@@ -1627,7 +1640,8 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
                                          kKind == kKeptFloat ? static_cast<void*>(c.exps) : c.g, static_cast<int>(c.piece)};
       tiles += tiles_of(m, c.all_scores.tile);
       if constexpr (kFine) {
-        const FloatArgs fa{static_cast<const float*>(weight), c.classes, c.features, 0, c.x_blocks, c.padded, 0, 0, c.zeros, c.counts};
+        const FloatArgs fa{static_cast<const float*>(weight) + first * c.features, c.classes - static_cast<int>(first), c.features, 0, c.x_blocks,
+                           c.padded, 0, 0, c.zeros, c.counts};
         return launch_floats<false>(s, fa, m, c.n_rows, c.all_scores, e);
       } else {
         return launch_product<L, false, false, kRowsN>(s, args, m, c.n_rows, c.all_scores, e);
@@ -1716,7 +1730,7 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
         more.tiles_n = static_cast<int>(tiles_of(classes, SmallTile::kBN));
         const int64_t blocks = static_cast<int64_t>(args.tiles_m) * args.tiles_n * c.row_product.splits;
         const int64_t all    = blocks + static_cast<int64_t>(more.tiles_m) * more.tiles_n * c.class_product.splits;
-        LBT_REQUIRE(all < (int64_t(1) << 31), "too many tiles");
+        LBT_REQUIRE(all <= most_groups(SmallTile::kThreads), "too many tiles");
         two_products_kernel<SmallTile, L::kProduct, L::kPlanes>
           <<<static_cast<unsigned>(all), SmallTile::kThreads, 0, s>>>(args, re, static_cast<unsigned>(blocks), more, ce);
         LBT_HIP(hipGetLastError());
@@ -1730,31 +1744,25 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
                                     static_cast<int>(classes), scaled}));
     } else if (c.class_product.splits > 1) {
       LBT_TRY(products(RowsEpilogue{c.class_sums, c.piece * c.cols, c.cols, true, static_cast<int>(classes), false}));
-      finish_classes_kernel<kDtype><<<static_cast<unsigned>(tiles_of(classes * ((c.features + 3) / 4), 256)), 256, 0, s>>>(
-        c.class_sums, c.class_product.splits, c.piece * c.cols, c.cols, first, classes, c.features, c.counts, scaled, grad_weight);
-      LBT_HIP(hipGetLastError());
+      LBT_TRY(launch_finish_classes<kDtype>(s, c, c.class_sums, c.piece * c.cols, first, classes, scaled, grad_weight));
     } else {
       LBT_TRY(products(ClassesEpilogue<kDtype>{grad_weight, static_cast<int>(first), c.classes, c.features, scaled}));
     }
   }
-  if (c.parts && ends) {
-    const int64_t blocks = tiles_of(static_cast<int64_t>(c.classes) * ((c.features + 3) / 4), 256);
-    LBT_REQUIRE(blocks < (int64_t(1) << 24), "too many values");
-    finish_classes_kernel<kDtype><<<static_cast<unsigned>(blocks), 256, 0, s>>>(c.class_sums, c.class_product.splits,
-                                                                                static_cast<int64_t>(c.classes) * c.cols, c.cols, 0, c.classes,
-                                                                                c.features, c.counts, false, grad_weight);
-    LBT_HIP(hipGetLastError());
-  }
+  if (c.parts && ends)
+    LBT_TRY(launch_finish_classes<kDtype>(s, c, c.class_sums, static_cast<int64_t>(c.classes) * c.cols, 0, c.classes, false, grad_weight));
   const int64_t blocks = tiles_of(c.n_rows * ((c.features + 3) / 4), 256);
-  LBT_REQUIRE(blocks < (int64_t(1) << 31), "too many values");
+  LBT_REQUIRE(blocks <= most_groups(256), "too many values");
   finish_rows_kernel<kDtype><<<static_cast<unsigned>(blocks), 256, 0, s>>>(c.row_sums, c.row_product.splits, c.padded * c.cols, c.cols,
                                                                            c.n_rows, c.features, c.rows, grad_X);
   LBT_HIP(hipGetLastError());
   if (grad_bias != nullptr) {
-    finish_bias_kernel<<<static_cast<unsigned>(tiles_of(c.classes, kJoinRows)), kJoinRows * kJoinSlices, 0, s>>>(c.bias_sums, c.classes,
-                                                                                       c.kept ? c.scale_rows : c.scores.tile, c.counts, kHalf,
-                                                                                       !begins, grad_bias);
-    LBT_HIP(hipGetLastError());
+    constexpr int kMost = 1 << 24;  // classes of a launch: 64 threads each
+    for (int first = 0; first < c.classes; first += kMost) {
+      finish_bias_kernel<<<static_cast<unsigned>(tiles_of(std::min(c.classes - first, kMost), kJoinRows)), kJoinRows * kJoinSlices, 0, s>>>(
+        c.bias_sums, first, c.classes, c.kept ? c.scale_rows : c.scores.tile, c.counts, kHalf, !begins, grad_bias);
+      LBT_HIP(hipGetLastError());
+    }
   }
   return LBT_OK;
 }
@@ -1762,7 +1770,7 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
 bool loss_shape(int64_t n_rows, int32_t n_features, int32_t n_outputs, int32_t dtype)
 {
   return (dtype == LBT_F32 || dtype == LBT_BF16 || dtype == LBT_F16) && n_rows >= 0 && n_features >= 1 && n_outputs >= 1 &&
-         n_rows <= (int64_t(1) << 30) && n_features <= (1 << 20) && n_outputs <= (1 << 30) &&
+         n_rows <= (int64_t(1) << 30) && n_features <= (1 << 20) && n_outputs <= (1 << 30) - 64 &&
          n_rows * n_features < (int64_t(1) << 38) && int64_t(n_outputs) * n_features < (int64_t(1) << 38);
 }
 

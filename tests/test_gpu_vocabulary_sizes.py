@@ -138,3 +138,64 @@ def test_long_sorts(t, rows, kind):
     # numbers that round: the same bits from call to call
     grad = torch.randn((t, 4), generator=gen, device="cuda").to(torch.bfloat16)
     assert torch.equal(ops.embed_rows_gradient(grad, tokens, rows, scale=1.3), ops.embed_rows_gradient(grad, tokens, rows, scale=1.3))
+
+
+# ---- more than 2^32 threads --------------------------------------------------------------------------
+# (a launch has fewer: these are several)
+
+
+@pytest.mark.parametrize("f,t", [(67, (1 << 26) + 1001), (9, (1 << 28) + 5)])  # 64 and 16 threads a row
+def test_lookups_of_many_tokens(f, t):
+    gen = torch.Generator(device="cuda").manual_seed(f)
+    table = torch.randn((77, f), generator=gen, device="cuda").to(torch.bfloat16)
+    tokens = torch.randint(-1, 78, (t,), generator=gen, device="cuda", dtype=torch.int32)
+    got = ops.embed_rows(table, tokens, 2.0)
+    clean = torch.cat([table * 2, torch.zeros((1, f), dtype=table.dtype, device="cuda")])  # (twice a number is exact)
+    for i in range(0, t, 1 << 24):
+        part = tokens[i:i + (1 << 24)].long()
+        assert torch.equal(got[i:i + (1 << 24)], clean[torch.where(part < 0, 77, part)])
+
+
+@pytest.mark.parametrize("t", [5, 3000])  # without sorting, and sorted with rows cleared apart
+def test_tables_of_many_rows(t):
+    rows = (1 << 30) - 64
+    gen = torch.Generator(device="cuda").manual_seed(t)
+    tokens = torch.randint(0, rows, (t,), generator=gen, device="cuda")
+    tokens[0], tokens[1], tokens[2] = rows - 1, 0, rows
+    grad = torch.randint(1, 9, (t, 1), generator=gen, device="cuda").to(torch.bfloat16)
+    got = ops.embed_rows_gradient(grad, tokens, rows)
+    named, where = torch.unique(tokens[tokens < rows], return_inverse=True)
+    want = torch.zeros(named.numel(), dtype=torch.float64).index_add_(0, where.cpu(), grad[tokens < rows, 0].double().cpu())
+    assert torch.equal(got[named, 0].double().cpu(), want)
+    assert sum(int(torch.count_nonzero(got[i:i + (1 << 28)])) for i in range(0, rows, 1 << 28)) == named.numel()
+    to = torch.ones((rows, 1), dtype=torch.bfloat16, device="cuda")
+    ops.embed_rows_gradient(grad, tokens, rows, add_to=to)
+    assert torch.equal(to[named, 0].double().cpu(), want + 1)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_bias_of_many_classes(dtype):
+    n, f, k = 6, 8, (1 << 26) + 1000
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.rand((n, f), generator=gen, device="cuda").to(TYPES[dtype])
+    w = (torch.randn((k, f), generator=gen, device="cuda") * 0.3).to(TYPES[dtype])
+    y = torch.randint(0, k, (n,), generator=gen, device="cuda")
+    bias = torch.randn(k, generator=gen, device="cuda")
+    y[0], y[1] = k - 1, 0
+    loss, _, _, gb = ops.linear_log_loss_gradient(x, w, y, bias=bias)
+    alone = ops.linear_log_loss(x, w, y, bias=bias)
+    want, off, sizes = (torch.zeros(k, dtype=torch.float64, device="cuda") for _ in range(3))
+    for r in range(n):  # as reference_by_rows, loss and grad_bias alone
+        s, size = bias.double(), bias.double().abs()
+        for i in range(f):
+            s, size = s + x[r, i].double() * w[:, i].double(), size + x[r, i].double().abs() * w[:, i].double().abs()
+        rel = float(2 * ((f + 8) * U + 2.0 ** -22) * size.max() + 1e-4)
+        lse = torch.logsumexp(s, dim=0)
+        assert abs(float(lse - s[y[r]] - loss[r])) <= rel + 8 * U * (abs(float(lse)) + 1.0)
+        assert abs(float(lse - s[y[r]] - alone[r])) <= rel + 8 * U * (abs(float(lse)) + 1.0)
+        p = torch.exp(s - lse)
+        off += p * rel
+        p[y[r]] -= 1.0
+        want += p
+        sizes += p.abs()
+    assert_within(gb, want, off + (n + 68) * U * sizes + want.abs() * U, "grad_bias")

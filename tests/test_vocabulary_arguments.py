@@ -147,3 +147,13 @@ def test_workspaces_of_many_rows():
             # G and its exponentials, the tops and totals, X in planes twice and the sums of its gradient, and those of grad_weight
             weights = 4 * 131072 * 1024
             assert q(4000000, 1024, 131072, dtype, gradient) < (4 << 30) + (1 << 31) + 2 * (2 << 30) + (4 << 30) + (1 << 29) + weights
+
+
+def test_the_largest_shapes():
+    q, e = L.lbt_linear_log_loss_workspace_bytes, L.lbt_embed_rows_gradient_workspace_bytes
+    for most, size in ((1 << 30, lambda v: q(v, 1, 1, _lib.LBT_BF16, 0)), ((1 << 30) - 64, lambda v: q(1, 1, v, _lib.LBT_BF16, 0)),
+                       (1 << 20, lambda v: q(1, v, 1, _lib.LBT_BF16, 0)), (1 << 30, lambda v: e(v, 1, 1, _lib.LBT_BF16)),
+                       ((1 << 30) - 64, lambda v: e(1, 1, v, _lib.LBT_BF16)), (1 << 24, lambda v: e(1, v, 1, _lib.LBT_BF16))):
+        assert size(most) > 0 and size(most + 1) == 0
+    assert loss(k=(1 << 30) - 63) == -1 and b"shape" in L.lbt_last_error()
+    assert L.lbt_embed_rows(None, AT, _lib.LBT_BF16, (1 << 30) - 63, 1, Y, 8, 5, 1.0, OUT) == -1 and b"shape" in L.lbt_last_error()
