@@ -628,6 +628,16 @@ __global__ void __launch_bounds__(kBoostThreads) feature_mask_kernel(MaskBits bi
 
 inline unsigned grid_for(int64_t n) { return static_cast<unsigned>((n + kBoostThreads - 1) / kBoostThreads); }
 
+// part(first, rows) for as many rows at a time, of `width` entries each, as a launch with a thread for each entry may have.
+constexpr int64_t kMostEntries = int64_t(1) << 31;
+template <class Part>
+int by_parts(int64_t n_rows, int64_t width, const Part& part)
+{
+  const int64_t most = std::max<int64_t>(kMostEntries / width, 1);
+  for (int64_t first = 0; first < n_rows; first += most) LBT_TRY(part(first, std::min(most, n_rows - first)));
+  return LBT_OK;
+}
+
 }  // namespace lbt
 
 extern "C" {
@@ -647,10 +657,21 @@ static int form_gradients(hipStream_t s, int32_t objective, const lbt::LeafAdd& 
   double* sum_g = abs_sum_chunks;
   double* sum_h = abs_sum_chunks != nullptr ? abs_sum_chunks + m : nullptr;
   const bool elementwise = objective == LBT_OBJ_SQUARED_ERROR || n_outputs == 1;
+  if (abs_sum_chunks == nullptr && n > lbt::kMostEntries)
+    return lbt::by_parts(n_rows, n_outputs, [&](int64_t first, int64_t rows) {
+      const int64_t at = first * n_outputs;
+      return form_gradients(s, objective, lbt::LeafAdd{add.leaf, add.n_nodes, add.leaf != nullptr ? add.row_leaf + first : nullptr}, pred + at,
+                            y + (elementwise ? at : first), sample_weight != nullptr ? sample_weight + first : nullptr, learning_rate, rows, n_outputs,
+                            g + at, h + at, nullptr);
+    });
   if (add.leaf != nullptr && !elementwise) {
     // a row's maximum needs all of its predictions
     lbt::ProfScope ps(LBT_PROF_OTHER, s, static_cast<double>(n) * 16.0 + static_cast<double>(n_rows) * 4.0);
-    lbt::add_leaf_values_kernel<<<lbt::grid_for(n), lbt::kBoostThreads, 0, s>>>(add.leaf, add.n_nodes, add.row_leaf, n, n_outputs, pred);
+    LBT_TRY(lbt::by_parts(n_rows, n_outputs, [&](int64_t first, int64_t rows) {
+      lbt::add_leaf_values_kernel<<<lbt::grid_for(rows * n_outputs), lbt::kBoostThreads, 0, s>>>(add.leaf, add.n_nodes, add.row_leaf + first,
+                                                                                               rows * n_outputs, n_outputs, pred + first * n_outputs);
+      return LBT_OK;
+    }));
   }
   lbt::ProfScope ps(LBT_PROF_OTHER, s, static_cast<double>(n) * (add.leaf != nullptr && elementwise ? 44.0 : 32.0));
   if (elementwise) {
@@ -836,9 +857,12 @@ int lbt_keep_rows(void* stream, const double* draw, double limit, int64_t n_rows
   hipStream_t s   = static_cast<hipStream_t>(stream);
   const int64_t n = n_rows * n_outputs;
   lbt::ProfScope ps(LBT_PROF_OTHER, s, static_cast<double>(n) * 8.0);
-  lbt::keep_rows_kernel<<<lbt::grid_for(n), lbt::kBoostThreads, 0, s>>>(draw, limit, n, n_outputs, g, h);
-  LBT_HIP(hipGetLastError());
-  return LBT_OK;
+  return lbt::by_parts(n_rows, n_outputs, [&](int64_t first, int64_t rows) {
+    lbt::keep_rows_kernel<<<lbt::grid_for(rows * n_outputs), lbt::kBoostThreads, 0, s>>>(draw + first, limit, rows * n_outputs, n_outputs,
+                                                                                         g + first * n_outputs, h + first * n_outputs);
+    LBT_HIP(hipGetLastError());
+    return LBT_OK;
+  });
 }
 
 int lbt_feature_mask(void* stream, const uint8_t* host_mask, int32_t n_features, uint8_t* feature_set)
@@ -870,6 +894,10 @@ int lbt_class_probabilities(void* stream, const double* raw, const double* init,
   const bool binary = n_outputs == 1;
   LBT_REQUIRE(raw != out, "the output may not alias the input");
   LBT_REQUIRE(!binary || reinterpret_cast<uintptr_t>(out) % 16 == 0, "the output must be 16-byte aligned: a row's two probabilities are stored together");
+  if (n > lbt::kMostEntries)
+    return lbt::by_parts(n_rows, n_outputs, [&](int64_t first, int64_t rows) {
+      return lbt_class_probabilities(stream, raw + first * n_outputs, init, rows, n_outputs, out + first * (binary ? 2 : n_outputs));
+    });
   lbt::ProfScope ps(LBT_PROF_OTHER, s, static_cast<double>(n) * (binary ? 24.0 : 16.0));
   if (binary) {
     lbt::two_class_probabilities_kernel<<<lbt::grid_for(n), lbt::kBoostThreads, 0, s>>>(raw, init, n, out);
@@ -919,10 +947,12 @@ int lbt_add_leaf_values(void* stream, const double* leaf_value, int32_t n_nodes,
   hipStream_t s   = static_cast<hipStream_t>(stream);
   const int64_t n = n_rows * n_outputs;
   lbt::ProfScope ps(LBT_PROF_OTHER, s, static_cast<double>(n) * 16.0 + static_cast<double>(n_rows) * 4.0);
-  lbt::add_leaf_values_kernel<<<lbt::grid_for(n), lbt::kBoostThreads, 0, s>>>(leaf_value, n_nodes, row_leaf, n,
-                                                                              n_outputs, pred);
-  LBT_HIP(hipGetLastError());
-  return LBT_OK;
+  return lbt::by_parts(n_rows, n_outputs, [&](int64_t first, int64_t rows) {
+    lbt::add_leaf_values_kernel<<<lbt::grid_for(rows * n_outputs), lbt::kBoostThreads, 0, s>>>(leaf_value, n_nodes, row_leaf + first, rows * n_outputs,
+                                                                                             n_outputs, pred + first * n_outputs);
+    LBT_HIP(hipGetLastError());
+    return LBT_OK;
+  });
 }
 
 int lbt_gather_rows(void* stream, const void* X, int32_t x_dtype, int64_t row_offset, int64_t n_rows,
@@ -942,16 +972,18 @@ int lbt_gather_rows(void* stream, const void* X, int32_t x_dtype, int64_t row_of
     LBT_HIP(hipMemcpyAsync(staging, sample_rows, sizeof(int64_t) * n_samples, hipMemcpyHostToDevice, s));
     rows = staging;
   }
-  const int64_t n = n_samples * n_features;
   lbt::ProfScope ps(LBT_PROF_OTHER, s);
-  if (x_dtype == LBT_F32)
-    lbt::gather_rows_kernel<float><<<lbt::grid_for(n), lbt::kBoostThreads, 0, s>>>(
-      static_cast<const float*>(X), row_offset, n_rows, n_features, rows, n, static_cast<float*>(out));
-  else
-    lbt::gather_rows_kernel<double><<<lbt::grid_for(n), lbt::kBoostThreads, 0, s>>>(
-      static_cast<const double*>(X), row_offset, n_rows, n_features, rows, n, static_cast<double*>(out));
-  LBT_HIP(hipGetLastError());
-  return LBT_OK;
+  return lbt::by_parts(n_samples, n_features, [&](int64_t first, int64_t some) {
+    const int64_t n = some * n_features, at = first * n_features;
+    if (x_dtype == LBT_F32)
+      lbt::gather_rows_kernel<float><<<lbt::grid_for(n), lbt::kBoostThreads, 0, s>>>(static_cast<const float*>(X), row_offset, n_rows, n_features,
+                                                                                     rows + first, n, static_cast<float*>(out) + at);
+    else
+      lbt::gather_rows_kernel<double><<<lbt::grid_for(n), lbt::kBoostThreads, 0, s>>>(static_cast<const double*>(X), row_offset, n_rows, n_features,
+                                                                                      rows + first, n, static_cast<double*>(out) + at);
+    LBT_HIP(hipGetLastError());
+    return LBT_OK;
+  });
 }
 
 }  // extern "C"
