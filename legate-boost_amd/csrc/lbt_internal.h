@@ -45,7 +45,7 @@ void set_error(const char* fmt, ...);
 // Workgroups that a launch may have along x: the runtime takes their threads modulo 2^32, and runs that many without an error.
 constexpr int64_t most_groups(int threads) { return (int64_t(1) << 32) / threads - 1; }
 
-// What a call reads or writes; null: nothing.
+// What a call reads or writes; null, or no bytes: nothing.
 struct MemoryRange {
   const void* begin;
   int64_t bytes;
@@ -56,7 +56,7 @@ inline bool ranges_apart(const MemoryRange* ranges, int written, int all)
   for (int i = 0; i < written; i++)
     for (int j = i + 1; j < all; j++) {
       const char *a = static_cast<const char*>(ranges[i].begin), *b = static_cast<const char*>(ranges[j].begin);
-      if (a != nullptr && b != nullptr && a < b + ranges[j].bytes && b < a + ranges[i].bytes) return false;
+      if (a != nullptr && b != nullptr && ranges[i].bytes > 0 && ranges[j].bytes > 0 && a < b + ranges[j].bytes && b < a + ranges[i].bytes) return false;
     }
   return true;
 }

@@ -157,3 +157,12 @@ def test_the_largest_shapes():
         assert size(most) > 0 and size(most + 1) == 0
     assert loss(k=(1 << 30) - 63) == -1 and b"shape" in L.lbt_last_error()
     assert L.lbt_embed_rows(None, AT, _lib.LBT_BF16, (1 << 30) - 63, 1, Y, 8, 5, 1.0, OUT) == -1 and b"shape" in L.lbt_last_error()
+
+
+def test_nothing_overlaps_an_empty_array():
+    """No rows, no tokens: their addresses are not looked at, wherever they point. The next check, that of the workspace, is reached."""
+    assert gradient(n=0, X=inside(GW), gx=inside(W), y=inside(GW, 32), out=inside(W, 48), w=inside(GW, 64)) == -3
+    assert b"workspace" in L.lbt_last_error()
+    grad = L.lbt_embed_rows_gradient
+    assert grad(None, inside(OUT), _lib.LBT_F32, inside(OUT, 64), 8, 0, 8, 10, 1.0, 0, OUT, None, 0) == -3
+    assert b"workspace" in L.lbt_last_error()
