@@ -466,7 +466,7 @@ int narrow_type(const at::Tensor& t, int64_t device)
 // Bytes of a token of a dense, contiguous tensor on device `device`; 0: something else
 int token_bytes(const at::Tensor& t, int64_t device)
 {
-  if (!t.defined() || t.layout() != at::kStrided || !t.is_cuda() || t.get_device() != device || !t.is_contiguous()) return 0;
+  if (!t.defined() || t.layout() != at::kStrided || !t.is_cuda() || t.get_device() != device || !t.is_contiguous() || t.is_neg()) return 0;
   return t.scalar_type() == at::kLong ? 8 : t.scalar_type() == at::kInt ? 4 : 0;
 }
 
@@ -475,8 +475,8 @@ const at::Tensor* numbers_of(PyObject* o, at::ScalarType type, int64_t n, int64_
 {
   if (!THPVariable_CheckExact(o)) return nullptr;
   const at::Tensor& t = THPVariable_Unpack(o);
-  if (!t.defined() || t.layout() != at::kStrided || !t.is_cuda() || t.get_device() != device || !t.is_contiguous() || t.scalar_type() != type ||
-      t.numel() != n)
+  if (!t.defined() || t.layout() != at::kStrided || !t.is_cuda() || t.get_device() != device || !t.is_contiguous() || t.is_neg() ||
+      t.scalar_type() != type || t.numel() != n)
     return nullptr;
   return &t;
 }

@@ -31,6 +31,8 @@ def as_device(a, dtype=None):
         t = t.to(dtype)
     if not t.is_cuda:
         t = t.cuda()
+    if t.is_neg():  # (the memory holds the negated values)
+        t = t.resolve_neg()
     return t.contiguous()
 
 
@@ -741,7 +743,8 @@ def embed_rows_gradient(grad, tokens, n_rows, scale=1.0, add_to=None):
     f, n_rows, dt = grad.shape[-1], int(n_rows), _DT_NARROW[grad.dtype]
     out = add_to
     if add_to is not None and not (isinstance(add_to, torch.Tensor) and add_to.shape == (n_rows, f) and add_to.dtype == grad.dtype
-                                   and add_to.device == grad.device and add_to.is_contiguous() and add_to.data_ptr() % 16 == 0):
+                                   and add_to.device == grad.device and add_to.is_contiguous() and not add_to.is_neg()
+                                   and add_to.data_ptr() % 16 == 0):
         raise _lib.LbtError("add_to must be a contiguous, 16-byte aligned [%d, %d] tensor of %s beside grad" % (n_rows, f, grad.dtype))
     with _On(grad.device):
         if out is None:
