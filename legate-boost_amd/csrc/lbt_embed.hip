@@ -250,7 +250,7 @@ __device__ __forceinline__ int digit_offset(const int32_t* __restrict__ counts, 
   return at;
 }
 
-// A wave takes 256 consecutive entries, 64 at a time: the lanes of equal digits find one another by ballots, the first of
+// A wave takes 64 * kSortEach consecutive entries, 64 at a time: the lanes of equal digits find one another by ballots, the first of
 // them moves the wave's count on. Ranks are then the block's offset, the waves before, and the place in the wave: stable.
 template <int kSortEach>
 __global__ void __launch_bounds__(kSortThreads)

@@ -10,9 +10,10 @@
 // lane, so the loop has no edges. The LDS holds 16-byte chunks in an order (an exclusive or with the row's number) in which
 // the 32 rows that a fragment reads lie on all banks.
 //
-// A large product of 16 bits runs at 1210 to 1310 TFLOP/s, where the card's library reaches 1240: the matrix cores are busy 57 to 63 % of
-// the cycles and the clock is at 1.85 GHz then, which is what bounds both. Measured and not better: stages of 32 of k four and five deep, waves
-// of 128 x 128, waves of raised priority.
+// A large product of 16 bits runs at 1210 to 1310 TFLOP/s, where the card's library reaches 1239 to 1304 by its size (8192 x 16384 x 4096 and
+// 8192^3). The matrix cores are busy 57 to 63 % of the cycles and the clock is at 1.85 GHz then, for the library's products too: most
+// likely the card's limit of power, which was not measured. Measured
+// and not better: stages of 32 of k four and five deep, waves of 128 x 128, waves of raised priority.
 //
 // float operands are sums of three bfloat16 planes (8 + 8 + 8 significant bits, exact); of the nine products of planes the
 // six that reach above 2^-24 of the result are added up, one walk over k each. (The scores, and grad_X of few rows, whose
@@ -42,7 +43,7 @@ struct ProductOperand {
   int32_t cols;
 };
 
-// What the rows of a call come down to; written on the device by prepare_rows_kernel.
+// What the rows of a call come down to; written on the device by prepare_rows_kernel or prepare_pack_kernel.
 struct RowCounts {
   int32_t rows;      // rows that count
   int32_t exponent;  // the largest exponent of a row's weight (half precision)

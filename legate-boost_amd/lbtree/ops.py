@@ -671,7 +671,8 @@ def linear_log_loss(X, weight, y, bias=None):
 def linear_log_loss_gradient(X, weight, y, sample_weight=None, bias=None):
     """linear_log_loss with the gradients of sum_r sample_weight[r] * loss[r]: (loss, grad_X, grad_weight), and grad_bias (float32)
     behind them where a bias is given. grad_X and grad_weight have the types of X and weight. sample_weight: [n_rows], all ones
-    where it is not given (1 / n_rows makes it the mean); the loss that is returned is not weighted."""
+    where it is not given (1 / n_rows makes it the mean); the loss that is returned is not weighted. The sums are float32, the entries
+    w (p - [c = y]) that they are of have X's type. The scratch holds these for up to 4 GiB of rows and classes (release_workspace)."""
     if _NATIVE is not None and torch.cuda.is_initialized():
         device = torch.cuda.current_device()
         got = _NATIVE.linear_log_loss_gradient(X, weight, y, bias, _scratch, _LOG_LOSS_GRADIENT, _LOG_LOSS_BYTES, _raw_stream(device), device,
@@ -707,7 +708,7 @@ def _tokens(tokens, device):
 def embed_rows(table, tokens, scale=1.0):
     """scale * table[tokens] for whole numbers `tokens` of any shape: [*tokens.shape, n_features] of the table's type (float32,
     bfloat16 or float16), multiplied in float32 and rounded once. A token that is no row of the table gives zeros. tokens may be
-    a tree's row_leaf (build_tree(row_leaf=True))."""
+    a tree's row_leaf (build_tree(row_leaf=True)). No autograd graph is recorded: embed_rows_gradient returns the gradient."""
     if _NATIVE is not None and torch.cuda.is_initialized():
         device = torch.cuda.current_device()
         got = _NATIVE.embed_rows(table, tokens, _EMBED, _raw_stream(device), device, scale)
@@ -728,7 +729,7 @@ def embed_rows_gradient(grad, tokens, n_rows, scale=1.0, add_to=None):
     """The gradient of embed_rows with respect to its table of n_rows rows: row v is scale times the sum of grad[t] over the t with
     tokens[t] = v, in float32 and in a fixed order. grad: [*tokens.shape, n_features]. add_to: a contiguous [n_rows, n_features]
     tensor of grad's type that the sums are added to in place, and which is returned, instead of a new one (a table that is also
-    the weight of linear_log_loss_gradient)."""
+    the weight of linear_log_loss_gradient): the sum of both is rounded to that type once more. No autograd graph is recorded."""
     if _NATIVE is not None and add_to is None and torch.cuda.is_initialized():
         device = torch.cuda.current_device()
         got = _NATIVE.embed_rows_gradient(grad, tokens, _scratch, _EMBED_GRADIENT, _EMBED_BYTES, _raw_stream(device), device, n_rows, scale)
