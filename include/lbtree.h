@@ -538,8 +538,8 @@ int lbt_gather_rows(void* stream, const void* X, int32_t x_dtype, int64_t row_of
  * Log loss of linear scores over many classes (a vocabulary), where lbt_weighted_gradient takes the scores themselves:
  *   s[r][c] = <X[r], weight[c]> + bias[c];   loss[r] = log sum_c exp(s[r][c]) - s[r][y[r]]
  * The scores are formed in tiles of rows and classes and never written (the gradient below holds a piece of them). Sums, tops and totals are held in 32 bits; LBT_F32
- * inputs are multiplied as three planes of bfloat16 each, which gives products as exact as those of float (an infinity among
- * the values of a row that counts, or of the weights, may come out as NaN).
+ * inputs are multiplied as three planes of bfloat16 each, which gives products as exact as those of float (but values below
+ * 2^-110 lose their last bits, and an infinity among the values of a row that counts, or of the weights, may come out as NaN).
  *   X       device [n_rows][n_features], dtype LBT_F32, LBT_BF16 or LBT_F16, 16-byte aligned
  *   weight  device [n_outputs][n_features], the same dtype, 16-byte aligned
  *   bias    device float [n_outputs], or NULL. A class whose bias is -inf takes no part (p = 0; a row with that label has an
@@ -564,7 +564,7 @@ int lbt_linear_log_loss(void* stream, const void* X, const void* weight, int32_t
  *   grad_X = G weight,  grad_weight = G^T X,  grad_bias[c] = sum_r G[r][c]
  * G is formed for a piece of the classes at a time, in the inputs' type (LBT_F16: times a power of two; LBT_F32: three planes of
  * bfloat16), and multiplied both ways with sums in 32 bits: an entry is off by half a step of that type, and for LBT_BF16 without
- * grad_bias by 2^-11 of p more. It is held together with the exponentials that it is made of, 2 to 16 bytes a row and class. A piece's share of the workspace is at most 4 GiB, whatever the
+ * grad_bias by 2^-11 of p more (down to 2^-62 of a row's largest p among 128 classes). It is held together with the exponentials that it is made of, 2 to 16 bytes a row and class. A piece's share of the workspace is at most 4 GiB, whatever the
  * vocabulary and the rows; classes that are one piece have their scores formed once, those of more pieces twice. Rows are taken in parts
  * of at most 131072 (fewer beyond 131072 classes, or where a row's planes are more than 8192 values): the workspace of more rows
  * is that of one part, and the sums of grad_weight in float beside it.

@@ -16,7 +16,7 @@
 //
 // What is rounded to fewer than 32 bits: an entry of G, to the type of the products (float: three planes, nothing lost above 2^-24 of
 // it), as products of two 16-bit types are all that the matrix cores do at full rate; sums stay in float. In bfloat16 without the
-// gradient of a bias u is held as half before that, 2^-11 of it beside the 2^-8 of G's own rounding. Against 64 bits the gradients
+// gradient of a bias u is held in 16 bits before that, 2^-11 of it beside the 2^-8 of G's own rounding. Against 64 bits the gradients
 // are off 1.1 to 1.5 times as far as those of the same formulas in float, whose only such rounding is that of the result (in the norm,
 // relative: 4096 rows, 32768 classes of 2048 bfloat16 0.0023 and 0.0017, 1531 rows of half precision 0.00029 and 0.00021). To hold G
 // in two planes would cost two products more. Losses, sums of the bias and all results of float are as exact as those or more so.
@@ -502,11 +502,26 @@ __device__ __forceinline__ void turn_rows(char* lds, int wave, int lane, Value v
 }
 
 // The shares of the rows' tops and totals: one of each row for the kWM classes of a wave. For scale_kernel also
-// u = exp(s - the share's top), [rows][piece]: as float, or, for G in bfloat16, as half times 2^15. Half is off by at most 2^-11 where
-// bfloat16 is by 2^-8 afterwards, and has all its bits down to 2^-29 of the top. (3687 rows, 32768 classes of 2048 bfloat16: 83 us for
-// G from halves, where a second product takes 450.)
-enum { kNotKept = 0, kKeptHalf = 1, kKeptFloat = 2 };
-constexpr float kKeptScale = 32768.f;
+// u = exp(s - the share's top), [rows][piece]: as float, or, for G in bfloat16, in 16 bits: 6 of its exponent and 10 of its significand, as
+// it has no sign. That is off by at most 2^-11 where bfloat16 is by 2^-8 afterwards, down to 2^-62 of the top (half precision keeps its
+// bits down to 2^-29: a row's small probabilities were off by more than its roundings). A float times 2^-64 has zeros above these 16
+// bits, which then are a shift and an addition away. (3687 rows, 32768 classes of 2048 bfloat16: 83 us for G from them, where a
+// second product takes 450.)
+enum { kNotKept = 0, kKeptShort = 1, kKeptFloat = 2 };
+constexpr float kKeptScale = 0x1p-64f;
+__device__ __forceinline__ uint2 shorten_four(const float (&u)[4])
+{
+  uint32_t r[4];
+#pragma unroll
+  for (int e = 0; e < 4; e++) r[e] = (__builtin_bit_cast(uint32_t, u[e] * kKeptScale) << 3) + 0x8000u;  // rounded in the upper half
+  return make_uint2(__builtin_amdgcn_perm(r[1], r[0], 0x07060302u), __builtin_amdgcn_perm(r[3], r[2], 0x07060302u));
+}
+// Two of them, times kKeptScale still.
+__device__ __forceinline__ void widen_two(uint32_t w, float& first, float& second)
+{
+  first  = __builtin_bit_cast(float, (w << 13) & 0x1fffe000u);
+  second = __builtin_bit_cast(float, (w >> 3) & 0x1fffe000u);
+}
 template <bool kExact, int kKeep>
 struct LossEpilogue {
   const float* bias;
@@ -562,10 +577,9 @@ struct LossEpilogue {
               u[e] = exp_of(acc[i][j][q * 4 + e] - from, kExact);
               total += u[e];
               v[e] = u[e];
-              if (kKeep == kKeptHalf) u[e] *= kKeptScale;
             }
-            if constexpr (kKeep == kKeptHalf) {
-              const uint2 w = narrow_four<LBT_F16>(u);
+            if constexpr (kKeep == kKeptShort) {
+              const uint2 w = shorten_four(u);
               __builtin_memcpy(v, &w, 8);
             }
           },
@@ -999,9 +1013,7 @@ __global__ void __launch_bounds__(kWaves * 64, 3)
         if constexpr (kKeep == kKeptFloat) {
           *reinterpret_cast<float4*>(static_cast<float*>(args.kept) + at) = make_float4(u[0], u[1], u[2], u[3]);
         } else {
-#pragma unroll
-          for (int e = 0; e < 4; e++) u[e] *= kKeptScale;
-          store_four<LBT_F16>(args.kept, at, u, 4);
+          *reinterpret_cast<uint2*>(static_cast<uint16_t*>(args.kept) + at) = shorten_four(u);
         }
       }
       total += __shfl_xor(total, 16);
@@ -1082,7 +1094,7 @@ __global__ void __launch_bounds__(kFewThreads)
 // 1000 classes of 256 floats: 30.5 us in all, 32.7 with the launch, 42.3 by 16 rows; 4096 rows, 32768 classes of 256 bfloat16: 444 us,
 // 488 by 4 rows.)
 constexpr int kScaleClasses = 2048;
-template <int kDtype, bool kKeptAsHalf, int kRows>
+template <int kDtype, bool kKeptAsShort, int kRows>
 __global__ void __launch_bounds__(256)
   scale_kernel(const void* kept, const float2* __restrict__ partial, int share_classes, int64_t share_step, int64_t row_step, int row_tile, LossRows rows,
                const RowCounts* __restrict__ counts, int n_classes, int piece, int64_t plane, uint16_t* g, uint16_t* g_blocks, int64_t padded, float* bias_sums,
@@ -1129,7 +1141,9 @@ __global__ void __launch_bounds__(256)
     float f           = 0.f;
     if (row < counted && class0 + s * share_classes < piece) {
       const float top = partial[(first + s) * share_step + row * row_step].x;
-      f = top == -INFINITY ? 0.f : exp_of(top - row_top[i % kRows], kDtype == LBT_F32) * row_inverse[i % kRows] * (kKeptAsHalf ? 1.f / kKeptScale : 1.f);
+      // (a row that holds NaN has it in its total, not in 16 bits: the factor is NaN, where all of a share's classes are masked, too)
+      const float p = top == -INFINITY ? 0.f : exp_of(top - row_top[i % kRows], kDtype == LBT_F32);
+      f = p * row_inverse[i % kRows] * (kKeptAsShort ? 1.f / kKeptScale : 1.f);
     }
     factor[i % kRows][s] = f;
   }
@@ -1146,10 +1160,12 @@ __global__ void __launch_bounds__(256)
     const float w   = rows.factor[row];
     const int label = rows.label[row] - c;
     float u[8];
-    if constexpr (kKeptAsHalf) {
-      const Half8 h = *reinterpret_cast<const Half8*>(static_cast<const uint16_t*>(kept) + at);
-#pragma unroll
-      for (int e = 0; e < 8; e++) u[e] = static_cast<float>(h[e]);
+    if constexpr (kKeptAsShort) {
+      const uint4 h = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(kept) + at);
+      widen_two(h.x, u[0], u[1]);
+      widen_two(h.y, u[2], u[3]);
+      widen_two(h.z, u[4], u[5]);
+      widen_two(h.w, u[6], u[7]);
     } else {
       const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(kept) + at);
       const float4 a = q[0], b = q[1];
@@ -1448,7 +1464,7 @@ struct LossCall {
     packed = type == LBT_F32 ? gradient && !floats_back : f % 8 != 0;
     // a piece's G and its packed weights within their bounds; pieces of one size
     int64_t most = round_up(k, 256);
-    kept                = type == LBT_BF16 && !with_bias ? kKeptHalf : kKeptFloat;  // (the sums for the bias are those of floats)
+    kept                = type == LBT_BF16 && !with_bias ? kKeptShort : kKeptFloat;  // (the sums for the bias are those of floats)
     const int64_t bytes = 2 * planes + (kept == kKeptFloat ? 4 : 0);                // of an entry of G
     if (gradient) most = std::min(most, kScoresBytes / (bytes * padded) / 256 * 256);
     if (packed) most = std::min(most, kPieceBytes / (2 * planes * int64_t(cols)) / 256 * 256);
@@ -1630,7 +1646,7 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
                           c.rows.order, c.rows.label, c.counts, c.kept == kKeptFloat ? static_cast<void*>(c.exps) : c.g,
                           static_cast<int>(c.piece)};
     if constexpr (kDtype == LBT_BF16)
-      LBT_TRY((c.kept == kKeptHalf ? launch_few<kDtype, kKeptHalf>(s, few, c.piece, true) : launch_few<kDtype, kKeptFloat>(s, few, c.piece, true)));
+      LBT_TRY((c.kept == kKeptShort ? launch_few<kDtype, kKeptShort>(s, few, c.piece, true) : launch_few<kDtype, kKeptFloat>(s, few, c.piece, true)));
     else
       LBT_TRY((launch_few<kDtype, kKeptFloat>(s, few, c.piece, true)));
   }
@@ -1657,8 +1673,8 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
       }
     };
     if constexpr (kDtype == LBT_BF16)
-      if (c.kept == kKeptHalf) {
-        LBT_TRY(scores(std::integral_constant<int, kKeptHalf>{}));
+      if (c.kept == kKeptShort) {
+        LBT_TRY(scores(std::integral_constant<int, kKeptShort>{}));
         continue;
       }
     LBT_TRY(c.kept == kNotKept ? scores(std::integral_constant<int, kNotKept>{}) : scores(std::integral_constant<int, kKeptFloat>{}));
@@ -1689,19 +1705,19 @@ int linear_log_loss(hipStream_t s, const LossCall& c, const void* X, const void*
     if (first > 0 || !laid_out) LBT_TRY(lay_out(first));
     const ProductOperand w = weights(first, classes);
     if (c.kept != kNotKept) {
-      auto scale = [&](auto half, auto each) {
+      auto scale = [&](auto narrow, auto each) {
         constexpr int kRows = decltype(each)::value;
-        scale_kernel<kDtype, decltype(half)::value, kRows>
+        scale_kernel<kDtype, decltype(narrow)::value, kRows>
           <<<static_cast<unsigned>(tiles_of(c.piece, kScaleClasses) * tiles_of(c.padded, kRows)), 256, 0, s>>>(
-            decltype(half)::value ? static_cast<const void*>(c.g) : c.exps, c.partial, share_classes, c.few ? 1 : c.padded, c.few ? shares : 1, std::max(c.row_product.tile, kProductK), c.rows, c.counts,
+            decltype(narrow)::value ? static_cast<const void*>(c.g) : c.exps, c.partial, share_classes, c.few ? 1 : c.padded, c.few ? shares : 1, std::max(c.row_product.tile, kProductK), c.rows, c.counts,
             c.classes, static_cast<int>(c.piece), c.padded * c.piece, c.g, c.g_blocks, c.padded, grad_bias != nullptr ? c.bias_sums : nullptr, join_here, loss);
       };
-      auto scale_by = [&](auto half) {
-        if (c.scale_rows == 16) scale(half, std::integral_constant<int, 16>{});
-        else scale(half, std::integral_constant<int, 4>{});
+      auto scale_by = [&](auto narrow) {
+        if (c.scale_rows == 16) scale(narrow, std::integral_constant<int, 16>{});
+        else scale(narrow, std::integral_constant<int, 4>{});
       };
       if constexpr (kDtype == LBT_BF16) {
-        if (c.kept == kKeptHalf) scale_by(std::true_type{});
+        if (c.kept == kKeptShort) scale_by(std::true_type{});
         else scale_by(std::false_type{});
       } else {
         scale_by(std::false_type{});

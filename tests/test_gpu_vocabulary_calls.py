@@ -1,5 +1,4 @@
-"""Calls of the operators for vocabularies that tensors of other kinds make: negated views, inputs on the host."""
-import numpy as np
+"""Calls of the operators for vocabularies with tensors and values of other kinds: negated views, probabilities far apart."""
 import pytest
 import torch
 
@@ -36,3 +35,30 @@ def test_negated_views(native, monkeypatch):
     # what is written in place is refused
     with pytest.raises(_lib.LbtError):
         ops.embed_rows_gradient(x, y, 60, add_to=neg(torch.zeros((60, 24), device="cuda")))
+
+
+@pytest.mark.parametrize("n,f,k", [(1, 8, 20), (5, 40, 3000), (40, 16, 9000), (300, 64, 700), (1100, 30, 5000)])
+def test_small_probabilities_keep_their_bits(n, f, k):
+    """bfloat16 without a bias holds exponentials in 16 bits before G: 11 significant bits of them, down to 2^-62 of the largest beside
+    them. Scores of which one leads by up to 40 (2^-58): each entry of grad_weight, of one row that counts, is p x within half a step of 11
+    bits (2^-11), of G (2^-8) and of the result (2^-8), and what the score is off by (`rel` below, as in test_gpu_vocabulary.reference)."""
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    x = torch.rand((n, f), generator=gen, device="cuda").add_(0.5).to(torch.bfloat16)
+    w = (torch.randn((k, f), generator=gen, device="cuda") * 0.1).to(torch.bfloat16)
+    y = torch.full((n,), -1, dtype=torch.int64, device="cuda")
+    at = n // 2
+    y[at] = 3
+    # the first feature lifts the label's score, and lowers the others' by up to 38
+    w[:, 0] = -torch.linspace(0, 24, k, device="cuda")[torch.randperm(k, generator=gen, device="cuda")].to(torch.bfloat16)
+    w[3, 0] = 2.0
+    x[at, 0] = 1.5
+    loss, gx, gw = ops.linear_log_loss_gradient(x, w, y)
+    X, W = x[at].double(), w.double()
+    s = W @ X
+    p = torch.exp(s - torch.logsumexp(s, 0))
+    assert 2.0 ** -62 < float(p.min()) < 2.0 ** -45
+    rest = torch.arange(k, device="cuda") != 3
+    want = p[rest, None] * X[None, :]
+    rel = float(2 * ((f + 8) * 2.0 ** -24 + 2.0 ** -22) * (W.abs() @ X.abs()).max() + 1e-4)
+    bound = (2.0 ** -11 + 2 * 2.0 ** -8 + rel) * (1 + 2.0 ** -6)
+    assert ((gw[rest].double() - want).abs() <= bound * want).all()

@@ -37,7 +37,7 @@ def reference_by_rows(x, w, y, bias, weight, t, step):
         wt = torch.ones(rows.numel(), **kinds) if weight is None else weight.double()[rows]
         g = g * wt[:, None]
         off = g.abs() * 4 * U + p * rel[:, None] * wt.abs()[:, None]
-        # an entry of G is rounded once; where bfloat16 has no bias the exponential is held as half before, half a step of which is 2^-11
+        # an entry of G is rounded once; where bfloat16 has no bias the exponential is held in 11 bits before, half a step of which is 2^-11
         entry = off + g.abs() * (ENTRY[t] + (2.0 ** -11 if t == "bf16" and bias is None else 0.0))
         gx[rows] = g @ W
         bx[rows] = (entry @ W.abs() + (k + 64) * U * (g.abs() @ W.abs())) * (1 + STEP[t]) + gx[rows].abs() * STEP[t] + LEAST[t]
