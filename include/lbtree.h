@@ -564,10 +564,11 @@ int lbt_linear_log_loss(void* stream, const void* X, const void* weight, int32_t
  *   grad_X = G weight,  grad_weight = G^T X,  grad_bias[c] = sum_r G[r][c]
  * G is formed for a piece of the classes at a time, in the inputs' type (LBT_F16: times a power of two; LBT_F32: three planes of
  * bfloat16), and multiplied both ways with sums in 32 bits: an entry is off by half a step of that type, and for LBT_BF16 without
- * grad_bias by 2^-11 of p more (down to 2^-62 of a row's largest p among 128 classes). It is held together with the exponentials that it is made of, 2 to 16 bytes a row and class. A piece's share of the workspace is at most 4 GiB, whatever the
- * vocabulary and the rows; classes that are one piece have their scores formed once, those of more pieces twice. Rows are taken in parts
- * of at most 131072 (fewer beyond 131072 classes, or where a row's planes are more than 8192 values): the workspace of more rows
- * is that of one part, and the sums of grad_weight in float beside it.
+ * grad_bias by 2^-11 of p more (down to 2^-62 of the largest p of the 16 to 128 classes beside it). It is held together with the
+ * exponentials that it is made of, 2 to 16 bytes a row and class. A piece's share of the workspace is at most 4 GiB, whatever the
+ * vocabulary and the rows; classes that are one piece have their scores formed once, those of more pieces twice. Rows are taken in
+ * parts of at most 131072 (fewer beyond 131072 classes, or where a row's planes are more than 8192 values): the workspace of more
+ * rows is that of one part, and the sums of grad_weight in float beside it.
  *   sample_weight  device float [n_rows], or NULL for ones
  *   grad_X, grad_weight  device, shape and dtype of X and weight, 16-byte aligned; overwritten (zeros for rows that do not count)
  *   grad_bias      device float [n_outputs], or NULL; only with a bias
