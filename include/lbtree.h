@@ -547,12 +547,15 @@ int lbt_gather_rows(void* stream, const void* X, int32_t x_dtype, int64_t row_of
  *   y       device int64 [n_rows]. A row whose label is not in [0, n_outputs) does not count: its loss is 0, nothing that
  *           it holds (NaN and infinities too) reaches any output
  *   loss    device float [n_rows]
- *   workspace  at least lbt_linear_log_loss_workspace_bytes(..., gradient = 0), 256-byte aligned. `gradient`: 0 for this
- *              call, 1 for lbt_linear_log_loss_gradient, 2 for that with grad_bias; 0 bytes for invalid arguments
- * Enqueues on the stream and does not wait. All results are the same from call to call. What is written (and the workspace) may
+ *   workspace  lbt_linear_log_loss_workspace_bytes(..., gradient = 0), 256-byte aligned. `gradient`: 0 for this
+ *              call, 1 for lbt_linear_log_loss_gradient, 2 for that with grad_bias; 0 bytes for invalid arguments.
+ *              With LBT_LEAST_WORKSPACE added, the least that is taken where there is no memory for that: classes go in smaller
+ *              pieces then, which takes longer and adds up in another order
+ * Enqueues on the stream and does not wait. All results are the same from call to call, workspaces of either size apart. What is written (and the workspace) may
  * not overlap what is read, or one another: LBT_ERR_INVALID, here and in the calls below. Up to 2^30 rows, 2^30 - 64 classes, 2^20
  * features and 2^38 values of X or weight.
  */
+#define LBT_LEAST_WORKSPACE 4
 size_t lbt_linear_log_loss_workspace_bytes(int64_t n_rows, int32_t n_features, int32_t n_outputs, int32_t dtype, int32_t gradient);
 int lbt_linear_log_loss(void* stream, const void* X, const void* weight, int32_t dtype, int64_t n_rows, int32_t n_features,
                         int32_t n_outputs, const float* bias, const int64_t* y, float* loss, void* workspace,

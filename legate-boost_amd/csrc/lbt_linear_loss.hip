@@ -42,6 +42,9 @@ namespace {
 constexpr int kHalfShift = 14;
 constexpr int64_t kPieceBytes  = int64_t(512) << 20;  // of packed weights at a time
 constexpr int64_t kScoresBytes = int64_t(4) << 30;    // of G and of what it is made from at a time
+// The same where the workspace is the least that is taken: 8192 rows, 131072 classes of 4096 bfloat16 then ask for 0.38 GiB instead of 2.25,
+// and take 28.7 ms, as the scores are formed twice, instead of 21.6.
+constexpr int64_t kLeastPieceBytes = int64_t(64) << 20, kLeastScoresBytes = int64_t(128) << 20;
 
 template <int kDtype>
 struct LossType;
@@ -1450,8 +1453,10 @@ struct LossCall {
   float2* partial;
   float *row_sums, *class_sums, *bias_sums, *exps;
 
-  LossCall(int64_t all_rows, int f, int k, int type, int grad) : features(f), classes(k), dtype(type), gradient(grad != 0), with_bias(grad > 1)
+  LossCall(int64_t all_rows, int f, int k, int type, int grad, bool least)
+    : features(f), classes(k), dtype(type), gradient(grad != 0), with_bias(grad > 1)
   {
+    const int64_t scores_bytes = least ? kLeastScoresBytes : kScoresBytes, piece_bytes = least ? kLeastPieceBytes : kPieceBytes;
     const int64_t n = n_rows = rows_at_once(all_rows, f, k, type);
     parts                    = n < all_rows;
     planes = type == LBT_F32 ? 3 : 1;
@@ -1460,14 +1465,14 @@ struct LossCall {
     // Where rows are few beside the features, laying out the weights and reading their planes up to six times costs more than G once more
     // in the other order. (1000 floats, 30000 classes: 17 rows 150 us, 271 with the weights laid out; 256 rows 372 and 458; 1024 rows 1213
     // and 1155.) Below 8 us of it the products of small gradients share a launch instead.
-    floats_back = type == LBT_F32 && gradient && 10.0 * (f - n) * k / 5e6 > 8.0 && 16 * padded * round_up(k, 256) <= kScoresBytes;
+    floats_back = type == LBT_F32 && gradient && 10.0 * (f - n) * k / 5e6 > 8.0 && 16 * padded * round_up(k, 256) <= scores_bytes;
     packed = type == LBT_F32 ? gradient && !floats_back : f % 8 != 0;
     // a piece's G and its packed weights within their bounds; pieces of one size
     int64_t most = round_up(k, 256);
     kept                = type == LBT_BF16 && !with_bias ? kKeptShort : kKeptFloat;  // (the sums for the bias are those of floats)
     const int64_t bytes = 2 * planes + (kept == kKeptFloat ? 4 : 0);                // of an entry of G
-    if (gradient) most = std::min(most, kScoresBytes / (bytes * padded) / 256 * 256);
-    if (packed) most = std::min(most, kPieceBytes / (2 * planes * int64_t(cols)) / 256 * 256);
+    if (gradient) most = std::min(most, scores_bytes / (bytes * padded) / 256 * 256);
+    if (packed) most = std::min(most, piece_bytes / (2 * planes * int64_t(cols)) / 256 * 256);
     most  = std::max<int64_t>(most, 256);
     piece = round_up(tiles_of(k, tiles_of(k, most)), 256);
     if (!gradient || piece < k) kept = kNotKept;
@@ -1823,7 +1828,8 @@ int run_loss(void* stream, const void* X, const void* weight, int32_t dtype, int
     set_error("a workspace aligned to 256 bytes is needed");
     return LBT_ERR_WORKSPACE;
   }
-  LossCall c(std::max<int64_t>(n_rows, 1), n_features, n_outputs, dtype, !gradient ? 0 : grad_bias == nullptr ? 1 : 2);
+  const int kind = !gradient ? 0 : grad_bias == nullptr ? 1 : 2;
+  LossCall c(std::max<int64_t>(n_rows, 1), n_features, n_outputs, dtype, kind, false);
   const bool few = !gradient && few_loss(n_rows, n_features, n_outputs, dtype);
   FewCall f;
   Arena arena;
@@ -1831,6 +1837,17 @@ int run_loss(void* stream, const void* X, const void* weight, int32_t dtype, int
   arena.cap  = workspace_bytes;
   if (few) f.carve(arena, n_rows, n_outputs, dtype);
   else c.carve(arena);
+  if (arena.failed && !few) {  // the least, perhaps
+    LossCall smaller(std::max<int64_t>(n_rows, 1), n_features, n_outputs, dtype, kind, true);
+    Arena there;
+    there.base = arena.base;
+    there.cap  = arena.cap;
+    smaller.carve(there);
+    if (!there.failed) {
+      c            = smaller;
+      arena.failed = false;
+    }
+  }
   if (arena.failed) {
     set_error("workspace of %zu bytes, %zu needed", workspace_bytes, arena.used);
     return LBT_ERR_WORKSPACE;
@@ -1873,8 +1890,10 @@ extern "C" {
 
 size_t lbt_linear_log_loss_workspace_bytes(int64_t n_rows, int32_t n_features, int32_t n_outputs, int32_t dtype, int32_t gradient)
 {
+  const bool least = gradient >= LBT_LEAST_WORKSPACE;
+  if (least) gradient -= LBT_LEAST_WORKSPACE;
   if (!lbt::loss_shape(n_rows, n_features, n_outputs, dtype) || gradient < 0 || gradient > 2) return 0;
-  lbt::LossCall c(std::max<int64_t>(n_rows, 1), n_features, n_outputs, dtype, gradient);
+  lbt::LossCall c(std::max<int64_t>(n_rows, 1), n_features, n_outputs, dtype, gradient, least);
   lbt::Arena arena;
   arena.measure = true;
   if (gradient == 0 && lbt::few_loss(n_rows, n_features, n_outputs, dtype)) {

@@ -23,6 +23,7 @@ LBT_F32 = 0
 LBT_F64 = 1
 LBT_BF16 = 2
 LBT_F16 = 3
+LBT_LEAST_WORKSPACE = 4
 LBT_MAX_SPLIT_SAMPLES = 2048
 LBT_OBJ_SQUARED_ERROR = 0
 LBT_OBJ_LOG_LOSS = 1

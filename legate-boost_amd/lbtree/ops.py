@@ -626,6 +626,19 @@ def _loss_arguments(X, weight, y, bias):
     return X, weight, y, bias
 
 
+def _loss_scratch(n, f, k, dt, gradient, device):
+    """The workspace of a loss; where there is no memory for it, the least that the call works with, as build_tree does."""
+    size = _lib.lib.lbt_linear_log_loss_workspace_bytes
+    need = size(n, f, k, dt, gradient)
+    try:
+        return _scratch(need, device)
+    except torch.OutOfMemoryError:
+        least = size(n, f, k, dt, gradient + _lib.LBT_LEAST_WORKSPACE)
+        if least >= need:
+            raise
+        return _scratch(least, device)
+
+
 def _ptr(a):
     return None if a is None else a.data_ptr()
 
@@ -652,7 +665,10 @@ def linear_log_loss(X, weight, y, bias=None):
     No autograd graph is recorded: linear_log_loss_gradient returns the gradients."""
     if _NATIVE is not None and torch.cuda.is_initialized():
         device = torch.cuda.current_device()
-        got = _NATIVE.linear_log_loss(X, weight, y, bias, _scratch, _LOG_LOSS, _LOG_LOSS_BYTES, _raw_stream(device), device)
+        try:
+            got = _NATIVE.linear_log_loss(X, weight, y, bias, _scratch, _LOG_LOSS, _LOG_LOSS_BYTES, _raw_stream(device), device)
+        except torch.OutOfMemoryError:
+            got = None  # (below with less)
         if got is not None:
             if not isinstance(got, torch.Tensor):
                 _lib.check(got)
@@ -662,7 +678,7 @@ def linear_log_loss(X, weight, y, bias=None):
     k, dt = weight.shape[0], _DT_NARROW[X.dtype]
     with _On(X.device):
         loss = torch.empty(n, dtype=torch.float32, device=X.device)
-        ws = _scratch(_lib.lib.lbt_linear_log_loss_workspace_bytes(n, f, k, dt, 0), X.device)
+        ws = _loss_scratch(n, f, k, dt, 0, X.device)
         _lib.check(_lib.lib.lbt_linear_log_loss(_stream(), X.data_ptr(), weight.data_ptr(), dt, n, f, k, _ptr(bias), y.data_ptr(),
                                                 loss.data_ptr(), ws.data_ptr(), ws.numel()))
     return loss
@@ -675,8 +691,11 @@ def linear_log_loss_gradient(X, weight, y, sample_weight=None, bias=None):
     w (p - [c = y]) that they are of have X's type. The scratch holds these for up to 4 GiB of rows and classes (release_workspace)."""
     if _NATIVE is not None and torch.cuda.is_initialized():
         device = torch.cuda.current_device()
-        got = _NATIVE.linear_log_loss_gradient(X, weight, y, bias, _scratch, _LOG_LOSS_GRADIENT, _LOG_LOSS_BYTES, _raw_stream(device), device,
-                                               sample_weight)
+        try:
+            got = _NATIVE.linear_log_loss_gradient(X, weight, y, bias, _scratch, _LOG_LOSS_GRADIENT, _LOG_LOSS_BYTES, _raw_stream(device),
+                                                   device, sample_weight)
+        except torch.OutOfMemoryError:
+            got = None  # (below with less)
         if got is not None:
             if not isinstance(got, tuple):
                 _lib.check(got)
@@ -693,7 +712,7 @@ def linear_log_loss_gradient(X, weight, y, sample_weight=None, bias=None):
         loss = torch.empty(n, dtype=torch.float32, device=X.device)
         grad_X, grad_weight = torch.empty_like(X), torch.empty_like(weight)
         grad_bias = None if bias is None else torch.empty(k, dtype=torch.float32, device=X.device)
-        ws = _scratch(_lib.lib.lbt_linear_log_loss_workspace_bytes(n, f, k, dt, 1 if bias is None else 2), X.device)
+        ws = _loss_scratch(n, f, k, dt, 1 if bias is None else 2, X.device)
         _lib.check(_lib.lib.lbt_linear_log_loss_gradient(
             _stream(), X.data_ptr(), weight.data_ptr(), dt, n, f, k, _ptr(bias), y.data_ptr(), _ptr(w), loss.data_ptr(),
             grad_X.data_ptr(), grad_weight.data_ptr(), _ptr(grad_bias), ws.data_ptr(), ws.numel()))

@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from lbtree import _lib, ops
-from test_gpu_vocabulary import inputs
+from test_gpu_vocabulary import TYPES, check, inputs
 
 pytestmark = pytest.mark.gpu
 
@@ -62,3 +62,43 @@ def test_small_probabilities_keep_their_bits(n, f, k):
     rel = float(2 * ((f + 8) * 2.0 ** -24 + 2.0 ** -22) * (W.abs() @ X.abs()).max() + 1e-4)
     bound = (2.0 ** -11 + 2 * 2.0 ** -8 + rel) * (1 + 2.0 ** -6)
     assert ((gw[rest].double() - want).abs() <= bound * want).all()
+
+
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("n,f,k", [(2000, 72, 60000), (1200, 520, 90001), (700, 2100, 20000)])
+def test_where_memory_is_short(n, f, k, dtype, native, monkeypatch):
+    """No room for the workspace that is asked for first: the least is, in pieces of the classes, and gives the same up to rounding."""
+    if not native:
+        monkeypatch.setattr(ops, "_NATIVE", None)
+    size = _lib.lib.lbt_linear_log_loss_workspace_bytes
+    kinds = [size(n, f, k, ops._DT_NARROW[TYPES[dtype]], kind) for kind in (1, 2, 5, 6)]
+    assert kinds[2] < kinds[0] and kinds[3] < kinds[1]
+    asked = []
+
+    def scratch(nbytes, device):
+        asked.append(nbytes)
+        if nbytes > max(kinds[2:]):
+            raise torch.OutOfMemoryError("no room")
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+    monkeypatch.setattr(ops, "_scratch", scratch)
+    x, w, y = inputs(n, f, k, dtype, seed=n)
+    y[::7] = -1
+    x[::7] = float("nan")
+    gen = torch.Generator(device="cuda").manual_seed(k)
+    bias = torch.randn(k, generator=gen, device="cuda")
+    weight = torch.rand(n, generator=gen, device="cuda") + 0.1
+    check(x, w, y, dtype)
+    assert kinds[0] in asked and kinds[2] in asked
+    check(x, w, y, dtype, bias=bias, weight=weight)
+    assert kinds[1] in asked and kinds[3] in asked
+
+    def none(nbytes, device):
+        raise torch.OutOfMemoryError("no room")
+
+    monkeypatch.setattr(ops, "_scratch", none)
+    with pytest.raises(torch.OutOfMemoryError):
+        ops.linear_log_loss_gradient(x, w, y)
+    with pytest.raises(torch.OutOfMemoryError):
+        ops.linear_log_loss(x, w, y)

@@ -166,3 +166,16 @@ def test_nothing_overlaps_an_empty_array():
     grad = L.lbt_embed_rows_gradient
     assert grad(None, inside(OUT), _lib.LBT_F32, inside(OUT, 64), 8, 0, 8, 10, 1.0, 0, OUT, None, 0) == -3
     assert b"workspace" in L.lbt_last_error()
+
+
+def test_the_least_workspace():
+    q, least = L.lbt_linear_log_loss_workspace_bytes, 4
+    for dtype in (_lib.LBT_BF16, _lib.LBT_F16, _lib.LBT_F32):
+        for kind in (0, 1, 2):
+            for n, f, k in ((10, 8, 100), (8192, 4096, 131072), (4096, 1000, 30000), (1, 1024, 32768), (300000, 64, 5000)):
+                assert 0 < q(n, f, k, dtype, least + kind) <= q(n, f, k, dtype, kind), (dtype, kind, n, f, k)
+        # X, its planes and sums, tops and totals, and those 128 MiB of G and 64 of weights
+        assert q(8192, 4096, 131072, dtype, least + 1) < (7 << 27) and q(8192, 4096, 131072, dtype, 1) > (5 << 28)
+        assert q(10, 8, 100, dtype, 7) == 0 and q(10, 0, 100, dtype, least) == 0
+    need, small = q(8192, 4096, 131072, _lib.LBT_BF16, 1), q(8192, 4096, 131072, _lib.LBT_BF16, least + 1)
+    assert gradient(n=8192, f=4096, k=131072, ws=WS, size=small - 1) == -3 and str(need).encode() in L.lbt_last_error()
