@@ -537,9 +537,10 @@ int lbt_gather_rows(void* stream, const void* X, int32_t x_dtype, int64_t row_of
 /*
  * Log loss of linear scores over many classes (a vocabulary), where lbt_weighted_gradient takes the scores themselves:
  *   s[r][c] = <X[r], weight[c]> + bias[c];   loss[r] = log sum_c exp(s[r][c]) - s[r][y[r]]
- * The scores are formed in tiles of rows and classes and never written (the gradient below holds a piece of them). Sums, tops and totals are held in 32 bits; LBT_F32
- * inputs are multiplied as three planes of bfloat16 each, which gives products as exact as those of float (but values below
- * 2^-110 lose their last bits, and an infinity among the values of a row that counts, or of the weights, may come out as NaN).
+ * The scores are formed in tiles of rows and classes and never written (the gradient below holds a piece of them). Sums, tops and
+ * totals are held in 32 bits; LBT_F32 inputs are multiplied as three planes of bfloat16 each, which gives products as exact as
+ * those of float (but values below 2^-110 lose their last bits, and an infinity among the values of a row that counts, or of the
+ * weights, may come out as NaN).
  *   X       device [n_rows][n_features], dtype LBT_F32, LBT_BF16 or LBT_F16, 16-byte aligned
  *   weight  device [n_outputs][n_features], the same dtype, 16-byte aligned
  *   bias    device float [n_outputs], or NULL. A class whose bias is -inf takes no part (p = 0; a row with that label has an

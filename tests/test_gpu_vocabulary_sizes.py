@@ -5,7 +5,7 @@ the sum of sizes; the values here have one sign for half of the classes, so that
 import pytest
 import torch
 
-from lbtree import ops
+from lbtree import _lib, ops
 from test_gpu_vocabulary import ENTRY, LEAST, STEP, TYPES, U, assert_within
 
 pytestmark = pytest.mark.gpu
@@ -93,6 +93,54 @@ def test_rows_in_parts_and_classes_in_pieces():
     for i, got in enumerate(ops.linear_log_loss_gradient(x, w, y)):
         assert_within(got, want[i], bound[i], ("loss", "grad_X", "grad_weight")[i])
     assert_within(ops.linear_log_loss(x, w, y), want[0], bound[0], "loss alone")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+def test_rows_in_parts_captured_and_replayed(dtype):
+    n, f, k = 140000, 10, 9
+    gen = torch.Generator(device="cuda").manual_seed(13)
+    x = torch.rand((n, f), generator=gen, device="cuda").to(TYPES[dtype])
+    w = torch.randn((k, f), generator=gen, device="cuda").to(TYPES[dtype])
+    y = torch.randint(-1, k, (n,), generator=gen, device="cuda")
+    weight, bias = torch.rand(n, generator=gen, device="cuda") * 1e-3, torch.randn(k, generator=gen, device="cuda")
+    ops.linear_log_loss_gradient(x, w, y, sample_weight=weight, bias=bias)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = ops.linear_log_loss_gradient(x, w, y, sample_weight=weight, bias=bias) + (ops.linear_log_loss(x, w, y),)
+    for _ in range(3):
+        y.copy_(torch.roll(y, 70001))
+        weight.mul_(3.0)
+        graph.replay()
+        want = ops.linear_log_loss_gradient(x, w, y, sample_weight=weight, bias=bias) + (ops.linear_log_loss(x, w, y),)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+def test_rows_in_parts_where_memory_is_short(dtype, monkeypatch):
+    """Two parts of the rows, and the least workspace: several pieces of the classes in each."""
+    n, f, k = 140000, 20, 3000
+    size = _lib.lib.lbt_linear_log_loss_workspace_bytes
+    full, least = (size(n, f, k, ops._DT_NARROW[TYPES[dtype]], kind) for kind in (2, 2 + _lib.LBT_LEAST_WORKSPACE))
+    assert least < full / 2
+
+    def scratch(nbytes, device):
+        if nbytes > least:
+            raise torch.OutOfMemoryError("no room")
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+    monkeypatch.setattr(ops, "_scratch", scratch)
+    gen = torch.Generator(device="cuda").manual_seed(11)
+    x = (torch.rand((n, f), generator=gen, device="cuda") * 0.5).to(TYPES[dtype])
+    w = (torch.randn((k, f), generator=gen, device="cuda") * 0.3).to(TYPES[dtype])
+    y = torch.randint(0, k // 2, (n,), generator=gen, device="cuda")
+    y[::5] = -1
+    x[::5] = float("nan")
+    weight = (torch.rand(n, generator=gen, device="cuda") + 0.5) * torch.where(torch.arange(n, device="cuda") < n // 2, 2e-3, 1e-2)
+    bias = torch.randn(k, generator=gen, device="cuda")
+    want, bound = reference_by_rows(x, w, y, bias, weight, dtype, 20000)
+    for i, got in enumerate(ops.linear_log_loss_gradient(x, w, y, sample_weight=weight, bias=bias)):
+        assert_within(got, want[i], bound[i], ("loss", "grad_X", "grad_weight", "grad_bias")[i])
 
 
 @pytest.mark.parametrize("dtype,n,f", [("f32", 9000, 66000), ("f16", 8300, 132000), ("bf16", 8300, 131073)])
