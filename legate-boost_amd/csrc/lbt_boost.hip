@@ -628,16 +628,6 @@ __global__ void __launch_bounds__(kBoostThreads) feature_mask_kernel(MaskBits bi
 
 inline unsigned grid_for(int64_t n) { return static_cast<unsigned>((n + kBoostThreads - 1) / kBoostThreads); }
 
-// part(first, rows) for as many rows at a time, of `width` entries each, as a launch with a thread for each entry may have.
-constexpr int64_t kMostEntries = int64_t(1) << 31;
-template <class Part>
-int by_parts(int64_t n_rows, int64_t width, const Part& part)
-{
-  const int64_t most = std::max<int64_t>(kMostEntries / width, 1);
-  for (int64_t first = 0; first < n_rows; first += most) LBT_TRY(part(first, std::min(most, n_rows - first)));
-  return LBT_OK;
-}
-
 }  // namespace lbt
 
 extern "C" {

@@ -45,6 +45,16 @@ void set_error(const char* fmt, ...);
 // Workgroups that a launch may have along x: the runtime takes their threads modulo 2^32, and runs that many without an error.
 constexpr int64_t most_groups(int threads) { return (int64_t(1) << 32) / threads - 1; }
 
+// part(first, rows) for as many rows at a time, of `width` entries each, as a launch with a thread for each entry may have.
+constexpr int64_t kMostEntries = int64_t(1) << 31;
+template <class Part>
+int by_parts(int64_t n_rows, int64_t width, const Part& part)
+{
+  const int64_t most = kMostEntries / width > 1 ? kMostEntries / width : 1;
+  for (int64_t first = 0; first < n_rows; first += most) LBT_TRY(part(first, most < n_rows - first ? most : n_rows - first));
+  return LBT_OK;
+}
+
 // What a call reads or writes; null, or no bytes: nothing.
 struct MemoryRange {
   const void* begin;

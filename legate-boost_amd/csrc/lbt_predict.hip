@@ -133,6 +133,7 @@ constexpr int kPackTrees    = 104; // trees packed per launch
 constexpr int kFirstBatches = 10;  // and batch descriptors written by the first one
 constexpr int kPackBatches  = 128; // batch descriptors written per launch of their own
 constexpr int kTileThreads  = 1024;
+constexpr int kMostLanes    = 16;  // threads of a row
 // L lanes share a row; a workgroup then covers 1024 / L rows, and a batch holds L * kLaneTrees
 // trees. Wide feature matrices take more lanes per row, so that the row tile still fits the LDS.
 // kFew: an ensemble of at most L trees (the one tree a boosting round predicts with): one tree
@@ -1139,6 +1140,12 @@ int lbt_predict_from(void* stream, const void* X, int32_t x_dtype, int64_t n_row
   LBT_REQUIRE(n_trees == 0 || (leaf && feature && split && tree_nodes), "null tree arrays");
   for (int i = 0; i < n_trees; i++)
     LBT_REQUIRE(leaf[i] && feature[i] && split[i] && tree_nodes[i] >= 1, "tree %d is incomplete", i);
+  const int64_t width = std::max<int64_t>(n_outputs, lbt::kMostLanes);
+  if (n_rows * width > lbt::kMostEntries)
+    return lbt::by_parts(n_rows, width, [&](int64_t first, int64_t rows) {
+      return lbt_predict_from(stream, static_cast<const char*>(X) + first * n_features * (x_dtype == LBT_F32 ? 4 : 8), x_dtype, rows, n_features, n_trees,
+                              leaf, feature, split, tree_nodes, n_outputs, init, out + first * n_outputs, workspace, workspace_bytes);
+    });
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (n_trees == 0) {
     lbt::zero_doubles_kernel<<<static_cast<unsigned>((n + 255) / 256), 256, 0, s>>>(out, n);
@@ -1221,6 +1228,11 @@ int lbt_predict_packed(void* stream, const void* X, int32_t x_dtype, int64_t n_r
               "corrupt ensemble descriptor (buffer size)");
   if (n_rows < 1) return LBT_OK;
   LBT_REQUIRE(X && out, "null X or output");
+  if (n_rows * lbt::kMostLanes > lbt::kMostEntries)
+    return lbt::by_parts(n_rows, lbt::kMostLanes, [&](int64_t first, int64_t rows) {
+      return lbt_predict_packed(stream, static_cast<const char*>(X) + first * n_features * (x_dtype == LBT_F32 ? 4 : 8), x_dtype, rows, n_features,
+                                ensemble, out + first * ensemble->n_outputs);
+    });
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (x_dtype == LBT_F32) return lbt::run_tiled<float>(s, static_cast<const float*>(X), n_rows, *ensemble, out);
   return lbt::run_tiled<double>(s, static_cast<const double*>(X), n_rows, *ensemble, out);

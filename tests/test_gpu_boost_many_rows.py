@@ -68,3 +68,36 @@ def test_gradients(objective):
         for i in range(0, times, 1 << 20):
             part = view[i:i + (1 << 20)]
             assert torch.equal(part[:, 0], one[0].expand(part.shape[0], k)) and not part[:, 1:].any()
+
+
+def test_predictions():
+    n, few = (1 << 30) + 1003, 59  # four threads a row, or more
+    values = torch.linspace(-1, 1, few, device="cuda").view(few, 1)
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    g = torch.randn((few, 1), generator=gen, device="cuda", dtype=torch.float64)
+    trees = [ops.build_tree(values, g * (i + 1), torch.ones_like(g), max_depth=3, split_samples=16, seed=i) for i in range(9)]
+    trees = [(t.leaf_value, t.feature, t.split_value) for t in trees]
+    X = values.repeat((-(-n // few), 1))[:n].contiguous()
+    packed = ops.PackedEnsemble(trees, 1, 1)
+    want = packed.predict(values)
+    assert want.unique().numel() > 5
+    init = torch.full((1,), 0.75, dtype=torch.float64, device="cuda")
+    for got, one in ((packed.predict(X), want), (ops.predict(X, trees, 1), want), (ops.predict(X, trees, 1, init=init), ops.predict(values, trees, 1, init=init))):
+        assert got.shape == (n, 1)
+        whole = n // few * few
+        view = got[:whole].view(-1, few)
+        for i in range(0, view.shape[0], 1 << 21):
+            assert torch.equal(view[i:i + (1 << 21)], one.view(1, few).expand(min(1 << 21, view.shape[0] - i), few))
+        assert torch.equal(got[whole:], one[:n - whole])
+
+
+def test_predictions_of_no_tree():
+    k = 8
+    n = (1 << 32) // k + 1007
+    X = torch.zeros((n, 1), device="cuda")
+    fill = torch.full((n * k,), 3.0, dtype=torch.float64, device="cuda")  # what the output's memory held
+    del fill
+    init = torch.arange(k, dtype=torch.float64, device="cuda")
+    got = ops.predict(X, [], k, init=init)
+    for i in range(0, n, 1 << 25):
+        assert torch.equal(got[i:i + (1 << 25)], init.expand(min(1 << 25, n - i), k))
